@@ -122,6 +122,12 @@ EXTRA_FLAGS = {
 PRECISE_MATH = {"loss.hip", "optim.hip", "bn_finalize.hip"}
 
 
+# No packed fp32 arithmetic (v_pk_add_f32, v_pk_mul_f32, v_pk_fma_f32): the compiler forms it from ordinary float code by
+# itself, and some of its forms have given wrong results now and then.  (hipcc's host pass warns that it does not know the
+# feature.)
+NO_PACKED_FP32 = ["-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+
+
 def _math_flags(name: str) -> List[str]:
     return ["-ffp-contract=fast", "-fno-math-errno"] if name in PRECISE_MATH else ["-ffast-math"]
 
@@ -132,7 +138,7 @@ def _compile_kernel(src: Path, headers: List[Path], force: bool) -> Path:
         _run(
             [
                 _hipcc(), "-O3", "-std=c++17", "-fPIC", "-c", f"--offload-arch={ARCH}", *_math_flags(src.name),
-                *EXTRA_FLAGS.get(src.name, []),
+                *EXTRA_FLAGS.get(src.name, []), *NO_PACKED_FP32,
                 "-Wall", "-Wno-unused-function", f"-I{CSRC / 'kernels'}", "-o", str(obj), str(src),
             ]
         )
