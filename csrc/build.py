@@ -109,6 +109,7 @@ def build_rccl(force: bool = False) -> Path:
 # to use VGPR destinations there.
 EXTRA_FLAGS = {
     "attention.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
+    "attention_packed.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form=1"],
 }
 
 # Floating-point model per file.  -ffast-math tells the compiler that no NaN or infinity ever occurs
@@ -119,7 +120,7 @@ EXTRA_FLAGS = {
 # (under finite-math-only even a bit test of the exponent field is folded away: the compiler may assume that no float
 # argument is an Inf or a NaN).  bn.hip's element-wise passes stay on the fast model - they run at the memory roof
 # and lose 2 % to the NaN-aware forms of max().
-PRECISE_MATH = {"loss.hip", "optim.hip", "bn_finalize.hip"}
+PRECISE_MATH = {"loss.hip", "optim.hip", "bn_finalize.hip", "attention_packed.hip"}
 
 
 # No packed fp32 arithmetic (v_pk_add_f32, v_pk_mul_f32, v_pk_fma_f32): the compiler forms it from ordinary float code by

@@ -9,11 +9,13 @@ kernel library is an error, not a fallback.
 
 from __future__ import annotations
 
+import math
 from typing import Optional
 
 import torch
 
 from . import reference as _ref
+from .packing import SequencePack, pack_sequences  # noqa: F401
 
 
 import os as _os
@@ -148,6 +150,62 @@ def attention_qkv(qkv, heads: int, causal: bool = False):
     if qkv.is_cuda:
         return _hip().attention_qkv(qkv, heads, causal)
     return _ref.attention_qkv(qkv, heads, causal)
+
+
+def _check_packed(x, pack, name: str) -> None:
+    if not isinstance(pack, SequencePack):
+        raise TypeError("pack: a SequencePack, made by ops.pack_sequences")
+    if x.device != pack.device:
+        raise ValueError(f"{name} on {x.device}, pack on {pack.device}")
+    if x.shape[0] != pack.rows:
+        raise ValueError(f"{name} has {x.shape[0]} rows, the pack {pack.rows}")
+    if not x.is_floating_point():
+        raise TypeError(f"{name} must be a floating-point tensor")
+
+
+def _check_scale(scale: Optional[float], head_dim: int) -> float:
+    scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
+    if not 0.0 < scale < math.inf:
+        raise ValueError("the softmax scale must be positive and finite")
+    return scale
+
+
+def attention_packed(q, k, v, pack: SequencePack, causal: bool = True, scale: Optional[float] = None):
+    """Attention inside every sequence of a pack, with grouped heads: ``q`` ``[T, H, D]``, ``k`` and ``v`` ``[T, Hk, D]`` ->
+    ``[T, H, D]``, query head ``h`` reading head ``h // (H // Hk)``.  A row attends to the rows of its own sequence, up to
+    itself if ``causal``; rows outside every sequence give 0 and get no gradient.  ``scale`` defaults to ``1 / sqrt(D)``.
+    On GPU: ``D`` of 64 or 128, computed in bf16 (fp32 softmax), any strides with a contiguous last axis."""
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+        raise ValueError(f"expected [T, H, D], [T, Hk, D], [T, Hk, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
+        raise ValueError(f"{q.shape[1]} query heads cannot share {k.shape[1]} key heads")
+    for x, name in ((q, "q"), (k, "k"), (v, "v")):
+        _check_packed(x, pack, name)
+    scale = _check_scale(scale, q.shape[2])
+    if q.is_cuda:
+        from . import hip_packed
+
+        return hip_packed.attention_packed(q, k, v, pack, causal, scale)
+    return _ref.attention_packed(q, k, v, pack.spans, causal, scale)
+
+
+def attention_packed_qkv(qkv, pack: SequencePack, heads: int, kv_heads: Optional[int] = None, causal: bool = True, scale: Optional[float] = None):
+    """:func:`attention_packed` on a joint projection ``[T, (heads + 2 * kv_heads) * D]`` (query heads, key heads, value
+    heads) -> ``[T, heads * D]``; on GPU the projection is read in place and its gradient written as one tensor."""
+    kv_heads = heads if kv_heads is None else kv_heads
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads cannot share {kv_heads} key heads")
+    if qkv.dim() != 2 or qkv.shape[1] == 0 or qkv.shape[1] % (heads + 2 * kv_heads):
+        raise ValueError(f"expected [T, ({heads} + 2 * {kv_heads}) * D], got {tuple(qkv.shape)}")
+    _check_packed(qkv, pack, "qkv")
+    scale = _check_scale(scale, qkv.shape[1] // (heads + 2 * kv_heads))
+    if qkv.is_cuda:
+        from . import hip_packed
+
+        return hip_packed.attention_packed_qkv(qkv, pack, heads, kv_heads, causal, scale)
+    x = qkv.view(qkv.shape[0], heads + 2 * kv_heads, -1)
+    out = _ref.attention_packed(x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:], pack.spans, causal, scale)
+    return out.reshape(qkv.shape[0], -1)
 
 
 def embedding(ids, weight):

@@ -1,0 +1,140 @@
+"""GPU attention over packed sequences with grouped heads (``csrc/kernels/attention_packed.hip``).
+
+Not exercised by the reference (its model is a CNN, /root/reference/src/main.py:49).
+"""
+
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .hip import _check, _ptr, _stream
+from .hip_transformer import _f, _i, _ll, _sig, _vp
+
+_pack_spans = _sig("pdt_pack_spans", [_vp, _i, _i, _vp, _vp, _vp])
+_fwd = _sig("pdt_packed_attention_fwd", [_vp] * 7 + [_i] * 4 + [_f, _i, _vp])
+_bwd = _sig("pdt_packed_attention_bwd", [_vp] * 11 + [_i, _vp, _vp] + [_i] * 4 + [_f, _i, _vp])
+_splits = _sig("pdt_packed_attention_splits", [_i] * 3)
+
+HEAD_DIMS = (64, 128)
+
+
+def pack_spans(offsets, rows: int):
+    with torch.cuda.device(offsets.device):
+        offsets = offsets.to(torch.int32).contiguous()
+        spans = torch.empty((rows, 2), dtype=torch.int32, device=offsets.device)
+        positions = torch.empty(rows, dtype=torch.int64, device=offsets.device)
+        if rows:
+            _check(_pack_spans(offsets.data_ptr(), offsets.numel() - 1, rows, spans.data_ptr(), positions.data_ptr(), _stream()), "pack_spans")
+    return spans, positions
+
+
+def _heads(x: torch.Tensor) -> torch.Tensor:
+    """[T, heads, D] in bf16 with unit stride along D and rows and heads on 16-byte boundaries (a view where it is one already)."""
+    if x.dtype != torch.bfloat16:
+        x = x.to(torch.bfloat16)
+    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.stride(0) <= 0 or x.stride(1) <= 0 or x.data_ptr() % 16:
+        x = x.clone(memory_format=torch.contiguous_format)
+    return x
+
+
+def _strides(*xs):
+    vals = [s for x in xs for s in (x.stride(0), x.stride(1))]
+    return (ctypes.c_longlong * len(vals))(*vals)
+
+
+def _forward(q, k, v, spans, causal: bool, scale: float):
+    t, h, d = q.shape
+    out = torch.empty((t, h, d), dtype=torch.bfloat16, device=q.device)
+    lse = torch.empty((h, t), dtype=torch.float32, device=q.device)
+    if out.numel():
+        _check(_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), spans.data_ptr(), _strides(q, k, v), t, h,
+                    k.shape[1], d, scale, int(causal), _stream()), "packed_attention_fwd")
+    return out, lse
+
+
+def _backward(q, k, v, out, lse, g, spans, causal: bool, scale: float, dq, dk, dv) -> None:
+    t, h, d = q.shape
+    hk = k.shape[1]
+    if not q.numel():
+        return
+    if g.dtype != torch.bfloat16:
+        g = g.to(torch.bfloat16)
+    if not g.is_contiguous() or g.data_ptr() % 16:
+        g = g.clone(memory_format=torch.contiguous_format)
+    delta = torch.empty((h, t), dtype=torch.float32, device=q.device)
+    splits = _splits(t, h, hk)
+    part = torch.empty((splits, 2, t, hk, d), dtype=torch.float32, device=q.device) if splits > 1 else None
+    _check(_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), g.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(),
+                dk.data_ptr(), dv.data_ptr(), _ptr(part), splits, spans.data_ptr(), _strides(q, k, v, dq, dk, dv), t, h, hk, d, scale,
+                int(causal), _stream()), "packed_attention_bwd")
+
+
+class _AttentionPacked(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, spans, causal: bool, scale: float):
+        with torch.cuda.device(q.device):
+            q, k, v = _heads(q), _heads(k), _heads(v)
+            out, lse = _forward(q, k, v, spans, causal, scale)
+        ctx.save_for_backward(q, k, v, out, lse, spans)
+        ctx.meta = (causal, scale)
+        return out
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        q, k, v, out, lse, spans = ctx.saved_tensors
+        with torch.cuda.device(q.device):
+            dq, dk, dv = (torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) for x in (q, k, v))
+            _backward(q, k, v, out, lse, g, spans, *ctx.meta, dq, dk, dv)
+        return dq, dk, dv, None, None, None
+
+
+def _split_qkv(qkv, heads: int, kv_heads: int):
+    t, width = qkv.shape
+    d = width // (heads + 2 * kv_heads)
+    x = qkv.view(t, heads + 2 * kv_heads, d)
+    return x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:]
+
+
+class _AttentionPackedQKV(torch.autograd.Function):
+    """On the projection's output, whose gradient is written as one tensor (no split in forward, no concatenation behind)."""
+
+    @staticmethod
+    def forward(ctx, qkv, heads: int, kv_heads: int, spans, causal: bool, scale: float):
+        with torch.cuda.device(qkv.device):
+            if qkv.dtype != torch.bfloat16:
+                qkv = qkv.to(torch.bfloat16)
+            if not qkv.is_contiguous() or qkv.data_ptr() % 16:
+                qkv = qkv.clone(memory_format=torch.contiguous_format)
+            out, lse = _forward(*_split_qkv(qkv, heads, kv_heads), spans, causal, scale)
+        ctx.save_for_backward(qkv, out, lse, spans)
+        ctx.meta = (heads, kv_heads, causal, scale)
+        return out.view(qkv.shape[0], -1)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, g):
+        qkv, out, lse, spans = ctx.saved_tensors
+        heads, kv_heads, causal, scale = ctx.meta
+        with torch.cuda.device(qkv.device):
+            dqkv = torch.empty_like(qkv)
+            _backward(*_split_qkv(qkv, heads, kv_heads), out, lse, g.reshape(out.shape), spans, causal, scale,
+                      *_split_qkv(dqkv, heads, kv_heads))
+        return dqkv, None, None, None, None, None
+
+
+def _check_head_dim(d: int) -> None:
+    if d not in HEAD_DIMS:
+        raise ValueError(f"the packed attention kernels need a head_dim of 64 or 128, got {d}")
+
+
+def attention_packed(q, k, v, pack, causal: bool, scale: float):
+    _check_head_dim(q.shape[2])
+    return _AttentionPacked.apply(q, k, v, pack.spans, bool(causal), scale)
+
+
+def attention_packed_qkv(qkv, pack, heads: int, kv_heads: int, causal: bool, scale: float):
+    _check_head_dim(qkv.shape[1] // (heads + 2 * kv_heads))
+    return _AttentionPackedQKV.apply(qkv, heads, kv_heads, pack.spans, bool(causal), scale)

@@ -108,6 +108,24 @@ def attention_qkv(qkv, heads: int, causal: bool = False):
     return attention(q, k, v, causal).transpose(1, 2).reshape(b, s, d)
 
 
+def attention_packed(q, k, v, spans, causal: bool, scale: float):
+    """Attention inside the sequences given by ``spans`` (``[T, 2]``, first row and end of each row's sequence); heads of
+    ``k`` / ``v`` are shared by equal groups of heads of ``q``.  Rows outside every sequence give zeros."""
+    group = q.shape[1] // k.shape[1]
+    out = q.new_zeros(q.shape) + 0.0 * q[:0].sum()  # (differentiable also where there is no sequence at all)
+    parts, end = [], 0
+    for first, stop in torch.unique(spans, dim=0).tolist():
+        if stop > first:
+            qs, ks, vs = (x[first:stop].transpose(0, 1) for x in (q, k.repeat_interleave(group, 1), v.repeat_interleave(group, 1)))
+            up = torch.promote_types(q.dtype, torch.float32)
+            s = (qs.to(up) @ ks.to(up).transpose(1, 2)) * scale
+            if causal:
+                s = s.masked_fill(torch.ones(s.shape[1:], dtype=torch.bool, device=s.device).triu(1), float("-inf"))
+            parts += [out[end:first], (torch.softmax(s, dim=-1) @ vs.to(up)).transpose(0, 1).to(q.dtype)]
+            end = stop
+    return torch.cat(parts + [out[end:]])
+
+
 def embedding(ids, weight):
     return F.embedding(ids, weight)
 

@@ -1,0 +1,260 @@
+"""Packed attention on the GPU against the formulas in 64 bits (needs an MI355X).
+
+Tolerances follow from the kernel's roundings alone, element by element: probabilities, score gradients and results are
+rounded to bf16, off by at most h = 2^-8 of the value each.  With P the exact probabilities,
+    |out - ref|  <= h (P |v|) + h |ref|                                                        =: E
+    |dv - ref|   <= h (P' |dout|) + h |ref|
+    |ds - ref|   <= h |ds| + P (|dout| E)   (the row term dout.out uses the rounded out)       =: F
+    |dq - ref|   <= scale (F |k|) + h |ref|,   |dk - ref| <= scale (F' |q|) + h |ref|
+Sums in 32 bits, exp2 (1 ulp of a 32-bit exponent of magnitude < 2^6) and second-order terms: 5 % on top, and 2e-5 of the
+sums' terms in place of zero.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+H = 2.0 ** -8
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from pytorch_distributed_training_amd import ops as m
+
+    return m
+
+
+def _inputs(t, h, hk, d, seed=0, std=1.0):
+    g = torch.Generator("cuda").manual_seed(seed)
+    r = lambda n: (torch.randn(t, n, d, generator=g, device="cuda") * std).to(torch.bfloat16)
+    return r(h), r(hk), r(hk), r(h)
+
+
+def _expected(q, k, v, do, offsets, causal, scale):
+    """(values, error bounds) of out, dq, dk, dv in 64 bits, one sequence and head at a time."""
+    q, k, v, do = (x.double() for x in (q, k, v, do))
+    group = q.shape[1] // k.shape[1]
+    val = [torch.zeros_like(x) for x in (q, q, k, v)]
+    err = [torch.zeros_like(x) for x in (q, q, k, v)]
+    for a, e in zip(offsets[:-1], offsets[1:]):
+        for j in range(q.shape[1]):
+            qs, ks, vs, ds_ = q[a:e, j], k[a:e, j // group], v[a:e, j // group], do[a:e, j]
+            s = qs @ ks.t() * scale
+            if causal:
+                s = s.masked_fill(torch.ones_like(s, dtype=torch.bool).triu(1), -math.inf)
+            p = torch.softmax(s, -1)
+            o = p @ vs
+            eo = (H + 2e-5) * (p @ vs.abs()) + H * o.abs()
+            dp = ds_ @ vs.t()
+            ds = p * (dp - (ds_ * o).sum(-1, keepdim=True))
+            f = H * ds.abs() + p * ((ds_.abs() * eo).sum(-1, keepdim=True) + 2e-5 * (ds_.abs() @ vs.abs().t()))
+            val[0][a:e, j], err[0][a:e, j] = o, eo
+            val[1][a:e, j], err[1][a:e, j] = scale * ds @ ks, scale * f @ ks.abs()
+            val[2][a:e, j // group] += scale * ds.t() @ qs
+            err[2][a:e, j // group] += scale * f.t() @ qs.abs()
+            val[3][a:e, j // group] += p.t() @ ds_
+            err[3][a:e, j // group] += (H + 2e-5) * p.t() @ ds_.abs()
+    return val, [e + (0 if i == 0 else H) * x.abs() for i, (x, e) in enumerate(zip(val, err))]
+
+
+def _check(got, val, err, what=("out", "dq", "dk", "dv")):
+    for name, x, y, e in zip(what, got, val, err):
+        assert x.shape == y.shape and bool(torch.isfinite(x).all()), name
+        over = (x.double() - y).abs() - 1.05 * e
+        assert float(over.max()) <= 0, f"{name}: {float(over.max()):.3g} over its bound at {int(over.argmax())}"
+
+
+def _offsets(lengths, first=0):
+    o = [first]
+    for n in lengths:
+        o.append(o[-1] + n)
+    return o
+
+
+CASES = [
+    # lengths, rows in front, rows behind, H, Hk, D, causal
+    ([1], 0, 0, 1, 1, 64, True),
+    ([2, 1, 0, 3], 0, 2, 2, 2, 128, True),
+    ([63, 64, 65, 1, 127, 129], 0, 3, 4, 2, 64, True),
+    ([63, 64, 65, 1, 127, 129], 5, 3, 4, 1, 128, False),
+    ([31, 33, 1, 1, 1, 200, 7, 300], 0, 0, 6, 3, 128, True),
+    ([1] * 200, 0, 1, 3, 3, 64, True),
+    ([1] * 130, 1, 0, 2, 1, 128, False),
+    ([700], 0, 0, 8, 1, 64, True),
+    ([1000, 24, 513], 0, 0, 5, 5, 64, False),
+    ([640, 383], 0, 0, 16, 2, 128, True),
+]
+
+
+@pytest.mark.parametrize("lengths,front,behind,h,hk,d,causal", CASES)
+def test_forward_and_gradients(ops, lengths, front, behind, h, hk, d, causal):
+    offsets = _offsets(lengths, front)
+    t = offsets[-1] + behind
+    q, k, v, do = _inputs(t, h, hk, d, seed=t)
+    for x in (q, k, v):
+        x.requires_grad_(True)
+    pack = ops.pack_sequences(torch.tensor(offsets, dtype=torch.int32, device="cuda"), t)
+    host = ops.pack_sequences(offsets, t)
+    assert torch.equal(pack.spans.cpu(), host.spans) and torch.equal(pack.positions.cpu(), host.positions)
+    out = ops.attention_packed(q, k, v, pack, causal=causal)
+    got = (out, *torch.autograd.grad(out, (q, k, v), do))
+    val, err = _expected(q.detach(), k.detach(), v.detach(), do, offsets, causal, d ** -0.5)
+    _check([x.detach() for x in got], val, err)  # (rows outside: values and bounds are zero)
+
+
+@pytest.mark.parametrize("h,hk,d", [(4, 2, 64), (3, 1, 128)])
+def test_joint_projection_views_and_scale(ops, h, hk, d):
+    """The joint form, views with gaps, other axis orders and another scale give what separate tensors give."""
+    offsets, t = _offsets([70, 3, 130]), 205
+    q, k, v, do = _inputs(t, h, hk, d, seed=7)
+    pack = ops.pack_sequences(offsets, t, device="cuda")
+    val, err = _expected(q, k, v, do, offsets, True, 0.11)
+    joint = torch.cat([q, k, v], 1).reshape(t, -1).requires_grad_(True)
+    out = ops.attention_packed_qkv(joint, pack, h, hk, scale=0.11)
+    (g,) = torch.autograd.grad(out, joint, do.reshape(t, -1))
+    g = g.view(t, h + 2 * hk, d)
+    a = [out.detach().view(t, h, d), g[:, :h], g[:, h:h + hk], g[:, h + hk:]]
+    _check(a, val, err)
+    wide = torch.zeros(t, h, d + 8, dtype=torch.bfloat16, device="cuda")
+    wide[:, :, :d] = q
+    qv = wide[:, :, :d].requires_grad_(True)                              # rows with gaps
+    kv = k.transpose(0, 1).contiguous().transpose(0, 1).requires_grad_(True)  # heads outermost
+    odd = torch.zeros(v.numel() + 1, dtype=torch.bfloat16, device="cuda")
+    vv = odd[1:].view(v.shape).copy_(v).requires_grad_(True)              # not on a 16-byte boundary
+    gout = do.transpose(0, 1).contiguous().transpose(0, 1)
+    out = ops.attention_packed(qv, kv, vv, pack, scale=0.11)
+    b = [out.detach(), *torch.autograd.grad(out, (qv, kv, vv), gout)]
+    for x, y in zip(a, b):
+        assert torch.equal(x, y)
+
+
+def test_fp32_inputs_are_computed_in_bf16(ops):
+    q, k, v, do = _inputs(40, 2, 2, 64)
+    pack = ops.pack_sequences([0, 40], 40, device="cuda")
+    ref = ops.attention_packed(q, k, v, pack)
+    qf = q.float().requires_grad_(True)
+    out = ops.attention_packed(qf, k.float(), v.float(), pack)
+    assert torch.equal(out.detach(), ref)
+    (g,) = torch.autograd.grad(out, qf, do)
+    assert g.dtype == torch.float32
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_large_scores_and_rising_maximum(ops, d):
+    """Scores far beyond the first keys' (the running maximum has to follow) and far below zero."""
+    offsets, t = _offsets([300, 200]), 500
+    q, k, v, do = _inputs(t, 2, 1, d, seed=3)
+    k[150:300] *= 16  # from the middle of the first sequence on
+    k[300:] *= 20
+    q[300:] = -k[300:, :1].clone() / 8  # the diagonal is hugely negative
+    pack = ops.pack_sequences(offsets, t, device="cuda")
+    with torch.no_grad():
+        out = ops.attention_packed(q, k, v, pack)
+    val, err = _expected(q, k, v, do, offsets, True, d ** -0.5)
+    # scores of magnitude s are off by s 2^-23 in 32 bits (products summed in fp32: s 2^-20 over d terms), so are exponents
+    s = float((q.double().abs().amax() * k.double().abs().amax()) * d ** 0.5)
+    slack = 2 * s * 2.0 ** -20
+    assert slack < 0.05
+    over = (out.double() - val[0]).abs() - 1.05 * err[0] - slack * v.double().abs().amax()
+    assert float(over.max()) <= 0
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_other_sequences_and_later_rows_do_not_show(ops, d, bad):
+    """NaN or infinity in one sequence, in rows outside and behind a row leave every other result as it is."""
+    offsets, t = [2, 40, 110, 150], 154
+    q, k, v, do = _inputs(t, 4, 2, d, seed=11)
+    pack = ops.pack_sequences(offsets, t, device="cuda")
+
+    def run(q, k, v, do):
+        q, k, v = (x.clone().requires_grad_(True) for x in (q, k, v))
+        out = ops.attention_packed(q, k, v, pack)
+        return [out.detach(), *torch.autograd.grad(out, (q, k, v), do)]
+
+    val, err = _expected(q, k, v, do, offsets, True, d ** -0.5)
+    q2, k2, v2, do2 = (x.clone() for x in (q, k, v, do))
+    for x in (q2, k2, v2, do2):
+        x[:2] = bad
+        x[150:] = bad
+        x[60:110] = bad  # the second sequence from its 20th row on
+    got = run(q2, k2, v2, do2)
+    keep = torch.ones(t, dtype=torch.bool, device="cuda")
+    keep[40:110] = False
+    _check([x[keep] for x in got], [x[keep] for x in val], [x[keep] for x in err])
+    for i in (0, 1):  # rows in front of the bad ones: their outputs and query gradients
+        _check([got[i][40:60]], [val[i][40:60]], [err[i][40:60]], [("out", "dq")[i]])
+    assert not torch.isfinite(got[0][60:110]).any()
+
+
+def test_offsets_beyond_the_rows_are_cut(ops):
+    q, k, v, _ = _inputs(20, 2, 2, 64)
+    far = ops.pack_sequences(torch.tensor([0, 5, 900], device="cuda"), 20)
+    cut = ops.pack_sequences([0, 5, 20], 20, device="cuda")
+    assert torch.equal(far.spans, cut.spans)
+    assert torch.equal(ops.attention_packed(q, k, v, far), ops.attention_packed(q, k, v, cut))
+
+
+def test_same_bits_every_time_and_on_another_stream(ops):
+    offsets, t = _offsets([300, 77, 400]), 777
+    q, k, v, do = _inputs(t, 8, 2, 128, seed=5)
+    for x in (q, k, v):
+        x.requires_grad_(True)
+    pack = ops.pack_sequences(offsets, t, device="cuda")
+
+    def run():
+        out = ops.attention_packed(q, k, v, pack)
+        return (out.detach(), *torch.autograd.grad(out, (q, k, v), do))
+
+    first = run()
+    torch.cuda.synchronize()
+    side = torch.cuda.Stream()
+    with torch.cuda.stream(side):
+        other = run()
+    side.synchronize()
+    for x, y, z in zip(first, run(), other):
+        assert torch.equal(x, y) and torch.equal(x, z)
+
+
+def test_captured_graph_follows_new_offsets_and_inputs(ops):
+    """Everything, the pack included, replayed over inputs and offsets written in place."""
+    t, h, hk, d = 260, 4, 2, 64
+    q, k, v, do = _inputs(t, h, hk, d)
+    offsets = torch.tensor([0, 100, 260], dtype=torch.int32, device="cuda")
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+
+    def run():
+        out = ops.attention_packed(q, k, v, ops.pack_sequences(offsets, t))
+        return (out, *torch.autograd.grad(out, leaves, do))
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = run()
+    for i, new in enumerate(([0, 1, 260], [0, 128, 256], [3, 200, 230], [0, 260, 260])):
+        offsets.copy_(torch.tensor(new, dtype=torch.int32))
+        with torch.no_grad():
+            for x, y in zip((q, k, v, do), _inputs(t, h, hk, d, seed=i + 50)):
+                x.copy_(y)
+        graph.replay()
+        torch.cuda.synchronize()
+        want = [x.detach().clone() for x in run()]
+        for x, y in zip(got, want):
+            assert torch.equal(x, y)
+
+
+def test_refusals(ops):
+    q, k, v, _ = _inputs(6, 2, 2, 64)
+    pack = ops.pack_sequences([0, 6], 6, device="cuda")
+    with pytest.raises(ValueError, match="head_dim"):
+        ops.attention_packed(q[..., :32], k[..., :32], v[..., :32], pack)
+    with pytest.raises(ValueError, match="pack on"):
+        ops.attention_packed(q, k, v, ops.pack_sequences([0, 6], 6))
+    with pytest.raises(ValueError, match="offsets on"):
+        ops.pack_sequences(torch.tensor([0, 6], device="cuda"), 6, device="cpu")

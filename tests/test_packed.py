@@ -1,0 +1,86 @@
+"""Packs of sequences and packed attention on the CPU: definitions, gradients and refusals."""
+import math
+
+import pytest
+import torch
+
+from pytorch_distributed_training_amd import ops
+
+
+def _pack(offsets, rows):
+    return ops.pack_sequences(offsets, rows)
+
+
+def test_pack_spans_and_positions():
+    p = _pack([1, 3, 3, 7], 9)
+    assert p.spans.tolist() == [[0, 0], [1, 3], [1, 3]] + [[3, 7]] * 4 + [[0, 0]] * 2
+    assert p.positions.tolist() == [0, 0, 1, 0, 1, 2, 3, 0, 0]
+    assert _pack(torch.tensor([0], dtype=torch.int32), 2).spans.tolist() == [[0, 0], [0, 0]]
+    assert _pack([0, 0], 0).spans.shape == (0, 2)
+
+
+@pytest.mark.parametrize("offsets,rows", [([0, 5, 4], 8), ([-1, 4], 8), ([0, 9], 8), ([], 8), ([0, 4], -1), ([[0, 4]], 8), ([0.0, 4.0], 8)])
+def test_pack_refusals(offsets, rows):
+    with pytest.raises(ValueError):
+        ops.pack_sequences(torch.tensor(offsets), rows)
+
+
+def _qkv(t, h, hk, d, dtype=torch.float64):
+    g = torch.Generator().manual_seed(t * 31 + h)
+    return [torch.randn(t, n, d, generator=g, dtype=dtype, requires_grad=True) for n in (h, hk, hk)]
+
+
+@pytest.mark.parametrize("causal", [True, False])
+def test_matches_masked_softmax(causal):
+    q, k, v = _qkv(12, 4, 2, 8)
+    pack = _pack([0, 1, 1, 6, 11], 12)
+    out = ops.attention_packed(q, k, v, pack, causal=causal)
+    row = torch.arange(12)
+    seq = torch.tensor([0] + [1] * 5 + [2] * 5 + [-1])
+    seen = (seq[:, None] == seq[None]) & (seq[:, None] >= 0)
+    if causal:
+        seen &= row[:, None] >= row[None]
+    s = torch.einsum("ihd,jhd->hij", q, k.repeat_interleave(2, 1)) / math.sqrt(8)
+    p = torch.softmax(s.masked_fill(~seen, -1e300), -1) * seen
+    ref = torch.einsum("hij,jhd->ihd", p, v.repeat_interleave(2, 1))
+    torch.testing.assert_close(out, ref, rtol=1e-12, atol=1e-12)
+    assert out[11].abs().max() == 0
+
+
+def test_gradients_against_differences():
+    q, k, v = _qkv(7, 2, 1, 4)
+    pack = _pack([0, 3, 6], 7)
+    assert torch.autograd.gradcheck(lambda a, b, c: ops.attention_packed(a, b, c, pack, scale=0.3), (q, k, v))
+    joint = torch.randn(7, 16, dtype=torch.float64, requires_grad=True)
+    assert torch.autograd.gradcheck(lambda x: ops.attention_packed_qkv(x, pack, 2, 1, causal=False), (joint,))
+
+
+def test_no_sequences():
+    q, k, v = _qkv(3, 2, 1, 4)
+    out = ops.attention_packed(q, k, v, _pack([0], 3))
+    out.sum().backward()
+    assert out.abs().max() == 0 and q.grad.abs().max() == 0
+
+
+def test_attention_refusals():
+    q, k, v = _qkv(6, 4, 2, 8)
+    pack = _pack([0, 6], 6)
+    with pytest.raises(ValueError, match="cannot share"):
+        ops.attention_packed(q[:, :3], k, v, pack)
+    with pytest.raises(ValueError, match="expected"):
+        ops.attention_packed(q, k, v[:, :1], pack)
+    with pytest.raises(ValueError, match="expected"):
+        ops.attention_packed(q[0], k, v, pack)
+    with pytest.raises(ValueError, match="rows"):
+        ops.attention_packed(q, k, v, _pack([0, 5], 5))
+    with pytest.raises(TypeError, match="pack"):
+        ops.attention_packed(q, k, v, torch.tensor([0, 6]))
+    with pytest.raises(TypeError, match="floating"):
+        ops.attention_packed(q.long(), k.long(), v.long(), pack)
+    for scale in (0.0, -1.0, math.inf, math.nan):
+        with pytest.raises(ValueError, match="scale"):
+            ops.attention_packed(q, k, v, pack, scale=scale)
+    with pytest.raises(ValueError, match="expected"):
+        ops.attention_packed_qkv(torch.zeros(6, 13), pack, 2, 1)
+    with pytest.raises(ValueError, match="cannot share"):
+        ops.attention_packed_qkv(torch.zeros(6, 14), pack, 3, 2)
