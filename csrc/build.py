@@ -120,7 +120,7 @@ EXTRA_FLAGS = {
 # (under finite-math-only even a bit test of the exponent field is folded away: the compiler may assume that no float
 # argument is an Inf or a NaN).  bn.hip's element-wise passes stay on the fast model - they run at the memory roof
 # and lose 2 % to the NaN-aware forms of max().
-PRECISE_MATH = {"loss.hip", "optim.hip", "bn_finalize.hip", "attention_packed.hip"}
+PRECISE_MATH = {"loss.hip", "optim.hip", "bn_finalize.hip", "attention_packed.hip", "vocab_loss.hip"}
 
 
 # No packed fp32 arithmetic (v_pk_add_f32, v_pk_mul_f32, v_pk_fma_f32): the compiler forms it from ordinary float code by

@@ -127,6 +127,94 @@ def lm_head_loss(x, weight, labels):
     return softmax_cross_entropy(logits.reshape(-1, logits.shape[-1]), labels.reshape(-1))
 
 
+MAX_TEACHER_TOP = 1024  # teacher logits of a row that the distillation losses take
+
+
+def _check_head(x, weight, what: str) -> None:
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1]:
+        raise ValueError(f"{what}: expected [..., width] and [vocabulary, width], got {tuple(x.shape)} and {tuple(weight.shape)}")
+    if not x.is_floating_point() or not weight.is_floating_point():
+        raise TypeError(f"{what} takes floating-point tensors")
+    if x.device != weight.device:
+        raise ValueError(f"{what}: x on {x.device}, weight on {weight.device}")
+    if x.is_cuda and weight.shape[1] % 64:
+        raise ValueError("in_features must be a multiple of 64")
+    if weight.numel() == 0 or weight.shape[0] >= 1 << 24:
+        raise ValueError(f"{what}: a vocabulary of 1 to 2^24 - 1 entries, got {weight.shape[0]}")
+
+
+def _check_targets(lead, ids, device, what: str, name: str) -> None:
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what}: {name} must be int64 or int32")
+    if tuple(ids.shape) != tuple(lead):
+        raise ValueError(f"{what}: {name} of shape {tuple(lead)} expected, got {tuple(ids.shape)}")
+    if ids.device != device:
+        raise ValueError(f"{what}: {name} on {ids.device}, expected on {device}")
+
+
+def _check_teacher(lead, teacher_logits, teacher_ids, temperature: float, device, what: str) -> float:
+    if teacher_ids.dim() != len(lead) + 1:
+        raise ValueError(f"{what}: teacher ids of shape {tuple(lead) + ('K',)} expected, got {tuple(teacher_ids.shape)}")
+    top = teacher_ids.shape[-1]
+    if not 1 <= top <= MAX_TEACHER_TOP:
+        raise ValueError(f"{what}: 1 to {MAX_TEACHER_TOP} teacher logits per row, got {top}")
+    _check_targets(tuple(lead) + (top,), teacher_ids, device, what, "teacher ids")
+    if teacher_logits.shape != teacher_ids.shape or teacher_logits.device != device or not teacher_logits.is_floating_point():
+        raise ValueError(f"{what}: teacher logits must be floating-point, of the ids' shape and device")
+    if teacher_logits.requires_grad:
+        raise ValueError(f"{what}: no gradient flows to the teacher; pass its logits detached")
+    temperature = float(temperature)
+    if not 0.0 < temperature < math.inf:
+        raise ValueError("the temperature must be positive and finite")
+    return temperature
+
+
+def linear_cross_entropy(x, weight, labels):
+    """Mean cross-entropy of the logits ``x W^T`` (``x`` ``[..., width]``, ``weight`` ``[vocabulary, width]``, no bias)
+    against ``labels`` ``[...]``, over the rows that have a label: a label outside ``[0, vocabulary)`` (-100, say) leaves
+    its row out, without gradient and not counted.  0 where no row has one.  On GPU the vocabulary, of any size, is worked
+    off in tiles and the logits are never stored; matrix products take bf16, loss and sums are fp32."""
+    _check_head(x, weight, "linear_cross_entropy")
+    _check_targets(x.shape[:-1], labels, x.device, "linear_cross_entropy", "labels")
+    if x.is_cuda and labels.numel():
+        from . import hip_vocab
+
+        return hip_vocab.head_loss(x, weight, labels.reshape(-1, 1).to(torch.int64).contiguous(), None, 1.0)
+    return _ref.linear_cross_entropy(x, weight, labels)
+
+
+def distillation_loss(logits, teacher_logits, teacher_ids, temperature: float = 1.0):
+    """``tau^2 KL(p || q)``, mean over rows, of a student's ``q = softmax(logits / tau)`` (``[..., vocabulary]``) from a
+    teacher's top logits: ``p = softmax(teacher_logits / tau)`` over its ``K`` entries ``[..., K]`` at ``teacher_ids``.
+    Entries with an id outside the vocabulary are absent; a row without any (or with -inf alone) is left out, without
+    gradient and not counted.  An id that occurs twice in a row counts with both its entries."""
+    if logits.dim() < 1 or not logits.is_floating_point() or not 1 <= logits.shape[-1] < 1 << 24:
+        raise ValueError("distillation_loss: logits are a floating-point tensor [..., vocabulary] of 1 to 2^24 - 1 entries")
+    tau = _check_teacher(logits.shape[:-1], teacher_logits, teacher_ids, temperature, logits.device, "distillation_loss")
+    if logits.is_cuda and logits.numel():
+        from . import hip_vocab
+
+        return hip_vocab.logits_distill(logits, *_teacher_rows(teacher_logits, teacher_ids), tau)
+    return _ref.distillation_loss(logits, teacher_logits, teacher_ids, tau)
+
+
+def linear_distillation_loss(x, weight, teacher_logits, teacher_ids, temperature: float = 1.0):
+    """:func:`distillation_loss` of the logits ``x W^T``, which on GPU are never stored (see :func:`linear_cross_entropy`)."""
+    _check_head(x, weight, "linear_distillation_loss")
+    tau = _check_teacher(x.shape[:-1], teacher_logits, teacher_ids, temperature, x.device, "linear_distillation_loss")
+    if x.is_cuda and teacher_ids.numel():
+        from . import hip_vocab
+
+        return hip_vocab.head_loss(x, weight, *_teacher_rows(teacher_logits, teacher_ids), tau)
+    return _ref.distillation_loss(linear(x, weight), teacher_logits, teacher_ids, tau)
+
+
+def _teacher_rows(teacher_logits, teacher_ids):
+    top = teacher_ids.shape[-1]
+    return (teacher_ids.reshape(-1, top).to(torch.int64).contiguous(),
+            teacher_logits.detach().reshape(-1, top).to(torch.float32).contiguous())
+
+
 def layer_norm(x, weight, bias, eps: float = 1e-5, link=None):
     if x.is_cuda:
         return _hip().layer_norm(x, weight, bias, eps, link)

@@ -77,6 +77,30 @@ def softmax_cross_entropy(logits: torch.Tensor, labels: torch.Tensor) -> torch.T
     return F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), labels.reshape(-1))
 
 
+def linear_cross_entropy(x, weight, labels):
+    """Mean cross-entropy of ``x W^T`` over the rows whose label lies in the vocabulary; 0 without any."""
+    up = torch.promote_types(x.dtype, torch.float32)
+    z = F.linear(x.reshape(-1, x.shape[-1]).to(up), weight.to(up))
+    y = labels.reshape(-1).to(torch.int64)
+    y = torch.where((y >= 0) & (y < weight.shape[0]), y, torch.full_like(y, -100))
+    return F.cross_entropy(z, y, ignore_index=-100, reduction="sum") / (y >= 0).sum().clamp(min=1)
+
+
+def distillation_loss(logits, teacher_logits, teacher_ids, temperature: float):
+    """``tau^2 sum_k p_k (log p_k - log q[id_k])``, mean over the rows with a present entry; 0 without any."""
+    up = torch.promote_types(logits.dtype, torch.float32)
+    vocab, top = logits.shape[-1], teacher_ids.shape[-1]
+    ids = teacher_ids.reshape(-1, top).to(torch.int64)
+    t = teacher_logits.reshape(-1, top).to(up)
+    t = t.masked_fill((ids < 0) | (ids >= vocab), float("-inf"))
+    some = (t != float("-inf")).any(1)
+    logp = torch.log_softmax((t - t.amax(1, keepdim=True)).masked_fill(~some[:, None], 0.0) / temperature, 1)
+    logq = torch.log_softmax(logits.reshape(-1, vocab).to(up) / temperature, 1).gather(1, ids.clamp(0, vocab - 1))
+    p = logp.exp()
+    each = torch.where((p != 0) & some[:, None], p * (torch.where(p != 0, logp, 0.0) - torch.where(p != 0, logq, 0.0)), 0.0)
+    return temperature ** 2 * each.sum() / some.sum().clamp(min=1)
+
+
 def layer_norm(x, weight, bias, eps: float = 1e-5, link=None):
     return F.layer_norm(x, (x.shape[-1],), weight, bias, eps)
 
