@@ -13,6 +13,7 @@
 // are joined, one pass turns the exponentials into q - p in place, and two more products give dx = (q - p) W and
 // dW = (q - p)^T x; the factor tau / rows is applied to their fp32 sums.
 #include "common.h"
+#include <type_traits>
 
 typedef __attribute__((address_space(3))) void vl_lds_void;
 typedef const __attribute__((address_space(1))) void vl_global_cvoid;
@@ -34,30 +35,87 @@ __device__ __forceinline__ float vl_exp2(float x) { return __builtin_amdgcn_exp2
 // of a row XOR-ed with (row & 3) | (row & 8) / 2, so that the rows {8g .. 8g + 3} two lane groups of a transposed read
 // touch at once fall on different banks.  The transposed reads take rows 8g .. 8g + 7 for lane group g, the k order of an
 // ordinary fragment, so the two kinds of operand go together.
+//
+// Schedule: a K-step is four phases of 16 MFMAs, each between two barriers, and the two wave rows run one barrier apart:
+// on every SIMD one wave's MFMAs cover the other's fragment reads and LDS-DMA requests.  Operands arrive in units of a
+// quarter stage, one per phase, six units ahead; a counted wait leaves four in flight.  Workgroups are persistent, so the
+// next tile's operands are on their way while a tile is written.
+//   A K-contiguous: a phase takes one half of the wave's rows (i) and one part of B - half the columns (B K-contiguous) or
+//     one 32-deep slice (B K-major); units {A lower, B part 0, B part 1, A upper}, phases (lower, 0) (lower, 1) (upper, 1) (upper, 0).
+//   A K-major: phases (slice, half of the rows); units {B slice 0, A slice 0, B slice 1, A slice 1}.
+// A unit is overwritten at least a phase behind its last reader's MFMAs in either order, for either wave row.
+//
+// Work: whole tiles first, a multiple of the workgroups; the tiles left over (all, where the tiles are few) are cut along k
+// into parts that fill the last round, summed in order by vocab_join_kernel.
 // ------------------------------------------------------------------------------------------------
 struct VocabGemm {
     const bf16 *a, *b;
     long long lda, ldb;
-    int M, N, K;
+    int M, N, K;             // K-contiguous operands hold K rounded up to 64 per row, a K-major A that many rows
     int tiles_m, tiles_n;
-    const bf16* zeros;     // 16 bytes of zeros
+    int whole, left, parts;  // units: `whole` tiles, then `left` tiles in `parts` parts each
+    int part_steps;
     // scores
-    float2* stats;         // [M][groups] {maximum (log2 units), sum}
-    bf16* e;               // [M][lde] exponentials, or nullptr
+    float2* stats;           // [M][groups] {maximum (log2 units), sum}
+    bf16* e;                 // [M][lde] exponentials, or nullptr
     long long lde;
     int groups;
-    float scale_log2;      // log2(e) / tau
+    float scale_log2;        // log2(e) / tau
     // dx, dW
-    const float* alpha;    // device factor of the result
-    bf16* out;             // bf16 result, or nullptr
-    float* out32;          // fp32 result; split products: [splits][M][N] partial sums
+    const float* alpha;      // device factor of the result
+    bf16* out;               // bf16 result, or nullptr
+    float* out32;            // fp32 result
     long long ldo;
-    int accumulate;        // add to out32
-    int k_per_split;       // multiple of 64
+    int accumulate;          // add to out32
+    float* part;             // [left][parts][32][512][4]: accumulators as the threads hold them
 };
+
+struct RowFrag {
+    u32x4 v;
+};
+struct TrFrag {
+    s16x4 lo, hi;
+};
+template <int OFF>
+__device__ __forceinline__ void vl_read(RowFrag& f, uint32_t at) { asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(f.v) : "v"(at), "n"(OFF) : "memory"); }
+template <int OFF>
+__device__ __forceinline__ void vl_read(TrFrag& f, uint32_t at) {
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(f.lo) : "v"(at), "n"(OFF) : "memory");
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(f.hi) : "v"(at), "n"(OFF + 4 * 256 * 2) : "memory");
+}
+// f(0), f(1), ... with compile-time indexes
+template <int N, typename F>
+__device__ __forceinline__ void vl_for(F f) {
+    if constexpr (N > 0) {
+        vl_for<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
+}
+// the values of reads issued above, taken over behind the wait for them: nothing that uses them can move in front of it
+__device__ __forceinline__ bf16x8 vl_take(RowFrag& f) {
+    asm volatile("" : "+v"(f.v));
+    return __builtin_bit_cast(bf16x8, f.v);
+}
+__device__ __forceinline__ bf16x8 vl_take(TrFrag& f) {
+    asm volatile("" : "+v"(f.lo), "+v"(f.hi));
+    const s16x8 v = {f.lo[0], f.lo[1], f.lo[2], f.lo[3], f.hi[0], f.hi[1], f.hi[2], f.hi[3]};
+    return __builtin_bit_cast(bf16x8, v);
+}
+template <int N>
+__device__ __forceinline__ void vl_wait_lds() {
+    asm volatile("s_waitcnt lgkmcnt(%0)" ::"n"(N) : "memory");
+    __builtin_amdgcn_sched_barrier(0);
+}
 
 template <bool KMAJOR>
 __device__ __forceinline__ int vl_swz(int row) { return KMAJOR ? (row & 3) | ((row >> 1) & 4) : row & 7; }
+
+// (tile row, tile column) in groups of eight rows of tiles: the 32 tiles an XCD works on at a time share 8 A and 4 B panels
+__device__ __forceinline__ void vl_tile(const VocabGemm& p, int u, int& m0, int& n0) {
+    const int per = 8 * p.tiles_n, grp = u / per, gm = min(8, p.tiles_m - grp * 8), in = u - grp * per;
+    m0 = (grp * 8 + in % gm) * 256;
+    n0 = (in / gm) * 256;
+}
 
 template <int KIND>
 __global__ __launch_bounds__(512) void vocab_gemm_kernel(const VocabGemm p) {
@@ -67,170 +125,412 @@ __global__ __launch_bounds__(512) void vocab_gemm_kernel(const VocabGemm p) {
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 2, wn = wave & 3;
     const int r16 = lane & 15, g4 = lane >> 4;
+    bf16* stage = vl_smem + 2 * STAGE + wave * (16 * 64);  // 16 rows of the wave's result at a time, as whole 128-byte rows
+    const int steps_all = (p.K + 63) / 64, units = p.whole + p.left * p.parts, G = gridDim.x;
+    const int first = xcd_remap(blockIdx.x, G);
+    float alpha = 1.f;
+    if constexpr (KIND != 0) alpha = p.alpha[0];
 
-    // tiles in groups of eight rows of tiles: the 32 tiles an XCD works on at a time share 8 A and 4 B panels
-    const int total = p.tiles_m * p.tiles_n;
-    const int lin = xcd_remap(blockIdx.x, gridDim.x), split = lin / total, u = lin - split * total;
-    const int per = 8 * p.tiles_n, grp = u / per, gm = min(8, p.tiles_m - grp * 8), in = u - grp * per;
-    const int m0 = (grp * 8 + in % gm) * 256, n0 = (in / gm) * 256;
-    const int k_lo = split * p.k_per_split, k_hi = min(p.K, k_lo + p.k_per_split);
-    const int nsteps = (k_hi - k_lo + 63) / 64;
+    struct Unit {
+        int m0, n0, k0, steps, part;  // part: -1 for a whole tile, else its place in p.part
+    };
+    auto unit_of = [&](int u) {
+        Unit r;
+        if (u < p.whole) {
+            vl_tile(p, u, r.m0, r.n0);
+            r.k0 = 0;
+            r.steps = steps_all;
+            r.part = -1;
+        } else {
+            const int v = u - p.whole, s = v / p.left, t = v - s * p.left;  // parts of one k range side by side: they share operand rows
+            vl_tile(p, p.whole + t, r.m0, r.n0);
+            r.k0 = s * p.part_steps * 64;
+            r.steps = min(p.part_steps, steps_all - s * p.part_steps);
+            r.part = t * p.parts + s;
+        }
+        return r;
+    };
 
-    // this lane's source of DMA piece i (four pieces of 1 KB per wave, operand and K-step) at k = 0
-    const bf16 *a_src[4], *b_src[4];
-    int a_k[4], b_k[4];  // K-major: the piece's row (its k inside the step)
-    auto setup = [&](const bf16* base, long long ld, int first, int count, bool km, const bf16*(&src)[4], int(&k)[4]) {
+    // ---- loader: wave-uniform base per operand, advanced by a K-step, and this lane's byte offset per DMA piece.  Pieces 2i'
+    // and 2i' + 1 of a wave belong to staging unit i' of their operand.
+    const char *a_base, *b_base;
+    uint32_t a_off[4], b_off[4];
+    int ld_u = first, ld_s = 0, ld_steps = 0, ld_slot = 0, ld_k = 0;
+    auto a_row = [&](int i) {
+        const int q = 2 * wave + (i & 1);
+        return A_KM ? (i >> 1) * 32 + q * 2 : (q >> 3) * 128 + (i >> 1) * 64 + (q & 7) * 8;
+    };
+    auto b_row = [&](int i) {
+        const int q = 2 * wave + (i & 1);
+        return B_KM ? (i >> 1) * 32 + q * 2 : (q >> 2) * 64 + (i >> 1) * 32 + (q & 3) * 8;
+    };
+    auto lane_off = [&](int row0, long long ld, int origin, int count, bool km) -> uint32_t {
+        if (km) {
+            const int row = row0 + (lane >> 5), pc = lane & 31;
+            const int col = (((pc >> 1) ^ vl_swz<true>(row)) << 4) | ((pc & 1) << 3);
+            const int c = min(origin + col, (count - 1) & ~7) - origin;  // (rows hold whole chunks of eight)
+            return (static_cast<uint32_t>(row) * static_cast<uint32_t>(ld) + c) * 2u;
+        }
+        const int row = row0 + (lane >> 3), slot = lane & 7;
+        return (static_cast<uint32_t>(min(origin + row, count - 1) - origin) * static_cast<uint32_t>(ld) + ((slot ^ vl_swz<false>(row)) << 3)) * 2u;
+    };
+    auto load_unit = [&](int u) {
+        const Unit r = unit_of(u < units ? u : first);  // (past its last unit the loader repeats the first: nothing reads it)
+        a_base = reinterpret_cast<const char*>(p.a + (A_KM ? r.k0 * p.lda + r.m0 : r.m0 * p.lda + r.k0));
+        b_base = reinterpret_cast<const char*>(p.b + (B_KM ? r.k0 * p.ldb + r.n0 : r.n0 * p.ldb + r.k0));
+        ld_steps = r.steps;
+        ld_k = r.k0;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            if (km) {
-                const int row = (wave * 4 + i) * 2 + (lane >> 5), pc = lane & 31;
-                const int col = (((pc >> 1) ^ vl_swz<true>(row)) << 4) | ((pc & 1) << 3);
-                const int last = (count - 1) & ~7;  // (rows have multiples of 8 elements: the last chunk is whole)
-                src[i] = base + min(first + col, last);
-                k[i] = row;
-            } else {
-                const int row = (wave * 4 + i) * 8 + (lane >> 3), slot = lane & 7;
-                src[i] = base + static_cast<long long>(min(first + row, count - 1)) * ld + ((slot ^ vl_swz<false>(row)) << 3);
-                k[i] = 0;
+            a_off[i] = lane_off(a_row(i), p.lda, r.m0, p.M, A_KM);
+            b_off[i] = lane_off(b_row(i), p.ldb, r.n0, p.N, B_KM);
+        }
+    };
+    auto load_a = [&](int half) {
+        bf16* tile = vl_smem + ld_slot * STAGE;
+#pragma unroll
+        for (int i = 2 * half; i < 2 * half + 2; ++i)
+            __builtin_amdgcn_global_load_lds((vl_global_cvoid*)(a_base + a_off[i]), (vl_lds_void*)(tile + a_row(i) * (A_KM ? 256 : 64)), 16, 0, 0);
+    };
+    auto load_b = [&](int half) {
+        bf16* tile = vl_smem + ld_slot * STAGE + 256 * 64;
+#pragma unroll
+        for (int i = 2 * half; i < 2 * half + 2; ++i) {
+            uint32_t off = b_off[i];
+            if constexpr (KIND == 1) {
+                // rows of W beyond the vocabulary repeat its last one (their products are with zeros)
+                const int over = ld_k + b_row(i) + (lane >> 5) - (p.K - 1);
+                off -= static_cast<uint32_t>(max(over, 0)) * static_cast<uint32_t>(p.ldb) * 2u;
+            }
+            __builtin_amdgcn_global_load_lds((vl_global_cvoid*)(b_base + off), (vl_lds_void*)(tile + b_row(i) * (B_KM ? 256 : 64)), 16, 0, 0);
+        }
+    };
+    auto load = [&](int r) {  // staging unit r of the K-step under the cursor
+        if constexpr (A_KM) {
+            if (r & 1) load_a(r >> 1);
+            else load_b(r >> 1);
+        } else {
+            if (r == 0 || r == 3) load_a(r == 3);
+            else load_b(r - 1);
+        }
+        if (r == 3) {
+            ld_slot ^= 1;
+            a_base += A_KM ? 64 * 2 * p.lda : 64 * 2;
+            b_base += B_KM ? 64 * 2 * p.ldb : 64 * 2;
+            ld_k += 64;
+            if (++ld_s == ld_steps) {
+                ld_s = 0;
+                ld_u += G;
+                load_unit(ld_u);
             }
         }
     };
-    setup(p.a, p.lda, m0, p.M, A_KM, a_src, a_k);
-    setup(p.b, p.ldb, n0, p.N, B_KM, b_src, b_k);
-    auto issue = [&](int s) {
-        const int k0 = k_lo + s * 64;
-        bf16* sA = vl_smem + (s & 1) * STAGE;
-        bf16* sB = sA + 256 * 64;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bf16* src;
-            // k beyond the end: zeros from A, so that whatever B holds there does not count (B repeats its last row)
-            if (A_KM) src = k0 + a_k[i] < k_hi ? a_src[i] + static_cast<long long>(k0 + a_k[i]) * p.lda : p.zeros;
-            else src = a_src[i] + k0;
-            __builtin_amdgcn_global_load_lds((vl_global_cvoid*)src, (vl_lds_void*)(sA + (wave * 4 + i) * 512), 16, 0, 0);
-        }
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const bf16* src = B_KM ? b_src[i] + static_cast<long long>(min(k0 + b_k[i], p.K - 1)) * p.ldb : b_src[i] + k0;
-            __builtin_amdgcn_global_load_lds((vl_global_cvoid*)src, (vl_lds_void*)(sB + (wave * 4 + i) * 512), 16, 0, 0);
-        }
-    };
-    auto fragment = [&](const bf16* tile, int first, int kk, bool km) -> bf16x8 {
-        if (km) {
-            const int row = kk * 32 + 8 * g4 + ((lane >> 2) & 3);  // (rows row and row + 4 are swizzled alike)
-            const bf16* at = tile + row * 256 + (((first >> 4) ^ vl_swz<true>(row)) << 4) + 4 * (lane & 3);
-            const s16x4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)at);
-            const s16x4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) s16x4*)(at + 4 * 256));
-            const s16x8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
-            return __builtin_bit_cast(bf16x8, v);
-        }
-        const int row = first + r16;
-        return *reinterpret_cast<const bf16x8*>(tile + row * 64 + (((kk * 4 + g4) ^ vl_swz<false>(row)) << 3));
-    };
+
+    // ---- fragment addresses (LDS bytes): a lane constant per operand, the rest as immediate offsets; the stage is bit 16
+    // (the kernel has no other LDS, so its dynamic part starts at 0).
+    // K-contiguous: rows 16 i + (lane & 15) of the wave's part at i * 2048, the second 32-deep slice with bit 6 turned.
+    // K-major: columns 16 i .. + 15 with i << 5 XOR-ed in, slices 16384 apart.
+    const uint32_t lds0 = static_cast<uint32_t>(reinterpret_cast<uintptr_t>((vl_lds_void*)vl_smem));
+    const int tr_row = 8 * g4 + ((lane >> 2) & 3);  // (rows row and row + 4 are swizzled alike)
+    const uint32_t row_lane = r16 * 128 + ((g4 ^ (r16 & 7)) << 4), tr_lane = tr_row * 512 + (vl_swz<true>(tr_row) << 5) + 8 * (lane & 3);
+    uint32_t at_a = lds0 + (A_KM ? tr_lane ^ (wm << 8) : row_lane + wm * 16384), at_b = lds0 + (B_KM ? tr_lane ^ (wn << 7) : row_lane + wn * 8192);
+    constexpr int B_AT = 256 * 64 * 2;
 
     f32x4 acc[8][4];
+    const f32x4 zero4 = {0.f, 0.f, 0.f, 0.f};
+    auto enter = [&]() {  // the unit the next phase reads has landed; everybody's waits meet
+        asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+        __builtin_amdgcn_s_setprio(1);
+    };
+    auto leave = [&]() {
+        __builtin_amdgcn_s_setprio(0);
+        __builtin_amdgcn_sched_barrier(0);
+        asm volatile("s_barrier" ::: "memory");
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    using C0 = std::integral_constant<int, 0>;
+    using C1 = std::integral_constant<int, 1>;
+    auto step = [&](auto first_step) {
+        constexpr bool FIRST = decltype(first_step)::value;
+        if constexpr (KIND == 0) {
+            RowFrag fa[2][4], fb[2][2][2];  // [kk][i], [part][kk][j]
+            bf16x8 b[2][2][2];
+            auto take_b = [&](int part, int kk) {
+                b[part][kk][0] = vl_take(fb[part][kk][0]);
+                b[part][kk][1] = vl_take(fb[part][kk][1]);
+            };
+            auto read_a = [&](auto half) {
+                vl_for<8>([&](auto n) { vl_read<(half * 4 + n % 4) * 2048>(fa[n / 4][n % 4], at_a ^ (n / 4 * 64)); });
+            };
+            auto read_b = [&](auto part) {
+                vl_for<4>([&](auto n) { vl_read<B_AT + (part * 2 + n % 2) * 2048>(fb[part][n / 2][n % 2], at_b ^ (n / 2 * 64)); });
+            };
+            bf16x8 a_[2][4];
+            auto pair = [&](int half, int part, int kk, int i, bool fresh = false) {
+                if (fresh) a_[kk][i] = vl_take(fa[kk][i]);
+                const bf16x8 a = a_[kk][i];
 #pragma unroll
-    for (int i = 0; i < 8; ++i)
+                for (int j = 0; j < 2; ++j) {
+                    f32x4& c = acc[half * 4 + i][part * 2 + j];
+                    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[part][kk][j], a, (FIRST && kk == 0) ? zero4 : c, 0, 0, 0);
+                }
+            };
+            auto falling = [&](int half, int part) {  // A fragments just requested: each pair of MFMAs waits for its own
+                vl_wait_lds<7>();
+                if (part == 0) {
+                    take_b(0, 0);
+                    take_b(0, 1);
+                }
+                pair(half, part, 0, 0, true);
+                vl_wait_lds<6>(); pair(half, part, 0, 1, true);
+                vl_wait_lds<5>(); pair(half, part, 0, 2, true);
+                vl_wait_lds<4>(); pair(half, part, 0, 3, true);
+                vl_wait_lds<3>(); pair(half, part, 1, 0, true);
+                vl_wait_lds<2>(); pair(half, part, 1, 1, true);
+                vl_wait_lds<1>(); pair(half, part, 1, 2, true);
+                vl_wait_lds<0>(); pair(half, part, 1, 3, true);
+            };
+            load(2);
+            read_b(C0{});
+            read_a(C0{});
+            enter();
+            falling(0, 0);
+            leave();
+            load(3);
+            read_b(C1{});
+            enter();
+            vl_wait_lds<2>();
+            take_b(1, 0);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (nsteps > 0) issue(0);
-    for (int s = 0; s < nsteps; ++s) {
-        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (s + 1 < nsteps) issue(s + 1);
-        const bf16* sA = vl_smem + (s & 1) * STAGE;
-        const bf16* sB = sA + 256 * 64;
+            for (int i = 0; i < 4; ++i) pair(0, 1, 0, i);
+            vl_wait_lds<0>();
+            take_b(1, 1);
 #pragma unroll
-        for (int kk = 0; kk < 2; ++kk) {
-            bf16x8 fb[4];
+            for (int i = 0; i < 4; ++i) pair(0, 1, 1, i);
+            leave();
+            load(0);
+            read_a(C1{});
+            enter();
+            falling(1, 1);
+            leave();
+            load(1);
+            enter();
 #pragma unroll
-            for (int j = 0; j < 4; ++j) fb[j] = fragment(sB, wn * 64 + j * 16, kk, B_KM);
+            for (int kk = 0; kk < 2; ++kk)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) pair(1, 0, kk, i);
+            leave();
+        } else if constexpr (KIND == 1) {
+            RowFrag fa[2][4];  // [kk][i]
+            TrFrag fb[2][4];   // [slice][j]
+            auto read_a = [&](auto half, auto kk) {
+                vl_for<4>([&](auto i) { vl_read<(half * 4 + i) * 2048>(fa[kk][i], at_a ^ (kk * 64)); });
+            };
+            auto read_b = [&](auto kk) {
+                vl_for<4>([&](auto j) { vl_read<B_AT + kk * 16384>(fb[kk][j], at_b ^ (j << 5)); });
+            };
+            bf16x8 a[2][4], b[2][4];
+            auto one = [&](int half, int kk, int i, int j) {
+                // the first slice a half of the rows meets starts from zero: slice 0 for the lower, slice 1 for the upper rows
+                f32x4& c = acc[half * 4 + i][j];
+                c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[kk][j], a[kk][i], (FIRST && kk == half) ? zero4 : c, 0, 0, 0);
+            };
+            auto row = [&](int half, int kk, int i) {
+                a[kk][i] = vl_take(fa[kk][i]);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) one(half, kk, i, j);
+            };
+            load(2);
+            read_b(C0{});
+            read_a(C0{}, C0{});
+            read_a(C0{}, C1{});
+            enter();
+            vl_wait_lds<7>();
+#pragma unroll
+            for (int j = 0; j < 4; ++j) b[0][j] = vl_take(fb[0][j]);
+            row(0, 0, 0);
+            vl_wait_lds<6>(); row(0, 0, 1);
+            vl_wait_lds<5>(); row(0, 0, 2);
+            vl_wait_lds<4>(); row(0, 0, 3);
+            leave();
+            load(3);
+            read_b(C1{});
+            enter();
+            auto column = [&](int j) {
+                b[1][j] = vl_take(fb[1][j]);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) one(0, 1, i, j);
+            };
+            vl_wait_lds<6>();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) a[1][i] = vl_take(fa[1][i]);
+            column(0);
+            vl_wait_lds<4>(); column(1);
+            vl_wait_lds<2>(); column(2);
+            vl_wait_lds<0>(); column(3);
+            leave();
+            load(0);
+            read_a(C1{}, C1{});
+            read_a(C1{}, C0{});
+            enter();
+            vl_wait_lds<7>(); row(1, 1, 0);
+            vl_wait_lds<6>(); row(1, 1, 1);
+            vl_wait_lds<5>(); row(1, 1, 2);
+            vl_wait_lds<4>(); row(1, 1, 3);
+            leave();
+            load(1);
+            enter();
+            vl_wait_lds<0>();
+#pragma unroll
+            for (int i = 0; i < 4; ++i) row(1, 0, i);
+            leave();
+        } else {
+            TrFrag fa[2][4], fb[4];  // [alternating][i], [j] of the slice
+            bf16x8 b[4];
+            auto phase = [&](auto kk_, auto half_) {
+                constexpr int kk = decltype(kk_)::value, half = decltype(half_)::value;
+                load((kk * 2 + half + 2) & 3);
+                if constexpr (half == 0) vl_for<4>([&](auto j) { vl_read<B_AT + kk * 16384>(fb[j], at_b ^ (j << 5)); });
+                vl_for<4>([&](auto i) { vl_read<kk * 16384>(fa[half][i], at_a ^ ((half * 4 + i) << 5)); });
+                enter();
+                auto row = [&](int i) {
+                    const bf16x8 a = vl_take(fa[half][i]);
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        f32x4& c = acc[half * 4 + i][j];
+                        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(b[j], a, (FIRST && kk == 0) ? zero4 : c, 0, 0, 0);
+                    }
+                };
+                vl_wait_lds<6>();
+                if constexpr (half == 0) vl_for<4>([&](auto j) { b[j] = vl_take(fb[j]); });
+                row(0);
+                vl_wait_lds<4>(); row(1);
+                vl_wait_lds<2>(); row(2);
+                vl_wait_lds<0>(); row(3);
+                leave();
+            };
+            phase(C0{}, C0{});
+            phase(C0{}, C1{});
+            phase(C1{}, C0{});
+            phase(C1{}, C1{});
+        }
+        at_a ^= STAGE * 2;
+        at_b ^= STAGE * 2;
+    };
+
+    load_unit(first);
+    load(0); load(1); load(2); load(3); load(0); load(1);
+    asm volatile("s_waitcnt vmcnt(8)\n\ts_barrier" ::: "memory");
+    if (wm == 1) asm volatile("s_barrier" ::: "memory");  // wave row 1 runs one barrier behind row 0 from here on
+    for (int u = first; u < units; u += G) {
+        const Unit w = unit_of(u);
+        step(std::true_type{});
+        for (int s = 1; s < w.steps; ++s) step(std::false_type{});
+        // both wave rows write their part at the same time: row 0 gives up its lead, row 1 falls back behind it afterwards
+        if (wm == 0) asm volatile("s_barrier" ::: "memory");
+        // lane: row m = 16 i + (lane & 15), columns n = 16 j + 4 (lane >> 4) + 0 .. 3 of the wave's 128 x 64
+        const int mw = w.m0 + wm * 128, nw = w.n0 + wn * 64;
+        if (KIND != 0 && w.part >= 0) {
+            float* dst = p.part + (static_cast<size_t>(w.part) * 32 * 512 + tid) * 4;
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) *reinterpret_cast<f32x4*>(dst + (i * 4 + j) * 2048) = acc[i][j];
+        } else {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const bf16x8 fa = fragment(sA, wm * 128 + i * 16, kk, A_KM);
+                const int m = mw + i * 16 + r16;
+                if constexpr (KIND == 0) {
+                    float mx = -VL_INF;
 #pragma unroll
-                for (int j = 0; j < 4; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[j], fa, acc[i][j], 0, 0, 0);
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            acc[i][j][e] = nw + j * 16 + 4 * g4 + e < p.N ? acc[i][j][e] * p.scale_log2 : -VL_INF;
+                            mx = fmaxf(mx, acc[i][j][e]);
+                        }
+                    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
+                    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                    const float ref = mx == -VL_INF ? 0.f : mx;  // (a group beyond the vocabulary, or one that is masked out)
+                    float sum = 0.f;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            acc[i][j][e] = vl_exp2(acc[i][j][e] - ref);
+                            sum += acc[i][j][e];
+                        }
+                    sum += __shfl_xor(sum, 16, 64);
+                    sum += __shfl_xor(sum, 32, 64);
+                    if (g4 == 0 && m < p.M && nw < p.N) p.stats[static_cast<size_t>(m) * p.groups + (nw >> 6)] = float2{mx, sum};
+                    if (p.e == nullptr) continue;
+                }
+                if (KIND == 0 || p.out != nullptr) {
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        bf16x4 v;
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) v[e] = f32_to_bf16(KIND == 0 ? acc[i][j][e] : acc[i][j][e] * alpha);
+                        *reinterpret_cast<bf16x4*>(stage + r16 * 64 + (((2 * j + (g4 >> 1)) ^ (r16 & 7)) << 3) + 4 * (g4 & 1)) = v;
+                    }
+#pragma unroll
+                    for (int ps = 0; ps < 2; ++ps) {
+                        const int row = ps * 8 + (lane >> 3), ch = lane & 7;
+                        const bf16x8 v = *reinterpret_cast<const bf16x8*>(stage + row * 64 + ((ch ^ (row & 7)) << 3));
+                        const int mm = mw + i * 16 + row, nn = nw + ch * 8;
+                        if (KIND == 0) {
+                            if (mm < p.M && nn < p.lde) *reinterpret_cast<bf16x8*>(p.e + mm * p.lde + nn) = v;
+                        } else {
+                            if (mm < p.M && nn < p.N) *reinterpret_cast<bf16x8*>(p.out + mm * p.ldo + nn) = v;
+                        }
+                    }
+                } else if (m < p.M) {
+                    float* dst = p.out32 + m * p.ldo + nw + 4 * g4;
+#pragma unroll
+                    for (int j = 0; j < 4; ++j)
+                        if (nw + j * 16 + 4 * g4 < p.N) {
+                            f32x4 v;
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * alpha;
+                            f32x4* at = reinterpret_cast<f32x4*>(dst + j * 16);
+                            *at = p.accumulate ? *at + v : v;
+                        }
+                }
             }
         }
+        if (wm == 1) asm volatile("s_barrier" ::: "memory");
     }
-    asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    // lane: row m = 16 i + (lane & 15), columns n = 16 j + 4 (lane >> 4) + 0 .. 3 of the wave's 128 x 64
-    bf16* stage = vl_smem + wave * (16 * 64);  // 16 rows of the wave at a time, as whole 128-byte rows
-    const int mw = m0 + wm * 128, nw = n0 + wn * 64;
-    float alpha = 1.f;
-    if constexpr (KIND != 0) alpha = p.out32 != nullptr && gridDim.x > static_cast<unsigned>(total) ? 1.f : p.alpha[0];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const int m = mw + i * 16 + r16;
-        if constexpr (KIND == 0) {
-            float mx = -VL_INF;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    acc[i][j][e] = nw + j * 16 + 4 * g4 + e < p.N ? acc[i][j][e] * p.scale_log2 : -VL_INF;
-                    mx = fmaxf(mx, acc[i][j][e]);
-                }
-            mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            const float ref = mx == -VL_INF ? 0.f : mx;  // (a group beyond the vocabulary, or one that is masked out)
-            float sum = 0.f;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    acc[i][j][e] = vl_exp2(acc[i][j][e] - ref);
-                    sum += acc[i][j][e];
-                }
-            sum += __shfl_xor(sum, 16, 64);
-            sum += __shfl_xor(sum, 32, 64);
-            if (g4 == 0 && m < p.M && nw < p.N) p.stats[static_cast<size_t>(m) * p.groups + (nw >> 6)] = float2{mx, sum};
-            if (p.e == nullptr) continue;
-        }
-        if (KIND == 0 || p.out != nullptr) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                bf16x4 v;
-#pragma unroll
-                for (int e = 0; e < 4; ++e) v[e] = f32_to_bf16(KIND == 0 ? acc[i][j][e] : acc[i][j][e] * alpha);
-                *reinterpret_cast<bf16x4*>(stage + r16 * 64 + (((2 * j + (g4 >> 1)) ^ (r16 & 7)) << 3) + 4 * (g4 & 1)) = v;
-            }
-#pragma unroll
-            for (int ps = 0; ps < 2; ++ps) {
-                const int row = ps * 8 + (lane >> 3), ch = lane & 7;
-                const bf16x8 v = *reinterpret_cast<const bf16x8*>(stage + row * 64 + ((ch ^ (row & 7)) << 3));
-                const int mm = mw + i * 16 + row, nn = nw + ch * 8;
-                if (KIND == 0) {
-                    if (mm < p.M && nn < p.lde) *reinterpret_cast<bf16x8*>(p.e + mm * p.lde + nn) = v;
-                } else {
-                    if (mm < p.M && nn < p.N) *reinterpret_cast<bf16x8*>(p.out + mm * p.ldo + nn) = v;
-                }
-            }
-        } else if (m < p.M) {
-            float* dst = p.out32 + static_cast<size_t>(split) * p.M * p.ldo + m * p.ldo + nw + 4 * g4;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-                if (nw + j * 16 + 4 * g4 < p.N) {
-                    f32x4 v;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) v[e] = acc[i][j][e] * alpha;
-                    f32x4* at = reinterpret_cast<f32x4*>(dst + j * 16);
-                    *at = p.accumulate ? *at + v : v;
-                }
-        }
-    }
+    if (wm == 0) asm volatile("s_barrier" ::: "memory");  // pairs with the last barrier of wave row 1
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the loader's trailing units
 }
 
-// out = alpha * (sum of the split product's parts, in order)
-__global__ __launch_bounds__(256) void vocab_join_kernel(const float* __restrict__ part, int splits, long long n, const float* __restrict__ alpha,
-                                                        bf16* __restrict__ out) {
-    const float a = alpha[0];
-    for (long long i = (blockIdx.x * 256ll + threadIdx.x) * 4; i < n; i += gridDim.x * 1024ll) {
-        f32x4 s = {0.f, 0.f, 0.f, 0.f};
-        for (int k = 0; k < splits; ++k) s += *reinterpret_cast<const f32x4*>(part + k * n + i);
-        bf16x4 r;
+// The tiles that were cut along k: their parts summed in order, times alpha.  A workgroup takes 16 rows of both wave rows.
+__global__ __launch_bounds__(512) void vocab_join_kernel(const VocabGemm p) {
+    const int t = blockIdx.x >> 3, i = blockIdx.x & 7, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    int m0, n0;
+    vl_tile(p, p.whole + t, m0, n0);
+    const int m = m0 + (wave >> 2) * 128 + i * 16 + (lane & 15);
+    const float alpha = p.alpha[0];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) r[e] = f32_to_bf16(s[e] * a);
-        *reinterpret_cast<bf16x4*>(out + i) = r;
+    for (int j = 0; j < 4; ++j) {
+        const int n = n0 + (wave & 3) * 64 + j * 16 + 4 * (lane >> 4);
+        if (m >= p.M || n >= p.N) continue;
+        f32x4 s = {0.f, 0.f, 0.f, 0.f};
+        const float* src = p.part + ((static_cast<size_t>(t) * p.parts * 32 + i * 4 + j) * 512 + tid) * 4;
+        for (int k = 0; k < p.parts; ++k) s += *reinterpret_cast<const f32x4*>(src + static_cast<size_t>(k) * 32 * 2048);
+        if (p.out != nullptr) {
+            bf16x4 r;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) r[e] = f32_to_bf16(s[e] * alpha);
+            *reinterpret_cast<bf16x4*>(p.out + m * p.ldo + n) = r;
+        } else {
+            f32x4* at = reinterpret_cast<f32x4*>(p.out32 + m * p.ldo + n);
+            f32x4 v;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = s[e] * alpha;
+            *at = p.accumulate ? *at + v : v;
+        }
     }
 }
 
@@ -245,7 +545,7 @@ struct Targets {
     int* valid;              // [rows]
     const bf16 *x, *w;       // behind a projection: [rows][width], [vocab][width]; else nullptr
     bf16* x_used;            // copy of x with zeros in the rows without a target, or nullptr: what such a row holds (NaN, say)
-                             // must not meet its zero gradient in the product that gives dW
+                             // must not meet its zero gradient in the product that gives dW; rows rounded up to 64, zeros behind the last
     int rows, top, width;
     long long vocab;
     float inv_tau;
@@ -261,7 +561,11 @@ __device__ __forceinline__ float vl_dot8(const bf16* a, const bf16* b, float s) 
 // one wave per row
 __global__ __launch_bounds__(256) void vocab_targets_kernel(const Targets t) {
     const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (row >= t.rows) return;
+    if (row >= t.rows) {
+        if (t.x_used != nullptr)
+            for (int c = lane * 8; c < t.width; c += 512) *reinterpret_cast<bf16x8*>(t.x_used + static_cast<size_t>(row) * t.width + c) = bf16x8{};
+        return;
+    }
     const long long* ids = t.ids + static_cast<size_t>(row) * t.top;
     auto present = [&](int k) { return ids[k] >= 0 && ids[k] < t.vocab; };
     float base = 0.f;
@@ -368,7 +672,8 @@ __device__ __forceinline__ bool vl_merged(const TargetLds& s, int k, int top, fl
     return true;
 }
 
-// ---- behind a projection: one workgroup per row joins the groups; training: exponentials -> q - p in place
+// ---- behind a projection: one workgroup per row joins the groups; training: exponentials -> q - p in place (e holds rows
+// rounded up to 64)
 struct Rows {
     const float2* stats;
     bf16* e;
@@ -378,7 +683,7 @@ struct Rows {
     const float* base;
     const int* valid;
     float* row_loss;
-    int groups, top;
+    int groups, top, rows;
     long long vocab;
 };
 
@@ -386,6 +691,10 @@ __global__ __launch_bounds__(256) void vocab_rows_kernel(const Rows a) {
     __shared__ float red[16];
     __shared__ TargetLds tg;
     const int row = blockIdx.x, tid = threadIdx.x;
+    if (row >= a.rows) {  // rows up to a multiple of 64: zeros for the product over the rows
+        for (long long c = tid * 8; c < a.lde; c += 2048) *reinterpret_cast<bf16x8*>(a.e + row * a.lde + c) = bf16x8{};
+        return;
+    }
     const float2* st = a.stats + static_cast<size_t>(row) * a.groups;
     float m = -VL_INF;
     for (int g = tid; g < a.groups; g += 256) m = fmaxf(m, st[g].x);
@@ -498,35 +807,70 @@ static int vl_grant_lds(K kernel, int bytes, unsigned long long& granted) {
     return static_cast<int>(e);
 }
 
-template <int KIND>
-static int vl_launch(VocabGemm& g, int splits, hipStream_t s) {
-    static unsigned long long granted;
-    constexpr int lds = 2 * 2 * 256 * 64 * 2;
-    if (int e = vl_grant_lds(vocab_gemm_kernel<KIND>, lds, granted)) return e;
+static int vl_cus() {
+    static int known[64];
+    int dev = 0, n = 0;
+    if (hipGetDevice(&dev) != hipSuccess || dev < 0 || dev >= 64) return 256;
+    if (known[dev] > 0) return known[dev];
+    if (hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    return known[dev] = n;
+}
+
+// Tiles in whole rounds of the CUs first; the rest in parts of at least eight K-steps that fill the last round, if it would
+// be less than 3/4 full.
+static void vl_plan(VocabGemm& g, bool split) {
     g.tiles_m = pdt_cdiv(g.M, 256);
     g.tiles_n = pdt_cdiv(g.N, 256);
-    const long long blocks = static_cast<long long>(g.tiles_m) * g.tiles_n * splits;
-    if (blocks >= (1ll << 31)) return -1;
-    hipLaunchKernelGGL(vocab_gemm_kernel<KIND>, dim3(static_cast<unsigned>(blocks)), dim3(512), lds, s, g);
+    const int tiles = g.tiles_m * g.tiles_n, steps = pdt_cdiv(g.K, 64), cus = vl_cus();
+    g.whole = tiles;
+    g.left = 0;
+    g.parts = g.part_steps = 1;
+    const int rest = tiles % cus;
+    if (!split || rest == 0 || rest * 4 >= cus * 3) return;
+    int parts = cus / rest;
+    if (parts > steps / 8) parts = steps / 8;
+    if (parts < 2) return;
+    g.part_steps = pdt_cdiv(steps, parts);
+    g.parts = pdt_cdiv(steps, g.part_steps);
+    g.left = rest;
+    g.whole = tiles - rest;
+}
+
+template <int KIND>
+static int vl_launch(const VocabGemm& g, hipStream_t s) {
+    static unsigned long long granted;
+    constexpr int lds = (2 * 2 * 256 * 64 + 8 * 16 * 64) * 2;
+    if (int e = vl_grant_lds(vocab_gemm_kernel<KIND>, lds, granted)) return e;
+    const int units = g.whole + g.left * g.parts, cus = vl_cus();
+    hipLaunchKernelGGL(vocab_gemm_kernel<KIND>, dim3(units < cus ? units : cus), dim3(512), lds, s, g);
+    if (g.left > 0) hipLaunchKernelGGL(vocab_join_kernel, dim3(g.left * 8), dim3(512), 0, s, g);
     return pdt_launch_status();
+}
+
+static bool vl_sizes_ok(int rows, int vocab, int width) {
+    // byte offsets inside a tile's rows and a whole number of tiles fit 32 bits
+    return rows > 0 && vocab > 0 && vocab < (1 << 22) && width > 0 && width <= (1 << 16) && (width % 64) == 0 &&
+           static_cast<long long>(pdt_cdiv(rows, 256)) * pdt_cdiv(vocab, 256) < (1ll << 30) &&
+           static_cast<long long>(pdt_cdiv(rows, 256)) * pdt_cdiv(width, 256) < (1ll << 30);
 }
 
 // Scores of `rows` rows against the vocabulary: stats [rows][ceil(vocab / 64)] {max, sum}; e [rows][lde] or nullptr, lde the
 // vocabulary rounded up to 64.
 PDT_API int pdt_vocab_scores(const void* x, const void* w, void* stats, void* e, int rows, int vocab, int width, long long lde, float inv_tau,
                              void* stream) {
-    if (rows <= 0 || vocab <= 0 || width <= 0 || (width % 64) != 0 || (e != nullptr && lde != (vocab + 63ll) / 64 * 64) || !(inv_tau > 0.f)) return -1;
+    if (!vl_sizes_ok(rows, vocab, width) || (e != nullptr && lde != (vocab + 63ll) / 64 * 64) || !(inv_tau > 0.f)) return -1;
     VocabGemm g = {};
     g.a = static_cast<const bf16*>(x);
     g.b = static_cast<const bf16*>(w);
     g.lda = g.ldb = width;
-    g.M = rows; g.N = vocab; g.K = g.k_per_split = width;
+    g.M = rows; g.N = vocab; g.K = width;
     g.stats = static_cast<float2*>(stats);
     g.e = static_cast<bf16*>(e);
     g.lde = lde;
     g.groups = pdt_cdiv(vocab, 64);
     g.scale_log2 = VL_LOG2E * inv_tau;
-    return vl_launch<0>(g, 1, static_cast<hipStream_t>(stream));
+    vl_plan(g, false);
+    return vl_launch<0>(g, static_cast<hipStream_t>(stream));
 }
 
 PDT_API int pdt_vocab_targets(const long long* ids, const float* teacher, float* p, float* base, int* valid, float* scal, const void* x, const void* w,
@@ -535,7 +879,7 @@ PDT_API int pdt_vocab_targets(const long long* ids, const float* teacher, float*
     if (teacher == nullptr && top != 1) return -1;
     hipStream_t s = static_cast<hipStream_t>(stream);
     Targets t = {ids, teacher, p, base, valid, static_cast<const bf16*>(x), static_cast<const bf16*>(w), static_cast<bf16*>(x_used), rows, top, width, vocab, 1.f / tau};
-    hipLaunchKernelGGL(vocab_targets_kernel, dim3(pdt_cdiv(rows, 4)), dim3(256), 0, s, t);
+    hipLaunchKernelGGL(vocab_targets_kernel, dim3(x_used == nullptr ? pdt_cdiv(rows, 4) : pdt_cdiv(rows, 64) * 16), dim3(256), 0, s, t);
     hipLaunchKernelGGL(vocab_count_kernel, dim3(1), dim3(1024), 0, s, valid, rows, tau, scal);
     return pdt_launch_status();
 }
@@ -543,8 +887,8 @@ PDT_API int pdt_vocab_targets(const long long* ids, const float* teacher, float*
 PDT_API int pdt_vocab_rows(const void* stats, void* e, const long long* ids, const float* p, const float* base, const int* valid, float* row_loss,
                            int rows, int vocab, int top, long long lde, void* stream) {
     if (rows <= 0 || vocab <= 0 || top <= 0 || top > VL_MAX_TOP) return -1;
-    Rows a = {static_cast<const float2*>(stats), static_cast<bf16*>(e), lde, ids, p, base, valid, row_loss, pdt_cdiv(vocab, 64), top, vocab};
-    hipLaunchKernelGGL(vocab_rows_kernel, dim3(rows), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    Rows a = {static_cast<const float2*>(stats), static_cast<bf16*>(e), lde, ids, p, base, valid, row_loss, pdt_cdiv(vocab, 64), top, rows, vocab};
+    hipLaunchKernelGGL(vocab_rows_kernel, dim3(e == nullptr ? rows : pdt_cdiv(rows, 64) * 64), dim3(256), 0, static_cast<hipStream_t>(stream), a);
     return pdt_launch_status();
 }
 
@@ -554,58 +898,54 @@ PDT_API int pdt_vocab_mean(const float* row_loss, const float* scal, float* loss
     return pdt_launch_status();
 }
 
-// Into how many parts the vocabulary is split for dx (1: no partial sums), so that few row tiles still fill the CUs.
-PDT_API int pdt_vocab_dx_splits(int rows, int vocab, int width) {
-    const int tiles = pdt_cdiv(rows, 256) * pdt_cdiv(width, 256), steps = pdt_cdiv(vocab, 64);
-    int s = 256 / tiles;
-    if (s > steps / 8) s = steps / 8;
-    return s < 1 ? 1 : s;
+// Floats of scratch that pdt_vocab_dx (which = 1) and pdt_vocab_dw (which = 2) need for tiles cut along k.
+PDT_API long long pdt_vocab_part_floats(int which, int rows, int vocab, int width) {
+    if (!vl_sizes_ok(rows, vocab, width)) return -1;
+    VocabGemm g = {};
+    g.M = which == 1 ? rows : vocab;
+    g.N = width;
+    g.K = which == 1 ? vocab : rows;
+    vl_plan(g, true);
+    return static_cast<long long>(g.left) * g.parts * 65536;
 }
 
-// dx [rows][width] bf16 = scal[0] * D w.  part: splits * rows * width floats, unused where splits is 1.
-PDT_API int pdt_vocab_dx(const void* d, const void* w, void* dx, float* part, int splits, const float* scal, int rows, int vocab, int width,
-                         long long ldd, void* stream) {
-    if (rows <= 0 || vocab <= 0 || width <= 0 || (width % 64) != 0 || ldd != (vocab + 63ll) / 64 * 64 || splits < 1 || (splits > 1 && part == nullptr))
-        return -1;
-    hipStream_t s = static_cast<hipStream_t>(stream);
+// dx [rows][width] bf16 = scal[0] * D w.
+PDT_API int pdt_vocab_dx(const void* d, const void* w, void* dx, float* part, const float* scal, int rows, int vocab, int width, long long ldd,
+                         void* stream) {
+    if (!vl_sizes_ok(rows, vocab, width) || ldd != (vocab + 63ll) / 64 * 64) return -1;
     VocabGemm g = {};
     g.a = static_cast<const bf16*>(d);
     g.b = static_cast<const bf16*>(w);
     g.lda = ldd; g.ldb = width;
     g.M = rows; g.N = width; g.K = vocab;
-    g.k_per_split = pdt_cdiv(pdt_cdiv(vocab, 64), splits) * 64;
     g.alpha = scal;
     g.ldo = width;
-    if (splits > 1) g.out32 = part;
-    else g.out = static_cast<bf16*>(dx);
-    if (int e = vl_launch<1>(g, splits, s)) return e;
-    if (splits > 1) {
-        const long long n = static_cast<long long>(rows) * width, blocks = (n / 4 + 255) / 256;
-        hipLaunchKernelGGL(vocab_join_kernel, dim3(static_cast<unsigned>(blocks < 4096 ? blocks : 4096)), dim3(256), 0, s, part, splits, n, scal,
-                           static_cast<bf16*>(dx));
-    }
-    return pdt_launch_status();
+    g.out = static_cast<bf16*>(dx);
+    g.part = part;
+    vl_plan(g, true);
+    if (g.left > 0 && part == nullptr) return -1;
+    return vl_launch<1>(g, static_cast<hipStream_t>(stream));
 }
 
-// dw [vocab][width] = scal[0] * D^T x, bf16 (dw) or fp32 (dw32, added to what it holds if accumulate)
-PDT_API int pdt_vocab_dw(const void* d, const void* x, void* dw, float* dw32, int accumulate, const float* scal, const void* zeros, int rows, int vocab,
+// dw [vocab][width] = scal[0] * D^T x, bf16 (dw) or fp32 (dw32, added to what it holds if accumulate).  D and x hold rows
+// rounded up to 64 rows, zeros behind the last.
+PDT_API int pdt_vocab_dw(const void* d, const void* x, void* dw, float* dw32, int accumulate, float* part, const float* scal, int rows, int vocab,
                          int width, long long ldd, void* stream) {
-    if (rows <= 0 || vocab <= 0 || width <= 0 || (width % 64) != 0 || ldd != (vocab + 63ll) / 64 * 64 || (dw == nullptr) == (dw32 == nullptr) ||
-        zeros == nullptr)
-        return -1;
+    if (!vl_sizes_ok(rows, vocab, width) || ldd != (vocab + 63ll) / 64 * 64 || (dw == nullptr) == (dw32 == nullptr)) return -1;
     VocabGemm g = {};
     g.a = static_cast<const bf16*>(d);
     g.b = static_cast<const bf16*>(x);
     g.lda = ldd; g.ldb = width;
     g.M = vocab; g.N = width; g.K = rows;
-    g.k_per_split = (rows + 63) / 64 * 64;
-    g.zeros = static_cast<const bf16*>(zeros);
     g.alpha = scal;
     g.out = static_cast<bf16*>(dw);
     g.out32 = dw32;
     g.accumulate = accumulate;
     g.ldo = width;
-    return vl_launch<2>(g, 1, static_cast<hipStream_t>(stream));
+    g.part = part;
+    vl_plan(g, true);
+    if (g.left > 0 && part == nullptr) return -1;
+    return vl_launch<2>(g, static_cast<hipStream_t>(stream));
 }
 
 // dtype: 0 fp32, 1 bf16 logits.  dz (may be nullptr) has the logits' type and row pitch ldd.

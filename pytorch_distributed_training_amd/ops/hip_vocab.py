@@ -10,15 +10,16 @@ import os
 
 import torch
 
-from .hip import SHADOWS, _axpy_dev, _check, _grad_sink, _ptr, _round_up, _scale_by_scalar, _stream, _zero_page
+from .hip import SHADOWS, _axpy_dev, _check, _grad_sink, _ptr, _round_up, _scale_by_scalar, _stream
 from .hip_transformer import _f, _i, _ll, _sig, _vp
 
 _scores = _sig("pdt_vocab_scores", [_vp] * 4 + [_i] * 3 + [_ll, _f, _vp])
 _targets = _sig("pdt_vocab_targets", [_vp] * 9 + [_i] * 4 + [_f, _vp])
 _rows = _sig("pdt_vocab_rows", [_vp] * 7 + [_i] * 3 + [_ll, _vp])
 _mean = _sig("pdt_vocab_mean", [_vp] * 3 + [_i, _vp])
-_dx_splits = _sig("pdt_vocab_dx_splits", [_i] * 3)
-_dx = _sig("pdt_vocab_dx", [_vp] * 4 + [_i, _vp] + [_i] * 3 + [_ll, _vp])
+_part_floats = _sig("pdt_vocab_part_floats", [_i] * 4)
+_part_floats.restype = _ll
+_dx = _sig("pdt_vocab_dx", [_vp] * 5 + [_i] * 3 + [_ll, _vp])
 _dw = _sig("pdt_vocab_dw", [_vp] * 4 + [_i, _vp, _vp] + [_i] * 3 + [_ll, _vp])
 _distill = _sig("pdt_logits_distill", [_vp] * 8 + [_i] * 3 + [_ll, _ll, _f, _i, _vp])
 
@@ -74,22 +75,23 @@ class _HeadLoss(torch.autograd.Function):
         with torch.cuda.device(x.device):
             x2, w = _matrix(x, width), _weight(weight)
             n, dev, top = x2.shape[0], x.device, ids.shape[1]
-            x_used = torch.empty_like(x2) if want_dw else None
+            x_used = torch.empty((_round_up(n, 64), width), dtype=torch.bfloat16, device=dev) if want_dw else None
             t = _Targets(ids, teacher, vocab, tau, x2, w, x_used)
             train = want_dx or want_dw
             pitch, groups = _round_up(vocab, 64), -(-vocab // 64)
             rows_c = n if not train else max(1, min(n, CHUNK_BYTES // (2 * pitch)))
-            if rows_c < n and rows_c > 256:
-                rows_c -= rows_c % 256
+            if rows_c < n:
+                rows_c = max(256, rows_c - rows_c % 256)
             stats = torch.empty((rows_c, groups, 2), dtype=torch.float32, device=dev)
-            e = torch.empty((rows_c, pitch), dtype=torch.bfloat16, device=dev) if train else None
+            e = torch.empty((_round_up(rows_c, 64), pitch), dtype=torch.bfloat16, device=dev) if train else None
             row_loss = torch.empty(n, dtype=torch.float32, device=dev)
             dx = torch.empty((n, width), dtype=torch.bfloat16, device=dev) if want_dx else None
             # one chunk and a bf16 weight: the gradient is rounded once, in the product's epilogue; else it is summed in fp32
             direct = want_dw and rows_c == n and weight.dtype == torch.bfloat16
             dw = torch.empty((vocab, width), dtype=torch.bfloat16 if direct else torch.float32, device=dev) if want_dw else None
-            splits = _dx_splits(rows_c, vocab, width)
-            part = torch.empty((splits, rows_c, width), dtype=torch.float32, device=dev) if want_dx and splits > 1 else None
+            chunks = {rows_c, n % rows_c or rows_c}
+            need = max(_part_floats(which, rows, vocab, width) for rows in chunks for which in (1, 2)) if train else 0
+            part = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
             for r0 in range(0, n, rows_c):
                 rows = min(rows_c, n - r0)
                 xc, idc = x2[r0:r0 + rows], ids[r0:r0 + rows]
@@ -98,11 +100,11 @@ class _HeadLoss(torch.autograd.Function):
                 _check(_rows(stats.data_ptr(), _ptr(e), idc.data_ptr(), None if t.p is None else t.p[r0:].data_ptr(), t.base[r0:].data_ptr(),
                              t.valid[r0:].data_ptr(), row_loss[r0:].data_ptr(), rows, vocab, top, pitch, _stream()), "vocab_rows")
                 if want_dx:
-                    _check(_dx(e.data_ptr(), w.data_ptr(), dx[r0:].data_ptr(), _ptr(part), splits, t.scal.data_ptr(), rows, vocab, width, pitch,
+                    _check(_dx(e.data_ptr(), w.data_ptr(), dx[r0:].data_ptr(), _ptr(part), t.scal.data_ptr(), rows, vocab, width, pitch,
                                _stream()), "vocab_dx")
                 if want_dw:
                     _check(_dw(e.data_ptr(), x_used[r0:].data_ptr(), dw.data_ptr() if direct else None, None if direct else dw.data_ptr(), int(r0 > 0),
-                               t.scal.data_ptr(), _zero_page(dev).data_ptr(), rows, vocab, width, pitch, _stream()), "vocab_dw")
+                               _ptr(part), t.scal.data_ptr(), rows, vocab, width, pitch, _stream()), "vocab_dw")
             loss = t.mean(row_loss)
         ctx.grads = [dx, dw]
         ctx.weight, ctx.shape = weight, x.shape
