@@ -36,6 +36,11 @@ struct PackedArgs {
 
 #define AP_INF __builtin_inff()
 
+// Tiles in LDS per streamed operand of the query-side kernels: three (two on their way while one is read) for heads of 64;
+// two for heads of 128, so that two workgroups fit a CU - with three, one wave per SIMD has nothing to cover its softmax.
+template <int NP>
+constexpr int ap_ring = NP == 1 ? AT_RING : 2;
+
 __device__ __forceinline__ bool ap_finite(float x) { return (__builtin_bit_cast(uint32_t, x) & 0x7f800000u) != 0x7f800000u; }
 
 // keys row i attends to / queries that attend to row i, as [lo, hi); empty for rows outside every sequence
@@ -211,20 +216,21 @@ __device__ __forceinline__ uint32_t bad_rows(const f32x16 (&a)[N], bool counts) 
     return static_cast<uint32_t>(b) | static_cast<uint32_t>(b >> 32);
 }
 
-// (block, head) of a workgroup: the units of consecutive workgroups of an XCD are the blocks of one head
+// (block, head) of a workgroup, heads fastest: consecutive workgroups go to the eight XCDs in turn, so an XCD keeps to a few
+// heads (one in eight where the heads are a multiple of eight) whose rows its L2 serves, and every XCD gets blocks of all
+// sizes.  Under a causal mask the blocks of a long sequence with the most tiles come first.
 __device__ __forceinline__ void ap_unit(const PackedArgs& p, int heads, int& blk, int& h) {
-    const int u = xcd_remap(blockIdx.x, p.nblk * heads);
-    h = u / p.nblk;
-    blk = u - h * p.nblk;
+    blk = blockIdx.x / heads;
+    h = blockIdx.x - blk * heads;
     if (p.causal) blk = p.nblk - 1 - blk;
 }
 
 template <int NP>
-__global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_fwd_kernel(const PackedArgs p) {
-    constexpr int TILE = NP * AT_TILE;
+__global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const PackedArgs p) {
+    constexpr int TILE = NP * AT_TILE, RING = ap_ring<NP>;
     extern __shared__ __attribute__((aligned(1024))) bf16 ap_smem[];
-    bf16* sK = ap_smem;                    // [AT_RING][TILE]
-    bf16* sV = ap_smem + AT_RING * TILE;   // [AT_RING][TILE]
+    bf16* sK = ap_smem;                    // [RING][TILE]
+    bf16* sV = ap_smem + RING * TILE;   // [RING][TILE]
     __shared__ int sB[8];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hi = lane >> 5, lq = lane & 31;
@@ -258,7 +264,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_fwd_kernel(const 
         ap_tile_issue<NP>(dma, vbase, p.v_row, k_lo + t * AT_T, k_hi - 1, sV + slot * TILE, wave);
     };
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < RING - 1; ++t)
         if (t < nt) issue(t, t);
 
     f32x16 o[2 * NP];
@@ -273,11 +279,11 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_fwd_kernel(const 
 
     int buf = 0;
     auto next_tile = [&](int t) {  // (the protocol of the fixed-length kernels)
-        if (t + 1 < nt) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * NP) : "memory");
+        if (RING > 2 && t + 1 < nt) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * NP) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t + 2 < nt) issue(t + 2, buf == 0 ? AT_RING - 1 : buf - 1);
+        if (t + RING - 1 < nt) issue(t + RING - 1, buf == 0 ? RING - 1 : buf - 1);
         const int cur = buf;
-        buf = buf == AT_RING - 1 ? 0 : buf + 1;
+        buf = buf == RING - 1 ? 0 : buf + 1;
         return cur;
     };
     for (int t = 0; t < min(t_lo, nt); ++t) next_tile(t);
@@ -288,18 +294,29 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_fwd_kernel(const 
         const bool masked = k0 < wb.max_lo || k0 + AT_T > wb.min_hi;
         const int rel_lo = span.x - k0 - 4 * hi;
         const uint32_t rel_n = static_cast<uint32_t>(span.y - span.x);  // offset o is valid: (unsigned)(o - rel_lo) < rel_n
-        auto scores = [&](f32x16& acc, const int kt) {
+        auto scores = [&](f32x16& acc, RowFrags(&kf)[NP]) {
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[e] = 0.f;
 #pragma unroll
-            for (int pn = 0; pn < NP; ++pn) {
-                RowFrags kf;
-                frag_rows_issue(kf, sk_tile + pn * (AT_TILE * 2), fa, kt);
-                lds_wait<0>();
-                taken(kf);
+            for (int pn = 0; pn < NP; ++pn)
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(kf, ks), qf[4 * pn + ks], acc, 0, 0, 0);
-            }
+                for (int ks = 0; ks < 4; ++ks) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(kf[pn], ks), qf[4 * pn + ks], acc, 0, 0, 0);
+        };
+        auto read_k = [&](RowFrags(&kf)[NP], const int kt) {
+#pragma unroll
+            for (int pn = 0; pn < NP; ++pn) frag_rows_issue(kf[pn], sk_tile + pn * (AT_TILE * 2), fa, kt);
+        };
+        auto take_k = [&](RowFrags(&kf)[NP]) {
+#pragma unroll
+            for (int pn = 0; pn < NP; ++pn) taken(kf[pn]);
+        };
+        auto read_v = [&](TrFrags(&vf)[2 * NP], const int kt) {
+#pragma unroll
+            for (int d = 0; d < 2 * NP; ++d) frag_tr_issue(vf[d], sv_tile + (d >> 1) * (AT_TILE * 2), fa, d & 1, kt);
+        };
+        auto take_v = [&](TrFrags(&vf)[2 * NP]) {
+#pragma unroll
+            for (int d = 0; d < 2 * NP; ++d) taken(vf[d]);
         };
         // scores -> probabilities about the running reference, in place; returns the lane's partial row sum.  Every lane's
         // first key lies in a half that starts at or before the wave's largest first key: those halves take the maximum;
@@ -333,28 +350,52 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_fwd_kernel(const 
             }
             return sum;
         };
-        f32x16 acc;
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            scores(acc, kt);
+        auto softmax_half = [&](f32x16& acc, const int kt) {
             const bool careful = k0 + 32 * kt <= wb.max_lo;
             float ls = probs(acc, 32 * kt, careful);
             if (!careful && __builtin_expect(__any(!(ls <= 1073741824.f)), 0)) {
-                scores(acc, kt);
+                RowFrags kf[NP];
+                read_k(kf, kt);
+                lds_wait<0>();
+                take_k(kf);
+                scores(acc, kf);
                 ls = probs(acc, 32 * kt, true);
             }
             lsum += ls;
+        };
+        auto values = [&](const f32x16& acc, const TrFrags(&vf)[2 * NP]) {
             const bf16x8 pb0 = pack_half(acc, 0), pb1 = pack_half(acc, 1);
 #pragma unroll
-            for (int d = 0; d < 2 * NP; ++d) {
-                TrFrags vf;
-                frag_tr_issue(vf, sv_tile + (d >> 1) * (AT_TILE * 2), fa, d & 1, kt);
-                lds_wait<0>();
-                taken(vf);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(vf, 0), pb0, o[d], 0, 0, 0);
-                o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(vf, 1), pb1, o[d], 0, 0, 0);
-            }
+            for (int d = 0; d < 2 * NP; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(vf[d], 0), pb0, o[d], 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < 2 * NP; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(vf[d], 1), pb1, o[d], 0, 0, 0);
+        };
+        // two halves of 32 keys, so that the matrix pipe has work while the vector ALU turns scores into probabilities:
+        //   S(0) S(1) | softmax(0) | PV(0) | softmax(1) | PV(1)
+        f32x16 acc0, acc1;
+        {
+            RowFrags kf[NP];
+            read_k(kf, 0);
+            lds_wait<0>();
+            take_k(kf);
+            scores(acc0, kf);
+            read_k(kf, 1);
+            lds_wait<0>();
+            take_k(kf);
+            scores(acc1, kf);
         }
+        TrFrags vf[2 * NP];
+        read_v(vf, 0);
+        softmax_half(acc0, 0);
+        lds_wait<0>();
+        take_v(vf);
+        values(acc0, vf);
+        read_v(vf, 1);
+        softmax_half(acc1, 1);
+        lds_wait<0>();
+        take_v(vf);
+        values(acc1, vf);
+        __builtin_amdgcn_sched_barrier(0);
     }
     for (int t = max(t_lo, t_hi); t < nt; ++t) next_tile(t);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
@@ -384,11 +425,11 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_fwd_kernel(const 
 }
 
 template <int NP>
-__global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dq_kernel(const PackedArgs p) {
-    constexpr int TILE = NP * AT_TILE;
+__global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const PackedArgs p) {
+    constexpr int TILE = NP * AT_TILE, RING = ap_ring<NP>;
     extern __shared__ __attribute__((aligned(1024))) bf16 ap_smem[];
     bf16* sK = ap_smem;
-    bf16* sV = ap_smem + AT_RING * TILE;
+    bf16* sV = ap_smem + RING * TILE;
     __shared__ int sB[8];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hi = lane >> 5, lq = lane & 31;
@@ -415,7 +456,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dq_kernel(const P
         ap_tile_issue<NP>(dma, vbase, p.v_row, k_lo + t * AT_T, k_hi - 1, sV + slot * TILE, wave);
     };
 #pragma unroll
-    for (int t = 0; t < 2; ++t)
+    for (int t = 0; t < RING - 1; ++t)
         if (t < nt) issue(t, t);
     bf16x8 qf[4 * NP], dof[4 * NP];
     float nl = 0.f, ndl = 0.f;  // minus log-sum-exp (log2 units), minus delta
@@ -446,11 +487,11 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dq_kernel(const P
 
     int buf = 0;
     auto next_tile = [&](int t) {
-        if (t + 1 < nt) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * NP) : "memory");
+        if (RING > 2 && t + 1 < nt) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * NP) : "memory");
         else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t + 2 < nt) issue(t + 2, buf == 0 ? AT_RING - 1 : buf - 1);
+        if (t + RING - 1 < nt) issue(t + RING - 1, buf == 0 ? RING - 1 : buf - 1);
         const int cur = buf;
-        buf = buf == AT_RING - 1 ? 0 : buf + 1;
+        buf = buf == RING - 1 ? 0 : buf + 1;
         return cur;
     };
     for (int t = 0; t < min(t_lo, nt); ++t) next_tile(t);
@@ -470,20 +511,25 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dq_kernel(const P
                 s[e] = 0.f;
                 dp[e] = ndl;
             }
+            {
+                RowFrags f[NP];
+                auto read = [&](uint32_t tile) {
 #pragma unroll
-            for (int pn = 0; pn < NP; ++pn) {
-                RowFrags kf, vf;
-                frag_rows_issue(kf, sk_tile + pn * (AT_TILE * 2), fa, kt);
-                frag_rows_issue(vf, sv_tile + pn * (AT_TILE * 2), fa, kt);
-                lds_wait<4>();
-                taken(kf);
+                    for (int pn = 0; pn < NP; ++pn) frag_rows_issue(f[pn], tile + pn * (AT_TILE * 2), fa, kt);
+                    lds_wait<0>();
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(kf, ks), qf[4 * pn + ks], s, 0, 0, 0);
-                lds_wait<0>();
-                taken(vf);
+                    for (int pn = 0; pn < NP; ++pn) taken(f[pn]);
+                };
+                read(sk_tile);
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(vf, ks), dof[4 * pn + ks], dp, 0, 0, 0);
+                for (int ks = 0; ks < 4 * NP; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), qf[ks], s, 0, 0, 0);
+                read(sv_tile);  // (under the products just issued)
+#pragma unroll
+                for (int ks = 0; ks < 4 * NP; ++ks) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), dof[ks], dp, 0, 0, 0);
             }
+            TrFrags kf[2 * NP];  // on their way during the vector work
+#pragma unroll
+            for (int d = 0; d < 2 * NP; ++d) frag_tr_issue(kf[d], sk_tile + (d >> 1) * (AT_TILE * 2), fa, d & 1, kt);
             if (masked) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
@@ -492,15 +538,14 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dq_kernel(const P
 #pragma unroll
             for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], p.scale_log2, nl)) * dp[r];
             const bf16x8 ds0 = pack_half(s, 0), ds1 = pack_half(s, 1);
+            lds_wait<0>();
 #pragma unroll
             for (int d = 0; d < 2 * NP; ++d) {
-                TrFrags kf;
-                frag_tr_issue(kf, sk_tile + (d >> 1) * (AT_TILE * 2), fa, d & 1, kt);
-                lds_wait<0>();
-                taken(kf);
-                dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(kf, 0), ds0, dq[d], 0, 0, 0);
-                dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(kf, 1), ds1, dq[d], 0, 0, 0);
+                taken(kf[d]);
+                dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(kf[d], 0), ds0, dq[d], 0, 0, 0);
+                dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(kf[d], 1), ds1, dq[d], 0, 0, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
         }
     }
     for (int t = max(t_lo, t_hi); t < nt; ++t) next_tile(t);
@@ -607,18 +652,18 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dkv_kernel(const 
             const bool masked = q0 < wb.max_lo || q0 + AT_T > wb.min_hi;
             const int rel_lo = span.x - q0 - 4 * hi;
             const uint32_t rel_n = static_cast<uint32_t>(span.y - span.x);
-#pragma unroll
-            for (int qt = 0; qt < 2; ++qt) {
-                if (q0 + 32 * qt >= wb.hi || q0 + 32 * qt + 32 <= wb.lo) continue;
-                f32x16 s, dp;
-                f32x4 l2[4], nd[4];
+            // S and dP of a half of 32 queries
+            auto products = [&](f32x16& s, f32x16& dp, const int qt) {
+                f32x4 nd[4];
+                RowFrags qf[NP], dof[NP];
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(nd[r4], row_tile + AT_T * 4 + (32 * qt + 8 * r4) * 4);
 #pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(l2[r4], row_tile + (32 * qt + 8 * r4) * 4);
-                lds_wait<0>();
+                for (int pn = 0; pn < NP; ++pn) frag_rows_issue(qf[pn], sq_tile + pn * (AT_TILE * 2), fa, qt);
+#pragma unroll
+                for (int pn = 0; pn < NP; ++pn) frag_rows_issue(dof[pn], sdo_tile + pn * (AT_TILE * 2), fa, qt);
+                lds_wait<4 * NP>();
                 taken(nd);
-                taken(l2);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) {
                     s[e] = 0.f;
@@ -626,18 +671,30 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dkv_kernel(const 
                 }
 #pragma unroll
                 for (int pn = 0; pn < NP; ++pn) {
-                    RowFrags qf, dof;
-                    frag_rows_issue(qf, sq_tile + pn * (AT_TILE * 2), fa, qt);
-                    frag_rows_issue(dof, sdo_tile + pn * (AT_TILE * 2), fa, qt);
-                    lds_wait<4>();
-                    taken(qf);
+                    taken(qf[pn]);
 #pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(qf, ks), kf[4 * pn + ks], s, 0, 0, 0);
-                    lds_wait<0>();
-                    taken(dof);
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(dof, ks), vf[4 * pn + ks], dp, 0, 0, 0);
+                    for (int ks = 0; ks < 4; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(qf[pn], ks), kf[4 * pn + ks], s, 0, 0, 0);
                 }
+                lds_wait<0>();
+#pragma unroll
+                for (int pn = 0; pn < NP; ++pn) {
+                    taken(dof[pn]);
+#pragma unroll
+                    for (int ks = 0; ks < 4; ++ks) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(dof[pn], ks), vf[4 * pn + ks], dp, 0, 0, 0);
+                }
+            };
+            auto finish = [&](f32x16& s, f32x16& dp, const int qt) {
+                f32x4 l2[4];
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(l2[r4], row_tile + (32 * qt + 8 * r4) * 4);
+                TrFrags dot[2], qtf[2];  // two column tiles of dO^T and Q^T at a time, on their way during the vector work
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    frag_tr_issue(dot[d], sdo_tile, fa, d, qt);
+                    frag_tr_issue(qtf[d], sq_tile, fa, d, qt);
+                }
+                lds_wait<15>();  // (the row terms are the oldest four of twenty reads; the counter ends at 15)
+                taken(l2);
                 if (masked) {
 #pragma unroll
                     for (int r = 0; r < 16; ++r)
@@ -655,20 +712,46 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dkv_kernel(const 
                     dsb[j] = pack_half(dp, j);
                 }
 #pragma unroll
-                for (int d = 0; d < 2 * NP; ++d) {
-                    TrFrags dot, qtf;
-                    frag_tr_issue(dot, sdo_tile + (d >> 1) * (AT_TILE * 2), fa, d & 1, qt);
-                    frag_tr_issue(qtf, sq_tile + (d >> 1) * (AT_TILE * 2), fa, d & 1, qt);
+                for (int pn = 0; pn < NP; ++pn) {
                     lds_wait<0>();
-                    taken(dot);
-                    taken(qtf);
+                    bf16x8 da[2][2], qa[2][2];
 #pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(dot, j), pb[j], dv[d], 0, 0, 0);
-                        dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(qtf, j), dsb[j], dk[d], 0, 0, 0);
+                    for (int d = 0; d < 2; ++d) {
+                        taken(dot[d]);
+                        taken(qtf[d]);
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            da[d][j] = frag_tr_get(dot[d], j);
+                            qa[d][j] = frag_tr_get(qtf[d], j);
+                        }
                     }
+                    if (pn + 1 < NP) {
+#pragma unroll
+                        for (int d = 0; d < 2; ++d) {
+                            frag_tr_issue(dot[d], sdo_tile + (pn + 1) * (AT_TILE * 2), fa, d, qt);
+                            frag_tr_issue(qtf[d], sq_tile + (pn + 1) * (AT_TILE * 2), fa, d, qt);
+                        }
+                    }
+#pragma unroll
+                    for (int d = 0; d < 2; ++d)
+#pragma unroll
+                        for (int j = 0; j < 2; ++j) {
+                            dv[2 * pn + d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(da[d][j], pb[j], dv[2 * pn + d], 0, 0, 0);
+                            dk[2 * pn + d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa[d][j], dsb[j], dk[2 * pn + d], 0, 0, 0);
+                        }
                 }
+            };
+            // (halves that no key of the wave meets are left out)
+            f32x16 s, dp;
+            if (q0 + 32 > wb.lo) {
+                products(s, dp, 0);
+                finish(s, dp, 0);
             }
+            if (q0 + 32 < wb.hi) {
+                products(s, dp, 1);
+                finish(s, dp, 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
         }
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     const bool some = span.y > span.x;
@@ -813,7 +896,7 @@ PDT_API int pdt_packed_attention_fwd(const void* q, const void* k, const void* v
     a.k_row = st[2]; a.k_head = st[3];
     a.v_row = st[4]; a.v_head = st[5];
     a.o_row = static_cast<long long>(H) * D;
-    const size_t lds = static_cast<size_t>(2 * AT_RING) * AT_T * D * sizeof(bf16);
+    const size_t lds = static_cast<size_t>(2 * (D == 64 ? ap_ring<1> : ap_ring<2>)) * AT_T * D * sizeof(bf16);
     const unsigned grid = static_cast<unsigned>(a.nblk) * H;
     static unsigned long long granted[2];
     return D == 64 ? ap_launch(packed_fwd_kernel<1>, granted[0], grid, lds, static_cast<hipStream_t>(stream), a)
@@ -857,11 +940,12 @@ PDT_API int pdt_packed_attention_bwd(const void* q, const void* k, const void* v
     a.dv_row = st[10]; a.dv_head = st[11];
     a.o_row = static_cast<long long>(H) * D;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    const size_t lds = static_cast<size_t>(2 * AT_RING) * AT_T * D * sizeof(bf16);
+    const size_t lds = static_cast<size_t>(2 * (D == 64 ? ap_ring<1> : ap_ring<2>)) * AT_T * D * sizeof(bf16);
+    const size_t lds_k = static_cast<size_t>(2 * AT_RING) * AT_T * D * sizeof(bf16);
     const unsigned gq = static_cast<unsigned>(a.nblk) * H, gk = static_cast<unsigned>(a.nblk) * Hk * splits;
     static unsigned long long granted[4];
     int rc = D == 64 ? ap_launch(packed_dq_kernel<1>, granted[0], gq, lds, s, a) : ap_launch(packed_dq_kernel<2>, granted[1], gq, lds, s, a);
-    if (rc == 0) rc = D == 64 ? ap_launch(packed_dkv_kernel<1>, granted[2], gk, lds, s, a) : ap_launch(packed_dkv_kernel<2>, granted[3], gk, lds, s, a);
+    if (rc == 0) rc = D == 64 ? ap_launch(packed_dkv_kernel<1>, granted[2], gk, lds_k, s, a) : ap_launch(packed_dkv_kernel<2>, granted[3], gk, lds_k, s, a);
     if (rc != 0) return rc;
     if (a.part != nullptr) {
         const long long n = 2ll * T * Hk * D / 4;

@@ -755,42 +755,91 @@ struct Logits {
     float scale_log2, inv_tau;
 };
 
+// 16 bytes of a row that may start at any element
 template <typename T>
-__global__ __launch_bounds__(512) void logits_distill_kernel(const Logits<T> a) {
+struct ChunkOf {
+    static constexpr int W = 16 / sizeof(T);
+    typedef T vec __attribute__((ext_vector_type(W)));
+    typedef T any __attribute__((ext_vector_type(W), aligned(sizeof(T))));
+};
+
+// The row stays in registers (NV chunks of 16 bytes per thread) between its maximum, its sum and the gradient: one read and
+// one write of the logits.  NV = 0: rows too long for that are read again from the caches.
+template <typename T, int THREADS, int NV>
+__global__ __launch_bounds__(THREADS) void logits_distill_kernel(const Logits<T> a) {
+    constexpr int W = 16 / sizeof(T);
     __shared__ float red[16];
     __shared__ TargetLds tg;
     const int row = blockIdx.x, tid = threadIdx.x;
     const T* z = a.z + row * a.ldz;
     const bool valid = a.valid[row] != 0;
     T* dz = a.dz == nullptr ? nullptr : a.dz + row * a.ldd;
+    const int chunks = (a.vocab + W - 1) / W;
     if (!valid) {
         if (tid == 0) a.row_loss[row] = 0.f;
         if (dz != nullptr)
-            for (int c = tid; c < a.vocab; c += 512) dz[c] = static_cast<T>(0.f);
+            for (int c = tid; c < a.vocab; c += THREADS) dz[c] = static_cast<T>(0.f);
         return;
     }
+    typedef typename ChunkOf<T>::vec vec;
+    auto load = [&](int c) -> vec {
+        if ((c + 1) * W <= a.vocab) return *reinterpret_cast<const typename ChunkOf<T>::any*>(z + c * W);
+        vec x;
+#pragma unroll
+        for (int e = 0; e < W; ++e) x[e] = c * W + e < a.vocab ? z[c * W + e] : static_cast<T>(-VL_INF);
+        return x;
+    };
+    vec held[NV > 0 ? NV : 1];
+    if constexpr (NV > 0) {
+#pragma unroll
+        for (int i = 0; i < NV; ++i)
+            if (tid + i * THREADS < chunks) held[i] = load(tid + i * THREADS);
+    }
+    auto each = [&](auto f) {  // f(chunk index, chunk) over this thread's chunks
+        if constexpr (NV > 0) {
+#pragma unroll
+            for (int i = 0; i < NV; ++i)
+                if (tid + i * THREADS < chunks) {
+                    u32x4 raw = __builtin_bit_cast(u32x4, held[i]);
+                    asm volatile("" : "+v"(raw));  // (converted anew in every pass: the converted row would not fit the registers)
+                    f(tid + i * THREADS, __builtin_bit_cast(vec, raw));
+                }
+        } else {
+            for (int c = tid; c < chunks; c += THREADS) f(c, load(c));
+        }
+    };
     vl_load_targets(tg, a.ids + static_cast<size_t>(row) * a.top, a.p + static_cast<size_t>(row) * a.top, a.top, a.vocab);
     float m = -VL_INF;
-    for (int c = tid; c < a.vocab; c += 512) m = fmaxf(m, static_cast<float>(z[c]));
+    each([&](int, vec x) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) m = fmaxf(m, static_cast<float>(x[e]));
+    });
     m = block_max(m, red);
     const float ref = m == -VL_INF ? 0.f : m;
-    float s = 0.f;
-    for (int c = tid; c < a.vocab; c += 512) s += vl_exp2((static_cast<float>(z[c]) - ref) * a.scale_log2);
-    s = block_sum(s, red);
-    float t = 0.f;
-    for (int k = tid; k < a.top; k += 512)
+    float s = 0.f, t = 0.f;
+    each([&](int, vec x) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) s += vl_exp2((static_cast<float>(x[e]) - ref) * a.scale_log2);
+    });
+    for (int k = tid; k < a.top; k += THREADS)
         if (tg.id[k] >= 0 && tg.p[k] != 0.f) t += tg.p[k] * (static_cast<float>(z[tg.id[k]]) - ref);
+    s = block_sum(s, red);
     t = block_sum(t, red);
     const float ls = log2f(s);
     if (tid == 0) a.row_loss[row] = a.base[row] - t * a.inv_tau + ls * VL_LN2;
     if (dz == nullptr) return;
     const float g = a.scal[0];
-    auto q_of = [&](int c) { return vl_exp2((static_cast<float>(z[c]) - ref) * a.scale_log2 - ls); };
-    for (int c = tid; c < a.vocab; c += 512) dz[c] = static_cast<T>(q_of(c) * g);
+    auto q_of = [&](float x) { return vl_exp2((x - ref) * a.scale_log2 - ls); };
+    each([&](int c, vec x) {  // (rows of dz are padded to whole chunks, on 16-byte boundaries)
+        vec r;
+#pragma unroll
+        for (int e = 0; e < W; ++e) r[e] = static_cast<T>(q_of(static_cast<float>(x[e])) * g);
+        *reinterpret_cast<vec*>(dz + c * W) = r;
+    });
     __syncthreads();
-    for (int k = tid; k < a.top; k += 512) {
+    for (int k = tid; k < a.top; k += THREADS) {
         float p;
-        if (vl_merged(tg, k, a.top, p)) dz[tg.id[k]] = static_cast<T>((q_of(tg.id[k]) - p) * g);
+        if (vl_merged(tg, k, a.top, p)) dz[tg.id[k]] = static_cast<T>((q_of(static_cast<float>(z[tg.id[k]])) - p) * g);
     }
 }
 
@@ -854,112 +903,176 @@ static bool vl_sizes_ok(int rows, int vocab, int width) {
            static_cast<long long>(pdt_cdiv(rows, 256)) * pdt_cdiv(width, 256) < (1ll << 30);
 }
 
-// Scores of `rows` rows against the vocabulary: stats [rows][ceil(vocab / 64)] {max, sum}; e [rows][lde] or nullptr, lde the
-// vocabulary rounded up to 64.
-PDT_API int pdt_vocab_scores(const void* x, const void* w, void* stats, void* e, int rows, int vocab, int width, long long lde, float inv_tau,
-                             void* stream) {
-    if (!vl_sizes_ok(rows, vocab, width) || (e != nullptr && lde != (vocab + 63ll) / 64 * 64) || !(inv_tau > 0.f)) return -1;
-    VocabGemm g = {};
-    g.a = static_cast<const bf16*>(x);
-    g.b = static_cast<const bf16*>(w);
-    g.lda = g.ldb = width;
-    g.M = rows; g.N = vocab; g.K = width;
-    g.stats = static_cast<float2*>(stats);
-    g.e = static_cast<bf16*>(e);
-    g.lde = lde;
-    g.groups = pdt_cdiv(vocab, 64);
-    g.scale_log2 = VL_LOG2E * inv_tau;
-    vl_plan(g, false);
-    return vl_launch<0>(g, static_cast<hipStream_t>(stream));
-}
-
-PDT_API int pdt_vocab_targets(const long long* ids, const float* teacher, float* p, float* base, int* valid, float* scal, const void* x, const void* w,
-                              void* x_used, int rows, int top, int width, int vocab, float tau, void* stream) {
-    if (rows <= 0 || top <= 0 || top > VL_MAX_TOP || vocab <= 0 || !(tau > 0.f) || (x != nullptr && (width <= 0 || (width % 8) != 0))) return -1;
-    if (teacher == nullptr && top != 1) return -1;
-    hipStream_t s = static_cast<hipStream_t>(stream);
+static int vl_targets(const long long* ids, const float* teacher, float* p, float* base, int* valid, float* scal, const void* x, const void* w,
+                      void* x_used, int rows, int top, int width, int vocab, float tau, hipStream_t s) {
     Targets t = {ids, teacher, p, base, valid, static_cast<const bf16*>(x), static_cast<const bf16*>(w), static_cast<bf16*>(x_used), rows, top, width, vocab, 1.f / tau};
     hipLaunchKernelGGL(vocab_targets_kernel, dim3(x_used == nullptr ? pdt_cdiv(rows, 4) : pdt_cdiv(rows, 64) * 16), dim3(256), 0, s, t);
     hipLaunchKernelGGL(vocab_count_kernel, dim3(1), dim3(1024), 0, s, valid, rows, tau, scal);
     return pdt_launch_status();
 }
 
-PDT_API int pdt_vocab_rows(const void* stats, void* e, const long long* ids, const float* p, const float* base, const int* valid, float* row_loss,
-                           int rows, int vocab, int top, long long lde, void* stream) {
-    if (rows <= 0 || vocab <= 0 || top <= 0 || top > VL_MAX_TOP) return -1;
-    Rows a = {static_cast<const float2*>(stats), static_cast<bf16*>(e), lde, ids, p, base, valid, row_loss, pdt_cdiv(vocab, 64), top, rows, vocab};
-    hipLaunchKernelGGL(vocab_rows_kernel, dim3(e == nullptr ? rows : pdt_cdiv(rows, 64) * 64), dim3(256), 0, static_cast<hipStream_t>(stream), a);
+static int vl_mean(const float* row_loss, const float* scal, float* loss, int rows, hipStream_t s) {
+    hipLaunchKernelGGL(vocab_mean_kernel, dim3(1), dim3(1024), 0, s, row_loss, rows, scal, loss);
     return pdt_launch_status();
 }
 
-PDT_API int pdt_vocab_mean(const float* row_loss, const float* scal, float* loss, int rows, void* stream) {
-    if (rows <= 0) return -1;
-    hipLaunchKernelGGL(vocab_mean_kernel, dim3(1), dim3(1024), 0, static_cast<hipStream_t>(stream), row_loss, rows, scal, loss);
-    return pdt_launch_status();
-}
-
-// Floats of scratch that pdt_vocab_dx (which = 1) and pdt_vocab_dw (which = 2) need for tiles cut along k.
-PDT_API long long pdt_vocab_part_floats(int which, int rows, int vocab, int width) {
-    if (!vl_sizes_ok(rows, vocab, width)) return -1;
-    VocabGemm g = {};
-    g.M = which == 1 ? rows : vocab;
-    g.N = width;
-    g.K = which == 1 ? vocab : rows;
-    vl_plan(g, true);
-    return static_cast<long long>(g.left) * g.parts * 65536;
-}
-
-// dx [rows][width] bf16 = scal[0] * D w.
-PDT_API int pdt_vocab_dx(const void* d, const void* w, void* dx, float* part, const float* scal, int rows, int vocab, int width, long long ldd,
-                         void* stream) {
-    if (!vl_sizes_ok(rows, vocab, width) || ldd != (vocab + 63ll) / 64 * 64) return -1;
-    VocabGemm g = {};
-    g.a = static_cast<const bf16*>(d);
-    g.b = static_cast<const bf16*>(w);
-    g.lda = ldd; g.ldb = width;
-    g.M = rows; g.N = width; g.K = vocab;
-    g.alpha = scal;
-    g.ldo = width;
-    g.out = static_cast<bf16*>(dx);
-    g.part = part;
-    vl_plan(g, true);
-    if (g.left > 0 && part == nullptr) return -1;
-    return vl_launch<1>(g, static_cast<hipStream_t>(stream));
-}
-
-// dw [vocab][width] = scal[0] * D^T x, bf16 (dw) or fp32 (dw32, added to what it holds if accumulate).  D and x hold rows
-// rounded up to 64 rows, zeros behind the last.
-PDT_API int pdt_vocab_dw(const void* d, const void* x, void* dw, float* dw32, int accumulate, float* part, const float* scal, int rows, int vocab,
-                         int width, long long ldd, void* stream) {
-    if (!vl_sizes_ok(rows, vocab, width) || ldd != (vocab + 63ll) / 64 * 64 || (dw == nullptr) == (dw32 == nullptr)) return -1;
-    VocabGemm g = {};
-    g.a = static_cast<const bf16*>(d);
-    g.b = static_cast<const bf16*>(x);
-    g.lda = ldd; g.ldb = width;
-    g.M = vocab; g.N = width; g.K = rows;
-    g.alpha = scal;
-    g.out = static_cast<bf16*>(dw);
-    g.out32 = dw32;
-    g.accumulate = accumulate;
-    g.ldo = width;
-    g.part = part;
-    vl_plan(g, true);
-    if (g.left > 0 && part == nullptr) return -1;
-    return vl_launch<2>(g, static_cast<hipStream_t>(stream));
-}
-
-// dtype: 0 fp32, 1 bf16 logits.  dz (may be nullptr) has the logits' type and row pitch ldd.
-PDT_API int pdt_logits_distill(const void* z, void* dz, const long long* ids, const float* p, const float* base, const int* valid, const float* scal,
-                               float* row_loss, int rows, int vocab, int top, long long ldz, long long ldd, float inv_tau, int dtype, void* stream) {
-    if (rows <= 0 || vocab <= 0 || top <= 0 || top > VL_MAX_TOP || ldz < 0 || (dz != nullptr && ldd < vocab) || !(inv_tau > 0.f)) return -1;
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    const float c = VL_LOG2E * inv_tau;
-    if (dtype == 1) {
-        Logits<bf16> a = {static_cast<const bf16*>(z), static_cast<bf16*>(dz), ldz, ldd, ids, p, base, valid, scal, row_loss, top, vocab, c, inv_tau};
-        hipLaunchKernelGGL(logits_distill_kernel<bf16>, dim3(rows), dim3(512), 0, s, a);
-    } else {
-        Logits<float> a = {static_cast<const float*>(z), static_cast<float*>(dz), ldz, ldd, ids, p, base, valid, scal, row_loss, top, vocab, c, inv_tau};
-        hipLaunchKernelGGL(logits_distill_kernel<float>, dim3(rows), dim3(512), 0, s, a);
+// Scratch of one call, carved from one allocation.
+struct Scratch {
+    char* at;
+    size_t used;
+    template <typename T>
+    T* take(size_t n) {
+        T* r = at == nullptr ? nullptr : reinterpret_cast<T*>(at + used);
+        used += (n * sizeof(T) + 255) & ~static_cast<size_t>(255);
+        return r;
     }
+};
+struct RowScratch {
+    float *p, *base, *scal, *row_loss;
+    int* valid;
+    RowScratch(Scratch& m, size_t rows, size_t top, bool teacher) {
+        p = teacher ? m.take<float>(rows * top) : nullptr;
+        base = m.take<float>(rows);
+        row_loss = m.take<float>(rows);
+        valid = m.take<int>(rows);
+        scal = m.take<float>(2);
+    }
+};
+struct HeadScratch {
+    RowScratch r;
+    float2* stats;
+    bf16 *e, *x_used;
+    float* part;
+    HeadScratch(Scratch& m, int rows, int top, int vocab, int width, int chunk, bool teacher, bool dx, bool dw) : r(m, rows, top, teacher) {
+        const size_t groups = pdt_cdiv(vocab, 64);
+        stats = m.take<float2>(chunk * groups);
+        e = dx || dw ? m.take<bf16>(static_cast<size_t>(pdt_cdiv(chunk, 64)) * 64 * groups * 64) : nullptr;
+        x_used = dw ? m.take<bf16>(static_cast<size_t>(pdt_cdiv(rows, 64)) * 64 * width) : nullptr;
+        size_t need = 0;
+        for (int k = 0; k < 2; ++k) {  // a whole chunk, and the last one
+            const int n = k == 0 ? chunk : rows % chunk;
+            if (n == 0) continue;
+            VocabGemm g = {};
+            g.N = width;
+            g.M = n; g.K = vocab;
+            if (dx) vl_plan(g, true);
+            if (dx && static_cast<size_t>(g.left) * g.parts > need) need = static_cast<size_t>(g.left) * g.parts;
+            g.M = vocab; g.K = n;
+            if (dw) vl_plan(g, true);
+            if (dw && static_cast<size_t>(g.left) * g.parts > need) need = static_cast<size_t>(g.left) * g.parts;
+        }
+        part = need > 0 ? m.take<float>(need * 65536) : nullptr;
+    }
+};
+
+static bool vl_head_ok(int rows, int top, int vocab, int width, int chunk) {
+    return vl_sizes_ok(rows, vocab, width) && top > 0 && top <= VL_MAX_TOP && chunk > 0 && chunk <= rows && (chunk == rows || (chunk % 256) == 0);
+}
+
+// Bytes of scratch that pdt_head_loss needs; rows are worked off `chunk` at a time (all, or a multiple of 256).
+PDT_API long long pdt_head_loss_scratch(int rows, int top, int vocab, int width, int chunk, int teacher, int dx, int dw) {
+    if (!vl_head_ok(rows, top, vocab, width, chunk)) return -1;
+    Scratch m = {nullptr, 0};
+    HeadScratch h(m, rows, top, vocab, width, chunk, teacher != 0, dx != 0, dw != 0);
+    return static_cast<long long>(m.used);
+}
+
+// Mean loss of x [rows][width] behind w [vocab][width] against ids [rows][top] with weights softmax(teacher / tau), or
+// against labels (teacher nullptr, top 1, tau 1); with dx [rows][width] bf16 and dw [vocab][width] in bf16 (dw, one chunk
+// only) or fp32 (dw32) where given.  All pointers 16-byte aligned.
+PDT_API int pdt_head_loss(const void* x, const void* w, const long long* ids, const float* teacher, float* loss, void* dx, void* dw, float* dw32,
+                          void* scratch, long long scratch_bytes, int rows, int top, int vocab, int width, int chunk, float tau, void* stream) {
+    if (!vl_head_ok(rows, top, vocab, width, chunk) || !(tau > 0.f) || (dw != nullptr && (dw32 != nullptr || chunk != rows))) return -1;
+    if (teacher == nullptr && (top != 1 || tau != 1.f)) return -1;
+    const bool want_dw = dw != nullptr || dw32 != nullptr, train = dx != nullptr || want_dw;
+    Scratch m = {static_cast<char*>(scratch), 0};
+    HeadScratch h(m, rows, top, vocab, width, chunk, teacher != nullptr, dx != nullptr, want_dw);
+    if (scratch == nullptr || static_cast<long long>(m.used) > scratch_bytes) return -1;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const long long pitch = (vocab + 63ll) / 64 * 64;
+    if (int e = vl_targets(ids, teacher, h.r.p, h.r.base, h.r.valid, h.r.scal, x, w, h.x_used, rows, top, width, vocab, tau, s)) return e;
+    for (int r0 = 0; r0 < rows; r0 += chunk) {
+        const int n = rows - r0 < chunk ? rows - r0 : chunk;
+        VocabGemm g = {};
+        g.a = static_cast<const bf16*>(x) + static_cast<size_t>(r0) * width;
+        g.b = static_cast<const bf16*>(w);
+        g.lda = g.ldb = width;
+        g.M = n; g.N = vocab; g.K = width;
+        g.stats = h.stats;
+        g.e = h.e;
+        g.lde = pitch;
+        g.groups = pdt_cdiv(vocab, 64);
+        g.scale_log2 = VL_LOG2E / tau;
+        vl_plan(g, false);
+        if (int e = vl_launch<0>(g, s)) return e;
+        Rows a = {h.stats, h.e, pitch, ids + static_cast<size_t>(r0) * top, h.r.p == nullptr ? nullptr : h.r.p + static_cast<size_t>(r0) * top,
+                  h.r.base + r0, h.r.valid + r0, h.r.row_loss + r0, g.groups, top, n, vocab};
+        hipLaunchKernelGGL(vocab_rows_kernel, dim3(train ? pdt_cdiv(n, 64) * 64 : n), dim3(256), 0, s, a);
+        g = {};
+        g.lda = pitch; g.ldb = width;
+        g.N = width;
+        g.a = h.e;
+        g.alpha = h.r.scal;
+        g.ldo = width;
+        g.part = h.part;
+        if (dx != nullptr) {
+            g.b = static_cast<const bf16*>(w);
+            g.M = n; g.K = vocab;
+            g.out = static_cast<bf16*>(dx) + static_cast<size_t>(r0) * width;
+            vl_plan(g, true);
+            if (int e = vl_launch<1>(g, s)) return e;
+        }
+        if (want_dw) {
+            g.b = h.x_used + static_cast<size_t>(r0) * width;
+            g.M = vocab; g.K = n;
+            g.out = static_cast<bf16*>(dw);
+            g.out32 = dw32;
+            g.accumulate = r0 > 0;
+            vl_plan(g, true);
+            if (int e = vl_launch<2>(g, s)) return e;
+        }
+    }
+    return vl_mean(h.r.row_loss, h.r.scal, loss, rows, s);
+}
+
+template <typename T>
+static int distill_launch(const Logits<T>& a, int rows, hipStream_t s) {
+    const int chunks = pdt_cdiv(a.vocab, 16 / static_cast<int>(sizeof(T)));
+#define PDT_LD(TH, NV) hipLaunchKernelGGL(HIP_KERNEL_NAME(logits_distill_kernel<T, TH, NV>), dim3(rows), dim3(TH), 0, s, a)
+    if (chunks <= 256) PDT_LD(256, 1);
+    else if (chunks <= 1024) PDT_LD(256, 4);
+    else if (chunks <= 4 * 512) PDT_LD(512, 4);
+    else if (chunks <= 8 * 512) PDT_LD(512, 8);
+    else if (chunks <= 13 * 512) PDT_LD(512, 13);
+    else if (chunks <= 16 * 512) PDT_LD(512, 16);
+    else if (chunks <= 13 * 1024) PDT_LD(1024, 13);
+    else if (chunks <= 16 * 1024) PDT_LD(1024, 16);
+    else PDT_LD(1024, 0);
+#undef PDT_LD
     return pdt_launch_status();
+}
+
+PDT_API long long pdt_distill_scratch(int rows, int top) {
+    if (rows <= 0 || top <= 0 || top > VL_MAX_TOP) return -1;
+    Scratch m = {nullptr, 0};
+    RowScratch r(m, rows, top, true);
+    return static_cast<long long>(m.used);
+}
+
+// dtype: 0 fp32, 1 bf16 logits.  dz (may be nullptr) has the logits' type, 16-byte aligned rows of pitch ldd and room for
+// whole 16-byte chunks.
+PDT_API int pdt_distill(const void* z, void* dz, const long long* ids, const float* teacher, float* loss, void* scratch, long long scratch_bytes, int rows,
+                        int vocab, int top, long long ldz, long long ldd, float tau, int dtype, void* stream) {
+    if (rows <= 0 || vocab <= 0 || vocab >= (1 << 24) || top <= 0 || top > VL_MAX_TOP || ldz < 0 || !(tau > 0.f) ||
+        (dz != nullptr && (ldd < (vocab + 7) / 8 * 8 || (ldd % 8) != 0)))
+        return -1;
+    Scratch m = {static_cast<char*>(scratch), 0};
+    RowScratch r(m, rows, top, true);
+    if (scratch == nullptr || static_cast<long long>(m.used) > scratch_bytes) return -1;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const float it = 1.f / tau, c = VL_LOG2E * it;
+    if (int e = vl_targets(ids, teacher, r.p, r.base, r.valid, r.scal, nullptr, nullptr, nullptr, rows, top, 0, vocab, tau, s)) return e;
+    const int e = dtype == 1 ? distill_launch(Logits<bf16>{static_cast<const bf16*>(z), static_cast<bf16*>(dz), ldz, ldd, ids, r.p, r.base, r.valid, r.scal, r.row_loss, top, vocab, c, it}, rows, s)
+                             : distill_launch(Logits<float>{static_cast<const float*>(z), static_cast<float*>(dz), ldz, ldd, ids, r.p, r.base, r.valid, r.scal, r.row_loss, top, vocab, c, it}, rows, s);
+    return e != 0 ? e : vl_mean(r.row_loss, r.scal, loss, rows, s);
 }

@@ -139,8 +139,8 @@ def _check_head(x, weight, what: str) -> None:
         raise ValueError(f"{what}: x on {x.device}, weight on {weight.device}")
     if x.is_cuda and weight.shape[1] % 64:
         raise ValueError("in_features must be a multiple of 64")
-    if weight.numel() == 0 or weight.shape[0] >= 1 << 24:
-        raise ValueError(f"{what}: a vocabulary of 1 to 2^24 - 1 entries, got {weight.shape[0]}")
+    if weight.numel() == 0 or weight.shape[0] >= 1 << 22:
+        raise ValueError(f"{what}: a vocabulary of 1 to 2^22 - 1 entries, got {weight.shape[0]}")
 
 
 def _check_targets(lead, ids, device, what: str, name: str) -> None:

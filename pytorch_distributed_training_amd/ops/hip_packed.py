@@ -10,7 +10,8 @@ import ctypes
 import torch
 
 from .hip import _check, _ptr, _stream
-from .hip_transformer import _f, _i, _ll, _sig, _vp
+from .hip_transformer import _f, _i, _sig, _vp
+from .hip_vocab import _on
 
 _pack_spans = _sig("pdt_pack_spans", [_vp, _i, _i, _vp, _vp, _vp])
 _fwd = _sig("pdt_packed_attention_fwd", [_vp] * 7 + [_i] * 4 + [_f, _i, _vp])
@@ -21,7 +22,7 @@ HEAD_DIMS = (64, 128)
 
 
 def pack_spans(offsets, rows: int):
-    with torch.cuda.device(offsets.device):
+    with _on(offsets.device):
         offsets = offsets.to(torch.int32).contiguous()
         spans = torch.empty((rows, 2), dtype=torch.int32, device=offsets.device)
         positions = torch.empty(rows, dtype=torch.int64, device=offsets.device)
@@ -74,7 +75,7 @@ def _backward(q, k, v, out, lse, g, spans, causal: bool, scale: float, dq, dk, d
 class _AttentionPacked(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, spans, causal: bool, scale: float):
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             q, k, v = _heads(q), _heads(k), _heads(v)
             out, lse = _forward(q, k, v, spans, causal, scale)
         ctx.save_for_backward(q, k, v, out, lse, spans)
@@ -85,7 +86,7 @@ class _AttentionPacked(torch.autograd.Function):
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
         q, k, v, out, lse, spans = ctx.saved_tensors
-        with torch.cuda.device(q.device):
+        with _on(q.device):
             dq, dk, dv = (torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) for x in (q, k, v))
             _backward(q, k, v, out, lse, g, spans, *ctx.meta, dq, dk, dv)
         return dq, dk, dv, None, None, None
@@ -103,7 +104,7 @@ class _AttentionPackedQKV(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, qkv, heads: int, kv_heads: int, spans, causal: bool, scale: float):
-        with torch.cuda.device(qkv.device):
+        with _on(qkv.device):
             if qkv.dtype != torch.bfloat16:
                 qkv = qkv.to(torch.bfloat16)
             if not qkv.is_contiguous() or qkv.data_ptr() % 16:
@@ -118,7 +119,7 @@ class _AttentionPackedQKV(torch.autograd.Function):
     def backward(ctx, g):
         qkv, out, lse, spans = ctx.saved_tensors
         heads, kv_heads, causal, scale = ctx.meta
-        with torch.cuda.device(qkv.device):
+        with _on(qkv.device):
             dqkv = torch.empty_like(qkv)
             _backward(*_split_qkv(qkv, heads, kv_heads), out, lse, g.reshape(out.shape), spans, causal, scale,
                       *_split_qkv(dqkv, heads, kv_heads))

@@ -6,6 +6,7 @@ Role parity: nn.CrossEntropyLoss at /root/reference/src/main.py:62,76,78 (on a c
 
 from __future__ import annotations
 
+import contextlib
 import os
 
 import torch
@@ -13,39 +14,20 @@ import torch
 from .hip import SHADOWS, _axpy_dev, _check, _grad_sink, _ptr, _round_up, _scale_by_scalar, _stream
 from .hip_transformer import _f, _i, _ll, _sig, _vp
 
-_scores = _sig("pdt_vocab_scores", [_vp] * 4 + [_i] * 3 + [_ll, _f, _vp])
-_targets = _sig("pdt_vocab_targets", [_vp] * 9 + [_i] * 4 + [_f, _vp])
-_rows = _sig("pdt_vocab_rows", [_vp] * 7 + [_i] * 3 + [_ll, _vp])
-_mean = _sig("pdt_vocab_mean", [_vp] * 3 + [_i, _vp])
-_part_floats = _sig("pdt_vocab_part_floats", [_i] * 4)
-_part_floats.restype = _ll
-_dx = _sig("pdt_vocab_dx", [_vp] * 5 + [_i] * 3 + [_ll, _vp])
-_dw = _sig("pdt_vocab_dw", [_vp] * 4 + [_i, _vp, _vp] + [_i] * 3 + [_ll, _vp])
-_distill = _sig("pdt_logits_distill", [_vp] * 8 + [_i] * 3 + [_ll, _ll, _f, _i, _vp])
+_head_scratch = _sig("pdt_head_loss_scratch", [_i] * 8)
+_head_scratch.restype = _ll
+_head = _sig("pdt_head_loss", [_vp] * 9 + [_ll] + [_i] * 5 + [_f, _vp])
+_distill_scratch = _sig("pdt_distill_scratch", [_i] * 2)
+_distill_scratch.restype = _ll
+_distill = _sig("pdt_distill", [_vp] * 6 + [_ll] + [_i] * 3 + [_ll, _ll, _f, _i, _vp])
 
-MAX_TOP = 1024  # targets of a row that fit the kernels' table
 # Rows worked off at a time: their exponentials (2 bytes per row and vocabulary entry) are the one large buffer.
 CHUNK_BYTES = int(os.environ.get("PDT_VOCAB_CHUNK_MB", "8192")) << 20
 
 
-class _Targets:
-    """Weights of the rows' targets, and the two factors (tau, tau^2 over the rows that have one)."""
-
-    def __init__(self, ids, teacher, vocab: int, tau: float, x=None, w=None, x_used=None):
-        n, top = ids.shape
-        dev = ids.device
-        self.ids, self.tau = ids, tau
-        self.p = torch.empty((n, top), dtype=torch.float32, device=dev) if teacher is not None else None
-        self.base = torch.empty(n, dtype=torch.float32, device=dev)
-        self.valid = torch.empty(n, dtype=torch.int32, device=dev)
-        self.scal = torch.empty(2, dtype=torch.float32, device=dev)
-        _check(_targets(ids.data_ptr(), _ptr(teacher), _ptr(self.p), self.base.data_ptr(), self.valid.data_ptr(), self.scal.data_ptr(), _ptr(x),
-                        _ptr(w), _ptr(x_used), n, top, 0 if x is None else x.shape[1], vocab, tau, _stream()), "vocab_targets")
-
-    def mean(self, row_loss):
-        loss = torch.empty((), dtype=torch.float32, device=row_loss.device)
-        _check(_mean(row_loss.data_ptr(), self.scal.data_ptr(), loss.data_ptr(), row_loss.numel(), _stream()), "vocab_mean")
-        return loss
+def _on(device):
+    """The device a kernel is launched on, made current where it is not."""
+    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _matrix(x: torch.Tensor, width: int) -> torch.Tensor:
@@ -72,40 +54,24 @@ class _HeadLoss(torch.autograd.Function):
     def forward(ctx, x, weight, ids, teacher, tau: float):
         vocab, width = weight.shape
         want_dx, want_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        with torch.cuda.device(x.device):
+        dev = x.device
+        with _on(dev):
             x2, w = _matrix(x, width), _weight(weight)
-            n, dev, top = x2.shape[0], x.device, ids.shape[1]
-            x_used = torch.empty((_round_up(n, 64), width), dtype=torch.bfloat16, device=dev) if want_dw else None
-            t = _Targets(ids, teacher, vocab, tau, x2, w, x_used)
-            train = want_dx or want_dw
-            pitch, groups = _round_up(vocab, 64), -(-vocab // 64)
-            rows_c = n if not train else max(1, min(n, CHUNK_BYTES // (2 * pitch)))
-            if rows_c < n:
-                rows_c = max(256, rows_c - rows_c % 256)
-            stats = torch.empty((rows_c, groups, 2), dtype=torch.float32, device=dev)
-            e = torch.empty((_round_up(rows_c, 64), pitch), dtype=torch.bfloat16, device=dev) if train else None
-            row_loss = torch.empty(n, dtype=torch.float32, device=dev)
-            dx = torch.empty((n, width), dtype=torch.bfloat16, device=dev) if want_dx else None
+            n, top = ids.shape
+            chunk = n if not (want_dx or want_dw) else min(n, CHUNK_BYTES // (2 * _round_up(vocab, 64)))
+            if chunk < n:
+                chunk = min(n, max(256, chunk - chunk % 256))
             # one chunk and a bf16 weight: the gradient is rounded once, in the product's epilogue; else it is summed in fp32
-            direct = want_dw and rows_c == n and weight.dtype == torch.bfloat16
+            direct = want_dw and chunk == n and weight.dtype == torch.bfloat16
+            dx = torch.empty((n, width), dtype=torch.bfloat16, device=dev) if want_dx else None
             dw = torch.empty((vocab, width), dtype=torch.bfloat16 if direct else torch.float32, device=dev) if want_dw else None
-            chunks = {rows_c, n % rows_c or rows_c}
-            need = max(_part_floats(which, rows, vocab, width) for rows in chunks for which in (1, 2)) if train else 0
-            part = torch.empty(need, dtype=torch.float32, device=dev) if need > 0 else None
-            for r0 in range(0, n, rows_c):
-                rows = min(rows_c, n - r0)
-                xc, idc = x2[r0:r0 + rows], ids[r0:r0 + rows]
-                _check(_scores(xc.data_ptr(), w.data_ptr(), stats.data_ptr(), _ptr(e), rows, vocab, width, pitch, 1.0 / tau, _stream()),
-                       "vocab_scores")
-                _check(_rows(stats.data_ptr(), _ptr(e), idc.data_ptr(), None if t.p is None else t.p[r0:].data_ptr(), t.base[r0:].data_ptr(),
-                             t.valid[r0:].data_ptr(), row_loss[r0:].data_ptr(), rows, vocab, top, pitch, _stream()), "vocab_rows")
-                if want_dx:
-                    _check(_dx(e.data_ptr(), w.data_ptr(), dx[r0:].data_ptr(), _ptr(part), t.scal.data_ptr(), rows, vocab, width, pitch,
-                               _stream()), "vocab_dx")
-                if want_dw:
-                    _check(_dw(e.data_ptr(), x_used[r0:].data_ptr(), dw.data_ptr() if direct else None, None if direct else dw.data_ptr(), int(r0 > 0),
-                               _ptr(part), t.scal.data_ptr(), rows, vocab, width, pitch, _stream()), "vocab_dw")
-            loss = t.mean(row_loss)
+            loss = torch.empty((), dtype=torch.float32, device=dev)
+            size = _head_scratch(n, top, vocab, width, chunk, int(teacher is not None), int(want_dx), int(want_dw))
+            if size < 0:
+                raise ValueError(f"the vocabulary kernels do not take {n} rows of {width} features against {vocab} entries")
+            scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+            _check(_head(x2.data_ptr(), w.data_ptr(), ids.data_ptr(), _ptr(teacher), loss.data_ptr(), _ptr(dx), _ptr(dw) if direct else None,
+                         None if direct else _ptr(dw), scratch.data_ptr(), size, n, top, vocab, width, chunk, tau, _stream()), "head_loss")
         ctx.grads = [dx, dw]
         ctx.weight, ctx.shape = weight, x.shape
         return loss
@@ -118,7 +84,7 @@ class _HeadLoss(torch.autograd.Function):
         if dx is None and dw is None:
             raise RuntimeError("the loss behind a projection handed its gradients out already (backward ran twice)")
         weight = ctx.weight
-        with torch.cuda.device(g.device):
+        with _on(g.device):
             g1 = g.reshape(1).to(torch.float32).contiguous()
             for d in (dx, dw):
                 if d is not None and d.dtype == torch.bfloat16:
@@ -143,22 +109,19 @@ class _LogitsDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, teacher, tau: float):
         vocab = logits.shape[-1]
-        with torch.cuda.device(logits.device):
+        with _on(logits.device):
             z = logits.reshape(-1, vocab)
             if z.dtype not in (torch.bfloat16, torch.float32):
                 z = z.to(torch.float32)
             if z.stride(1) != 1 and vocab > 1:
                 z = z.contiguous()
             n, top = ids.shape
-            t = _Targets(ids, teacher, vocab, tau)
-            row_loss = torch.empty(n, dtype=torch.float32, device=z.device)
-            dz = None
-            if ctx.needs_input_grad[0]:
-                dz = torch.empty((n, _round_up(vocab, 64)), dtype=z.dtype, device=z.device)
-            _check(_distill(z.data_ptr(), _ptr(dz), ids.data_ptr(), t.p.data_ptr(), t.base.data_ptr(), t.valid.data_ptr(), t.scal.data_ptr(),
-                            row_loss.data_ptr(), n, vocab, top, z.stride(0), 0 if dz is None else dz.stride(0), 1.0 / tau,
-                            int(z.dtype == torch.bfloat16), _stream()), "logits_distill")
-            loss = t.mean(row_loss)
+            dz = torch.empty((n, _round_up(vocab, 64)), dtype=z.dtype, device=z.device) if ctx.needs_input_grad[0] else None
+            loss = torch.empty((), dtype=torch.float32, device=z.device)
+            size = _distill_scratch(n, top)
+            scratch = torch.empty(size, dtype=torch.uint8, device=z.device)
+            _check(_distill(z.data_ptr(), _ptr(dz), ids.data_ptr(), teacher.data_ptr(), loss.data_ptr(), scratch.data_ptr(), size, n, vocab, top,
+                            z.stride(0), 0 if dz is None else dz.stride(0), tau, int(z.dtype == torch.bfloat16), _stream()), "distill")
         ctx.dz, ctx.shape = dz, logits.shape
         return loss
 
@@ -168,7 +131,7 @@ class _LogitsDistill(torch.autograd.Function):
         dz, ctx.dz = ctx.dz, None
         if dz is None:
             raise RuntimeError("the distillation loss handed its gradient out already (backward ran twice)")
-        with torch.cuda.device(g.device):
+        with _on(g.device):
             g1 = g.reshape(1).to(torch.float32).contiguous()
             if dz.dtype == torch.bfloat16:
                 _check(_scale_by_scalar(dz.data_ptr(), g1.data_ptr(), dz.numel(), _stream()), "scale_by_scalar")
