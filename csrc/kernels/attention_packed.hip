@@ -19,6 +19,7 @@
 // interval only (row_* functions: one row per wave, no matrix instructions), so what one sequence or a later position
 // holds never shows in another row.
 #include "attention_tile.h"
+#include <type_traits>
 
 struct PackedArgs {
     const bf16 *q, *k, *v, *o, *dout;
@@ -60,38 +61,83 @@ struct Bounds {
     int lo, hi;          // union
     int max_lo, min_hi;  // beyond these an element-wise mask is not needed
 };
-__device__ __forceinline__ int wave_min_i(int v) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64));
-    return v;
+// The lane, opaque to the compiler: what is computed from it behind a loop is not computed (and kept in registers) before.
+__device__ __forceinline__ int ap_late(int lane) {
+    asm volatile("" : "+v"(lane));
+    return lane;
 }
-__device__ __forceinline__ int wave_max_i(int v) {
+
+// (the partners' lanes are computed from `lane` and not shared with other shuffles: six registers that would live across
+// the kernel's main loop)
+__device__ __forceinline__ int wave_min_i(int v, int lane) {
 #pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64));
+    for (int o = 32; o > 0; o >>= 1) v = min(v, __builtin_amdgcn_ds_bpermute((lane ^ o) << 2, v));
     return v;
 }
 // (rows without an interval put no bounds on the mask: whatever their lanes compute is dropped)
-__device__ __forceinline__ Bounds wave_bounds(int2 s) {
+__device__ __forceinline__ Bounds wave_bounds(int2 s, int lane) {
     const bool some = s.y > s.x;
+    const int l = ap_late(lane);
     Bounds b;
-    b.lo = __builtin_amdgcn_readfirstlane(wave_min_i(some ? s.x : INT32_MAX));
-    b.hi = __builtin_amdgcn_readfirstlane(wave_max_i(some ? s.y : 0));
-    b.max_lo = __builtin_amdgcn_readfirstlane(wave_max_i(some ? s.x : 0));
-    b.min_hi = __builtin_amdgcn_readfirstlane(wave_min_i(some ? s.y : INT32_MAX));
+    b.lo = __builtin_amdgcn_readfirstlane(wave_min_i(some ? s.x : INT32_MAX, l));
+    b.hi = -__builtin_amdgcn_readfirstlane(wave_min_i(some ? -s.y : 0, l));
+    b.max_lo = -__builtin_amdgcn_readfirstlane(wave_min_i(some ? -s.x : 0, l));
+    b.min_hi = __builtin_amdgcn_readfirstlane(wave_min_i(some ? s.y : INT32_MAX, l));
     return b;
 }
 
-// 64 rows from row r0 (clamped to `last`, the last row that any lane wants) of a [*, row] matrix, D / 64 panels
+// 64 rows from row r0 (clamped to `last`, the last row that any lane wants) of a [*, row] matrix, D / 64 panels.  The
+// address is a wave-uniform base and a 32-bit lane offset: running 64-bit addresses per lane cost registers the kernels
+// do not have (the host keeps 64 rows below 2^31 bytes).
 template <int NP>
 __device__ __forceinline__ void ap_tile_issue(const TileDma& d, const bf16* base, long long row, int r0, int last, bf16* tile, int wave) {
+    const char* first = reinterpret_cast<const char*>(base + r0 * row);
+    const uint32_t pitch = static_cast<uint32_t>(row) * 2u;
+    const int limit = last - r0;
 #pragma unroll
     for (int j = 0; j < 2; ++j) {
-        const bf16* src = base + static_cast<long long>(min(r0 + static_cast<int>(d.row[j]), last)) * row + d.off[j];
+        const uint32_t off = static_cast<uint32_t>(min(static_cast<int>(d.row[j]), limit)) * pitch + d.off[j] * 2u;
 #pragma unroll
         for (int pn = 0; pn < NP; ++pn)
-            __builtin_amdgcn_global_load_lds((at_global_cvoid*)(src + 64 * pn), (at_lds_void*)(tile + pn * AT_TILE + (2 * wave + j) * 512), 16, 0, 0);
+            __builtin_amdgcn_global_load_lds((at_global_cvoid*)(first + 128 * pn + off), (at_lds_void*)(tile + pn * AT_TILE + (2 * wave + j) * 512), 16, 0, 0);
     }
 }
+
+// Fragment reads of a tile (attention_tile.h) with everything but the lane's part in the immediate offset: one set of
+// eight addresses per tile serves both operands, all panels and halves.
+struct TileAt {
+    uint32_t row[4], tr[2][2];
+};
+__device__ __forceinline__ TileAt tile_at(const FragAddr& fa, uint32_t base) {
+    TileAt t;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) t.row[ks] = base + fa.row[ks];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) t.tr[i >> 1][i & 1] = base + fa.tr[i >> 1][i & 1];
+    return t;
+}
+template <int OFF>
+__device__ __forceinline__ void read_rows(RowFrags& f, const uint32_t (&at)[4]) {
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(f.v[ks]) : "v"(at[ks]), "n"(OFF) : "memory");
+}
+template <int OFF>
+__device__ __forceinline__ void read_tr(TrFrags& f, const uint32_t (&at)[2]) {
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(f.lo[0]) : "v"(at[0]), "n"(OFF) : "memory");
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(f.hi[0]) : "v"(at[1]), "n"(OFF) : "memory");
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(f.lo[1]) : "v"(at[0]), "n"(OFF + 2048) : "memory");
+    asm volatile("ds_read_b64_tr_b16 %0, %1 offset:%2" : "=v"(f.hi[1]) : "v"(at[1]), "n"(OFF + 2048) : "memory");
+}
+// f(0), f(1), ... with compile-time indexes
+template <int N, typename F>
+__device__ __forceinline__ void ap_for(F f) {
+    if constexpr (N > 0) {
+        ap_for<N - 1>(f);
+        f(std::integral_constant<int, N - 1>{});
+    }
+}
+using C0 = std::integral_constant<int, 0>;
+using C1 = std::integral_constant<int, 1>;
 
 // the values of reads issued by inline assembly, taken over behind the wait: nothing that uses them can move in front of it
 __device__ __forceinline__ void taken(RowFrags& f) { asm volatile("" : "+v"(f.v[0]), "+v"(f.v[1]), "+v"(f.v[2]), "+v"(f.v[3])); }
@@ -159,16 +205,16 @@ __device__ __forceinline__ void row_dq(const PackedArgs& p, int h, int row, int 
     for (int e = 0; e < NP; ++e) p.dq[row * p.dq_row + h * p.dq_head + lane + 64 * e] = f32_to_bf16(dq[e] * p.scale);
 }
 
-// heads [h0, h1) of the key's group
-template <int NP>
+// dK or dV (IS_V) from heads [h0, h1) of the key's group
+template <int NP, bool IS_V>
 __device__ __forceinline__ void row_dkv(const PackedArgs& p, int hk, int h0, int h1, int split, int row, int lane) {
     const int2 s = ap_queries_of(p, row);
-    float kv[NP], vv[NP], dk[NP], dv[NP];
+    float kv[NP], vv[NP], acc[NP];
 #pragma unroll
     for (int e = 0; e < NP; ++e) {
         kv[e] = bf16_to_f32(p.k[row * p.k_row + hk * p.k_head + lane + 64 * e]);
         vv[e] = bf16_to_f32(p.v[row * p.v_row + hk * p.v_head + lane + 64 * e]);
-        dk[e] = dv[e] = 0.f;
+        acc[e] = 0.f;
     }
     for (int h = h0; h < h1; ++h)
         for (int i = s.x; i < s.y; ++i) {
@@ -185,22 +231,33 @@ __device__ __forceinline__ void row_dkv(const PackedArgs& p, int hk, int h0, int
             const float pr = fast_exp2(a * p.scale_log2 - p.lse[static_cast<size_t>(h) * p.T + i]);
             const float ds = pr * (b + p.delta[static_cast<size_t>(h) * p.T + i]);
 #pragma unroll
-            for (int e = 0; e < NP; ++e) {
-                dk[e] += ds * qv[e];
-                dv[e] += pr * dov[e];
-            }
+            for (int e = 0; e < NP; ++e) acc[e] += IS_V ? pr * dov[e] : ds * qv[e];
         }
 #pragma unroll
     for (int e = 0; e < NP; ++e) {
+        const float x = IS_V ? acc[e] : acc[e] * p.scale;
+        const int c = lane + 64 * e;
         if (p.part != nullptr) {
             const size_t one = static_cast<size_t>(p.T) * p.Hk * (64 * NP);
-            float* dst = p.part + static_cast<size_t>(split) * 2 * one + (static_cast<size_t>(row) * p.Hk + hk) * (64 * NP) + lane + 64 * e;
-            dst[0] = dk[e] * p.scale;
-            dst[one] = dv[e];
+            p.part[(static_cast<size_t>(split) * 2 + IS_V) * one + (static_cast<size_t>(row) * p.Hk + hk) * (64 * NP) + c] = x;
+        } else if (IS_V) {
+            p.dv[row * p.dv_row + hk * p.dv_head + c] = f32_to_bf16(x);
         } else {
-            p.dk[row * p.dk_row + hk * p.dk_head + lane + 64 * e] = f32_to_bf16(dk[e] * p.scale);
-            p.dv[row * p.dv_row + hk * p.dv_head + lane + 64 * e] = f32_to_bf16(dv[e]);
+            p.dk[row * p.dk_row + hk * p.dk_head + c] = f32_to_bf16(x);
         }
+    }
+}
+
+// Scores of 32 streamed rows (register r holds row (r & 3) + 8 (r >> 2), the upper half wave 4 more) that lie outside
+// [lo, hi) become -inf.  The interval is a bit mask first: two instructions per score, none of them a comparison.
+__device__ __forceinline__ void mask_outside(f32x16& a, int lo, int hi) {
+    auto below = [](int x) { return x >= 32 ? 0xffffffffu : (1u << max(x, 0)) - 1u; };
+    const uint32_t in = below(hi) & ~below(lo);
+#pragma unroll
+    for (int r = 0; r < 16; ++r) {
+        const uint32_t keep = static_cast<uint32_t>(static_cast<int>(in << (31 - (r & 3) - 8 * (r >> 2))) >> 31);
+        const float x = a[r];  // (a bit cast of a vector's element itself reads element 0)
+        a[r] = __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, x) & keep) | (0xff800000u & ~keep));
     }
 }
 
@@ -239,7 +296,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
     const int hk = h / p.group;
     const int qw0 = blk * AT_BR + 32 * wave, qrow = qw0 + lq;
     const int2 span = ap_keys_of(p, qrow);
-    const Bounds wb = wave_bounds(span);
+    const Bounds wb = wave_bounds(span, lane);
     if (lane == 0) {
         sB[wave] = wb.lo;
         sB[4 + wave] = wb.hi;
@@ -275,7 +332,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
     float lsum = 0.f;      // this lane's share of the row sum
     float m = -AP_INF;     // running maximum (log2 units) ...
     float ref = 0.f;       // ... and what the exponents are taken about: the maximum, 0 before the first key
-    const uint32_t sk_lds = lds_addr(sK), sv_lds = lds_addr(sV);
+    const uint32_t sk_lds = lds_addr(sK);
 
     int buf = 0;
     auto next_tile = [&](int t) {  // (the protocol of the fixed-length kernels)
@@ -286,118 +343,121 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
         buf = buf == RING - 1 ? 0 : buf + 1;
         return cur;
     };
-    for (int t = 0; t < min(t_lo, nt); ++t) next_tile(t);
-    for (int t = t_lo; t < t_hi; ++t) {
-        const int k0 = k_lo + t * AT_T;
-        const int cur = next_tile(t);
-        const uint32_t sk_tile = sk_lds + static_cast<uint32_t>(cur) * (TILE * 2), sv_tile = sv_lds + static_cast<uint32_t>(cur) * (TILE * 2);
-        const bool masked = k0 < wb.max_lo || k0 + AT_T > wb.min_hi;
-        const int rel_lo = span.x - k0 - 4 * hi;
-        const uint32_t rel_n = static_cast<uint32_t>(span.y - span.x);  // offset o is valid: (unsigned)(o - rel_lo) < rel_n
-        auto scores = [&](f32x16& acc, RowFrags(&kf)[NP]) {
+    constexpr int PANEL = AT_TILE * 2, V_AT = RING * TILE * 2;  // bytes
+    TileAt at;
+    auto enter_tile = [&](int t) { at = tile_at(fa, sk_lds + static_cast<uint32_t>(next_tile(t)) * (TILE * 2)); };
+    // scores of a half of 32 keys, masked with -inf
+    auto scores = [&](f32x16& acc, auto kt) {
+        RowFrags kf[NP];
+        ap_for<NP>([&](auto pn) { read_rows<pn * PANEL + kt * 4096>(kf[pn], at.row); });
+        lds_wait<0>();
 #pragma unroll
-            for (int e = 0; e < 16; ++e) acc[e] = 0.f;
+        for (int pn = 0; pn < NP; ++pn) taken(kf[pn]);
 #pragma unroll
-            for (int pn = 0; pn < NP; ++pn)
+        for (int ks = 0; ks < 4 * NP; ++ks)
+            acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(kf[ks >> 2], ks & 3), qf[ks], ks == 0 ? f32x16{} : acc, 0, 0, 0);
+    };
+    auto mask = [&](f32x16& acc, int k0, const int kt) {
+        if (k0 >= wb.max_lo && k0 + AT_T <= wb.min_hi) return;
+        const int first = k0 + 32 * kt + 4 * hi;
+        mask_outside(acc, span.x - first, span.y - first);
+    };
+    auto probs = [&](f32x16& acc) {  // in place; returns the lane's partial row sum
+        float sum = 0.f;
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) acc = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(kf[pn], ks), qf[4 * pn + ks], acc, 0, 0, 0);
-        };
-        auto read_k = [&](RowFrags(&kf)[NP], const int kt) {
-#pragma unroll
-            for (int pn = 0; pn < NP; ++pn) frag_rows_issue(kf[pn], sk_tile + pn * (AT_TILE * 2), fa, kt);
-        };
-        auto take_k = [&](RowFrags(&kf)[NP]) {
-#pragma unroll
-            for (int pn = 0; pn < NP; ++pn) taken(kf[pn]);
-        };
-        auto read_v = [&](TrFrags(&vf)[2 * NP], const int kt) {
-#pragma unroll
-            for (int d = 0; d < 2 * NP; ++d) frag_tr_issue(vf[d], sv_tile + (d >> 1) * (AT_TILE * 2), fa, d & 1, kt);
-        };
-        auto take_v = [&](TrFrags(&vf)[2 * NP]) {
-#pragma unroll
-            for (int d = 0; d < 2 * NP; ++d) taken(vf[d]);
-        };
-        // scores -> probabilities about the running reference, in place; returns the lane's partial row sum.  Every lane's
-        // first key lies in a half that starts at or before the wave's largest first key: those halves take the maximum;
-        // later ones only when a partial sum outgrows 2^30 (the maximum rose by 30 octaves).
-        auto probs = [&](f32x16& acc, const int koff, const bool careful) {
-            if (masked) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    acc[r] = static_cast<uint32_t>(koff + (r & 3) + 8 * (r >> 2) - rel_lo) < rel_n ? acc[r] : -AP_INF;
-            }
-            if (careful) {
-                float mx = acc[0];
-#pragma unroll
-                for (int r = 1; r < 16; ++r) mx = fmaxf(mx, acc[r]);
-                mx = other_half_max(mx) * p.scale_log2;
-                const float m_new = fmaxf(m, mx), next = m_new == -AP_INF ? 0.f : m_new;
-                const float alpha = m == -AP_INF ? 0.f : fast_exp2(ref - next);  // (before the row's first key there is nothing to keep)
-                lsum *= alpha;
-#pragma unroll
-                for (int d = 0; d < 2 * NP; ++d)
-#pragma unroll
-                    for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
-                m = m_new;
-                ref = next;
-            }
-            float sum = 0.f;
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                acc[r] = fast_exp2(fmaf(acc[r], p.scale_log2, -ref));
-                sum += acc[r];
-            }
-            return sum;
-        };
-        auto softmax_half = [&](f32x16& acc, const int kt) {
-            const bool careful = k0 + 32 * kt <= wb.max_lo;
-            float ls = probs(acc, 32 * kt, careful);
-            if (!careful && __builtin_expect(__any(!(ls <= 1073741824.f)), 0)) {
-                RowFrags kf[NP];
-                read_k(kf, kt);
-                lds_wait<0>();
-                take_k(kf);
-                scores(acc, kf);
-                ls = probs(acc, 32 * kt, true);
-            }
-            lsum += ls;
-        };
-        auto values = [&](const f32x16& acc, const TrFrags(&vf)[2 * NP]) {
-            const bf16x8 pb0 = pack_half(acc, 0), pb1 = pack_half(acc, 1);
-#pragma unroll
-            for (int d = 0; d < 2 * NP; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(vf[d], 0), pb0, o[d], 0, 0, 0);
-#pragma unroll
-            for (int d = 0; d < 2 * NP; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(vf[d], 1), pb1, o[d], 0, 0, 0);
-        };
-        // two halves of 32 keys, so that the matrix pipe has work while the vector ALU turns scores into probabilities:
-        //   S(0) S(1) | softmax(0) | PV(0) | softmax(1) | PV(1)
-        f32x16 acc0, acc1;
-        {
-            RowFrags kf[NP];
-            read_k(kf, 0);
-            lds_wait<0>();
-            take_k(kf);
-            scores(acc0, kf);
-            read_k(kf, 1);
-            lds_wait<0>();
-            take_k(kf);
-            scores(acc1, kf);
+        for (int r = 0; r < 16; ++r) {
+            acc[r] = fast_exp2(fmaf(acc[r], p.scale_log2, -ref));
+            sum += acc[r];
         }
-        TrFrags vf[2 * NP];
-        read_v(vf, 0);
-        softmax_half(acc0, 0);
+        return sum;
+    };
+    TrFrags vf[2 * NP];
+    auto read_v = [&](auto kt) {
+        ap_for<2 * NP>([&](auto d) { read_tr<V_AT + (d >> 1) * PANEL + kt * 4096>(vf[d], at.tr[d & 1]); });
+    };
+    auto values = [&](const f32x16& acc) {
+        const bf16x8 pb0 = pack_half(acc, 0), pb1 = pack_half(acc, 1);
         lds_wait<0>();
-        take_v(vf);
-        values(acc0, vf);
-        read_v(vf, 1);
-        softmax_half(acc1, 1);
-        lds_wait<0>();
-        take_v(vf);
-        values(acc1, vf);
+#pragma unroll
+        for (int d = 0; d < 2 * NP; ++d) taken(vf[d]);
+#pragma unroll
+        for (int d = 0; d < 2 * NP; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(vf[d], 0), pb0, o[d], 0, 0, 0);
+#pragma unroll
+        for (int d = 0; d < 2 * NP; ++d) o[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(vf[d], 1), pb1, o[d], 0, 0, 0);
+    };
+    // a half with the maximum taken first and the sums so far rescaled
+    auto careful_half = [&](int k0, auto kt) {
+        f32x16 acc;
+        scores(acc, kt);
+        read_v(kt);
+        mask(acc, k0, kt);
+        float mx = acc[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, acc[r]);
+        mx = other_half_max(mx) * p.scale_log2;
+        const float m_new = fmaxf(m, mx), next = m_new == -AP_INF ? 0.f : m_new;
+        const float alpha = m == -AP_INF ? 0.f : fast_exp2(ref - next);  // (before the row's first key there is nothing to keep)
+        m = m_new;
+        ref = next;
+        lsum = lsum * alpha + probs(acc);
+#pragma unroll
+        for (int d = 0; d < 2 * NP; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] *= alpha;
+        values(acc);
         __builtin_amdgcn_sched_barrier(0);
+    };
+    // Every lane's first key lies in a tile that starts at or before the wave's largest first key: those tiles take the
+    // maximum.  The tiles behind them do not - one multiply-add, one exponential and one addition per score - unless a
+    // partial sum outgrows 2^30 (the maximum rose by 30 octaves): that half and the rest of its tile are then done carefully.
+    // (Two loops, not a branch in one: around a branch the compiler keeps a second copy of the output's registers.)
+    for (int t = 0; t < min(t_lo, nt); ++t) next_tile(t);
+    int t = t_lo, kt0 = 0;
+    bool entered = false;
+    while (t < t_hi) {
+        do {
+            const int k0 = k_lo + t * AT_T;
+            if (!entered) enter_tile(t);
+            if (kt0 == 0) careful_half(k0, C0{});
+            careful_half(k0, C1{});
+            entered = false;
+            kt0 = 0;
+            ++t;
+        } while (t < t_hi && k_lo + t * AT_T <= wb.max_lo);
+        for (; t < t_hi; ++t) {
+            // two halves of 32 keys, so that the matrix pipe has work while the vector ALU turns scores into probabilities:
+            //   S(0) S(1) | softmax(0) | PV(0) | softmax(1) | PV(1)
+            const int k0 = k_lo + t * AT_T;
+            enter_tile(t);
+            f32x16 acc0, acc1;
+            scores(acc0, C0{});
+            scores(acc1, C1{});
+            read_v(C0{});
+            mask(acc0, k0, 0);
+            const float l0 = probs(acc0);
+            entered = true;
+            if (__builtin_expect(__any(!(l0 <= 1073741824.f)), 0)) {
+                lds_wait<0>();  // (the value fragments are read again)
+                break;
+            }
+            lsum += l0;
+            values(acc0);
+            read_v(C1{});
+            mask(acc1, k0, 1);
+            const float l1 = probs(acc1);
+            kt0 = 1;
+            if (__builtin_expect(__any(!(l1 <= 1073741824.f)), 0)) {
+                lds_wait<0>();
+                break;
+            }
+            lsum += l1;
+            values(acc1);
+            entered = false;
+            kt0 = 0;
+            __builtin_amdgcn_sched_barrier(0);
+        }
     }
-    for (int t = max(t_lo, t_hi); t < nt; ++t) next_tile(t);
+    for (t = max(t_lo, t_hi); t < nt; ++t) next_tile(t);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     const bool some = span.y > span.x;
     const float lt = other_half_sum(lsum);
@@ -409,18 +469,19 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
             for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
     }
     if (hi == 0 && qrow < p.T) p.lse[static_cast<size_t>(h) * p.T + qrow] = some ? log2f(lt) + ref : 0.f;
+    const int el = ap_late(lane);
     bf16* orow0 = p.out + qw0 * p.o_row + h * (64 * NP);
     bf16* so = sK + wave * (32 * AT_D);
 #pragma unroll
     for (int pn = 0; pn < NP; ++pn)
-        store_rows32(so, o + 2 * pn, inv, lane, p.T - qw0, [&](int row) { return orow0 + row * p.o_row + 64 * pn; });
+        store_rows32(so, o + 2 * pn, inv, el, p.T - qw0, [&](int row) { return orow0 + row * p.o_row + 64 * pn; });
     uint32_t bad = bad_rows(o, some);
     const unsigned long long bl = __ballot(some && !ap_finite(lt));
     bad |= static_cast<uint32_t>(bl) | static_cast<uint32_t>(bl >> 32);
     if (__builtin_expect(bad != 0, 0)) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");  // the rows just stored are written over
         for (int r = 0; r < 32; ++r)
-            if ((bad >> r) & 1) row_forward<NP>(p, h, qw0 + r, lane);
+            if ((bad >> r) & 1) row_forward<NP>(p, h, qw0 + r, el);
     }
 }
 
@@ -438,7 +499,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
     const int hk = h / p.group;
     const int qw0 = blk * AT_BR + 32 * wave, qrow = qw0 + lq;
     const int2 span = ap_keys_of(p, qrow);
-    const Bounds wb = wave_bounds(span);
+    const Bounds wb = wave_bounds(span, lane);
     if (lane == 0) {
         sB[wave] = wb.lo;
         sB[4 + wave] = wb.hi;
@@ -483,7 +544,8 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
     for (int d = 0; d < 2 * NP; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
-    const uint32_t sk_lds = lds_addr(sK), sv_lds = lds_addr(sV);
+    const uint32_t sk_lds = lds_addr(sK);
+    constexpr int PANEL = AT_TILE * 2, V_AT = RING * TILE * 2;  // bytes
 
     int buf = 0;
     auto next_tile = [&](int t) {
@@ -498,55 +560,53 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
     for (int t = t_lo; t < t_hi; ++t) {
         const int k0 = k_lo + t * AT_T;
         const int cur = next_tile(t);
-        const uint32_t sk_tile = sk_lds + static_cast<uint32_t>(cur) * (TILE * 2), sv_tile = sv_lds + static_cast<uint32_t>(cur) * (TILE * 2);
+        const TileAt at = tile_at(fa, sk_lds + static_cast<uint32_t>(cur) * (TILE * 2));
         const bool masked = k0 < wb.max_lo || k0 + AT_T > wb.min_hi;
-        const int rel_lo = span.x - k0 - 4 * hi;
-        const uint32_t rel_n = static_cast<uint32_t>(span.y - span.x);
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt) {
-            if (k0 + 32 * kt >= wb.hi || k0 + 32 * kt + 32 <= wb.lo) continue;  // a half that no row of the wave reaches
+        auto half = [&](auto kt) {
+            if (k0 + 32 * kt >= wb.hi || k0 + 32 * kt + 32 <= wb.lo) return;  // no row of the wave reaches it
             f32x16 s, dp;
+            // delta is the initial accumulator of dP where the registers allow (16 equal ones, set once), else an addition
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                s[e] = 0.f;
-                dp[e] = ndl;
-            }
+            for (int e = 0; e < 16; ++e) dp[e] = NP == 1 ? ndl : 0.f;
             {
                 RowFrags f[NP];
-                auto read = [&](uint32_t tile) {
+                ap_for<NP>([&](auto pn) { read_rows<pn * PANEL + kt * 4096>(f[pn], at.row); });
+                lds_wait<0>();
 #pragma unroll
-                    for (int pn = 0; pn < NP; ++pn) frag_rows_issue(f[pn], tile + pn * (AT_TILE * 2), fa, kt);
-                    lds_wait<0>();
+                for (int pn = 0; pn < NP; ++pn) taken(f[pn]);
 #pragma unroll
-                    for (int pn = 0; pn < NP; ++pn) taken(f[pn]);
-                };
-                read(sk_tile);
+                for (int ks = 0; ks < 4 * NP; ++ks)
+                    s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), qf[ks], ks == 0 ? f32x16{} : s, 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                ap_for<NP>([&](auto pn) { read_rows<V_AT + pn * PANEL + kt * 4096>(f[pn], at.row); });  // (under the products just issued)
+                lds_wait<0>();
 #pragma unroll
-                for (int ks = 0; ks < 4 * NP; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), qf[ks], s, 0, 0, 0);
-                read(sv_tile);  // (under the products just issued)
+                for (int pn = 0; pn < NP; ++pn) taken(f[pn]);
 #pragma unroll
-                for (int ks = 0; ks < 4 * NP; ++ks) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), dof[ks], dp, 0, 0, 0);
+                for (int ks = 0; ks < 4 * NP; ++ks)
+                    dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), dof[ks], dp, 0, 0, 0);
             }
+            __builtin_amdgcn_sched_barrier(0);
             TrFrags kf[2 * NP];  // on their way during the vector work
-#pragma unroll
-            for (int d = 0; d < 2 * NP; ++d) frag_tr_issue(kf[d], sk_tile + (d >> 1) * (AT_TILE * 2), fa, d & 1, kt);
+            ap_for<2 * NP>([&](auto d) { read_tr<(d >> 1) * PANEL + kt * 4096>(kf[d], at.tr[d & 1]); });
             if (masked) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    s[r] = static_cast<uint32_t>(32 * kt + (r & 3) + 8 * (r >> 2) - rel_lo) < rel_n ? s[r] : -AP_INF;
+                const int first = k0 + 32 * kt + 4 * hi;
+                mask_outside(s, span.x - first, span.y - first);
             }
 #pragma unroll
-            for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], p.scale_log2, nl)) * dp[r];
+            for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], p.scale_log2, nl)) * (NP == 1 ? dp[r] : dp[r] + ndl);
             const bf16x8 ds0 = pack_half(s, 0), ds1 = pack_half(s, 1);
             lds_wait<0>();
 #pragma unroll
-            for (int d = 0; d < 2 * NP; ++d) {
-                taken(kf[d]);
-                dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(kf[d], 0), ds0, dq[d], 0, 0, 0);
-                dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(kf[d], 1), ds1, dq[d], 0, 0, 0);
-            }
+            for (int d = 0; d < 2 * NP; ++d) taken(kf[d]);
+#pragma unroll
+            for (int d = 0; d < 2 * NP; ++d) dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(kf[d], 0), ds0, dq[d], 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < 2 * NP; ++d) dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(kf[d], 1), ds1, dq[d], 0, 0, 0);
             __builtin_amdgcn_sched_barrier(0);
-        }
+        };
+        half(C0{});
+        half(C1{});
     }
     for (int t = max(t_lo, t_hi); t < nt; ++t) next_tile(t);
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
@@ -557,21 +617,63 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
 #pragma unroll
             for (int e = 0; e < 16; ++e) dq[d][e] = 0.f;
     }
+    const int el = ap_late(lane);
     bf16* drow0 = p.dq + qw0 * p.dq_row + h * p.dq_head;
     bf16* so = sK + wave * (32 * AT_D);
 #pragma unroll
     for (int pn = 0; pn < NP; ++pn)
-        store_rows32(so, dq + 2 * pn, p.scale, lane, p.T - qw0, [&](int row) { return drow0 + row * p.dq_row + 64 * pn; });
+        store_rows32(so, dq + 2 * pn, p.scale, el, p.T - qw0, [&](int row) { return drow0 + row * p.dq_row + 64 * pn; });
     const uint32_t bad = bad_rows(dq, some);
     if (__builtin_expect(bad != 0, 0)) {
         asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
         for (int r = 0; r < 32; ++r)
-            if ((bad >> r) & 1) row_dq<NP>(p, h, qw0 + r, lane);
+            if ((bad >> r) & 1) row_dq<NP>(p, h, qw0 + r, el);
     }
 }
 
-template <int NP>
-__global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dkv_kernel(const PackedArgs p) {
+// dK or dV (IS_V) of a wave's 32 keys: bf16 rows (through `so`, 4 KB of LDS of the wave's own) or fp32 partial sums
+template <int NP, bool IS_V>
+__device__ __forceinline__ void dkv_store(const PackedArgs& p, f32x16 (&acc)[2 * NP], bf16* so, int hk, int h0, int h1, int split, int kw0, bool some,
+                                          int lane) {
+    const float mult = IS_V ? 1.f : p.scale;
+    if (!some) {
+#pragma unroll
+        for (int d = 0; d < 2 * NP; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+    }
+    const int el = ap_late(lane);
+    if (p.part != nullptr) {
+        const size_t one = static_cast<size_t>(p.T) * p.Hk * (64 * NP);
+        const int row = kw0 + (el & 31);
+        float* dst = p.part + (static_cast<size_t>(split) * 2 + IS_V) * one + (static_cast<size_t>(row) * p.Hk + hk) * (64 * NP) + 4 * (el >> 5);
+        if (row < p.T) {
+#pragma unroll
+            for (int d = 0; d < 2 * NP; ++d)
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    f32x4 a;
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) a[e] = acc[d][4 * r4 + e] * mult;
+                    *reinterpret_cast<f32x4*>(dst + 32 * d + 8 * r4) = a;
+                }
+        }
+    } else {
+        const long long pitch = IS_V ? p.dv_row : p.dk_row;
+        bf16* row0 = IS_V ? p.dv + kw0 * p.dv_row + hk * p.dv_head : p.dk + kw0 * p.dk_row + hk * p.dk_head;
+#pragma unroll
+        for (int pn = 0; pn < NP; ++pn) store_rows32(so, acc + 2 * pn, mult, el, p.T - kw0, [&](int row) { return row0 + row * pitch + 64 * pn; });
+    }
+    const uint32_t bad = bad_rows(acc, some);
+    if (__builtin_expect(bad != 0, 0)) {
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        for (int r = 0; r < 32; ++r)
+            if ((bad >> r) & 1) row_dkv<NP, IS_V>(p, hk, h0, h1, split, kw0 + r, el);
+    }
+}
+
+__global__ __launch_bounds__(256, 2) void packed_dkv64_kernel(const PackedArgs p) {
+    constexpr int NP = 1;
     constexpr int TILE = NP * AT_TILE;
     extern __shared__ __attribute__((aligned(1024))) bf16 ap_smem[];
     bf16* sQ = ap_smem;
@@ -587,7 +689,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dkv_kernel(const 
     const int h0 = hk * p.group + split * p.group / p.splits, h1 = hk * p.group + (split + 1) * p.group / p.splits;
     const int kw0 = blk * AT_BR + 32 * wave, key = kw0 + lq;
     const int2 span = ap_queries_of(p, key);
-    const Bounds wb = wave_bounds(span);
+    const Bounds wb = wave_bounds(span, lane);
     if (lane == 0) {
         sB[wave] = wb.lo;
         sB[4 + wave] = wb.hi;
@@ -630,7 +732,8 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dkv_kernel(const 
     for (int d = 0; d < 2 * NP; ++d)
 #pragma unroll
         for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
-    const uint32_t sq_lds = lds_addr(sQ), sdo_lds = lds_addr(sDO), srow_lds = lds_addr(&sRow[0][0][0]);
+    constexpr int DO_AT = AT_RING * TILE * 2;  // bytes
+    const uint32_t sq_lds = lds_addr(sQ), srow_lds = lds_addr(&sRow[0][0][0]);
 
     int buf = 0, done = 0;
     auto next_tile = [&]() {
@@ -647,59 +750,42 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dkv_kernel(const 
             const int cur = next_tile();
             if (t < t_lo || t >= t_hi) continue;
             const int q0 = q_lo + t * AT_T;
-            const uint32_t sq_tile = sq_lds + static_cast<uint32_t>(cur) * (TILE * 2), sdo_tile = sdo_lds + static_cast<uint32_t>(cur) * (TILE * 2);
+            const TileAt at = tile_at(fa, sq_lds + static_cast<uint32_t>(cur) * (TILE * 2));
             const uint32_t row_tile = srow_lds + static_cast<uint32_t>(cur) * (4 * AT_T * 4) + 16 * hi;
             const bool masked = q0 < wb.max_lo || q0 + AT_T > wb.min_hi;
-            const int rel_lo = span.x - q0 - 4 * hi;
-            const uint32_t rel_n = static_cast<uint32_t>(span.y - span.x);
-            // S and dP of a half of 32 queries
-            auto products = [&](f32x16& s, f32x16& dp, const int qt) {
-                f32x4 nd[4];
-                RowFrags qf[NP], dof[NP];
+            auto half = [&](auto qt) {
+                if (q0 + 32 * qt >= wb.hi || q0 + 32 * qt + 32 <= wb.lo) return;  // no key of the wave meets it
+                f32x16 s, dp;
+                f32x4 nd[4], l2[4];
+                RowFrags qf, dof;
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(nd[r4], row_tile + AT_T * 4 + (32 * qt + 8 * r4) * 4);
-#pragma unroll
-                for (int pn = 0; pn < NP; ++pn) frag_rows_issue(qf[pn], sq_tile + pn * (AT_TILE * 2), fa, qt);
-#pragma unroll
-                for (int pn = 0; pn < NP; ++pn) frag_rows_issue(dof[pn], sdo_tile + pn * (AT_TILE * 2), fa, qt);
-                lds_wait<4 * NP>();
+                read_rows<qt * 4096>(qf, at.row);
+                read_rows<DO_AT + qt * 4096>(dof, at.row);
+                lds_wait<4>();
                 taken(nd);
+                taken(qf);
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    s[e] = 0.f;
-                    dp[e] = nd[e >> 2][e & 3];
-                }
+                for (int e = 0; e < 16; ++e) dp[e] = nd[e >> 2][e & 3];
 #pragma unroll
-                for (int pn = 0; pn < NP; ++pn) {
-                    taken(qf[pn]);
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(qf[pn], ks), kf[4 * pn + ks], s, 0, 0, 0);
-                }
+                for (int ks = 0; ks < 4; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(qf, ks), kf[ks], ks == 0 ? f32x16{} : s, 0, 0, 0);
                 lds_wait<0>();
+                taken(dof);
 #pragma unroll
-                for (int pn = 0; pn < NP; ++pn) {
-                    taken(dof[pn]);
-#pragma unroll
-                    for (int ks = 0; ks < 4; ++ks) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(dof[pn], ks), vf[4 * pn + ks], dp, 0, 0, 0);
-                }
-            };
-            auto finish = [&](f32x16& s, f32x16& dp, const int qt) {
-                f32x4 l2[4];
+                for (int ks = 0; ks < 4; ++ks) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(dof, ks), vf[ks], dp, 0, 0, 0);
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(l2[r4], row_tile + (32 * qt + 8 * r4) * 4);
-                TrFrags dot[2], qtf[2];  // two column tiles of dO^T and Q^T at a time, on their way during the vector work
-#pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    frag_tr_issue(dot[d], sdo_tile, fa, d, qt);
-                    frag_tr_issue(qtf[d], sq_tile, fa, d, qt);
+                TrFrags dot[2], qtf[2];  // dO^T and Q^T, on their way during the vector work
+                ap_for<2>([&](auto d) {
+                    read_tr<DO_AT + qt * 4096>(dot[d], at.tr[d]);
+                    read_tr<qt * 4096>(qtf[d], at.tr[d]);
+                });
+                if (masked) {
+                    const int first = q0 + 32 * qt + 4 * hi;
+                    mask_outside(s, span.x - first, span.y - first);
                 }
                 lds_wait<15>();  // (the row terms are the oldest four of twenty reads; the counter ends at 15)
                 taken(l2);
-                if (masked) {
-#pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        s[r] = static_cast<uint32_t>(32 * qt + (r & 3) + 8 * (r >> 2) - rel_lo) < rel_n ? s[r] : -AP_INF;
-                }
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
                     s[r] = fast_exp2(fmaf(s[r], p.scale_log2, -l2[r >> 2][r & 3]));
@@ -711,90 +797,200 @@ __global__ __launch_bounds__(256, NP == 1 ? 2 : 1) void packed_dkv_kernel(const 
                     pb[j] = pack_half(s, j);
                     dsb[j] = pack_half(dp, j);
                 }
+                lds_wait<0>();
 #pragma unroll
-                for (int pn = 0; pn < NP; ++pn) {
-                    lds_wait<0>();
-                    bf16x8 da[2][2], qa[2][2];
+                for (int d = 0; d < 2; ++d) {
+                    taken(dot[d]);
+                    taken(qtf[d]);
+                }
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
 #pragma unroll
                     for (int d = 0; d < 2; ++d) {
-                        taken(dot[d]);
-                        taken(qtf[d]);
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            da[d][j] = frag_tr_get(dot[d], j);
-                            qa[d][j] = frag_tr_get(qtf[d], j);
-                        }
+                        dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(dot[d], j), pb[j], dv[d], 0, 0, 0);
+                        dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(qtf[d], j), dsb[j], dk[d], 0, 0, 0);
                     }
-                    if (pn + 1 < NP) {
-#pragma unroll
-                        for (int d = 0; d < 2; ++d) {
-                            frag_tr_issue(dot[d], sdo_tile + (pn + 1) * (AT_TILE * 2), fa, d, qt);
-                            frag_tr_issue(qtf[d], sq_tile + (pn + 1) * (AT_TILE * 2), fa, d, qt);
-                        }
-                    }
-#pragma unroll
-                    for (int d = 0; d < 2; ++d)
-#pragma unroll
-                        for (int j = 0; j < 2; ++j) {
-                            dv[2 * pn + d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(da[d][j], pb[j], dv[2 * pn + d], 0, 0, 0);
-                            dk[2 * pn + d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(qa[d][j], dsb[j], dk[2 * pn + d], 0, 0, 0);
-                        }
-                }
+                __builtin_amdgcn_sched_barrier(0);
             };
-            // (halves that no key of the wave meets are left out)
-            f32x16 s, dp;
-            if (q0 + 32 > wb.lo) {
-                products(s, dp, 0);
-                finish(s, dp, 0);
-            }
-            if (q0 + 32 < wb.hi) {
-                products(s, dp, 1);
-                finish(s, dp, 1);
-            }
-            __builtin_amdgcn_sched_barrier(0);
+            half(C0{});
+            half(C1{});
         }
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-    const bool some = span.y > span.x;
-    if (!some) {
-#pragma unroll
-        for (int d = 0; d < 2 * NP; ++d)
-#pragma unroll
-            for (int e = 0; e < 16; ++e) dk[d][e] = dv[d][e] = 0.f;
+    dkv_store<1, false>(p, dk, sQ + wave * (32 * AT_D), hk, h0, h1, split, kw0, span.y > span.x, lane);
+    dkv_store<1, true>(p, dv, sQ + wave * (32 * AT_D), hk, h0, h1, split, kw0, span.y > span.x, lane);
+}
+
+// Heads of 128: dK and dV of 32 keys together with both operands' fragments do not leave two waves per SIMD their
+// registers, and one wave per SIMD has nothing to run under its softmax.  So a workgroup has two kinds of waves, one pair per
+// 32 keys, which the hardware puts on one SIMD:
+//   P waves:  S = Q K^T, P = 2^(S - lse), dV += dO^T P            dS waves:  dP = dO V^T - delta, dS = P dP, dK += Q^T dS
+// P goes from the one to the other through LDS in fp32, register for register (the two products have the same layout).  The
+// work is a sequence of phases of 32 queries with a barrier each; the dS waves run one phase behind.  Tiles are 64 queries
+// (32 KB with dO) in a ring of three: one arriving, one of the P waves, one that the dS waves may still need.
+__global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs p) {
+    constexpr int TILE = 2 * AT_TILE, PANEL = AT_TILE * 2, DO_AT = AT_RING * TILE * 2;  // elements; bytes
+    extern __shared__ __attribute__((aligned(1024))) bf16 ap_smem[];
+    bf16* sQ = ap_smem;                    // [AT_RING][TILE]
+    bf16* sDO = ap_smem + AT_RING * TILE;  // [AT_RING][TILE]
+    float* sP = reinterpret_cast<float*>(ap_smem + 2 * AT_RING * TILE);  // [2][4 pairs][16 registers / 4][64 lanes][4]
+    __shared__ __attribute__((aligned(1024))) float sRow[AT_RING][8][AT_T];  // a wave's own row terms: lse (P waves) or -delta
+    __shared__ int sB[8];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int hi = lane >> 5, lq = lane & 31, pair = wave & 3;
+    const bool is_p = wave < 4;
+    int blk, u;
+    ap_unit(p, p.Hk * p.splits, blk, u);
+    if (p.causal) blk = p.nblk - 1 - blk;  // here the first key blocks carry the most query tiles
+    const int hk = u / p.splits, split = u - hk * p.splits;
+    const int h0 = hk * p.group + split * p.group / p.splits, h1 = hk * p.group + (split + 1) * p.group / p.splits;
+    const int kw0 = blk * AT_BR + 32 * pair, key = kw0 + lq;
+    const int2 span = ap_queries_of(p, key);
+    const Bounds wb = wave_bounds(span, lane);
+    if (lane == 0 && is_p) {
+        sB[wave] = wb.lo;
+        sB[4 + wave] = wb.hi;
     }
-    if (p.part != nullptr) {
-        const size_t one = static_cast<size_t>(p.T) * p.Hk * (64 * NP);
-        float* dst = p.part + static_cast<size_t>(split) * 2 * one + (static_cast<size_t>(key) * p.Hk + hk) * (64 * NP) + 4 * hi;
-        if (key < p.T) {
+    __syncthreads();
+    const int q_lo = min(min(sB[0], sB[1]), min(sB[2], sB[3])), q_hi = max(max(sB[4], sB[5]), max(sB[6], sB[7]));
+    const int nt1 = q_hi > q_lo ? (q_hi - q_lo + AT_T - 1) / AT_T : 0;  // tiles of one head; the heads follow each other
+    const int nt = nt1 * (h1 - h0);
+    const FragAddr fa = frag_addr_setup(lane);
+    // DMA pieces of eight rows: wave w fetches rows 8w .. 8w + 7 of each of the tile's four panels
+    const int d_row = wave * 8 + (lane >> 3);
+    const uint32_t d_off = ((lane & 7) ^ at_swz(d_row)) << 3;
+    bf16x8 own[8];  // B operand: K^T (P waves) or V^T fragments of this lane's key
+    {
+        const int kc = min(key, p.T - 1);
+        const bf16* src = is_p ? p.k + kc * p.k_row + hk * p.k_head : p.v + kc * p.v_row + hk * p.v_head;
 #pragma unroll
-            for (int d = 0; d < 2 * NP; ++d)
+        for (int ks = 0; ks < 8; ++ks) own[ks] = *reinterpret_cast<const bf16x8*>(src + 8 * hi + 16 * ks);
+    }
+    int is_h = h0, is_t = 0;  // the loader's head and tile
+    auto issue = [&](int slot) {
+        const int r0 = q_lo + is_t * AT_T;
+        const uint32_t row = static_cast<uint32_t>(min(d_row, q_hi - 1 - r0));
+        auto one = [&](const bf16* base, long long pitch, bf16* tile) {
+            const char* first = reinterpret_cast<const char*>(base + r0 * pitch);
+            const uint32_t off = row * (static_cast<uint32_t>(pitch) * 2u) + d_off * 2u;
 #pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4) {
-                    f32x4 a, b;
-#pragma unroll
-                    for (int e = 0; e < 4; ++e) {
-                        a[e] = dk[d][4 * r4 + e] * p.scale;
-                        b[e] = dv[d][4 * r4 + e];
-                    }
-                    *reinterpret_cast<f32x4*>(dst + 32 * d + 8 * r4) = a;
-                    *reinterpret_cast<f32x4*>(dst + one + 32 * d + 8 * r4) = b;
-                }
+            for (int pn = 0; pn < 2; ++pn)
+                __builtin_amdgcn_global_load_lds((at_global_cvoid*)(first + 128 * pn + off), (at_lds_void*)(tile + pn * AT_TILE + wave * 512), 16, 0, 0);
+        };
+        one(p.q + is_h * p.q_head, p.q_row, sQ + slot * TILE);
+        one(p.dout + is_h * 128, p.o_row, sDO + slot * TILE);
+        const float* rows = (is_p ? p.lse : p.delta) + static_cast<size_t>(is_h) * p.T;
+        __builtin_amdgcn_global_load_lds((at_global_cvoid*)(rows + min(r0 + lane, q_hi - 1)), (at_lds_void*)&sRow[slot][wave][0], 4, 0, 0);
+        if (++is_t == nt1) {
+            is_t = 0;
+            ++is_h;
         }
-    } else {
-        bf16* so = sQ + wave * (32 * AT_D);
-        bf16* krow0 = p.dk + kw0 * p.dk_row + hk * p.dk_head;
-        bf16* vrow0 = p.dv + kw0 * p.dv_row + hk * p.dv_head;
+    };
+    if (nt > 0) issue(0);
+    if (nt > 1) issue(1);
+    f32x16 acc[4];  // dV (P waves) or dK of the 32 keys
 #pragma unroll
-        for (int pn = 0; pn < NP; ++pn) {
-            store_rows32(so, dk + 2 * pn, p.scale, lane, p.T - kw0, [&](int row) { return krow0 + row * p.dk_row + 64 * pn; });
-            store_rows32(so, dv + 2 * pn, 1.f, lane, p.T - kw0, [&](int row) { return vrow0 + row * p.dv_row + 64 * pn; });
+    for (int d = 0; d < 4; ++d)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
+    const uint32_t sq_lds = lds_addr(sQ), srow_lds = lds_addr(&sRow[0][wave][0]) + 16 * hi;
+    const uint32_t sp_lds = lds_addr(sP) + pair * 4096 + lane * 16;
+
+    // phase n of a wave: queries [q_lo + 64 t + 32 half, + 32) of its current head, tile in ring slot `slot`, P buffer n & 1
+    auto reached = [&](int t, int half) {
+        const int q0 = q_lo + t * AT_T + 32 * half;
+        return q0 < wb.hi && q0 + 32 > wb.lo;
+    };
+    // first product of the phase: rows of Q (P waves) or dO with the wave's own fragments
+    auto product = [&](f32x16& c, const TileAt& at, auto first_at, auto half) {
+        RowFrags f[2];
+        read_rows<first_at + half * 4096>(f[0], at.row);
+        read_rows<first_at + PANEL + half * 4096>(f[1], at.row);
+        lds_wait<4>();
+        taken(f[0]);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[0], ks), own[ks], ks == 0 ? f32x16{} : c, 0, 0, 0);
+        lds_wait<0>();
+        taken(f[1]);
+#pragma unroll
+        for (int ks = 0; ks < 4; ++ks) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[1], ks), own[4 + ks], c, 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    // second product: acc += rows^T (of dO or Q) x c, c packed to bf16
+    auto accumulate = [&](TrFrags(&f)[4], const f32x16& c) {
+        const bf16x8 b0 = pack_half(c, 0), b1 = pack_half(c, 1);
+        lds_wait<0>();
+#pragma unroll
+        for (int d = 0; d < 4; ++d) taken(f[d]);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(f[d], 0), b0, acc[d], 0, 0, 0);
+#pragma unroll
+        for (int d = 0; d < 4; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(f[d], 1), b1, acc[d], 0, 0, 0);
+        __builtin_amdgcn_sched_barrier(0);
+    };
+    using Q_AT = std::integral_constant<int, 0>;
+    using DO_OFF = std::integral_constant<int, DO_AT>;
+    auto p_phase = [&](int t, int slot, auto half) {
+        if (!reached(t, half)) return;
+        const int q0 = q_lo + t * AT_T + 32 * half;
+        const TileAt at = tile_at(fa, sq_lds + static_cast<uint32_t>(slot) * (TILE * 2));
+        f32x16 s;
+        f32x4 l2[4];
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(l2[r4], srow_lds + static_cast<uint32_t>(slot) * (8 * AT_T * 4) + (32 * half + 8 * r4) * 4);
+        product(s, at, Q_AT{}, half);
+        taken(l2);
+        TrFrags f[4];  // on their way during the vector work
+        ap_for<4>([&](auto d) { read_tr<DO_AT + (d >> 1) * PANEL + half * 4096>(f[d], at.tr[d & 1]); });
+        if (q0 < wb.max_lo || q0 + 32 > wb.min_hi) mask_outside(s, span.x - q0 - 4 * hi, span.y - q0 - 4 * hi);
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], p.scale_log2, -l2[r >> 2][r & 3]));
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) {
+            const f32x4 v = {s[4 * r4], s[4 * r4 + 1], s[4 * r4 + 2], s[4 * r4 + 3]};
+            asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(sp_lds), "v"(v), "n"(half * 16384 + r4 * 1024) : "memory");
         }
+        accumulate(f, s);
+    };
+    auto ds_phase = [&](int t, int slot, auto half) {
+        if (!reached(t, half)) return;
+        const TileAt at = tile_at(fa, sq_lds + static_cast<uint32_t>(slot) * (TILE * 2));
+        f32x16 dp;
+        product(dp, at, DO_OFF{}, half);
+        f32x4 nd[4], pr[4];
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(nd[r4], srow_lds + static_cast<uint32_t>(slot) * (8 * AT_T * 4) + (32 * half + 8 * r4) * 4);
+#pragma unroll
+        for (int r4 = 0; r4 < 4; ++r4) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(pr[r4]) : "v"(sp_lds), "n"(half * 16384 + r4 * 1024) : "memory");
+        lds_wait<0>();
+        taken(nd);
+        taken(pr);
+        TrFrags f[4];
+        ap_for<4>([&](auto d) { read_tr<(d >> 1) * PANEL + half * 4096>(f[d], at.tr[d & 1]); });
+#pragma unroll
+        for (int r = 0; r < 16; ++r) dp[r] = (dp[r] + nd[r >> 2][r & 3]) * pr[r >> 2][r & 3];
+        accumulate(f, dp);
+    };
+    // (every barrier: the wave's own LDS writes are done - P - and, where a tile is entered, its DMA pieces have landed)
+    int slot = 0, prev = 0, t = 0, t_prev = 0;
+    for (int n = 0; n < nt; ++n) {
+        if (n + 1 < nt) asm volatile("s_waitcnt vmcnt(5) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (is_p) p_phase(t, slot, C0{});
+        else if (n > 0) ds_phase(t_prev, prev, C1{});
+        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (n + 2 < nt) issue(slot == 0 ? AT_RING - 1 : slot - 1);  // nobody reads the tile before this one any more
+        if (is_p) p_phase(t, slot, C1{});
+        else ds_phase(t, slot, C0{});
+        prev = slot;
+        t_prev = t;
+        slot = slot == AT_RING - 1 ? 0 : slot + 1;
+        if (++t == nt1) t = 0;
     }
-    const uint32_t bad = bad_rows(dk, some) | bad_rows(dv, some);
-    if (__builtin_expect(bad != 0, 0)) {
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        for (int r = 0; r < 32; ++r)
-            if ((bad >> r) & 1) row_dkv<NP>(p, hk, h0, h1, split, kw0 + r, lane);
-    }
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (!is_p && nt > 0) ds_phase(t_prev, prev, C1{});
+    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    if (is_p) dkv_store<2, true>(p, acc, sQ + wave * (32 * AT_D), hk, h0, h1, split, kw0, span.y > span.x, lane);
+    else dkv_store<2, false>(p, acc, sQ + wave * (32 * AT_D), hk, h0, h1, split, kw0, span.y > span.x, lane);
 }
 
 // dK, dV = the sum of the splits' parts, in order
@@ -845,7 +1041,7 @@ PDT_API int pdt_pack_spans(const int* offsets, int sequences, int rows, void* sp
 
 static bool ap_stride_ok(const long long* st, int n) {
     for (int i = 0; i < n; ++i)
-        if (st[i] <= 0 || (st[i] % 8) != 0) return false;
+        if (st[i] <= 0 || (st[i] % 8) != 0 || (i % 2 == 0 && st[i] >= (1 << 24))) return false;
     return true;
 }
 
@@ -876,9 +1072,9 @@ static int ap_lds(K kernel, size_t bytes, unsigned long long& granted) {
 }
 
 template <typename K>
-static int ap_launch(K kernel, unsigned long long& granted, unsigned grid, size_t lds, hipStream_t stream, const PackedArgs& a) {
+static int ap_launch(K kernel, unsigned long long& granted, unsigned grid, size_t lds, hipStream_t stream, const PackedArgs& a, int threads = 256) {
     if (int e = ap_lds(kernel, lds, granted)) return e;
-    hipLaunchKernelGGL(kernel, dim3(grid), dim3(256), lds, stream, a);
+    hipLaunchKernelGGL(kernel, dim3(grid), dim3(threads), lds, stream, a);
     return pdt_launch_status();
 }
 
@@ -941,11 +1137,11 @@ PDT_API int pdt_packed_attention_bwd(const void* q, const void* k, const void* v
     a.o_row = static_cast<long long>(H) * D;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const size_t lds = static_cast<size_t>(2 * (D == 64 ? ap_ring<1> : ap_ring<2>)) * AT_T * D * sizeof(bf16);
-    const size_t lds_k = static_cast<size_t>(2 * AT_RING) * AT_T * D * sizeof(bf16);
+    const size_t lds_k = static_cast<size_t>(2 * AT_RING) * AT_T * D * sizeof(bf16) + (D == 128 ? 2 * 4 * 4096 : 0);
     const unsigned gq = static_cast<unsigned>(a.nblk) * H, gk = static_cast<unsigned>(a.nblk) * Hk * splits;
     static unsigned long long granted[4];
     int rc = D == 64 ? ap_launch(packed_dq_kernel<1>, granted[0], gq, lds, s, a) : ap_launch(packed_dq_kernel<2>, granted[1], gq, lds, s, a);
-    if (rc == 0) rc = D == 64 ? ap_launch(packed_dkv_kernel<1>, granted[2], gk, lds_k, s, a) : ap_launch(packed_dkv_kernel<2>, granted[3], gk, lds_k, s, a);
+    if (rc == 0) rc = D == 64 ? ap_launch(packed_dkv64_kernel, granted[2], gk, lds_k, s, a) : ap_launch(packed_dkv128_kernel, granted[3], gk, lds_k, s, a, 512);
     if (rc != 0) return rc;
     if (a.part != nullptr) {
         const long long n = 2ll * T * Hk * D / 4;

@@ -35,7 +35,7 @@ def _heads(x: torch.Tensor) -> torch.Tensor:
     """[T, heads, D] in bf16 with unit stride along D and rows and heads on 16-byte boundaries (a view where it is one already)."""
     if x.dtype != torch.bfloat16:
         x = x.to(torch.bfloat16)
-    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or x.stride(0) <= 0 or x.stride(1) <= 0 or x.data_ptr() % 16:
+    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or not 0 < x.stride(0) < 1 << 24 or x.stride(1) <= 0 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
