@@ -887,110 +887,129 @@ __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs 
     };
     if (nt > 0) issue(0);
     if (nt > 1) issue(1);
-    f32x16 acc[4];  // dV (P waves) or dK of the 32 keys
-#pragma unroll
-    for (int d = 0; d < 4; ++d)
-#pragma unroll
-        for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
     const uint32_t sq_lds = lds_addr(sQ), srow_lds = lds_addr(&sRow[0][wave][0]) + 16 * hi;
     const uint32_t sp_lds = lds_addr(sP) + pair * 4096 + lane * 16;
 
-    // phase n of a wave: queries [q_lo + 64 t + 32 half, + 32) of its current head, tile in ring slot `slot`, P buffer n & 1
-    auto reached = [&](int t, int half) {
-        const int q0 = q_lo + t * AT_T + 32 * half;
-        return q0 < wb.hi && q0 + 32 > wb.lo;
-    };
-    // first product of the phase: rows of Q (P waves) or dO with the wave's own fragments
-    auto product = [&](f32x16& c, const TileAt& at, auto first_at, auto half) {
+    // The loop of one kind of waves.  The rows of Q (P waves) or dO that a phase starts from are read during the phase before
+    // it, everything else at its start, so that the reads run under products and vector work.  They are waited for before
+    // the phase ends: registers with a read under way must not meet a branch (the compiler may move them there).
+    // Phases that no key of the wave meets are worked off like others, all masked: the pair waits for the barrier either way.
+    auto run = [&](auto role) {
+        constexpr bool IS_P = role == 0;
+        constexpr int ROWS_AT = IS_P ? 0 : DO_AT, T_AT = IS_P ? DO_AT : 0;
+        f32x16 acc[4];  // dV or dK of the 32 keys
+#pragma unroll
+        for (int d = 0; d < 4; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
         RowFrags f[2];
-        read_rows<first_at + half * 4096>(f[0], at.row);
-        read_rows<first_at + PANEL + half * 4096>(f[1], at.row);
-        lds_wait<4>();
-        taken(f[0]);
+        auto fetch = [&](int slot, auto half) {
+            const uint32_t base = sq_lds + static_cast<uint32_t>(slot) * (TILE * 2);
+            uint32_t at[4];
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[0], ks), own[ks], ks == 0 ? f32x16{} : c, 0, 0, 0);
-        lds_wait<0>();
-        taken(f[1]);
+            for (int ks = 0; ks < 4; ++ks) at[ks] = base + fa.row[ks];
+            read_rows<ROWS_AT + half * 4096>(f[0], at);
+            read_rows<ROWS_AT + PANEL + half * 4096>(f[1], at);
+        };
+        auto fetched = [&]() {
+            lds_wait<0>();
+            taken(f[0]);
+            taken(f[1]);
+        };
+        // queries [q_lo + 64 t + 32 half, + 32) of the current head, tile in ring slot `slot`; then the rows of half2 in slot2
+        auto phase = [&](int t, int slot, auto half, int slot2, auto half2) {
+            const uint32_t base = sq_lds + static_cast<uint32_t>(slot) * (TILE * 2), row_at = srow_lds + static_cast<uint32_t>(slot) * (8 * AT_T * 4);
+            f32x16 c;
+            f32x4 rt[4], pr[4];  // row terms; P of the other wave
+            TrFrags ft[4];
 #pragma unroll
-        for (int ks = 0; ks < 4; ++ks) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[1], ks), own[4 + ks], c, 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    // second product: acc += rows^T (of dO or Q) x c, c packed to bf16
-    auto accumulate = [&](TrFrags(&f)[4], const f32x16& c) {
-        const bf16x8 b0 = pack_half(c, 0), b1 = pack_half(c, 1);
-        lds_wait<0>();
+            for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(rt[r4], row_at + (32 * half + 8 * r4) * 4);
+            if constexpr (!IS_P) {
 #pragma unroll
-        for (int d = 0; d < 4; ++d) taken(f[d]);
+                for (int r4 = 0; r4 < 4; ++r4) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(pr[r4]) : "v"(sp_lds), "n"(half * 16384 + r4 * 1024) : "memory");
+            }
+            {
+                uint32_t at[2][2];
 #pragma unroll
-        for (int d = 0; d < 4; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(f[d], 0), b0, acc[d], 0, 0, 0);
+                for (int i = 0; i < 4; ++i) at[i >> 1][i & 1] = base + fa.tr[i >> 1][i & 1];
+                ap_for<4>([&](auto d) { read_tr<T_AT + (d >> 1) * PANEL + half * 4096>(ft[d], at[d & 1]); });
+            }
 #pragma unroll
-        for (int d = 0; d < 4; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(f[d], 1), b1, acc[d], 0, 0, 0);
-        __builtin_amdgcn_sched_barrier(0);
-    };
-    using Q_AT = std::integral_constant<int, 0>;
-    using DO_OFF = std::integral_constant<int, DO_AT>;
-    auto p_phase = [&](int t, int slot, auto half) {
-        if (!reached(t, half)) return;
-        const int q0 = q_lo + t * AT_T + 32 * half;
-        const TileAt at = tile_at(fa, sq_lds + static_cast<uint32_t>(slot) * (TILE * 2));
-        f32x16 s;
-        f32x4 l2[4];
+            for (int ks = 0; ks < 8; ++ks) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), own[ks], ks == 0 ? f32x16{} : c, 0, 0, 0);
+            if constexpr (IS_P) {
+                lds_wait<15>();  // (the row terms are the oldest four of twenty reads; the counter ends at 15)
+                taken(rt);
+                const int q0 = q_lo + t * AT_T + 32 * half;
+                if (q0 < wb.max_lo || q0 + 32 > wb.min_hi) mask_outside(c, span.x - q0 - 4 * hi, span.y - q0 - 4 * hi);
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(l2[r4], srow_lds + static_cast<uint32_t>(slot) * (8 * AT_T * 4) + (32 * half + 8 * r4) * 4);
-        product(s, at, Q_AT{}, half);
-        taken(l2);
-        TrFrags f[4];  // on their way during the vector work
-        ap_for<4>([&](auto d) { read_tr<DO_AT + (d >> 1) * PANEL + half * 4096>(f[d], at.tr[d & 1]); });
-        if (q0 < wb.max_lo || q0 + 32 > wb.min_hi) mask_outside(s, span.x - q0 - 4 * hi, span.y - q0 - 4 * hi);
+                for (int r = 0; r < 16; ++r) c[r] = fast_exp2(fmaf(c[r], p.scale_log2, -rt[r >> 2][r & 3]));
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = fast_exp2(fmaf(s[r], p.scale_log2, -l2[r >> 2][r & 3]));
+                for (int r4 = 0; r4 < 4; ++r4) {
+                    const f32x4 v = {c[4 * r4], c[4 * r4 + 1], c[4 * r4 + 2], c[4 * r4 + 3]};
+                    asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(sp_lds), "v"(v), "n"(half * 16384 + r4 * 1024) : "memory");
+                }
+            }
+            lds_wait<0>();
 #pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) {
-            const f32x4 v = {s[4 * r4], s[4 * r4 + 1], s[4 * r4 + 2], s[4 * r4 + 3]};
-            asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(sp_lds), "v"(v), "n"(half * 16384 + r4 * 1024) : "memory");
+            for (int d = 0; d < 4; ++d) taken(ft[d]);
+            if constexpr (!IS_P) {
+                taken(rt);
+                taken(pr);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) c[r] = (c[r] + rt[r >> 2][r & 3]) * pr[r >> 2][r & 3];
+            }
+            const bf16x8 b0 = pack_half(c, 0), b1 = pack_half(c, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            fetch(slot2, half2);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(ft[d], 0), b0, acc[d], 0, 0, 0);
+#pragma unroll
+            for (int d = 0; d < 4; ++d) acc[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(ft[d], 1), b1, acc[d], 0, 0, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            fetched();
+        };
+        // Tile n + 1 has landed by the second phase of tile n, in which tile n + 2 is requested (into the slot of tile n - 1,
+        // which nobody reads any more).
+        auto middle = [&](int n, int slot) {
+            asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            if (n + 2 < nt) issue(slot == 0 ? AT_RING - 1 : slot - 1);
+        };
+        if (nt > 0) {
+            if (nt > 1) asm volatile("s_waitcnt vmcnt(5)\n\ts_barrier" ::: "memory");
+            else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+            fetch(0, C0{});
+            fetched();
+            int slot = 0, t = 0;
+            if constexpr (IS_P) {
+                for (int n = 0; n < nt; ++n) {
+                    const int next = slot == AT_RING - 1 ? 0 : slot + 1;
+                    phase(t, slot, C0{}, slot, C1{});
+                    middle(n, slot);
+                    phase(t, slot, C1{}, n + 1 < nt ? next : slot, C0{});
+                    asm volatile("s_barrier" ::: "memory");
+                    slot = next;
+                    if (++t == nt1) t = 0;
+                }
+            } else {
+                middle(0, 0);
+                phase(0, 0, C0{}, 0, C1{});
+                asm volatile("s_barrier" ::: "memory");
+                for (int n = 1; n < nt; ++n) {
+                    const int next = slot == AT_RING - 1 ? 0 : slot + 1;
+                    phase(0, slot, C1{}, next, C0{});
+                    slot = next;
+                    middle(n, slot);
+                    phase(0, slot, C0{}, slot, C1{});
+                    asm volatile("s_barrier" ::: "memory");
+                }
+                phase(0, slot, C1{}, slot, C0{});
+            }
         }
-        accumulate(f, s);
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        dkv_store<2, IS_P>(p, acc, sQ + wave * (32 * AT_D), hk, h0, h1, split, kw0, span.y > span.x, lane);
     };
-    auto ds_phase = [&](int t, int slot, auto half) {
-        if (!reached(t, half)) return;
-        const TileAt at = tile_at(fa, sq_lds + static_cast<uint32_t>(slot) * (TILE * 2));
-        f32x16 dp;
-        product(dp, at, DO_OFF{}, half);
-        f32x4 nd[4], pr[4];
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(nd[r4], srow_lds + static_cast<uint32_t>(slot) * (8 * AT_T * 4) + (32 * half + 8 * r4) * 4);
-#pragma unroll
-        for (int r4 = 0; r4 < 4; ++r4) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(pr[r4]) : "v"(sp_lds), "n"(half * 16384 + r4 * 1024) : "memory");
-        lds_wait<0>();
-        taken(nd);
-        taken(pr);
-        TrFrags f[4];
-        ap_for<4>([&](auto d) { read_tr<(d >> 1) * PANEL + half * 4096>(f[d], at.tr[d & 1]); });
-#pragma unroll
-        for (int r = 0; r < 16; ++r) dp[r] = (dp[r] + nd[r >> 2][r & 3]) * pr[r >> 2][r & 3];
-        accumulate(f, dp);
-    };
-    // (every barrier: the wave's own LDS writes are done - P - and, where a tile is entered, its DMA pieces have landed)
-    int slot = 0, prev = 0, t = 0, t_prev = 0;
-    for (int n = 0; n < nt; ++n) {
-        if (n + 1 < nt) asm volatile("s_waitcnt vmcnt(5) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        else asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (is_p) p_phase(t, slot, C0{});
-        else if (n > 0) ds_phase(t_prev, prev, C1{});
-        asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (n + 2 < nt) issue(slot == 0 ? AT_RING - 1 : slot - 1);  // nobody reads the tile before this one any more
-        if (is_p) p_phase(t, slot, C1{});
-        else ds_phase(t, slot, C0{});
-        prev = slot;
-        t_prev = t;
-        slot = slot == AT_RING - 1 ? 0 : slot + 1;
-        if (++t == nt1) t = 0;
-    }
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (!is_p && nt > 0) ds_phase(t_prev, prev, C1{});
-    asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    if (is_p) dkv_store<2, true>(p, acc, sQ + wave * (32 * AT_D), hk, h0, h1, split, kw0, span.y > span.x, lane);
-    else dkv_store<2, false>(p, acc, sQ + wave * (32 * AT_D), hk, h0, h1, split, kw0, span.y > span.x, lane);
+    if (is_p) run(C0{});
+    else run(C1{});
 }
 
 // dK, dV = the sum of the splits' parts, in order
