@@ -2,7 +2,7 @@
 //
 //   q   : [T, H, D]   bf16   T rows: the tokens of all sequences, one sequence behind the other
 //   k, v: [T, Hk, D]  bf16   query head h reads key / value head h / (H / Hk)
-//   out : [T, H, D]   bf16   lse, delta: [H, T] fp32 (log2 units / minus rowsum(dO * O))
+//   out : [T, H, D]   bf16   lse, delta: [H, T] fp32 (log2 units / minus rowsum(dO * O))   rest: [T, H, D] bf16, out's rounding
 //   spans: [T] {first, end}: the sequence a row belongs to; {0, 0} for a row outside every sequence (its results are 0)
 //
 //   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i.k_j - lse_i),  j in [first, i] (causal) or [first, end)
@@ -24,6 +24,7 @@
 struct PackedArgs {
     const bf16 *q, *k, *v, *o, *dout;
     bf16 *out, *dq, *dk, *dv;
+    bf16* rest;           // [T, H, D]: what rounding took from out, written for the backward pass (nullptr: no backward pass)
     float* lse;
     float* delta;
     float* part;          // split dK / dV: [splits][2][T][Hk][D] fp32 partial sums, or nullptr
@@ -168,7 +169,13 @@ __device__ __forceinline__ void row_forward(const PackedArgs& p, int h, int row,
         m = mn;
     }
 #pragma unroll
-    for (int e = 0; e < NP; ++e) p.out[row * p.o_row + h * (64 * NP) + lane + 64 * e] = f32_to_bf16(o[e] / l);
+    for (int e = 0; e < NP; ++e) {
+        const long long at = row * p.o_row + h * (64 * NP) + lane + 64 * e;
+        const float x = o[e] / l;
+        const bf16 r = f32_to_bf16(x);
+        p.out[at] = r;
+        if (p.rest != nullptr) p.rest[at] = f32_to_bf16(x - bf16_to_f32(r));
+    }
     if (lane == 0) p.lse[static_cast<size_t>(h) * p.T + row] = log2f(l) + m;
 }
 
@@ -183,7 +190,7 @@ __device__ __forceinline__ void row_dq(const PackedArgs& p, int h, int row, int 
         const long long at = row * p.o_row + h * (64 * NP) + lane + 64 * e;
         qv[e] = bf16_to_f32(p.q[row * p.q_row + h * p.q_head + lane + 64 * e]);
         dov[e] = bf16_to_f32(p.dout[at]);
-        dl += dov[e] * bf16_to_f32(p.o[at]);
+        dl += dov[e] * (bf16_to_f32(p.o[at]) + bf16_to_f32(p.rest[at]));
         dq[e] = 0.f;
     }
     dl = wave_sum(dl);
@@ -476,6 +483,21 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
     for (int pn = 0; pn < NP; ++pn)
         store_rows32(so, o + 2 * pn, inv, el, p.T - qw0, [&](int row) { return orow0 + row * p.o_row + 64 * pn; });
     uint32_t bad = bad_rows(o, some);
+    if (p.rest != nullptr) {
+        // The backward pass takes dout . out as the row term of dS = P (dP - term).  Where few keys share a row P (dP - term) is
+        // a small difference, and the rounding of out would be its largest error: the term is formed from out and its rest.
+        bf16* rrow0 = p.rest + qw0 * p.o_row + h * (64 * NP);
+#pragma unroll
+        for (int d = 0; d < 2 * NP; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+                const float x = o[d][e] * inv;
+                o[d][e] = x - bf16_to_f32(f32_to_bf16(x));
+            }
+#pragma unroll
+        for (int pn = 0; pn < NP; ++pn)
+            store_rows32(so, o + 2 * pn, 1.f, el, p.T - qw0, [&](int row) { return rrow0 + row * p.o_row + 64 * pn; });
+    }
     const unsigned long long bl = __ballot(some && !ap_finite(lt));
     bad |= static_cast<uint32_t>(bl) | static_cast<uint32_t>(bl >> 32);
     if (__builtin_expect(bad != 0, 0)) {
@@ -531,8 +553,9 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
             qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
             dof[ks] = *reinterpret_cast<const bf16x8*>(p.dout + orow + 16 * ks);
             const bf16x8 ov = *reinterpret_cast<const bf16x8*>(p.o + orow + 16 * ks);
+            const bf16x8 rv = *reinterpret_cast<const bf16x8*>(p.rest + orow + 16 * ks);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dl += bf16_to_f32(dof[ks][e]) * bf16_to_f32(ov[e]);
+            for (int e = 0; e < 8; ++e) dl += bf16_to_f32(dof[ks][e]) * (bf16_to_f32(ov[e]) + bf16_to_f32(rv[e]));
         }
         ndl = -other_half_sum(dl);
         const size_t off = static_cast<size_t>(h) * p.T + qc;
@@ -1097,8 +1120,9 @@ static int ap_launch(K kernel, unsigned long long& granted, unsigned grid, size_
     return pdt_launch_status();
 }
 
-// st: row and head strides of q, k, v in elements (multiples of 8; 16-byte aligned pointers); out is [T, H, D] without gaps.
-PDT_API int pdt_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, float* lse, const void* spans, const long long* st,
+// st: row and head strides of q, k, v in elements (multiples of 8; 16-byte aligned pointers); out is [T, H, D] without gaps,
+// rest (nullptr without a backward pass) like it.
+PDT_API int pdt_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, void* rest, float* lse, const void* spans, const long long* st,
                                      int T, int H, int Hk, int D, float scale, int causal, void* stream) {
     PackedArgs a = {};
     if (ap_args(a, spans, T, H, Hk, D, scale, causal) != 0 || !ap_stride_ok(st, 6)) return -1;
@@ -1106,6 +1130,7 @@ PDT_API int pdt_packed_attention_fwd(const void* q, const void* k, const void* v
     a.k = static_cast<const bf16*>(k);
     a.v = static_cast<const bf16*>(v);
     a.out = static_cast<bf16*>(out);
+    a.rest = static_cast<bf16*>(rest);
     a.lse = lse;
     a.q_row = st[0]; a.q_head = st[1];
     a.k_row = st[2]; a.k_head = st[3];
@@ -1129,7 +1154,7 @@ PDT_API int pdt_packed_attention_splits(int T, int H, int Hk) {
 
 // st: row and head strides of q, k, v, dq, dk, dv; o and dout are [T, H, D] without gaps.  delta: scratch, H * T floats.
 // part: scratch, splits * 2 * T * Hk * D floats, unused (may be nullptr) where splits is 1.
-PDT_API int pdt_packed_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* dout, const float* lse, float* delta,
+PDT_API int pdt_packed_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* rest, const void* dout, const float* lse, float* delta,
                                      void* dq, void* dk, void* dv, float* part, int splits, const void* spans, const long long* st, int T, int H,
                                      int Hk, int D, float scale, int causal, void* stream) {
     PackedArgs a = {};
@@ -1139,6 +1164,7 @@ PDT_API int pdt_packed_attention_bwd(const void* q, const void* k, const void* v
     a.k = static_cast<const bf16*>(k);
     a.v = static_cast<const bf16*>(v);
     a.o = static_cast<const bf16*>(o);
+    a.rest = const_cast<bf16*>(static_cast<const bf16*>(rest));
     a.dout = static_cast<const bf16*>(dout);
     a.lse = const_cast<float*>(lse);
     a.delta = delta;

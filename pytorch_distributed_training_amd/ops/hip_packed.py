@@ -14,8 +14,8 @@ from .hip_transformer import _f, _i, _sig, _vp
 from .hip_vocab import _on
 
 _pack_spans = _sig("pdt_pack_spans", [_vp, _i, _i, _vp, _vp, _vp])
-_fwd = _sig("pdt_packed_attention_fwd", [_vp] * 7 + [_i] * 4 + [_f, _i, _vp])
-_bwd = _sig("pdt_packed_attention_bwd", [_vp] * 11 + [_i, _vp, _vp] + [_i] * 4 + [_f, _i, _vp])
+_fwd = _sig("pdt_packed_attention_fwd", [_vp] * 8 + [_i] * 4 + [_f, _i, _vp])
+_bwd = _sig("pdt_packed_attention_bwd", [_vp] * 12 + [_i, _vp, _vp] + [_i] * 4 + [_f, _i, _vp])
 _splits = _sig("pdt_packed_attention_splits", [_i] * 3)
 
 HEAD_DIMS = (64, 128)
@@ -45,17 +45,18 @@ def _strides(*xs):
     return (ctypes.c_longlong * len(vals))(*vals)
 
 
-def _forward(q, k, v, spans, causal: bool, scale: float):
+def _forward(q, k, v, spans, causal: bool, scale: float, train: bool):
     t, h, d = q.shape
     out = torch.empty((t, h, d), dtype=torch.bfloat16, device=q.device)
+    rest = torch.empty_like(out) if train else None  # what rounding took from out: the backward pass's row terms need it
     lse = torch.empty((h, t), dtype=torch.float32, device=q.device)
     if out.numel():
-        _check(_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), lse.data_ptr(), spans.data_ptr(), _strides(q, k, v), t, h,
-                    k.shape[1], d, scale, int(causal), _stream()), "packed_attention_fwd")
-    return out, lse
+        _check(_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(rest), lse.data_ptr(), spans.data_ptr(), _strides(q, k, v),
+                    t, h, k.shape[1], d, scale, int(causal), _stream()), "packed_attention_fwd")
+    return out, rest, lse
 
 
-def _backward(q, k, v, out, lse, g, spans, causal: bool, scale: float, dq, dk, dv) -> None:
+def _backward(q, k, v, out, rest, lse, g, spans, causal: bool, scale: float, dq, dk, dv) -> None:
     t, h, d = q.shape
     hk = k.shape[1]
     if not q.numel():
@@ -67,8 +68,8 @@ def _backward(q, k, v, out, lse, g, spans, causal: bool, scale: float, dq, dk, d
     delta = torch.empty((h, t), dtype=torch.float32, device=q.device)
     splits = _splits(t, h, hk)
     part = torch.empty((splits, 2, t, hk, d), dtype=torch.float32, device=q.device) if splits > 1 else None
-    _check(_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), g.data_ptr(), lse.data_ptr(), delta.data_ptr(), dq.data_ptr(),
-                dk.data_ptr(), dv.data_ptr(), _ptr(part), splits, spans.data_ptr(), _strides(q, k, v, dq, dk, dv), t, h, hk, d, scale,
+    _check(_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr(), g.data_ptr(), lse.data_ptr(), delta.data_ptr(),
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(part), splits, spans.data_ptr(), _strides(q, k, v, dq, dk, dv), t, h, hk, d, scale,
                 int(causal), _stream()), "packed_attention_bwd")
 
 
@@ -77,18 +78,18 @@ class _AttentionPacked(torch.autograd.Function):
     def forward(ctx, q, k, v, spans, causal: bool, scale: float):
         with _on(q.device):
             q, k, v = _heads(q), _heads(k), _heads(v)
-            out, lse = _forward(q, k, v, spans, causal, scale)
-        ctx.save_for_backward(q, k, v, out, lse, spans)
+            out, rest, lse = _forward(q, k, v, spans, causal, scale, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, out, rest, lse, spans)
         ctx.meta = (causal, scale)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        q, k, v, out, lse, spans = ctx.saved_tensors
+        q, k, v, out, rest, lse, spans = ctx.saved_tensors
         with _on(q.device):
             dq, dk, dv = (torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) for x in (q, k, v))
-            _backward(q, k, v, out, lse, g, spans, *ctx.meta, dq, dk, dv)
+            _backward(q, k, v, out, rest, lse, g, spans, *ctx.meta, dq, dk, dv)
         return dq, dk, dv, None, None, None
 
 
@@ -109,19 +110,19 @@ class _AttentionPackedQKV(torch.autograd.Function):
                 qkv = qkv.to(torch.bfloat16)
             if not qkv.is_contiguous() or qkv.data_ptr() % 16:
                 qkv = qkv.clone(memory_format=torch.contiguous_format)
-            out, lse = _forward(*_split_qkv(qkv, heads, kv_heads), spans, causal, scale)
-        ctx.save_for_backward(qkv, out, lse, spans)
+            out, rest, lse = _forward(*_split_qkv(qkv, heads, kv_heads), spans, causal, scale, ctx.needs_input_grad[0])
+        ctx.save_for_backward(qkv, out, rest, lse, spans)
         ctx.meta = (heads, kv_heads, causal, scale)
         return out.view(qkv.shape[0], -1)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        qkv, out, lse, spans = ctx.saved_tensors
+        qkv, out, rest, lse, spans = ctx.saved_tensors
         heads, kv_heads, causal, scale = ctx.meta
         with _on(qkv.device):
             dqkv = torch.empty_like(qkv)
-            _backward(*_split_qkv(qkv, heads, kv_heads), out, lse, g.reshape(out.shape), spans, causal, scale,
+            _backward(*_split_qkv(qkv, heads, kv_heads), out, rest, lse, g.reshape(out.shape), spans, causal, scale,
                       *_split_qkv(dqkv, heads, kv_heads))
         return dqkv, None, None, None, None, None
 
