@@ -29,6 +29,7 @@ struct PackedArgs {
     float* delta;
     float* part;          // split dK / dV: [splits][2][T][Hk][D] fp32 partial sums, or nullptr
     const int2* spans;
+    const int* order;     // [nblk]: blocks of 128 rows, the ones with the most tiles first
     long long q_row, k_row, v_row, o_row, dq_row, dk_row, dv_row;   // elements between rows ...
     long long q_head, k_head, v_head, dq_head, dk_head, dv_head;    // ... and between heads (o, dout, out: o_row, D)
     int T, H, Hk, group;
@@ -282,11 +283,12 @@ __device__ __forceinline__ uint32_t bad_rows(const f32x16 (&a)[N], bool counts) 
 
 // (block, head) of a workgroup, heads fastest: consecutive workgroups go to the eight XCDs in turn, so an XCD keeps to a few
 // heads (one in eight where the heads are a multiple of eight) whose rows its L2 serves, and every XCD gets blocks of all
-// sizes.  Under a causal mask the blocks of a long sequence with the most tiles come first.
+// sizes.  The blocks with the most tiles come first (pack_order_kernel): 16384 rows of documents of 1 to 1024 tokens fill
+// the CUs 2.7 times, and in the order of the rows the last round left them a quarter idle.
 __device__ __forceinline__ void ap_unit(const PackedArgs& p, int heads, int& blk, int& h) {
-    blk = blockIdx.x / heads;
-    h = blockIdx.x - blk * heads;
-    if (p.causal) blk = p.nblk - 1 - blk;
+    const int rank = blockIdx.x / heads;
+    h = blockIdx.x - rank * heads;
+    blk = p.order[rank];
 }
 
 template <int NP>
@@ -707,7 +709,6 @@ __global__ __launch_bounds__(256, 2) void packed_dkv64_kernel(const PackedArgs p
     const int hi = lane >> 5, lq = lane & 31;
     int blk, u;
     ap_unit(p, p.Hk * p.splits, blk, u);
-    if (p.causal) blk = p.nblk - 1 - blk;  // here the first key blocks carry the most query tiles
     const int hk = u / p.splits, split = u - hk * p.splits;
     const int h0 = hk * p.group + split * p.group / p.splits, h1 = hk * p.group + (split + 1) * p.group / p.splits;
     const int kw0 = blk * AT_BR + 32 * wave, key = kw0 + lq;
@@ -863,7 +864,6 @@ __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs 
     const bool is_p = wave < 4;
     int blk, u;
     ap_unit(p, p.Hk * p.splits, blk, u);
-    if (p.causal) blk = p.nblk - 1 - blk;  // here the first key blocks carry the most query tiles
     const int hk = u / p.splits, split = u - hk * p.splits;
     const int h0 = hk * p.group + split * p.group / p.splits, h1 = hk * p.group + (split + 1) * p.group / p.splits;
     const int kw0 = blk * AT_BR + 32 * pair, key = kw0 + lq;
@@ -1054,30 +1054,78 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PackedArgs p, in
 
 // Sequence of every row: offsets[s] <= row < offsets[s + 1], cut to the rows there are.  The last sequence that starts at or
 // before the row is the only one that can hold it (empty sequences share their start with the one behind them).
-__global__ __launch_bounds__(256) void pack_spans_kernel(const int* __restrict__ offsets, int n, int rows, int2* __restrict__ spans,
-                                                        long long* __restrict__ positions) {
-    const int row = blockIdx.x * 256 + threadIdx.x;
-    if (row >= rows) return;
+__device__ __forceinline__ int2 pack_span_of(const int* offsets, int n, int rows, int row) {
     int lo = 0, hi = n;  // offsets[0 .. lo) start at or before the row
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
         if (offsets[mid] <= row) lo = mid + 1;
         else hi = mid;
     }
-    int2 s = {0, 0};
     if (lo > 0) {
         const int first = max(offsets[lo - 1], 0), end = min(offsets[lo], rows);
-        if (row < end) s = {first, end};
+        if (row < end) return {first, end};
     }
-    spans[row] = s;
-    positions[row] = s.y > 0 ? row - s.x : 0;
+    return {0, 0};
 }
 
-// offsets: [sequences + 1] int32, not falling.
-PDT_API int pdt_pack_spans(const int* offsets, int sequences, int rows, void* spans, long long* positions, void* stream) {
-    if (sequences < 0 || rows <= 0) return -1;
-    hipLaunchKernelGGL(pack_spans_kernel, dim3(pdt_cdiv(rows, 256)), dim3(256), 0, static_cast<hipStream_t>(stream), offsets, sequences, rows,
-                       static_cast<int2*>(spans), positions);
+// work: [3][blocks], rows that a block of 128 streams: causal query side, causal key side, not causal.  order (if given): the
+// rows' own order of the blocks instead.
+__global__ __launch_bounds__(256) void pack_spans_kernel(const int* __restrict__ offsets, int n, int rows, int2* __restrict__ spans,
+                                                        long long* __restrict__ positions, int* __restrict__ work, int* __restrict__ order) {
+    const int row = blockIdx.x * 256 + threadIdx.x;
+    if (row >= rows) return;
+    const int2 s = pack_span_of(offsets, n, rows, row);
+    spans[row] = s;
+    positions[row] = s.y > 0 ? row - s.x : 0;
+    if (row % AT_BR == 0) {
+        const int last = min(row + AT_BR, rows) - 1, blocks = (rows + AT_BR - 1) / AT_BR, b = row / AT_BR;
+        const int2 e = pack_span_of(offsets, n, rows, last);
+        const int first = s.y > 0 ? s.x : row, end = e.y > 0 ? e.y : last + 1;  // (a block's edge may lie outside every sequence)
+        if (order != nullptr) {
+            order[b] = blocks - 1 - b;  // causal, query side: the last blocks of a long sequence have the most keys
+            order[blocks + b] = b;
+            order[2 * static_cast<size_t>(blocks) + b] = b;
+        } else {
+            work[b] = last + 1 - first;
+            work[blocks + b] = end - row;
+            work[2 * static_cast<size_t>(blocks) + b] = end - first;
+        }
+    }
+}
+
+// order[k][rank] = block, by falling work (equal ones as the rows go).  Counted, not sorted: a few thousand blocks at most.
+__global__ __launch_bounds__(256) void pack_order_kernel(const int* __restrict__ work, int blocks, int* __restrict__ order) {
+    __shared__ __attribute__((aligned(16))) int w[256];
+    const int* src = work + static_cast<size_t>(blockIdx.y) * blocks;
+    const int b = blockIdx.x * 256 + threadIdx.x, mine = b < blocks ? src[b] : 0;
+    int rank = 0;
+    for (int j0 = 0; j0 < blocks; j0 += 256) {
+        __syncthreads();
+        w[threadIdx.x] = j0 + static_cast<int>(threadIdx.x) < blocks ? src[j0 + threadIdx.x] : -1;
+        __syncthreads();
+        const int before = b - j0;  // equal work counts from the blocks in front of this one
+#pragma unroll 16
+        for (int j = 0; j < 256; j += 4) {
+            const int4 x = *reinterpret_cast<const int4*>(w + j);
+            rank += (x.x >= mine + (j >= before)) + (x.y >= mine + (j + 1 >= before)) + (x.z >= mine + (j + 2 >= before)) + (x.w >= mine + (j + 3 >= before));
+        }
+    }
+    if (b < blocks) order[static_cast<size_t>(blockIdx.y) * blocks + rank] = b;
+}
+
+// Packs of few blocks (one round of workgroups) and of very many (the last round does not matter) keep the rows' own order.
+#define AP_ORDER_FROM 16
+#define AP_ORDER_TO 8192
+
+// offsets: [sequences + 1] int32, not falling.  order: [3][ceil(rows / 128)]; work: scratch of the same size.
+PDT_API int pdt_pack_spans(const int* offsets, int sequences, int rows, void* spans, long long* positions, int* order, int* work, void* stream) {
+    if (sequences < 0 || rows <= 0 || rows >= (1 << 30)) return -1;
+    hipStream_t s = static_cast<hipStream_t>(stream);
+    const int blocks = pdt_cdiv(rows, AT_BR);
+    const bool sorted = blocks > AP_ORDER_FROM && blocks <= AP_ORDER_TO;
+    hipLaunchKernelGGL(pack_spans_kernel, dim3(pdt_cdiv(rows, 256)), dim3(256), 0, s, offsets, sequences, rows, static_cast<int2*>(spans), positions, work,
+                       sorted ? nullptr : order);
+    if (sorted) hipLaunchKernelGGL(pack_order_kernel, dim3(pdt_cdiv(blocks, 256), 3), dim3(256), 0, s, work, blocks, order);
     return pdt_launch_status();
 }
 
@@ -1087,7 +1135,7 @@ static bool ap_stride_ok(const long long* st, int n) {
     return true;
 }
 
-static int ap_args(PackedArgs& a, const void* spans, int T, int H, int Hk, int D, float scale, int causal) {
+static int ap_args(PackedArgs& a, const void* spans, const int* order, int T, int H, int Hk, int D, float scale, int causal) {
     if (T <= 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || (D != 64 && D != 128) || !(scale > 0.f) || !(scale < 3.0e38f)) return -1;
     a.spans = static_cast<const int2*>(spans);
     a.T = T; a.H = H; a.Hk = Hk;
@@ -1095,6 +1143,7 @@ static int ap_args(PackedArgs& a, const void* spans, int T, int H, int Hk, int D
     a.nblk = pdt_cdiv(T, AT_BR);
     a.causal = causal != 0;
     a.splits = 1;
+    a.order = order + (causal != 0 ? 0 : 2 * static_cast<size_t>(a.nblk));
     a.scale = scale;
     a.scale_log2 = scale * 1.4426950408889634f;
     if (static_cast<long long>(a.nblk) * H >= (1ll << 31) || T >= (1 << 30)) return -1;
@@ -1120,12 +1169,12 @@ static int ap_launch(K kernel, unsigned long long& granted, unsigned grid, size_
     return pdt_launch_status();
 }
 
-// st: row and head strides of q, k, v in elements (multiples of 8; 16-byte aligned pointers); out is [T, H, D] without gaps,
+// spans, order: pdt_pack_spans.  st: row and head strides of q, k, v in elements (multiples of 8; 16-byte aligned pointers); out is [T, H, D] without gaps,
 // rest (nullptr without a backward pass) like it.
-PDT_API int pdt_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, void* rest, float* lse, const void* spans, const long long* st,
+PDT_API int pdt_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, void* rest, float* lse, const void* spans, const int* order, const long long* st,
                                      int T, int H, int Hk, int D, float scale, int causal, void* stream) {
     PackedArgs a = {};
-    if (ap_args(a, spans, T, H, Hk, D, scale, causal) != 0 || !ap_stride_ok(st, 6)) return -1;
+    if (ap_args(a, spans, order, T, H, Hk, D, scale, causal) != 0 || !ap_stride_ok(st, 6)) return -1;
     a.q = static_cast<const bf16*>(q);
     a.k = static_cast<const bf16*>(k);
     a.v = static_cast<const bf16*>(v);
@@ -1155,10 +1204,10 @@ PDT_API int pdt_packed_attention_splits(int T, int H, int Hk) {
 // st: row and head strides of q, k, v, dq, dk, dv; o and dout are [T, H, D] without gaps.  delta: scratch, H * T floats.
 // part: scratch, splits * 2 * T * Hk * D floats, unused (may be nullptr) where splits is 1.
 PDT_API int pdt_packed_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* rest, const void* dout, const float* lse, float* delta,
-                                     void* dq, void* dk, void* dv, float* part, int splits, const void* spans, const long long* st, int T, int H,
+                                     void* dq, void* dk, void* dv, float* part, int splits, const void* spans, const int* order, const long long* st, int T, int H,
                                      int Hk, int D, float scale, int causal, void* stream) {
     PackedArgs a = {};
-    if (ap_args(a, spans, T, H, Hk, D, scale, causal) != 0 || !ap_stride_ok(st, 12)) return -1;
+    if (ap_args(a, spans, order, T, H, Hk, D, scale, causal) != 0 || !ap_stride_ok(st, 12)) return -1;
     if (splits < 1 || splits > a.group || (splits > 1 && part == nullptr) || static_cast<long long>(a.nblk) * Hk * splits >= (1ll << 31)) return -1;
     a.q = static_cast<const bf16*>(q);
     a.k = static_cast<const bf16*>(k);
@@ -1186,6 +1235,7 @@ PDT_API int pdt_packed_attention_bwd(const void* q, const void* k, const void* v
     const unsigned gq = static_cast<unsigned>(a.nblk) * H, gk = static_cast<unsigned>(a.nblk) * Hk * splits;
     static unsigned long long granted[4];
     int rc = D == 64 ? ap_launch(packed_dq_kernel<1>, granted[0], gq, lds, s, a) : ap_launch(packed_dq_kernel<2>, granted[1], gq, lds, s, a);
+    if (a.causal) a.order += a.nblk;  // the key side
     if (rc == 0) rc = D == 64 ? ap_launch(packed_dkv64_kernel, granted[2], gk, lds_k, s, a) : ap_launch(packed_dkv128_kernel, granted[3], gk, lds_k, s, a, 512);
     if (rc != 0) return rc;
     if (a.part != nullptr) {

@@ -13,12 +13,13 @@ from .hip import _check, _ptr, _stream
 from .hip_transformer import _f, _i, _sig, _vp
 from .hip_vocab import _on
 
-_pack_spans = _sig("pdt_pack_spans", [_vp, _i, _i, _vp, _vp, _vp])
-_fwd = _sig("pdt_packed_attention_fwd", [_vp] * 8 + [_i] * 4 + [_f, _i, _vp])
-_bwd = _sig("pdt_packed_attention_bwd", [_vp] * 12 + [_i, _vp, _vp] + [_i] * 4 + [_f, _i, _vp])
+_pack_spans = _sig("pdt_pack_spans", [_vp, _i, _i] + [_vp] * 5)
+_fwd = _sig("pdt_packed_attention_fwd", [_vp] * 9 + [_i] * 4 + [_f, _i, _vp])
+_bwd = _sig("pdt_packed_attention_bwd", [_vp] * 12 + [_i, _vp, _vp, _vp] + [_i] * 4 + [_f, _i, _vp])
 _splits = _sig("pdt_packed_attention_splits", [_i] * 3)
 
 HEAD_DIMS = (64, 128)
+BLOCK_ROWS = 128  # rows of a workgroup
 
 
 def pack_spans(offsets, rows: int):
@@ -26,9 +27,11 @@ def pack_spans(offsets, rows: int):
         offsets = offsets.to(torch.int32).contiguous()
         spans = torch.empty((rows, 2), dtype=torch.int32, device=offsets.device)
         positions = torch.empty(rows, dtype=torch.int64, device=offsets.device)
+        order, work = torch.empty((2, 3, -(-rows // BLOCK_ROWS)), dtype=torch.int32, device=offsets.device)
         if rows:
-            _check(_pack_spans(offsets.data_ptr(), offsets.numel() - 1, rows, spans.data_ptr(), positions.data_ptr(), _stream()), "pack_spans")
-    return spans, positions
+            _check(_pack_spans(offsets.data_ptr(), offsets.numel() - 1, rows, spans.data_ptr(), positions.data_ptr(), order.data_ptr(),
+                               work.data_ptr(), _stream()), "pack_spans")
+    return spans, positions, order
 
 
 def _heads(x: torch.Tensor) -> torch.Tensor:
@@ -45,18 +48,18 @@ def _strides(*xs):
     return (ctypes.c_longlong * len(vals))(*vals)
 
 
-def _forward(q, k, v, spans, causal: bool, scale: float, train: bool):
+def _forward(q, k, v, spans, order, causal: bool, scale: float, train: bool):
     t, h, d = q.shape
     out = torch.empty((t, h, d), dtype=torch.bfloat16, device=q.device)
     rest = torch.empty_like(out) if train else None  # what rounding took from out: the backward pass's row terms need it
     lse = torch.empty((h, t), dtype=torch.float32, device=q.device)
     if out.numel():
-        _check(_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(rest), lse.data_ptr(), spans.data_ptr(), _strides(q, k, v),
+        _check(_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(rest), lse.data_ptr(), spans.data_ptr(), order.data_ptr(), _strides(q, k, v),
                     t, h, k.shape[1], d, scale, int(causal), _stream()), "packed_attention_fwd")
     return out, rest, lse
 
 
-def _backward(q, k, v, out, rest, lse, g, spans, causal: bool, scale: float, dq, dk, dv) -> None:
+def _backward(q, k, v, out, rest, lse, g, spans, order, causal: bool, scale: float, dq, dk, dv) -> None:
     t, h, d = q.shape
     hk = k.shape[1]
     if not q.numel():
@@ -69,28 +72,28 @@ def _backward(q, k, v, out, rest, lse, g, spans, causal: bool, scale: float, dq,
     splits = _splits(t, h, hk)
     part = torch.empty((splits, 2, t, hk, d), dtype=torch.float32, device=q.device) if splits > 1 else None
     _check(_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr(), g.data_ptr(), lse.data_ptr(), delta.data_ptr(),
-                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(part), splits, spans.data_ptr(), _strides(q, k, v, dq, dk, dv), t, h, hk, d, scale,
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(part), splits, spans.data_ptr(), order.data_ptr(), _strides(q, k, v, dq, dk, dv), t, h, hk, d, scale,
                 int(causal), _stream()), "packed_attention_bwd")
 
 
 class _AttentionPacked(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, spans, causal: bool, scale: float):
+    def forward(ctx, q, k, v, spans, order, causal: bool, scale: float):
         with _on(q.device):
             q, k, v = _heads(q), _heads(k), _heads(v)
-            out, rest, lse = _forward(q, k, v, spans, causal, scale, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(q, k, v, out, rest, lse, spans)
+            out, rest, lse = _forward(q, k, v, spans, order, causal, scale, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, out, rest, lse, spans, order)
         ctx.meta = (causal, scale)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        q, k, v, out, rest, lse, spans = ctx.saved_tensors
+        q, k, v, out, rest, lse, spans, order = ctx.saved_tensors
         with _on(q.device):
             dq, dk, dv = (torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) for x in (q, k, v))
-            _backward(q, k, v, out, rest, lse, g, spans, *ctx.meta, dq, dk, dv)
-        return dq, dk, dv, None, None, None
+            _backward(q, k, v, out, rest, lse, g, spans, order, *ctx.meta, dq, dk, dv)
+        return dq, dk, dv, None, None, None, None
 
 
 def _split_qkv(qkv, heads: int, kv_heads: int):
@@ -104,27 +107,27 @@ class _AttentionPackedQKV(torch.autograd.Function):
     """On the projection's output, whose gradient is written as one tensor (no split in forward, no concatenation behind)."""
 
     @staticmethod
-    def forward(ctx, qkv, heads: int, kv_heads: int, spans, causal: bool, scale: float):
+    def forward(ctx, qkv, heads: int, kv_heads: int, spans, order, causal: bool, scale: float):
         with _on(qkv.device):
             if qkv.dtype != torch.bfloat16:
                 qkv = qkv.to(torch.bfloat16)
             if not qkv.is_contiguous() or qkv.data_ptr() % 16:
                 qkv = qkv.clone(memory_format=torch.contiguous_format)
-            out, rest, lse = _forward(*_split_qkv(qkv, heads, kv_heads), spans, causal, scale, ctx.needs_input_grad[0])
-        ctx.save_for_backward(qkv, out, rest, lse, spans)
+            out, rest, lse = _forward(*_split_qkv(qkv, heads, kv_heads), spans, order, causal, scale, ctx.needs_input_grad[0])
+        ctx.save_for_backward(qkv, out, rest, lse, spans, order)
         ctx.meta = (heads, kv_heads, causal, scale)
         return out.view(qkv.shape[0], -1)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        qkv, out, rest, lse, spans = ctx.saved_tensors
+        qkv, out, rest, lse, spans, order = ctx.saved_tensors
         heads, kv_heads, causal, scale = ctx.meta
         with _on(qkv.device):
             dqkv = torch.empty_like(qkv)
-            _backward(*_split_qkv(qkv, heads, kv_heads), out, rest, lse, g.reshape(out.shape), spans, causal, scale,
+            _backward(*_split_qkv(qkv, heads, kv_heads), out, rest, lse, g.reshape(out.shape), spans, order, causal, scale,
                       *_split_qkv(dqkv, heads, kv_heads))
-        return dqkv, None, None, None, None, None
+        return dqkv, None, None, None, None, None, None
 
 
 def _check_head_dim(d: int) -> None:
@@ -134,9 +137,9 @@ def _check_head_dim(d: int) -> None:
 
 def attention_packed(q, k, v, pack, causal: bool, scale: float):
     _check_head_dim(q.shape[2])
-    return _AttentionPacked.apply(q, k, v, pack.spans, bool(causal), scale)
+    return _AttentionPacked.apply(q, k, v, pack.spans, pack.order, bool(causal), scale)
 
 
 def attention_packed_qkv(qkv, pack, heads: int, kv_heads: int, causal: bool, scale: float):
     _check_head_dim(qkv.shape[1] // (heads + 2 * kv_heads))
-    return _AttentionPackedQKV.apply(qkv, heads, kv_heads, pack.spans, bool(causal), scale)
+    return _AttentionPackedQKV.apply(qkv, heads, kv_heads, pack.spans, pack.order, bool(causal), scale)

@@ -13,12 +13,13 @@ import torch
 
 class SequencePack:
     """``spans``: int32 ``[rows, 2]``, first row and end of the sequence a row belongs to (0, 0 outside every sequence);
-    ``positions``: int64 ``[rows]``, a row's position inside its sequence (0 outside)."""
+    ``positions``: int64 ``[rows]``, a row's position inside its sequence (0 outside); ``order``: on GPU, in which order the
+    attention kernels take the rows."""
 
-    __slots__ = ("spans", "positions", "rows", "device")
+    __slots__ = ("spans", "positions", "order", "rows", "device")
 
-    def __init__(self, spans: torch.Tensor, positions: torch.Tensor):
-        self.spans, self.positions = spans, positions
+    def __init__(self, spans: torch.Tensor, positions: torch.Tensor, order: Optional[torch.Tensor] = None):
+        self.spans, self.positions, self.order = spans, positions, order
         self.rows, self.device = spans.shape[0], spans.device
 
 
