@@ -442,23 +442,26 @@ __global__ __launch_bounds__(512) void vocab_gemm_kernel(const VocabGemm p) {
             for (int i = 0; i < 8; ++i) {
                 const int m = mw + i * 16 + r16;
                 if constexpr (KIND == 0) {
-                    float mx = -VL_INF;
+                    if (nw + 64 > p.N) {  // (the last columns of the vocabulary)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j)
+#pragma unroll
+                            for (int e = 0; e < 4; ++e) acc[i][j][e] = nw + j * 16 + 4 * g4 + e < p.N ? acc[i][j][e] : -VL_INF;
+                    }
+                    float mx = acc[i][0][0];
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            acc[i][j][e] = nw + j * 16 + 4 * g4 + e < p.N ? acc[i][j][e] * p.scale_log2 : -VL_INF;
-                            mx = fmaxf(mx, acc[i][j][e]);
-                        }
+                        for (int e = 0; e < 4; ++e) mx = fmaxf(mx, acc[i][j][e]);
                     mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+                    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * p.scale_log2;
                     const float ref = mx == -VL_INF ? 0.f : mx;  // (a group beyond the vocabulary, or one that is masked out)
                     float sum = 0.f;
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) {
-                            acc[i][j][e] = vl_exp2(acc[i][j][e] - ref);
+                            acc[i][j][e] = vl_exp2(fmaf(acc[i][j][e], p.scale_log2, -ref));
                             sum += acc[i][j][e];
                         }
                     sum += __shfl_xor(sum, 16, 64);
@@ -505,32 +508,37 @@ __global__ __launch_bounds__(512) void vocab_gemm_kernel(const VocabGemm p) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");      // the loader's trailing units
 }
 
-// The tiles that were cut along k: their parts summed in order, times alpha.  A workgroup takes 16 rows of both wave rows.
+// The tiles that were cut along k: their parts summed in order, times alpha.  A workgroup takes 16 rows of both wave rows
+// and 16 columns of every wave column, a thread the four values that one thread of the product held.
 __global__ __launch_bounds__(512) void vocab_join_kernel(const VocabGemm p) {
-    const int t = blockIdx.x >> 3, i = blockIdx.x & 7, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int t = blockIdx.x >> 5, ij = blockIdx.x & 31, i = ij >> 2, j = ij & 3, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int m0, n0;
     vl_tile(p, p.whole + t, m0, n0);
-    const int m = m0 + (wave >> 2) * 128 + i * 16 + (lane & 15);
+    const int m = m0 + (wave >> 2) * 128 + i * 16 + (lane & 15), n = n0 + (wave & 3) * 64 + j * 16 + 4 * (lane >> 4);
+    if (m >= p.M || n >= p.N) return;
     const float alpha = p.alpha[0];
+    const float* src = p.part + ((static_cast<size_t>(t) * p.parts * 32 + ij) * 512 + tid) * 4;
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
+    int k = 0;
+    for (; k + 8 <= p.parts; k += 8) {
+        f32x4 v[8];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-        const int n = n0 + (wave & 3) * 64 + j * 16 + 4 * (lane >> 4);
-        if (m >= p.M || n >= p.N) continue;
-        f32x4 s = {0.f, 0.f, 0.f, 0.f};
-        const float* src = p.part + ((static_cast<size_t>(t) * p.parts * 32 + i * 4 + j) * 512 + tid) * 4;
-        for (int k = 0; k < p.parts; ++k) s += *reinterpret_cast<const f32x4*>(src + static_cast<size_t>(k) * 32 * 2048);
-        if (p.out != nullptr) {
-            bf16x4 r;
+        for (int e = 0; e < 8; ++e) v[e] = *reinterpret_cast<const f32x4*>(src + static_cast<size_t>(k + e) * 32 * 2048);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) r[e] = f32_to_bf16(s[e] * alpha);
-            *reinterpret_cast<bf16x4*>(p.out + m * p.ldo + n) = r;
-        } else {
-            f32x4* at = reinterpret_cast<f32x4*>(p.out32 + m * p.ldo + n);
-            f32x4 v;
+        for (int e = 0; e < 8; ++e) s += v[e];
+    }
+    for (; k < p.parts; ++k) s += *reinterpret_cast<const f32x4*>(src + static_cast<size_t>(k) * 32 * 2048);
+    if (p.out != nullptr) {
+        bf16x4 r;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = s[e] * alpha;
-            *at = p.accumulate ? *at + v : v;
-        }
+        for (int e = 0; e < 4; ++e) r[e] = f32_to_bf16(s[e] * alpha);
+        *reinterpret_cast<bf16x4*>(p.out + m * p.ldo + n) = r;
+    } else {
+        f32x4* at = reinterpret_cast<f32x4*>(p.out32 + m * p.ldo + n);
+        f32x4 v;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = s[e] * alpha;
+        *at = p.accumulate ? *at + v : v;
     }
 }
 
@@ -550,13 +558,6 @@ struct Targets {
     long long vocab;
     float inv_tau;
 };
-
-__device__ __forceinline__ float vl_dot8(const bf16* a, const bf16* b, float s) {
-    const bf16x8 u = *reinterpret_cast<const bf16x8*>(a), v = *reinterpret_cast<const bf16x8*>(b);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) s = fmaf(bf16_to_f32(u[e]), bf16_to_f32(v[e]), s);
-    return s;
-}
 
 // one wave per row
 __global__ __launch_bounds__(256) void vocab_targets_kernel(const Targets t) {
@@ -598,14 +599,34 @@ __global__ __launch_bounds__(256) void vocab_targets_kernel(const Targets t) {
         __threadfence_block();  // (the weights are read again by all lanes below)
     }
     if (t.x != nullptr && some) {
+        // sum_k p_k x . W[id_k], eight targets at a time: their rows of W are on their way together
         const bf16* x = t.x + static_cast<size_t>(row) * t.width;
-        for (int k = 0; k < t.top; ++k) {
-            const float pk = t.teacher == nullptr ? 1.f : t.p[static_cast<size_t>(row) * t.top + k];
-            if (pk == 0.f || !present(k)) continue;
-            const bf16* w = t.w + ids[k] * t.width;
-            float s = 0.f;
-            for (int c = lane * 8; c < t.width; c += 512) s = vl_dot8(x + c, w + c, s);
-            base -= pk * s * t.inv_tau;
+        const float* p = t.teacher == nullptr ? nullptr : t.p + static_cast<size_t>(row) * t.top;
+        for (int k0 = 0; k0 < t.top; k0 += 8) {
+            const bf16* w[8];
+            float pk[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int k = min(k0 + i, t.top - 1);
+                const bool ok = k0 + i < t.top && present(k);
+                pk[i] = ok ? (p == nullptr ? 1.f : p[k]) : 0.f;
+                w[i] = t.w + (pk[i] != 0.f ? ids[k] : 0ll) * t.width;
+            }
+            for (int c = lane * 8; c < t.width; c += 512) {
+                const bf16x8 xv = *reinterpret_cast<const bf16x8*>(x + c);
+                bf16x8 wv[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    if (pk[i] != 0.f) wv[i] = *reinterpret_cast<const bf16x8*>(w[i] + c);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    if (pk[i] == 0.f) continue;  // (not multiplied by 0: what an absent target's row holds does not count)
+                    float s = 0.f;
+#pragma unroll
+                    for (int e = 0; e < 8; ++e) s = fmaf(bf16_to_f32(xv[e]), bf16_to_f32(wv[i][e]), s);
+                    base -= pk[i] * s * t.inv_tau;
+                }
+            }
         }
     }
     if (t.x_used != nullptr)
@@ -892,7 +913,7 @@ static int vl_launch(const VocabGemm& g, hipStream_t s) {
     if (int e = vl_grant_lds(vocab_gemm_kernel<KIND>, lds, granted)) return e;
     const int units = g.whole + g.left * g.parts, cus = vl_cus();
     hipLaunchKernelGGL(vocab_gemm_kernel<KIND>, dim3(units < cus ? units : cus), dim3(512), lds, s, g);
-    if (g.left > 0) hipLaunchKernelGGL(vocab_join_kernel, dim3(g.left * 8), dim3(512), 0, s, g);
+    if (g.left > 0) hipLaunchKernelGGL(vocab_join_kernel, dim3(g.left * 32), dim3(512), 0, s, g);
     return pdt_launch_status();
 }
 

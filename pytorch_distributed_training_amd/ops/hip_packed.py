@@ -22,16 +22,17 @@ HEAD_DIMS = (64, 128)
 BLOCK_ROWS = 128  # rows of a workgroup
 
 
-def pack_spans(offsets, rows: int):
+def pack_plan(offsets, rows: int):
+    """One int64 buffer: ``rows`` positions, ``rows`` spans (two int32), three orders of the blocks and as much scratch."""
     with _on(offsets.device):
         offsets = offsets.to(torch.int32).contiguous()
-        spans = torch.empty((rows, 2), dtype=torch.int32, device=offsets.device)
-        positions = torch.empty(rows, dtype=torch.int64, device=offsets.device)
-        order, work = torch.empty((2, 3, -(-rows // BLOCK_ROWS)), dtype=torch.int32, device=offsets.device)
+        blocks = -(-rows // BLOCK_ROWS)
+        plan = torch.empty(2 * rows + 3 * blocks, dtype=torch.int64, device=offsets.device)
         if rows:
-            _check(_pack_spans(offsets.data_ptr(), offsets.numel() - 1, rows, spans.data_ptr(), positions.data_ptr(), order.data_ptr(),
-                               work.data_ptr(), _stream()), "pack_spans")
-    return spans, positions, order
+            at = plan.data_ptr()
+            order = at + 16 * rows
+            _check(_pack_spans(offsets.data_ptr(), offsets.numel() - 1, rows, at + 8 * rows, at, order, order + 12 * blocks, _stream()), "pack_spans")
+    return plan
 
 
 def _heads(x: torch.Tensor) -> torch.Tensor:
@@ -48,18 +49,18 @@ def _strides(*xs):
     return (ctypes.c_longlong * len(vals))(*vals)
 
 
-def _forward(q, k, v, spans, order, causal: bool, scale: float, train: bool):
+def _forward(q, k, v, plan, causal: bool, scale: float, train: bool):
     t, h, d = q.shape
     out = torch.empty((t, h, d), dtype=torch.bfloat16, device=q.device)
     rest = torch.empty_like(out) if train else None  # what rounding took from out: the backward pass's row terms need it
     lse = torch.empty((h, t), dtype=torch.float32, device=q.device)
     if out.numel():
-        _check(_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(rest), lse.data_ptr(), spans.data_ptr(), order.data_ptr(), _strides(q, k, v),
+        _check(_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(rest), lse.data_ptr(), plan.data_ptr() + 8 * t, plan.data_ptr() + 16 * t, _strides(q, k, v),
                     t, h, k.shape[1], d, scale, int(causal), _stream()), "packed_attention_fwd")
     return out, rest, lse
 
 
-def _backward(q, k, v, out, rest, lse, g, spans, order, causal: bool, scale: float, dq, dk, dv) -> None:
+def _backward(q, k, v, out, rest, lse, g, plan, causal: bool, scale: float, dq, dk, dv) -> None:
     t, h, d = q.shape
     hk = k.shape[1]
     if not q.numel():
@@ -72,28 +73,28 @@ def _backward(q, k, v, out, rest, lse, g, spans, order, causal: bool, scale: flo
     splits = _splits(t, h, hk)
     part = torch.empty((splits, 2, t, hk, d), dtype=torch.float32, device=q.device) if splits > 1 else None
     _check(_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr(), g.data_ptr(), lse.data_ptr(), delta.data_ptr(),
-                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(part), splits, spans.data_ptr(), order.data_ptr(), _strides(q, k, v, dq, dk, dv), t, h, hk, d, scale,
+                dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(part), splits, plan.data_ptr() + 8 * t, plan.data_ptr() + 16 * t, _strides(q, k, v, dq, dk, dv), t, h, hk, d, scale,
                 int(causal), _stream()), "packed_attention_bwd")
 
 
 class _AttentionPacked(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, spans, order, causal: bool, scale: float):
+    def forward(ctx, q, k, v, plan, causal: bool, scale: float):
         with _on(q.device):
             q, k, v = _heads(q), _heads(k), _heads(v)
-            out, rest, lse = _forward(q, k, v, spans, order, causal, scale, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(q, k, v, out, rest, lse, spans, order)
+            out, rest, lse = _forward(q, k, v, plan, causal, scale, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, out, rest, lse, plan)
         ctx.meta = (causal, scale)
         return out
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        q, k, v, out, rest, lse, spans, order = ctx.saved_tensors
+        q, k, v, out, rest, lse, plan = ctx.saved_tensors
         with _on(q.device):
             dq, dk, dv = (torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) for x in (q, k, v))
-            _backward(q, k, v, out, rest, lse, g, spans, order, *ctx.meta, dq, dk, dv)
-        return dq, dk, dv, None, None, None, None
+            _backward(q, k, v, out, rest, lse, g, plan, *ctx.meta, dq, dk, dv)
+        return dq, dk, dv, None, None, None
 
 
 def _split_qkv(qkv, heads: int, kv_heads: int):
@@ -107,27 +108,27 @@ class _AttentionPackedQKV(torch.autograd.Function):
     """On the projection's output, whose gradient is written as one tensor (no split in forward, no concatenation behind)."""
 
     @staticmethod
-    def forward(ctx, qkv, heads: int, kv_heads: int, spans, order, causal: bool, scale: float):
+    def forward(ctx, qkv, heads: int, kv_heads: int, plan, causal: bool, scale: float):
         with _on(qkv.device):
             if qkv.dtype != torch.bfloat16:
                 qkv = qkv.to(torch.bfloat16)
             if not qkv.is_contiguous() or qkv.data_ptr() % 16:
                 qkv = qkv.clone(memory_format=torch.contiguous_format)
-            out, rest, lse = _forward(*_split_qkv(qkv, heads, kv_heads), spans, order, causal, scale, ctx.needs_input_grad[0])
-        ctx.save_for_backward(qkv, out, rest, lse, spans, order)
+            out, rest, lse = _forward(*_split_qkv(qkv, heads, kv_heads), plan, causal, scale, ctx.needs_input_grad[0])
+        ctx.save_for_backward(qkv, out, rest, lse, plan)
         ctx.meta = (heads, kv_heads, causal, scale)
         return out.view(qkv.shape[0], -1)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        qkv, out, rest, lse, spans, order = ctx.saved_tensors
+        qkv, out, rest, lse, plan = ctx.saved_tensors
         heads, kv_heads, causal, scale = ctx.meta
         with _on(qkv.device):
             dqkv = torch.empty_like(qkv)
-            _backward(*_split_qkv(qkv, heads, kv_heads), out, rest, lse, g.reshape(out.shape), spans, order, causal, scale,
+            _backward(*_split_qkv(qkv, heads, kv_heads), out, rest, lse, g.reshape(out.shape), plan, causal, scale,
                       *_split_qkv(dqkv, heads, kv_heads))
-        return dqkv, None, None, None, None, None, None
+        return dqkv, None, None, None, None, None
 
 
 def _check_head_dim(d: int) -> None:
@@ -137,9 +138,9 @@ def _check_head_dim(d: int) -> None:
 
 def attention_packed(q, k, v, pack, causal: bool, scale: float):
     _check_head_dim(q.shape[2])
-    return _AttentionPacked.apply(q, k, v, pack.spans, pack.order, bool(causal), scale)
+    return _AttentionPacked.apply(q, k, v, pack.plan, bool(causal), scale)
 
 
 def attention_packed_qkv(qkv, pack, heads: int, kv_heads: int, causal: bool, scale: float):
     _check_head_dim(qkv.shape[1] // (heads + 2 * kv_heads))
-    return _AttentionPackedQKV.apply(qkv, heads, kv_heads, pack.spans, pack.order, bool(causal), scale)
+    return _AttentionPackedQKV.apply(qkv, heads, kv_heads, pack.plan, bool(causal), scale)

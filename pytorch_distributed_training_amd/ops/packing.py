@@ -13,14 +13,22 @@ import torch
 
 class SequencePack:
     """``spans``: int32 ``[rows, 2]``, first row and end of the sequence a row belongs to (0, 0 outside every sequence);
-    ``positions``: int64 ``[rows]``, a row's position inside its sequence (0 outside); ``order``: on GPU, in which order the
-    attention kernels take the rows."""
+    ``positions``: int64 ``[rows]``, a row's position inside its sequence (0 outside).  ``plan``: what the attention kernels
+    read on GPU (positions, spans and the order they take the rows in, one buffer)."""
 
-    __slots__ = ("spans", "positions", "order", "rows", "device")
+    __slots__ = ("rows", "device", "plan", "_host")
 
-    def __init__(self, spans: torch.Tensor, positions: torch.Tensor, order: Optional[torch.Tensor] = None):
-        self.spans, self.positions, self.order = spans, positions, order
-        self.rows, self.device = spans.shape[0], spans.device
+    def __init__(self, rows: int, plan: Optional[torch.Tensor] = None, host=None):
+        self.rows, self.plan, self._host = rows, plan, host
+        self.device = plan.device if host is None else host[0].device
+
+    @property
+    def spans(self) -> torch.Tensor:
+        return self._host[0] if self._host is not None else self.plan[self.rows:2 * self.rows].view(torch.int32).view(-1, 2)
+
+    @property
+    def positions(self) -> torch.Tensor:
+        return self._host[1] if self._host is not None else self.plan[:self.rows]
 
 
 def _check_on_host(offsets: torch.Tensor, rows: int) -> None:
@@ -52,7 +60,7 @@ def pack_sequences(offsets, rows: int, device: Optional[torch.device] = None) ->
     if offsets.is_cuda:
         from . import hip_packed
 
-        return SequencePack(*hip_packed.pack_spans(offsets, rows))
+        return SequencePack(rows, hip_packed.pack_plan(offsets, rows))
     offsets = offsets.to(torch.int64)
     row = torch.arange(rows)
     at = torch.searchsorted(offsets, row, right=True) - 1  # the last sequence that starts at or before the row
@@ -60,4 +68,4 @@ def pack_sequences(offsets, rows: int, device: Optional[torch.device] = None) ->
     at = at.clamp(0, max(offsets.numel() - 2, 0))
     ends = offsets[1:] if offsets.numel() > 1 else offsets
     spans = torch.stack([offsets[at], ends[at]], 1) * inside[:, None]
-    return SequencePack(spans.to(torch.int32), torch.where(inside, row - spans[:, 0], 0))
+    return SequencePack(rows, host=(spans.to(torch.int32), torch.where(inside, row - spans[:, 0], 0)))
