@@ -546,8 +546,8 @@ PDT_API int pdt_embedding_bwd(const long long* ids, const void* g, float* dw, lo
 // the batch, so no atomics and no [B, S, D] -> [S, D] reduction pass; the token table uses embedding_bwd.
 // ------------------------------------------------------------------------------------------------
 __global__ __launch_bounds__(256) void embedding_pos_fwd_kernel(const long long* __restrict__ ids, const float* __restrict__ w,
-                                                               const float* __restrict__ pos, bf16* __restrict__ out, long long n,
-                                                               int D, long long vocab, int S) {
+                                                               const float* __restrict__ pos, const long long* __restrict__ at,
+                                                               bf16* __restrict__ out, long long n, int D, long long vocab, int S) {
     const int dvec = D >> 3;
     const long long nvec = n * dvec;
     for (long long v = blockIdx.x * 256ll + threadIdx.x; v < nvec; v += gridDim.x * 256ll) {
@@ -555,7 +555,8 @@ __global__ __launch_bounds__(256) void embedding_pos_fwd_kernel(const long long*
         const int c = static_cast<int>(v - i * dvec) << 3;
         long long id = ids[i];
         id = id < 0 ? 0 : (id >= vocab ? vocab - 1 : id);
-        const int t = static_cast<int>(i % S);
+        // (positions given: packed sequences; the table's S rows bound them as the vocabulary bounds the ids)
+        const int t = at == nullptr ? static_cast<int>(i % S) : static_cast<int>(at[i] < 0 ? 0 : (at[i] >= S ? S - 1 : at[i]));
         const f32x4 a = *reinterpret_cast<const f32x4*>(w + id * D + c), b = *reinterpret_cast<const f32x4*>(w + id * D + c + 4);
         const f32x4 pa = *reinterpret_cast<const f32x4*>(pos + static_cast<long long>(t) * D + c),
                     pb = *reinterpret_cast<const f32x4*>(pos + static_cast<long long>(t) * D + c + 4);
@@ -612,11 +613,11 @@ __global__ __launch_bounds__(256) void batch_rowsum_kernel(const bf16* __restric
     }
 }
 
-PDT_API int pdt_embedding_pos_fwd(const long long* ids, const float* w, const float* pos, void* out, long long n, int D,
-                                  long long vocab, int S, void* stream) {
+PDT_API int pdt_embedding_pos_fwd(const long long* ids, const float* w, const float* pos, const long long* at, void* out, long long n,
+                                  int D, long long vocab, int S, void* stream) {
     if (n <= 0 || D <= 0 || (D % 8) != 0 || vocab <= 0 || S <= 0) return -1;
     hipLaunchKernelGGL(embedding_pos_fwd_kernel, dim3(ew_grid8(n * (D / 8))), dim3(256), 0, static_cast<hipStream_t>(stream), ids, w,
-                       pos, static_cast<bf16*>(out), n, D, vocab, S);
+                       pos, at, static_cast<bf16*>(out), n, D, vocab, S);
     return pdt_launch_status();
 }
 

@@ -5,7 +5,9 @@ the large-gradient data-parallel workload (~355 M parameters, tied input/output
 embeddings) that stresses the bucket reducer and the fused AdamW step.
 The forward pass returns logits; with ``targets`` it returns the mean next-token
 cross-entropy from the fused output-projection + loss operator, which works through the rows
-in chunks and never materialises logits or probabilities for the whole batch.
+in chunks and never materialises logits or probabilities for the whole batch; with ``teacher``
+the divergence from a teacher's top logits, in the same way.  Documents of different lengths
+train without padding, packed one behind the other along one axis (``pack``).
 """
 
 from __future__ import annotations
@@ -44,16 +46,28 @@ class GPT2(nn.Module):
         elif isinstance(m, nn.Embedding):
             nn.init.normal_(m.weight, std=0.02)
 
-    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None) -> torch.Tensor:
-        b, s = idx.shape
-        if s > self.n_ctx:
-            raise ValueError(f"sequence length {s} exceeds context {self.n_ctx}")
-        x = ops.token_position_embedding(idx, self.wte.weight, self.wpe.weight)
+    def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, pack: Optional[ops.SequencePack] = None,
+                teacher: Optional[tuple] = None, temperature: float = 1.0) -> torch.Tensor:
+        """``idx`` ``[B, S]``, or ``[rows]`` with ``pack`` (:func:`ops.pack_sequences`): documents one behind the other,
+        each with positions of its own from 0 and attending to itself alone.  ``targets`` of the shape of ``idx`` (packed:
+        tokens whose target lies outside the vocabulary, -100 at a document's end say, do not count), or ``teacher``:
+        (logits, ids) of the shape of ``idx`` plus ``K``, see :func:`ops.distillation_loss`."""
+        if targets is not None and teacher is not None:
+            raise ValueError("targets or a teacher, not both")
+        if pack is None:
+            b, s = idx.shape
+            if s > self.n_ctx:
+                raise ValueError(f"sequence length {s} exceeds context {self.n_ctx}")
+        x = ops.token_position_embedding(idx, self.wte.weight, self.wpe.weight, pack)
         for blk in self.h:
-            x = blk(x)
+            x = blk(x, pack)
         x = ops.layer_norm(x, self.ln_f.weight, self.ln_f.bias, self.ln_f.eps)
+        if teacher is not None:
+            return ops.linear_distillation_loss(x, self.wte.weight, *teacher, temperature=temperature)
         if targets is None:
             return ops.linear(x, self.wte.weight, None)  # tied output projection
+        if pack is not None or self.vocab_size > 65536:
+            return ops.linear_cross_entropy(x, self.wte.weight, targets)
         # projection + loss in one operator: the [b * s, vocabulary] logits are never held as a whole
         return ops.lm_head_loss(x, self.wte.weight, targets)
 

@@ -36,9 +36,12 @@ class SelfAttention(nn.Module):
         self.qkv = nn.Linear(dim, 3 * dim)
         self.proj = nn.Linear(dim, dim)
 
-    def forward(self, x, residual, link=None):
+    def forward(self, x, residual, link=None, pack=None):
         qkv = ops.linear(x, self.qkv.weight, self.qkv.bias)  # [b, s, 3*d], consumed in place by the attention kernel
-        o = ops.attention_qkv(qkv, self.heads, causal=self.causal)
+        if pack is None:
+            o = ops.attention_qkv(qkv, self.heads, causal=self.causal)
+        else:  # [rows, 3*d]: sequences packed one behind the other
+            o = ops.attention_packed_qkv(qkv, pack, self.heads, causal=self.causal)
         return ops.linear(o, self.proj.weight, self.proj.bias, residual=residual, link=link)
 
 
@@ -50,10 +53,10 @@ class EncoderBlock(nn.Module):
         self.ln_2 = nn.LayerNorm(dim, eps=1e-6)
         self.mlp = MLP(dim, mlp_dim)
 
-    def forward(self, x):
+    def forward(self, x, pack=None):
         # each branch's skip gradient is handed to the LayerNorm at its head (ops.skip_link)
         l1 = ops.skip_link(x)
-        x = self.attn(ops.layer_norm(x, self.ln_1.weight, self.ln_1.bias, self.ln_1.eps, link=l1), x, l1)
+        x = self.attn(ops.layer_norm(x, self.ln_1.weight, self.ln_1.bias, self.ln_1.eps, link=l1), x, l1, pack)
         l2 = ops.skip_link(x)
         return self.mlp(ops.layer_norm(x, self.ln_2.weight, self.ln_2.bias, self.ln_2.eps, link=l2), x, l2)
 

@@ -302,12 +302,22 @@ def embedding(ids, weight):
     return _ref.embedding(ids, weight)
 
 
-def token_position_embedding(ids, wte, wpe):
-    """Input embedding of a language model: ``wte[ids] + wpe[position]`` for ``ids`` of shape ``[B, S]``."""
+def token_position_embedding(ids, wte, wpe, pack: Optional[SequencePack] = None):
+    """Input embedding of a language model: ``wte[ids] + wpe[position]`` for ``ids`` of shape ``[B, S]``, or of shape
+    ``[rows]`` with ``pack``, where positions count from the start of each sequence (and are 0 outside)."""
+    if pack is not None:
+        if ids.dim() != 1 or ids.shape[0] != pack.rows or ids.device != pack.device:
+            raise ValueError(f"packed tokens of shape ({pack.rows},) on {pack.device} expected, got {tuple(ids.shape)} on {ids.device}")
+        if pack.longest is not None and pack.longest > wpe.shape[0]:
+            raise ValueError(f"a sequence of {pack.longest} tokens exceeds the {wpe.shape[0]} positions of the table")
     if wte.is_cuda:
         from . import hip_transformer as ht
 
+        if pack is not None:
+            return ht.packed_embedding(ids, pack.positions, wte, wpe)
         return ht.token_position_embedding(ids, wte, wpe)
+    if pack is not None:
+        return _ref.packed_embedding(ids, pack.positions, wte, wpe)
     return _ref.token_position_embedding(ids, wte, wpe)
 
 

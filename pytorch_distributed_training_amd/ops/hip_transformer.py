@@ -33,7 +33,7 @@ _gelu_bwd = _sig("pdt_gelu_bwd", [_vp, _vp, _vp, _ll, _vp])
 _bias_res = _sig("pdt_bias_residual", [_vp, _vp, _vp, _vp, _ll, _i, _vp])
 _emb_fwd = _sig("pdt_embedding_fwd", [_vp, _vp, _vp, _ll, _i, _ll, _vp])
 _emb_bwd = _sig("pdt_embedding_bwd", [_vp, _vp, _vp, _ll, _i, _ll, _vp])
-_emb_pos_fwd = _sig("pdt_embedding_pos_fwd", [_vp, _vp, _vp, _vp, _ll, _i, _ll, _i, _vp])
+_emb_pos_fwd = _sig("pdt_embedding_pos_fwd", [_vp, _vp, _vp, _vp, _vp, _ll, _i, _ll, _i, _vp])
 _batch_rowsum = _sig("pdt_batch_rowsum", [_vp, _vp, _i, _i, _i, _i, _i, _vp])
 _vit_asm_fwd = _sig("pdt_vit_assemble_fwd", [_vp, _vp, _vp, _vp, _i, _i, _i, _vp])
 _vit_asm_bwd = _sig("pdt_vit_assemble_bwd", [_vp, _vp, _i, _i, _i, _vp])
@@ -228,7 +228,7 @@ class _TokenPositionEmbedding(torch.autograd.Function):
         if wpe.shape[0] < s or wpe.shape[1] != d or not wte.is_contiguous() or not wpe.is_contiguous():
             raise ValueError("position table too short or of a different width")
         out = torch.empty((b, s, d), dtype=torch.bfloat16, device=wte.device)
-        _check(_emb_pos_fwd(ids_c.data_ptr(), wte.data_ptr(), wpe.data_ptr(), out.data_ptr(), ids_c.numel(), d, vocab, s,
+        _check(_emb_pos_fwd(ids_c.data_ptr(), wte.data_ptr(), wpe.data_ptr(), None, out.data_ptr(), ids_c.numel(), d, vocab, s,
                             _stream()), "embedding_pos_fwd")
         ctx.save_for_backward(ids_c)
         ctx.tables = (wte, wpe)
@@ -274,6 +274,43 @@ def _embedding_grad(ids_c, g2, buf, d: int, vocab: int) -> None:
 
 def token_position_embedding(ids, wte, wpe):
     return _TokenPositionEmbedding.apply(ids, wte, wpe)
+
+
+class _PackedEmbedding(torch.autograd.Function):
+    """``wte[ids] + wpe[positions]`` -> bf16 ``[rows, D]`` for packed sequences: rows of equal position lie anywhere, so the
+    position table's gradient is a scatter-add like the token table's."""
+
+    @staticmethod
+    def forward(ctx, ids, positions, wte, wpe):
+        ids_c = ids.to(torch.int64).contiguous()
+        vocab, d = wte.shape
+        if wpe.shape[1] != d or not wte.is_contiguous() or not wpe.is_contiguous():
+            raise ValueError("position table of a different width")
+        out = torch.empty((ids_c.numel(), d), dtype=torch.bfloat16, device=wte.device)
+        if out.numel():
+            _check(_emb_pos_fwd(ids_c.data_ptr(), wte.data_ptr(), wpe.data_ptr(), positions.data_ptr(), out.data_ptr(), ids_c.numel(), d,
+                                vocab, wpe.shape[0], _stream()), "embedding_pos_fwd")
+        ctx.save_for_backward(ids_c, positions)
+        ctx.tables = (wte, wpe)
+        return out
+
+    @staticmethod
+    def backward(ctx, g):
+        grads = []
+        g2 = _bf16c(g)
+        for need, table, ids in zip(ctx.needs_input_grad[2:], ctx.tables, ctx.saved_tensors):
+            if not need:
+                grads.append(None)
+                continue
+            buf, own = _param_grad_target(table, tuple(table.shape), g.device)
+            if ids.numel():
+                _embedding_grad(ids, g2, buf, table.shape[1], table.shape[0])
+            grads.append(None if own else buf)
+        return None, None, *grads
+
+
+def packed_embedding(ids, positions, wte, wpe):
+    return _PackedEmbedding.apply(ids, positions, wte, wpe)
 
 
 class _VitAssemble(torch.autograd.Function):

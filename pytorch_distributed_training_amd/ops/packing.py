@@ -14,12 +14,13 @@ import torch
 class SequencePack:
     """``spans``: int32 ``[rows, 2]``, first row and end of the sequence a row belongs to (0, 0 outside every sequence);
     ``positions``: int64 ``[rows]``, a row's position inside its sequence (0 outside).  ``plan``: what the attention kernels
-    read on GPU (positions, spans and the order they take the rows in, one buffer)."""
+    read on GPU (positions, spans and the order they take the rows in, one buffer).  ``longest``: length of the longest
+    sequence, ``None`` where the offsets were on the GPU."""
 
-    __slots__ = ("rows", "device", "plan", "_host")
+    __slots__ = ("rows", "device", "plan", "longest", "_host")
 
-    def __init__(self, rows: int, plan: Optional[torch.Tensor] = None, host=None):
-        self.rows, self.plan, self._host = rows, plan, host
+    def __init__(self, rows: int, plan: Optional[torch.Tensor] = None, host=None, longest: Optional[int] = None):
+        self.rows, self.plan, self._host, self.longest = rows, plan, host, longest
         self.device = plan.device if host is None else host[0].device
 
     @property
@@ -51,8 +52,10 @@ def pack_sequences(offsets, rows: int, device: Optional[torch.device] = None) ->
     rows = int(rows)
     if not 0 <= rows < 1 << 30:
         raise ValueError(f"a pack holds 0 to 2^30 - 1 rows, got {rows}")
+    longest = None
     if not offsets.is_cuda:
         _check_on_host(offsets, rows)
+        longest = int((offsets[1:] - offsets[:-1]).max()) if offsets.numel() > 1 else 0
         if device is not None:
             offsets = offsets.to(device)
     elif device is not None and torch.device(device) != offsets.device:
@@ -60,7 +63,7 @@ def pack_sequences(offsets, rows: int, device: Optional[torch.device] = None) ->
     if offsets.is_cuda:
         from . import hip_packed
 
-        return SequencePack(rows, hip_packed.pack_plan(offsets, rows))
+        return SequencePack(rows, hip_packed.pack_plan(offsets, rows), longest=longest)
     offsets = offsets.to(torch.int64)
     row = torch.arange(rows)
     at = torch.searchsorted(offsets, row, right=True) - 1  # the last sequence that starts at or before the row
@@ -68,4 +71,4 @@ def pack_sequences(offsets, rows: int, device: Optional[torch.device] = None) ->
     at = at.clamp(0, max(offsets.numel() - 2, 0))
     ends = offsets[1:] if offsets.numel() > 1 else offsets
     spans = torch.stack([offsets[at], ends[at]], 1) * inside[:, None]
-    return SequencePack(rows, host=(spans.to(torch.int32), torch.where(inside, row - spans[:, 0], 0)))
+    return SequencePack(rows, host=(spans.to(torch.int32), torch.where(inside, row - spans[:, 0], 0)), longest=longest)

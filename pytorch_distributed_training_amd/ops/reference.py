@@ -160,6 +160,10 @@ def token_position_embedding(ids, wte, wpe):
     return F.embedding(ids, wte) + wpe[:s_].unsqueeze(0)
 
 
+def packed_embedding(ids, positions, wte, wpe):
+    return F.embedding(ids, wte) + F.embedding(positions, wpe)
+
+
 def vit_assemble(tok, cls, pos):
     """``cat([cls, tok], dim=1) + pos``: class token in front of the patch tokens, position table added."""
     b = tok.shape[0]

@@ -258,3 +258,61 @@ def test_refusals(ops):
         ops.attention_packed(q, k, v, ops.pack_sequences([0, 6], 6))
     with pytest.raises(ValueError, match="offsets on"):
         ops.pack_sequences(torch.tensor([0, 6], device="cuda"), 6, device="cpu")
+
+
+def test_packed_embedding(ops):
+    g = torch.Generator("cuda").manual_seed(0)
+    wte, wpe = torch.randn(50, 64, generator=g, device="cuda"), torch.randn(20, 64, generator=g, device="cuda")
+    ids = torch.randint(0, 50, (33,), generator=g, device="cuda")
+    pack = ops.pack_sequences([0, 20, 20, 31], 33, device="cuda")
+    wte.requires_grad_(True), wpe.requires_grad_(True)
+    out = ops.token_position_embedding(ids, wte, wpe, pack)
+    assert torch.equal(out, (wte[ids] + wpe[pack.positions]).to(torch.bfloat16))  # one rounding of the fp32 sum
+    do = torch.randn(33, 64, generator=g, device="cuda").to(torch.bfloat16)
+    a, b = torch.autograd.grad(out, (wte, wpe), do)
+    ra = torch.zeros_like(wte, dtype=torch.float64).index_add_(0, ids, do.double())
+    rb = torch.zeros_like(wpe, dtype=torch.float64).index_add_(0, pack.positions, do.double())
+    # fp32 sums of at most 33 terms of magnitude below 8
+    assert float((a.double() - ra).abs().max()) < 33 * 33 * 8 * 2.0 ** -24 and float((b.double() - rb).abs().max()) < 33 * 33 * 8 * 2.0 ** -24
+    with pytest.raises(ValueError, match="exceeds"):
+        ops.token_position_embedding(ids, wte, wpe[:19], pack)
+    with pytest.raises(ValueError, match="packed tokens"):
+        ops.token_position_embedding(ids.cpu(), wte, wpe, pack)
+
+
+@pytest.mark.parametrize("with_teacher", [False, True])
+def test_gpt2_trains_on_packed_documents(ops, with_teacher):
+    """Embedding, attention, projection and loss together: the packed GPU model against the fp32 model on the CPU, with the
+    gradients left in .grad by the kernels and an optimizer step behind them."""
+    import copy
+
+    from pytorch_distributed_training_amd.models.gpt2 import gpt2_tiny
+    from pytorch_distributed_training_amd.optim import build_optimizer
+
+    torch.manual_seed(0)
+    ref = gpt2_tiny(vocab_size=2000, n_ctx=64)
+    gpu = ops.prepare_module(copy.deepcopy(ref).cuda())
+    for p in gpu.parameters():
+        p.grad = torch.zeros_like(p)
+    offsets, rows = _offsets([60, 1, 33, 64, 5]), 165
+    idx = torch.randint(0, 2000, (rows,))
+    targets = torch.roll(idx, -1)
+    targets[[o - 1 for o in offsets[1:]]] = -100
+    targets[163:] = -100
+    teacher = (torch.randn(rows, 8) * 3, torch.randint(0, 2000, (rows, 8)))
+    cpu_pack, gpu_pack = ops.pack_sequences(offsets, rows), ops.pack_sequences(offsets, rows, device="cuda")
+    if with_teacher:
+        a = ref(idx, pack=cpu_pack, teacher=teacher, temperature=2.0)
+        b = gpu(idx.cuda(), pack=gpu_pack, teacher=tuple(t.cuda() for t in teacher), temperature=2.0)
+    else:
+        a, b = ref(idx, targets, pack=cpu_pack), gpu(idx.cuda(), targets.cuda(), pack=gpu_pack)
+    a.backward(), b.backward()
+    # bf16 activations through two blocks: each rounds at 2^-8 of the value a dozen times, at random
+    assert abs(float(a) - float(b)) < 12 * 2.0 ** -8
+    for (n, x), y in zip(ref.named_parameters(), gpu.parameters()):
+        cos = torch.nn.functional.cosine_similarity(x.grad.flatten(), y.grad.cpu().flatten(), dim=0)
+        assert cos > 0.99, (n, float(cos))
+    before = [p.detach().clone() for p in gpu.parameters()]
+    build_optimizer(gpu.parameters(), "adamw", 1e-3, 0.0, 0.9).step()
+    again = gpu(idx.cuda(), targets.cuda(), pack=gpu_pack)
+    assert torch.isfinite(again) and any(not torch.equal(x, y) for x, y in zip(before, gpu.parameters()))

@@ -84,3 +84,43 @@ def test_attention_refusals():
         ops.attention_packed_qkv(torch.zeros(6, 13), pack, 2, 1)
     with pytest.raises(ValueError, match="cannot share"):
         ops.attention_packed_qkv(torch.zeros(6, 14), pack, 3, 2)
+
+
+def test_gpt2_on_packed_documents():
+    """The packed model against one forward per document: loss and every gradient."""
+    from pytorch_distributed_training_amd.models.gpt2 import gpt2_tiny
+
+    torch.manual_seed(0)
+    model = gpt2_tiny(vocab_size=97, n_ctx=32)
+    lengths = [5, 1, 32, 11]
+    docs = [torch.randint(0, 97, (n,)) for n in lengths]
+    targets = [torch.cat([d[1:], torch.tensor([-100])]) for d in docs]
+    offsets = [0, 5, 6, 38, 49]
+    pack = _pack(offsets, 51)
+    assert pack.longest == 32
+    pad = torch.zeros(2, dtype=torch.int64)
+    idx, tgt = torch.cat(docs + [pad]), torch.cat(targets + [pad - 100])
+    loss = model(idx, tgt, pack=pack)
+    loss.backward()
+    got = [p.grad.clone() for p in model.parameters()]
+    model.zero_grad()
+    count = sum(n - 1 for n in lengths)
+    total = 0.0
+    for d, t in zip(docs, targets):
+        logits = model(d[None])[0]
+        total = total + torch.nn.functional.cross_entropy(logits, t, ignore_index=-100, reduction="sum") / count
+    total.backward()
+    torch.testing.assert_close(loss, total, rtol=1e-5, atol=1e-5)
+    for a, p in zip(got, model.parameters()):
+        torch.testing.assert_close(a, p.grad, rtol=1e-4, atol=1e-5)
+    logits = model(idx, pack=pack)
+    t, ids = logits.detach().topk(4, dim=-1)
+    t = t + 1.0  # (a shift of the teacher's logits changes nothing)
+    loss = model(idx, pack=pack, teacher=(t, ids), temperature=2.0)
+    torch.testing.assert_close(loss, ops.distillation_loss(logits, t, ids, 2.0))
+    with pytest.raises(ValueError, match="exceeds"):
+        model(torch.zeros(40, dtype=torch.int64), pack=_pack([0, 40], 40))
+    with pytest.raises(ValueError, match="packed tokens"):
+        model(idx[:10], pack=pack)
+    with pytest.raises(ValueError, match="not both"):
+        model(idx, tgt, pack=pack, teacher=(t, ids))
