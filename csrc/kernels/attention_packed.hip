@@ -58,34 +58,25 @@ __device__ __forceinline__ int2 ap_queries_of(const PackedArgs& p, int row) {
     return s;
 }
 
-// bounds of a wave's / workgroup's intervals
-struct Bounds {
-    int lo, hi;          // union
-    int max_lo, min_hi;  // beyond these an element-wise mask is not needed
-};
 // The lane, opaque to the compiler: what is computed from it behind a loop is not computed (and kept in registers) before.
 __device__ __forceinline__ int ap_late(int lane) {
     asm volatile("" : "+v"(lane));
     return lane;
 }
 
-// (the partners' lanes are computed from `lane` and not shared with other shuffles: six registers that would live across
-// the kernel's main loop)
-__device__ __forceinline__ int wave_min_i(int v, int lane) {
-#pragma unroll
-    for (int o = 32; o > 0; o >>= 1) v = min(v, __builtin_amdgcn_ds_bpermute((lane ^ o) << 2, v));
-    return v;
-}
-// (rows without an interval put no bounds on the mask: whatever their lanes compute is dropped)
-__device__ __forceinline__ Bounds wave_bounds(int2 s, int lane) {
-    const bool some = s.y > s.x;
-    const int l = ap_late(lane);
-    Bounds b;
-    b.lo = __builtin_amdgcn_readfirstlane(wave_min_i(some ? s.x : INT32_MAX, l));
-    b.hi = -__builtin_amdgcn_readfirstlane(wave_min_i(some ? -s.y : 0, l));
-    b.max_lo = -__builtin_amdgcn_readfirstlane(wave_min_i(some ? -s.x : 0, l));
-    b.min_hi = __builtin_amdgcn_readfirstlane(wave_min_i(some ? s.y : INT32_MAX, l));
-    return b;
+// Bounds of a wave's intervals.  Neither end of them falls from row to row, so the first and the last row that has one give
+// all four (lanes 32 .. 63 repeat the rows of lanes 0 .. 31).  Rows without an interval put no bounds on the mask: whatever
+// their lanes compute is dropped.
+struct Bounds {
+    int lo, hi;          // union
+    int max_lo, min_hi;  // beyond these an element-wise mask is not needed
+};
+__device__ __forceinline__ Bounds wave_bounds(int2 s) {
+    const uint32_t some = static_cast<uint32_t>(__ballot(s.y > s.x));
+    if (some == 0) return {INT32_MAX, 0, 0, INT32_MAX};
+    const int first = __builtin_ctz(some), last = 31 - __builtin_clz(some);
+    return {__builtin_amdgcn_readlane(s.x, first), __builtin_amdgcn_readlane(s.y, last), __builtin_amdgcn_readlane(s.x, last),
+            __builtin_amdgcn_readlane(s.y, first)};
 }
 
 // 64 rows from row r0 (clamped to `last`, the last row that any lane wants) of a [*, row] matrix, D / 64 panels.  The
@@ -304,8 +295,14 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
     ap_unit(p, p.H, blk, h);
     const int hk = h / p.group;
     const int qw0 = blk * AT_BR + 32 * wave, qrow = qw0 + lq;
+    bf16x8 qf[4 * NP];  // B operand of S^T
+    {
+        const bf16* qp = p.q + min(qrow, p.T - 1) * p.q_row + h * p.q_head + 8 * hi;
+#pragma unroll
+        for (int ks = 0; ks < 4 * NP; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
+    }
     const int2 span = ap_keys_of(p, qrow);
-    const Bounds wb = wave_bounds(span, lane);
+    const Bounds wb = wave_bounds(span);
     if (lane == 0) {
         sB[wave] = wb.lo;
         sB[4 + wave] = wb.hi;
@@ -319,12 +316,6 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
     const TileDma dma = tile_dma_setup(wave, lane);
     const FragAddr fa = frag_addr_setup(lane);
 
-    bf16x8 qf[4 * NP];  // B operand of S^T
-    {
-        const bf16* qp = p.q + min(qrow, p.T - 1) * p.q_row + h * p.q_head + 8 * hi;
-#pragma unroll
-        for (int ks = 0; ks < 4 * NP; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
-    }
     auto issue = [&](int t, int slot) {
         ap_tile_issue<NP>(dma, kbase, p.k_row, k_lo + t * AT_T, k_hi - 1, sK + slot * TILE, wave);
         ap_tile_issue<NP>(dma, vbase, p.v_row, k_lo + t * AT_T, k_hi - 1, sV + slot * TILE, wave);
@@ -523,7 +514,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
     const int hk = h / p.group;
     const int qw0 = blk * AT_BR + 32 * wave, qrow = qw0 + lq;
     const int2 span = ap_keys_of(p, qrow);
-    const Bounds wb = wave_bounds(span, lane);
+    const Bounds wb = wave_bounds(span);
     if (lane == 0) {
         sB[wave] = wb.lo;
         sB[4 + wave] = wb.hi;
@@ -713,7 +704,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkv64_kernel(const PackedArgs p
     const int h0 = hk * p.group + split * p.group / p.splits, h1 = hk * p.group + (split + 1) * p.group / p.splits;
     const int kw0 = blk * AT_BR + 32 * wave, key = kw0 + lq;
     const int2 span = ap_queries_of(p, key);
-    const Bounds wb = wave_bounds(span, lane);
+    const Bounds wb = wave_bounds(span);
     if (lane == 0) {
         sB[wave] = wb.lo;
         sB[4 + wave] = wb.hi;
@@ -868,7 +859,7 @@ __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs 
     const int h0 = hk * p.group + split * p.group / p.splits, h1 = hk * p.group + (split + 1) * p.group / p.splits;
     const int kw0 = blk * AT_BR + 32 * pair, key = kw0 + lq;
     const int2 span = ap_queries_of(p, key);
-    const Bounds wb = wave_bounds(span, lane);
+    const Bounds wb = wave_bounds(span);
     if (lane == 0 && is_p) {
         sB[wave] = wb.lo;
         sB[4 + wave] = wb.hi;

@@ -39,13 +39,14 @@ def _heads(x: torch.Tensor) -> torch.Tensor:
     """[T, heads, D] in bf16 with unit stride along D and rows and heads on 16-byte boundaries (a view where it is one already)."""
     if x.dtype != torch.bfloat16:
         x = x.to(torch.bfloat16)
-    if x.stride(2) != 1 or x.stride(0) % 8 or x.stride(1) % 8 or not 0 < x.stride(0) < 1 << 24 or x.stride(1) <= 0 or x.data_ptr() % 16:
+    rows, heads, one = x.stride()
+    if one != 1 or rows % 8 or heads % 8 or not 0 < rows < 1 << 24 or heads <= 0 or x.data_ptr() % 16:
         x = x.clone(memory_format=torch.contiguous_format)
     return x
 
 
 def _strides(*xs):
-    vals = [s for x in xs for s in (x.stride(0), x.stride(1))]
+    vals = [s for x in xs for s in x.stride()[:2]]
     return (ctypes.c_longlong * len(vals))(*vals)
 
 
@@ -138,6 +139,9 @@ def _check_head_dim(d: int) -> None:
 
 def attention_packed(q, k, v, pack, causal: bool, scale: float):
     _check_head_dim(q.shape[2])
+    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+        with _on(q.device):
+            return _forward(_heads(q), _heads(k), _heads(v), pack.plan, causal, scale, False)[0]
     return _AttentionPacked.apply(q, k, v, pack.plan, bool(causal), scale)
 
 

@@ -46,33 +46,37 @@ def _weight(weight: torch.Tensor) -> torch.Tensor:
     return _matrix(weight.detach(), weight.shape[1])
 
 
+def _head_forward(x, weight, ids, teacher, tau: float, want_dx: bool, want_dw: bool):
+    """(loss, dx, dW), the gradients for an incoming one of 1."""
+    vocab, width = weight.shape
+    dev = x.device
+    with _on(dev):
+        x2, w = _matrix(x, width), _weight(weight)
+        n, top = ids.shape
+        chunk = n if not (want_dx or want_dw) else min(n, CHUNK_BYTES // (2 * _round_up(vocab, 64)))
+        if chunk < n:
+            chunk = min(n, max(256, chunk - chunk % 256))
+        # one chunk and a bf16 weight: the gradient is rounded once, in the product's epilogue; else it is summed in fp32
+        direct = want_dw and chunk == n and weight.dtype == torch.bfloat16
+        dx = torch.empty((n, width), dtype=torch.bfloat16, device=dev) if want_dx else None
+        dw = torch.empty((vocab, width), dtype=torch.bfloat16 if direct else torch.float32, device=dev) if want_dw else None
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        size = _head_scratch(n, top, vocab, width, chunk, int(teacher is not None), int(want_dx), int(want_dw))
+        if size < 0:
+            raise ValueError(f"the vocabulary kernels do not take {n} rows of {width} features against {vocab} entries")
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+        _check(_head(x2.data_ptr(), w.data_ptr(), ids.data_ptr(), _ptr(teacher), loss.data_ptr(), _ptr(dx), _ptr(dw) if direct else None,
+                     None if direct else _ptr(dw), scratch.data_ptr(), size, n, top, vocab, width, chunk, tau, _stream()), "head_loss")
+    return loss, dx, dw
+
+
 class _HeadLoss(torch.autograd.Function):
     """Loss of ``x W^T`` against a few targets per row.  The rows are worked off in chunks; the forward pass leaves ``dx``
     and ``dW`` for an incoming gradient of 1, the backward pass multiplies them by the incoming one (a device scalar)."""
 
     @staticmethod
     def forward(ctx, x, weight, ids, teacher, tau: float):
-        vocab, width = weight.shape
-        want_dx, want_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
-        dev = x.device
-        with _on(dev):
-            x2, w = _matrix(x, width), _weight(weight)
-            n, top = ids.shape
-            chunk = n if not (want_dx or want_dw) else min(n, CHUNK_BYTES // (2 * _round_up(vocab, 64)))
-            if chunk < n:
-                chunk = min(n, max(256, chunk - chunk % 256))
-            # one chunk and a bf16 weight: the gradient is rounded once, in the product's epilogue; else it is summed in fp32
-            direct = want_dw and chunk == n and weight.dtype == torch.bfloat16
-            dx = torch.empty((n, width), dtype=torch.bfloat16, device=dev) if want_dx else None
-            dw = torch.empty((vocab, width), dtype=torch.bfloat16 if direct else torch.float32, device=dev) if want_dw else None
-            loss = torch.empty((), dtype=torch.float32, device=dev)
-            size = _head_scratch(n, top, vocab, width, chunk, int(teacher is not None), int(want_dx), int(want_dw))
-            if size < 0:
-                raise ValueError(f"the vocabulary kernels do not take {n} rows of {width} features against {vocab} entries")
-            scratch = torch.empty(size, dtype=torch.uint8, device=dev)
-            _check(_head(x2.data_ptr(), w.data_ptr(), ids.data_ptr(), _ptr(teacher), loss.data_ptr(), _ptr(dx), _ptr(dw) if direct else None,
-                         None if direct else _ptr(dw), scratch.data_ptr(), size, n, top, vocab, width, chunk, tau, _stream()), "head_loss")
-        ctx.grads = [dx, dw]
+        loss, *ctx.grads = _head_forward(x, weight, ids, teacher, tau, *ctx.needs_input_grad[:2])
         ctx.weight, ctx.shape = weight, x.shape
         return loss
 
@@ -100,7 +104,29 @@ class _HeadLoss(torch.autograd.Function):
 
 
 def head_loss(x, weight, ids, teacher, tau: float):
+    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
+        return _head_forward(x, weight, ids, teacher, tau, False, False)[0]
     return _HeadLoss.apply(x, weight, ids, teacher, tau)
+
+
+def _distill_forward(logits, ids, teacher, tau: float, want: bool):
+    """(loss, gradient of the logits for an incoming one of 1, rows padded to whole 128 bytes)."""
+    vocab = logits.shape[-1]
+    dev = logits.device
+    with _on(dev):
+        z = logits.reshape(-1, vocab)
+        if z.dtype not in (torch.bfloat16, torch.float32):
+            z = z.to(torch.float32)
+        if z.stride(1) != 1 and vocab > 1:
+            z = z.contiguous()
+        n, top = ids.shape
+        dz = torch.empty((n, _round_up(vocab, 64)), dtype=z.dtype, device=dev) if want else None
+        loss = torch.empty((), dtype=torch.float32, device=dev)
+        size = _distill_scratch(n, top)
+        scratch = torch.empty(size, dtype=torch.uint8, device=dev)
+        _check(_distill(z.data_ptr(), _ptr(dz), ids.data_ptr(), teacher.data_ptr(), loss.data_ptr(), scratch.data_ptr(), size, n, vocab, top,
+                        z.stride(0), 0 if dz is None else dz.stride(0), tau, int(z.dtype == torch.bfloat16), _stream()), "distill")
+    return loss, dz
 
 
 class _LogitsDistill(torch.autograd.Function):
@@ -108,21 +134,8 @@ class _LogitsDistill(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, logits, ids, teacher, tau: float):
-        vocab = logits.shape[-1]
-        with _on(logits.device):
-            z = logits.reshape(-1, vocab)
-            if z.dtype not in (torch.bfloat16, torch.float32):
-                z = z.to(torch.float32)
-            if z.stride(1) != 1 and vocab > 1:
-                z = z.contiguous()
-            n, top = ids.shape
-            dz = torch.empty((n, _round_up(vocab, 64)), dtype=z.dtype, device=z.device) if ctx.needs_input_grad[0] else None
-            loss = torch.empty((), dtype=torch.float32, device=z.device)
-            size = _distill_scratch(n, top)
-            scratch = torch.empty(size, dtype=torch.uint8, device=z.device)
-            _check(_distill(z.data_ptr(), _ptr(dz), ids.data_ptr(), teacher.data_ptr(), loss.data_ptr(), scratch.data_ptr(), size, n, vocab, top,
-                            z.stride(0), 0 if dz is None else dz.stride(0), tau, int(z.dtype == torch.bfloat16), _stream()), "distill")
-        ctx.dz, ctx.shape = dz, logits.shape
+        loss, ctx.dz = _distill_forward(logits, ids, teacher, tau, True)
+        ctx.shape = logits.shape
         return loss
 
     @staticmethod
@@ -141,4 +154,6 @@ class _LogitsDistill(torch.autograd.Function):
 
 
 def logits_distill(logits, ids, teacher, tau: float):
+    if not (torch.is_grad_enabled() and logits.requires_grad):
+        return _distill_forward(logits, ids, teacher, tau, False)[0]
     return _LogitsDistill.apply(logits, ids, teacher, tau)
