@@ -2,7 +2,7 @@
 //
 //   q   : [T, H, D]   bf16   T rows: the tokens of all sequences, one sequence behind the other
 //   k, v: [T, Hk, D]  bf16   query head h reads key / value head h / (H / Hk)
-//   out : [T, H, D]   bf16   lse, delta: [H, T] fp32 (log2 units / minus rowsum(dO * O))   rest: [T, H, D] bf16, out's rounding
+//   out : [T, H, D]   bf16   lse, delta: [H, T] fp32 (log2 units / minus rowsum(dO * O))   rest: [T, H, D] 8 bits, out's rounding
 //   spans: [T] {first, end}: the sequence a row belongs to; {0, 0} for a row outside every sequence (its results are 0)
 //
 //   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i.k_j - lse_i),  j in [first, i] (causal) or [first, end)
@@ -24,7 +24,7 @@
 struct PackedArgs {
     const bf16 *q, *k, *v, *o, *dout;
     bf16 *out, *dq, *dk, *dv;
-    bf16* rest;           // [T, H, D]: what rounding took from out, written for the backward pass (nullptr: no backward pass)
+    uint8_t* rest;        // [T, H, D] e5m2, see rest_place: what rounding took from out, for the backward pass (or nullptr)
     float* lse;
     float* delta;
     float* part;          // split dK / dV: [splits][2][T][Hk][D] fp32 partial sums, or nullptr
@@ -137,6 +137,27 @@ __device__ __forceinline__ void taken(RowFrags& f) { asm volatile("" : "+v"(f.v[
 __device__ __forceinline__ void taken(TrFrags& f) { asm volatile("" : "+v"(f.lo[0]), "+v"(f.lo[1]), "+v"(f.hi[0]), "+v"(f.hi[1])); }
 __device__ __forceinline__ void taken(f32x4 (&f)[4]) { asm volatile("" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3])); }
 
+// What rounding to bf16 took from an output, 2^-9 of it at most, in 8 bits (e5m2, times 256, saturating): an eighth of it is
+// all that is lost.  The bytes of a row lie as the dQ kernel's lanes read them: element d at half d / 8 % 2, 8 (d / 16) + d % 8.
+template <int NP>
+__device__ __forceinline__ int rest_place(int d) { return ((d >> 3) & 1) * (32 * NP) + ((d >> 4) << 3) + (d & 7); }
+__device__ __forceinline__ float rest_of(float x) {
+    const float r = (x - bf16_to_f32(f32_to_bf16(x))) * 256.f;
+    return fminf(fmaxf(r, -57344.f), 57344.f);
+}
+__device__ __forceinline__ uint32_t rest_pack(float a, float b, float c, float d) {
+    const int lo = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false);
+    return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_bf8_f32(c, d, lo, true));
+}
+// sum over four elements of g[e] (o[e] + rest[e])
+__device__ __forceinline__ float rest_dot(uint32_t rest, const bf16* g, const bf16* o, float s) {
+    const f32x2 a = __builtin_amdgcn_cvt_pk_f32_bf8(static_cast<int>(rest), false), b = __builtin_amdgcn_cvt_pk_f32_bf8(static_cast<int>(rest), true);
+    const float r[4] = {a[0], a[1], b[0], b[1]};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) s = fmaf(bf16_to_f32(g[e]), fmaf(r[e], 1.f / 256.f, bf16_to_f32(o[e])), s);
+    return s;
+}
+
 // ---- one row by a whole wave (lane = element lane, lane + 64), over its own interval only
 template <int NP>
 __device__ __forceinline__ void row_forward(const PackedArgs& p, int h, int row, int lane) {
@@ -166,7 +187,8 @@ __device__ __forceinline__ void row_forward(const PackedArgs& p, int h, int row,
         const float x = o[e] / l;
         const bf16 r = f32_to_bf16(x);
         p.out[at] = r;
-        if (p.rest != nullptr) p.rest[at] = f32_to_bf16(x - bf16_to_f32(r));
+        if (p.rest != nullptr)
+            p.rest[row * p.o_row + h * (64 * NP) + rest_place<NP>(lane + 64 * e)] = static_cast<uint8_t>(rest_pack(rest_of(x), 0.f, 0.f, 0.f));
     }
     if (lane == 0) p.lse[static_cast<size_t>(h) * p.T + row] = log2f(l) + m;
 }
@@ -182,7 +204,8 @@ __device__ __forceinline__ void row_dq(const PackedArgs& p, int h, int row, int 
         const long long at = row * p.o_row + h * (64 * NP) + lane + 64 * e;
         qv[e] = bf16_to_f32(p.q[row * p.q_row + h * p.q_head + lane + 64 * e]);
         dov[e] = bf16_to_f32(p.dout[at]);
-        dl += dov[e] * (bf16_to_f32(p.o[at]) + bf16_to_f32(p.rest[at]));
+        const int rest = p.rest[row * p.o_row + h * (64 * NP) + rest_place<NP>(lane + 64 * e)];
+        dl += dov[e] * (bf16_to_f32(p.o[at]) + __builtin_amdgcn_cvt_f32_bf8(rest, 0) * (1.f / 256.f));
         dq[e] = 0.f;
     }
     dl = wave_sum(dl);
@@ -479,17 +502,25 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
     if (p.rest != nullptr) {
         // The backward pass takes dout . out as the row term of dS = P (dP - term).  Where few keys share a row P (dP - term) is
         // a small difference, and the rounding of out would be its largest error: the term is formed from out and its rest.
-        bf16* rrow0 = p.rest + qw0 * p.o_row + h * (64 * NP);
+        // A lane holds elements 4 hi .. 4 hi + 3 of every eight; swapped with the other half of the wave it has whole eights,
+        // every other one: the half of the row that lane reads again.
+        uint8_t* at = p.rest + (qw0 + (el & 31)) * p.o_row + h * (64 * NP) + (el >> 5) * (32 * NP);
+        const bool there = qw0 + (el & 31) < p.T;
 #pragma unroll
-        for (int d = 0; d < 2 * NP; ++d)
+        for (int d = 0; d < 2 * NP; ++d) {
+            u32x4 w;
 #pragma unroll
-            for (int e = 0; e < 16; ++e) {
-                const float x = o[d][e] * inv;
-                o[d][e] = x - bf16_to_f32(f32_to_bf16(x));
+            for (int r2 = 0; r2 < 2; ++r2) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] = rest_of(o[d][8 * r2 + e] * inv);
+                float even = __builtin_bit_cast(float, rest_pack(x[0], x[1], x[2], x[3])), odd = __builtin_bit_cast(float, rest_pack(x[4], x[5], x[6], x[7]));
+                swap_rows32(even, odd);
+                w[2 * r2] = __builtin_bit_cast(uint32_t, even);
+                w[2 * r2 + 1] = __builtin_bit_cast(uint32_t, odd);
             }
-#pragma unroll
-        for (int pn = 0; pn < NP; ++pn)
-            store_rows32(so, o + 2 * pn, 1.f, el, p.T - qw0, [&](int row) { return rrow0 + row * p.o_row + 64 * pn; });
+            if (there) *reinterpret_cast<u32x4*>(at + 16 * d) = w;
+        }
     }
     const unsigned long long bl = __ballot(some && !ap_finite(lt));
     bad |= static_cast<uint32_t>(bl) | static_cast<uint32_t>(bl >> 32);
@@ -545,10 +576,23 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
         for (int ks = 0; ks < 4 * NP; ++ks) {
             qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
             dof[ks] = *reinterpret_cast<const bf16x8*>(p.dout + orow + 16 * ks);
-            const bf16x8 ov = *reinterpret_cast<const bf16x8*>(p.o + orow + 16 * ks);
-            const bf16x8 rv = *reinterpret_cast<const bf16x8*>(p.rest + orow + 16 * ks);
+        }
+        const uint8_t* rest = p.rest + qc * p.o_row + h * (64 * NP) + hi * (32 * NP);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) dl += bf16_to_f32(dof[ks][e]) * (bf16_to_f32(ov[e]) + bf16_to_f32(rv[e]));
+        for (int j = 0; j < 2 * NP; ++j) {
+            const u32x4 rv = *reinterpret_cast<const u32x4*>(rest + 16 * j);
+#pragma unroll
+            for (int k = 0; k < 2; ++k) {
+                const bf16x8 ov = *reinterpret_cast<const bf16x8*>(p.o + orow + 16 * (2 * j + k));
+                bf16 g[8], o[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    g[e] = dof[2 * j + k][e];
+                    o[e] = ov[e];
+                }
+                dl = rest_dot(rv[2 * k], g, o, dl);
+                dl = rest_dot(rv[2 * k + 1], g + 4, o + 4, dl);
+            }
         }
         ndl = -other_half_sum(dl);
         const size_t off = static_cast<size_t>(h) * p.T + qc;
@@ -1161,7 +1205,7 @@ static int ap_launch(K kernel, unsigned long long& granted, unsigned grid, size_
 }
 
 // spans, order: pdt_pack_spans.  st: row and head strides of q, k, v in elements (multiples of 8; 16-byte aligned pointers); out is [T, H, D] without gaps,
-// rest (nullptr without a backward pass) like it.
+// rest (nullptr without a backward pass) has one byte for each of its elements.
 PDT_API int pdt_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, void* rest, float* lse, const void* spans, const int* order, const long long* st,
                                      int T, int H, int Hk, int D, float scale, int causal, void* stream) {
     PackedArgs a = {};
@@ -1170,7 +1214,7 @@ PDT_API int pdt_packed_attention_fwd(const void* q, const void* k, const void* v
     a.k = static_cast<const bf16*>(k);
     a.v = static_cast<const bf16*>(v);
     a.out = static_cast<bf16*>(out);
-    a.rest = static_cast<bf16*>(rest);
+    a.rest = static_cast<uint8_t*>(rest);
     a.lse = lse;
     a.q_row = st[0]; a.q_head = st[1];
     a.k_row = st[2]; a.k_head = st[3];
@@ -1204,7 +1248,7 @@ PDT_API int pdt_packed_attention_bwd(const void* q, const void* k, const void* v
     a.k = static_cast<const bf16*>(k);
     a.v = static_cast<const bf16*>(v);
     a.o = static_cast<const bf16*>(o);
-    a.rest = const_cast<bf16*>(static_cast<const bf16*>(rest));
+    a.rest = const_cast<uint8_t*>(static_cast<const uint8_t*>(rest));
     a.dout = static_cast<const bf16*>(dout);
     a.lse = const_cast<float*>(lse);
     a.delta = delta;

@@ -53,7 +53,7 @@ def _strides(*xs):
 def _forward(q, k, v, plan, causal: bool, scale: float, train: bool):
     t, h, d = q.shape
     out = torch.empty((t, h, d), dtype=torch.bfloat16, device=q.device)
-    rest = torch.empty_like(out) if train else None  # what rounding took from out: the backward pass's row terms need it
+    rest = torch.empty((t, h, d), dtype=torch.uint8, device=q.device) if train else None  # what rounding took from out: the backward pass's row terms need it
     lse = torch.empty((h, t), dtype=torch.float32, device=q.device)
     if out.numel():
         _check(_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(rest), lse.data_ptr(), plan.data_ptr() + 8 * t, plan.data_ptr() + 16 * t, _strides(q, k, v),
