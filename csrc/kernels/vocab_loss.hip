@@ -457,6 +457,7 @@ __global__ __launch_bounds__(512) void vocab_gemm_kernel(const VocabGemm p) {
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int m = mw + i * 16 + r16;
+                if (mw + i * 16 >= p.M) break;  // (few rows: most of the tile)
                 if constexpr (KIND == 0) {
                     if (nw + 64 > p.N) {  // (the last columns of the vocabulary)
 #pragma unroll
