@@ -21,6 +21,7 @@ typedef const __attribute__((address_space(1))) void vl_global_cvoid;
 #define VL_INF __builtin_inff()
 #define VL_GROUP 64   // vocabulary entries that share a maximum
 #define VL_MAX_TOP 1024
+#define VL_MAX_ROWS (1 << 22)  // a workgroup of up to 1024 threads a row, 2^32 threads a launch
 
 // A buffer far larger than the caches is written around them (measured on 8192 x 50257 bf16: the scores kernel 798 -> 757 us,
 // the pass over the rows 365 -> 311 us, distillation on logits 409 -> 379 us); a smaller one is read again from them.
@@ -938,7 +939,7 @@ static int vl_launch(const VocabGemm& g, hipStream_t s) {
 
 static bool vl_sizes_ok(int rows, int vocab, int width) {
     // byte offsets inside a tile's rows and a whole number of tiles fit 32 bits
-    return rows > 0 && vocab > 0 && vocab < (1 << 22) && width > 0 && width <= (1 << 16) && (width % 64) == 0 &&
+    return rows > 0 && rows < VL_MAX_ROWS && vocab > 0 && vocab < (1 << 22) && width > 0 && width <= (1 << 16) && (width % 64) == 0 &&
            static_cast<long long>(pdt_cdiv(rows, 256)) * pdt_cdiv(vocab, 256) < (1ll << 30) &&
            static_cast<long long>(pdt_cdiv(rows, 256)) * pdt_cdiv(width, 256) < (1ll << 30);
 }
@@ -1095,7 +1096,7 @@ static int distill_launch(const Logits<T>& a, int rows, hipStream_t s) {
 }
 
 PDT_API long long pdt_distill_scratch(int rows, int top) {
-    if (rows <= 0 || top <= 0 || top > VL_MAX_TOP) return -1;
+    if (rows <= 0 || rows >= VL_MAX_ROWS || top <= 0 || top > VL_MAX_TOP) return -1;
     Scratch m = {nullptr, 0};
     RowScratch r(m, rows, top, true);
     return static_cast<long long>(m.used);
@@ -1105,7 +1106,7 @@ PDT_API long long pdt_distill_scratch(int rows, int top) {
 // whole 16-byte chunks.
 PDT_API int pdt_distill(const void* z, void* dz, const long long* ids, const float* teacher, float* loss, void* scratch, long long scratch_bytes, int rows,
                         int vocab, int top, long long ldz, long long ldd, float tau, int dtype, void* stream) {
-    if (rows <= 0 || vocab <= 0 || vocab >= (1 << 24) || top <= 0 || top > VL_MAX_TOP || ldz < 0 || !(tau > 0.f) ||
+    if (rows <= 0 || rows >= VL_MAX_ROWS || vocab <= 0 || vocab >= (1 << 24) || top <= 0 || top > VL_MAX_TOP || ldz < 0 || !(tau > 0.f) ||
         (dz != nullptr && (ldd < (vocab + 7) / 8 * 8 || (ldd % 8) != 0)))
         return -1;
     Scratch m = {static_cast<char*>(scratch), 0};

@@ -164,8 +164,8 @@ def _check_teacher(lead, teacher_logits, teacher_ids, temperature: float, device
     if teacher_logits.requires_grad:
         raise ValueError(f"{what}: no gradient flows to the teacher; pass its logits detached")
     temperature = float(temperature)
-    if not 0.0 < temperature < math.inf:
-        raise ValueError("the temperature must be positive and finite")
+    if not 1e-6 <= temperature <= 1e6:  # (its square and its inverse are fp32 factors)
+        raise ValueError(f"a temperature between 1e-6 and 1e6, got {temperature}")
     return temperature
 
 
@@ -206,7 +206,8 @@ def linear_distillation_loss(x, weight, teacher_logits, teacher_ids, temperature
         from . import hip_vocab
 
         return hip_vocab.head_loss(x, weight, *_teacher_rows(teacher_logits, teacher_ids), tau)
-    return _ref.distillation_loss(linear(x, weight), teacher_logits, teacher_ids, tau)
+    up = torch.promote_types(x.dtype, torch.float32)
+    return _ref.distillation_loss(_ref.linear(x.to(up), weight.to(up)), teacher_logits, teacher_ids, tau)
 
 
 def _teacher_rows(teacher_logits, teacher_ids):
@@ -253,8 +254,8 @@ def _check_packed(x, pack, name: str) -> None:
 
 def _check_scale(scale: Optional[float], head_dim: int) -> float:
     scale = 1.0 / math.sqrt(head_dim) if scale is None else float(scale)
-    if not 0.0 < scale < math.inf:
-        raise ValueError("the softmax scale must be positive and finite")
+    if not 1e-30 <= scale <= 1e30:  # (an fp32 factor)
+        raise ValueError(f"a softmax scale between 1e-30 and 1e30, got {scale}")
     return scale
 
 
@@ -263,7 +264,7 @@ def attention_packed(q, k, v, pack: SequencePack, causal: bool = True, scale: Op
     ``[T, H, D]``, query head ``h`` reading head ``h // (H // Hk)``.  A row attends to the rows of its own sequence, up to
     itself if ``causal``; rows outside every sequence give 0 and get no gradient.  ``scale`` defaults to ``1 / sqrt(D)``.
     On GPU: ``D`` of 64 or 128, computed in bf16 (fp32 softmax), any strides with a contiguous last axis."""
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
+    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2] or q.shape[2] == 0:
         raise ValueError(f"expected [T, H, D], [T, Hk, D], [T, Hk, D], got {tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
     if k.shape[1] == 0 or q.shape[1] == 0 or q.shape[1] % k.shape[1]:
         raise ValueError(f"{q.shape[1]} query heads cannot share {k.shape[1]} key heads")
@@ -291,9 +292,9 @@ def attention_packed_qkv(qkv, pack: SequencePack, heads: int, kv_heads: Optional
         from . import hip_packed
 
         return hip_packed.attention_packed_qkv(qkv, pack, heads, kv_heads, causal, scale)
-    x = qkv.view(qkv.shape[0], heads + 2 * kv_heads, -1)
+    x = qkv.reshape(qkv.shape[0], heads + 2 * kv_heads, qkv.shape[1] // (heads + 2 * kv_heads))
     out = _ref.attention_packed(x[:, :heads], x[:, heads:heads + kv_heads], x[:, heads + kv_heads:], pack.spans, causal, scale)
-    return out.reshape(qkv.shape[0], -1)
+    return out.flatten(1)
 
 
 def embedding(ids, weight):
@@ -304,10 +305,18 @@ def embedding(ids, weight):
 
 def token_position_embedding(ids, wte, wpe, pack: Optional[SequencePack] = None):
     """Input embedding of a language model: ``wte[ids] + wpe[position]`` for ``ids`` of shape ``[B, S]``, or of shape
-    ``[rows]`` with ``pack``, where positions count from the start of each sequence (and are 0 outside)."""
+    ``[rows]`` with ``pack``, where positions count from the start of each sequence (and are 0 outside).  A sequence longer
+    than the table is refused where the pack knows its lengths; of one made from offsets on the GPU the tokens behind the
+    table's end take its last row."""
     if pack is not None:
+        if not isinstance(pack, SequencePack):
+            raise TypeError("pack: a SequencePack, made by ops.pack_sequences")
         if ids.dim() != 1 or ids.shape[0] != pack.rows or ids.device != pack.device:
             raise ValueError(f"packed tokens of shape ({pack.rows},) on {pack.device} expected, got {tuple(ids.shape)} on {ids.device}")
+        if ids.dtype not in (torch.int64, torch.int32):
+            raise TypeError("packed tokens must be int64 or int32")
+        if wte.device != ids.device or wpe.device != ids.device:
+            raise ValueError(f"tokens on {ids.device}, tables on {wte.device} and {wpe.device}")
         if pack.longest is not None and pack.longest > wpe.shape[0]:
             raise ValueError(f"a sequence of {pack.longest} tokens exceeds the {wpe.shape[0]} positions of the table")
     if wte.is_cuda:

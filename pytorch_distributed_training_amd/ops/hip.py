@@ -16,6 +16,7 @@ Role parity: the ATen/cuDNN/cuBLAS kernels implicitly launched by
 
 from __future__ import annotations
 
+import contextlib as _contextlib
 import ctypes
 import math
 import os as _os
@@ -105,6 +106,11 @@ def _stream() -> int:
     if _raw_stream is not None:
         return _raw_stream(torch.cuda.current_device())
     return torch.cuda.current_stream().cuda_stream
+
+
+def _on(device: torch.device):
+    """The device a kernel is launched on, made current where it is not."""
+    return _contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
 
 
 def _ptr(t: Optional[torch.Tensor]):

@@ -9,9 +9,8 @@ import ctypes
 
 import torch
 
-from .hip import _check, _ptr, _stream
+from .hip import _check, _on, _ptr, _stream
 from .hip_transformer import _f, _i, _sig, _vp
-from .hip_vocab import _on
 
 _pack_spans = _sig("pdt_pack_spans", [_vp, _i, _i] + [_vp] * 5)
 _fwd = _sig("pdt_packed_attention_fwd", [_vp] * 9 + [_i] * 4 + [_f, _i, _vp])
@@ -25,6 +24,8 @@ BLOCK_ROWS = 128  # rows of a workgroup
 def pack_plan(offsets, rows: int):
     """One int64 buffer: ``rows`` positions, ``rows`` spans (two int32), three orders of the blocks and as much scratch."""
     with _on(offsets.device):
+        if offsets.dtype == torch.int64:
+            offsets = offsets.clamp(-1, rows)  # (what lies beyond is cut off, and must not wrap around in 32 bits)
         offsets = offsets.to(torch.int32).contiguous()
         blocks = -(-rows // BLOCK_ROWS)
         plan = torch.empty(2 * rows + 3 * blocks, dtype=torch.int64, device=offsets.device)
@@ -118,7 +119,7 @@ class _AttentionPackedQKV(torch.autograd.Function):
             out, rest, lse = _forward(*_split_qkv(qkv, heads, kv_heads), plan, causal, scale, ctx.needs_input_grad[0])
         ctx.save_for_backward(qkv, out, rest, lse, plan)
         ctx.meta = (heads, kv_heads, causal, scale)
-        return out.view(qkv.shape[0], -1)
+        return out.flatten(1)
 
     @staticmethod
     @torch.autograd.function.once_differentiable

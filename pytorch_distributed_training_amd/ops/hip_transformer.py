@@ -13,7 +13,7 @@ from typing import Optional
 
 import torch
 
-from .hip import _check, _colsum, _grad_sink, _lib, _ptr, _stream
+from .hip import _check, _colsum, _grad_sink, _lib, _on, _ptr, _stream
 
 _vp, _i, _f, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
 
@@ -286,10 +286,13 @@ class _PackedEmbedding(torch.autograd.Function):
         vocab, d = wte.shape
         if wpe.shape[1] != d or not wte.is_contiguous() or not wpe.is_contiguous():
             raise ValueError("position table of a different width")
+        if wte.dtype != torch.float32 or wpe.dtype != torch.float32:
+            raise TypeError("token and position tables must be float32")
         out = torch.empty((ids_c.numel(), d), dtype=torch.bfloat16, device=wte.device)
         if out.numel():
-            _check(_emb_pos_fwd(ids_c.data_ptr(), wte.data_ptr(), wpe.data_ptr(), positions.data_ptr(), out.data_ptr(), ids_c.numel(), d,
-                                vocab, wpe.shape[0], _stream()), "embedding_pos_fwd")
+            with _on(wte.device):
+                _check(_emb_pos_fwd(ids_c.data_ptr(), wte.data_ptr(), wpe.data_ptr(), positions.data_ptr(), out.data_ptr(), ids_c.numel(), d,
+                                    vocab, wpe.shape[0], _stream()), "embedding_pos_fwd")
         ctx.save_for_backward(ids_c, positions)
         ctx.tables = (wte, wpe)
         return out
@@ -304,7 +307,8 @@ class _PackedEmbedding(torch.autograd.Function):
                 continue
             buf, own = _param_grad_target(table, tuple(table.shape), g.device)
             if ids.numel():
-                _embedding_grad(ids, g2, buf, table.shape[1], table.shape[0])
+                with _on(g.device):
+                    _embedding_grad(ids, g2, buf, table.shape[1], table.shape[0])
             grads.append(None if own else buf)
         return None, None, *grads
 

@@ -6,12 +6,11 @@ Role parity: nn.CrossEntropyLoss at /root/reference/src/main.py:62,76,78 (on a c
 
 from __future__ import annotations
 
-import contextlib
 import os
 
 import torch
 
-from .hip import SHADOWS, _axpy_dev, _check, _grad_sink, _ptr, _round_up, _scale_by_scalar, _stream
+from .hip import SHADOWS, _axpy_dev, _check, _grad_sink, _on, _ptr, _round_up, _scale_by_scalar, _stream
 from .hip_transformer import _f, _i, _ll, _sig, _vp
 
 _head_scratch = _sig("pdt_head_loss_scratch", [_i] * 8)
@@ -23,11 +22,12 @@ _distill = _sig("pdt_distill", [_vp] * 6 + [_ll] + [_i] * 3 + [_ll, _ll, _f, _i,
 
 # Rows worked off at a time: their exponentials (2 bytes per row and vocabulary entry) are the one large buffer.
 CHUNK_BYTES = int(os.environ.get("PDT_VOCAB_CHUNK_MB", "8192")) << 20
+MAX_ROWS = 1 << 22  # rows of a call stay below (a workgroup of up to 1024 threads each, 2^32 threads in a launch)
 
 
-def _on(device):
-    """The device a kernel is launched on, made current where it is not."""
-    return contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)
+def _check_rows(n: int) -> None:
+    if n >= MAX_ROWS:
+        raise ValueError(f"the vocabulary losses take fewer than {MAX_ROWS} rows at a time, got {n}")
 
 
 def _matrix(x: torch.Tensor, width: int) -> torch.Tensor:
@@ -53,6 +53,7 @@ def _head_forward(x, weight, ids, teacher, tau: float, want_dx: bool, want_dw: b
     with _on(dev):
         x2, w = _matrix(x, width), _weight(weight)
         n, top = ids.shape
+        _check_rows(n)
         chunk = n if not (want_dx or want_dw) else min(n, CHUNK_BYTES // (2 * _round_up(vocab, 64)))
         if chunk < n:
             chunk = min(n, max(256, chunk - chunk % 256))
@@ -120,6 +121,7 @@ def _distill_forward(logits, ids, teacher, tau: float, want: bool):
         if z.stride(1) != 1 and vocab > 1:
             z = z.contiguous()
         n, top = ids.shape
+        _check_rows(n)
         dz = torch.empty((n, _round_up(vocab, 64)), dtype=z.dtype, device=dev) if want else None
         loss = torch.empty((), dtype=torch.float32, device=dev)
         size = _distill_scratch(n, top)

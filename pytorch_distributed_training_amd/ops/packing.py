@@ -46,7 +46,7 @@ def pack_sequences(offsets, rows: int, device: Optional[torch.device] = None) ->
     and behind the last belong to none.  Offsets on the host are checked and sent to ``device``; offsets on the GPU are not
     read back (no synchronisation): they must not fall, and what reaches beyond ``rows`` is cut off."""
     if not isinstance(offsets, torch.Tensor):
-        offsets = torch.tensor(offsets, dtype=torch.int64)
+        offsets = torch.tensor(offsets)
     if offsets.dim() != 1 or offsets.numel() < 1 or offsets.dtype not in (torch.int32, torch.int64):
         raise ValueError("sequence offsets are a one-dimensional int32 or int64 tensor of at least one element")
     rows = int(rows)
@@ -58,7 +58,7 @@ def pack_sequences(offsets, rows: int, device: Optional[torch.device] = None) ->
         longest = int((offsets[1:] - offsets[:-1]).max()) if offsets.numel() > 1 else 0
         if device is not None:
             offsets = offsets.to(device)
-    elif device is not None and torch.device(device) != offsets.device:
+    elif device is not None and torch.device(device) not in (offsets.device, torch.device(offsets.device.type)):
         raise ValueError(f"sequence offsets on {offsets.device}, pack wanted on {device}")
     if offsets.is_cuda:
         from . import hip_packed

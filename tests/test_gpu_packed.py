@@ -316,3 +316,104 @@ def test_gpt2_trains_on_packed_documents(ops, with_teacher):
     build_optimizer(gpu.parameters(), "adamw", 1e-3, 0.0, 0.9).step()
     again = gpu(idx.cuda(), targets.cuda(), pack=gpu_pack)
     assert torch.isfinite(again) and any(not torch.equal(x, y) for x, y in zip(before, gpu.parameters()))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_offsets_of_64_bits_and_rows_far_apart(ops, d):
+    """Row strides that carry the last rows past 2^32 bytes and 2^31 elements; 64-bit offsets past 2^32 are cut off."""
+    t, h, hk = 300, 2, 1
+    q, k, v, do = _inputs(t, h, hk, d, seed=11)
+    room = torch.empty(t, 1 << 23, dtype=torch.bfloat16, device="cuda")
+    far = []
+    for i, x in enumerate((q, k, v)):
+        at = room[:, 1024 * i:1024 * i + x.shape[1] * d].unflatten(1, (x.shape[1], d))
+        far.append(at.copy_(x).detach().requires_grad_(True))
+    assert far[0].stride(0) * (t - 1) > 1 << 31
+    pack = ops.pack_sequences(torch.tensor([0, 100, (1 << 32) + 5], device="cuda"), t)
+    same = ops.pack_sequences([0, 100, t], t, device="cuda")
+    assert torch.equal(pack.spans, same.spans)
+    near = [x.requires_grad_(True) for x in (q, k, v)]
+    a, b = ops.attention_packed(*far, pack), ops.attention_packed(*near, same)
+    assert torch.equal(a, b)
+    for x, y in zip(torch.autograd.grad(a, far, do), torch.autograd.grad(b, near, do)):
+        assert torch.equal(x, y)
+
+
+def test_no_rows_no_sequences_and_some_gradients(ops):
+    q, k, v, do = _inputs(70, 4, 2, 64)
+    none = ops.pack_sequences(torch.zeros(1, dtype=torch.int64, device="cuda"), 70)
+    out = ops.attention_packed(q.requires_grad_(True), k, v, none)
+    (dq,) = torch.autograd.grad(out, q, do)
+    assert out.abs().max() == 0 and dq.abs().max() == 0
+    nothing = ops.pack_sequences([0, 0], 0, device="cuda")
+    empty = [x[:0].detach().requires_grad_(True) for x in (q, k, v)]
+    out = ops.attention_packed(*empty, nothing)
+    assert out.shape == (0, 4, 64) and all(g.shape == x.shape for g, x in zip(torch.autograd.grad(out.sum(), empty), empty))
+    assert ops.attention_packed_qkv(torch.zeros(0, 8 * 64, device="cuda"), nothing, 4, 2).shape == (0, 256)
+    pack = ops.pack_sequences([0, 33, 70], 70, device="cuda")
+    q, k, v = (x.detach().requires_grad_(True) for x in (q, k, v))
+    every = torch.autograd.grad(ops.attention_packed(q, k, v, pack), (q, k, v), do)
+    for i, name in enumerate("qkv"):
+        leaf = (q, k, v)[i]
+        (one,) = torch.autograd.grad(ops.attention_packed(*(x if x is leaf else x.detach() for x in (q, k, v)), pack), leaf, do)
+        assert torch.equal(one, every[i]), name
+    # keys and values given as one head expanded over the key heads
+    k1, v1 = (x.detach()[:, :1].expand(-1, 2, -1).requires_grad_(True) for x in (k, v))
+    a = ops.attention_packed(q, k1, v1, pack)
+    b = ops.attention_packed(q, k1.detach().contiguous(), v1.detach().contiguous(), pack)
+    assert torch.equal(a, b)
+    # the first pass' graph used twice
+    out = ops.attention_packed(q, k, v, pack)
+    once, twice = torch.autograd.grad(out, (q, k, v), do, retain_graph=True), torch.autograd.grad(out, (q, k, v), do)
+    assert all(torch.equal(x, y) for x, y in zip(once, twice))
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+def test_other_input_types(ops, dtype):
+    q, k, v, do = (x.to(torch.float16).to(torch.bfloat16) for x in _inputs(40, 2, 1, 128, seed=3))  # (values that every type holds)
+    pack = ops.pack_sequences([0, 40], 40, device="cuda")
+    other = [x.to(dtype).requires_grad_(True) for x in (q, k, v)]
+    own = [x.requires_grad_(True) for x in (q, k, v)]
+    a, b = ops.attention_packed(*other, pack), ops.attention_packed(*own, pack)
+    assert a.dtype == torch.bfloat16 and torch.equal(a, b)
+    for x, y in zip(torch.autograd.grad(a, other, do), torch.autograd.grad(b, own, do)):
+        assert x.dtype == dtype and torch.equal(x, y.to(dtype))
+
+
+def test_two_streams_at_once_with_one_pack(ops):
+    t = 3000
+    pack = ops.pack_sequences([0, 900, 901, 2990], t, device="cuda")
+    sets = [[x.requires_grad_(i < 3) for i, x in enumerate(_inputs(t, 8, 2, d, seed=d))] for d in (64, 128)]
+
+    def run(s):
+        out = ops.attention_packed(*s[:3], pack)
+        return (out.detach(), *torch.autograd.grad(out, s[:3], s[3]))
+
+    want = [run(s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(sets[i]))
+    torch.cuda.synchronize()
+    for w, g in zip(want, got):
+        for each in g:
+            assert all(torch.equal(x, y) for x, y in zip(w, each))
+
+
+def test_pack_devices_and_embedding_refusals(ops):
+    offsets = torch.tensor([0, 6], device="cuda")
+    pack = ops.pack_sequences(offsets, 6, device="cuda")  # any index
+    assert pack.device == offsets.device
+    table = torch.zeros(10, 64, device="cuda")
+    ids = torch.zeros(6, dtype=torch.int64, device="cuda")
+    with pytest.raises(ValueError, match="tables on"):
+        ops.token_position_embedding(ids.cpu(), table, table, ops.pack_sequences([0, 6], 6))
+    with pytest.raises(TypeError, match="float32"):
+        ops.token_position_embedding(ids, table.to(torch.bfloat16), table, pack)
+    long = ops.pack_sequences(torch.tensor([0, 12], device="cuda"), 12)  # lengths unknown on the host: the table's last row
+    wpe = torch.arange(10.0, device="cuda")[:, None].repeat(1, 64)
+    got = ops.token_position_embedding(torch.zeros(12, dtype=torch.int64, device="cuda"), table, wpe, long)
+    assert got[:, 0].tolist() == [0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 9, 9]

@@ -298,3 +298,156 @@ def test_refusals(ops):
         ops.linear_cross_entropy(x, wt, y.cpu())
     with pytest.raises(ValueError, match="teacher ids on"):
         ops.distillation_loss(x, torch.zeros(4, 2), torch.zeros(4, 2, dtype=torch.int64))
+
+
+def _sampled_check(got, x, w, labels, cols, scale_sum):
+    """A cross-entropy whose matrices are too large for 64 bits at once: every row's loss and dx in pieces of rows, dW at
+    some vocabulary entries.  Bounds as in _head_check, with the scores' error from the largest absolute sum."""
+    n, v = x.shape[0], w.shape[0]
+    ok = (labels >= 0) & (labels < v)
+    count = max(int(ok.sum()), 1)
+    s = x.shape[1] * 2.0 ** -24 * scale_sum + 2e-5
+    loss = torch.zeros((), dtype=torch.float64, device="cuda")
+    wc = w[cols].double()
+    dw, dwe = torch.zeros_like(wc), torch.zeros_like(wc)
+    for r in range(0, n, 512):
+        xs, ys, oks = x[r:r + 512].double(), labels[r:r + 512], ok[r:r + 512]
+        lse = torch.full((xs.shape[0],), -math.inf, dtype=torch.float64, device="cuda")
+        for c in range(0, v, 1 << 18):
+            lse = torch.logaddexp(lse, torch.logsumexp(xs @ w[c:c + (1 << 18)].double().t(), 1))
+        zy = (xs * w[ys.clamp(0, v - 1)].double()).sum(1)
+        loss += torch.where(oks, lse - zy, 0.0).sum() / count
+        q = torch.exp(xs @ wc.t() - lse[:, None]) * oks[:, None] / count
+        dz = q - ((cols[None] == ys[:, None]) & oks[:, None]).double() / count
+        dw += dz.t() @ xs
+        dwe += (H * q + H * dz.abs() + s * q).t() @ xs.abs()
+    assert abs(float(got[0]) - float(loss)) <= s * (1 + float(loss)) + s
+    over = (got[2][cols].double() - dw).abs() - 1.05 * (dwe + H * dw.abs() + 1e-30)
+    assert float(over.max()) <= 0, f"dw: {float(over.max()):.3g} over its bound"
+    return ok
+
+
+def test_exponentials_past_32_bits(ops):
+    """34 000 rows of 65 537 exponentials (4.5 GB) in one piece."""
+    n, v, w = 34000, 65537, 64
+    x, wt = _head(n, v, w)
+    y = _labels(n, v)
+    x.requires_grad_(True), wt.requires_grad_(True)
+    loss = ops.linear_cross_entropy(x, wt, y)
+    dx, dw = torch.autograd.grad(loss, (x, wt))
+    cols = torch.cat([torch.arange(0, 40, device="cuda"), y[(y >= 0) & (y < v)][-60:], torch.arange(v - 40, v, device="cuda")])
+    big = float(x.detach().double().abs().sum(1).max()) * float(wt.detach().abs().max())
+    ok = _sampled_check((loss.detach(), dx, dw), x.detach(), wt.detach(), y, cols, big)
+    # the last rows again by themselves: their share of the whole mean
+    last = slice(n - 300, n)
+    xs = x.detach()[last].clone().requires_grad_(True)
+    (dl,) = torch.autograd.grad(ops.linear_cross_entropy(xs, wt.detach(), y[last]), xs)
+    share = int(ok[last].sum()) / int(ok.sum())
+    a, b = dx[last].double(), dl.double() * share
+    # either side: sum_v (h q + h |q - p|) |W| / rows <= 3 h max |W| / rows, and the result's own rounding
+    bound = 2 * (3 * H * float(wt.detach().abs().max()) / int(ok.sum()) + H * float(b.abs().max()))
+    assert float((a - b).abs().max()) <= 1.05 * bound
+
+
+def test_weights_past_32_bits(ops):
+    """A vocabulary of 1.1 million entries (4.6 GB of weights), most of a row's blocks empty."""
+    n, v, w = 3, 1_100_003, 2112
+    g = _gen(0)
+    x = torch.randn(n, w, generator=g, device="cuda").to(torch.bfloat16).requires_grad_(True)
+    wt = torch.empty(v, w, dtype=torch.bfloat16, device="cuda").normal_(0, 0.03, generator=g).requires_grad_(True)
+    y = torch.tensor([v - 1, 5, -100], device="cuda")
+    loss = ops.linear_cross_entropy(x, wt, y)
+    dx, dw = torch.autograd.grad(loss, (x, wt))
+    cols = torch.cat([torch.arange(0, 50, device="cuda"), torch.arange(v - 50, v, device="cuda")])
+    big = float(x.detach().double().abs().sum(1).max()) * float(wt.detach().abs().max())
+    _sampled_check((loss.detach(), dx, dw), x.detach(), wt.detach(), y, cols, big)
+    assert dx[2].abs().max() == 0 and bool(torch.isfinite(dx).all())
+
+
+@pytest.mark.parametrize("k", [1023, 1024])
+def test_as_many_targets_as_there_may_be(ops, k):
+    n, v, w = 9, 700, 64  # more targets than entries: every row repeats some
+    x, wt = _head(n, v, w)
+    t, ids = _teacher(n, v, k)
+    x.requires_grad_(True), wt.requires_grad_(True)
+    loss = ops.linear_distillation_loss(x, wt, t, ids, 2.0)
+    _head_check((loss.detach(), *torch.autograd.grad(loss, (x, wt))), x.detach(), wt.detach(), None, (t, ids), 2.0)
+
+
+@pytest.mark.parametrize("dtype", [torch.float16, torch.float64])
+def test_other_input_types(ops, dtype):
+    n, v, w = 20, 300, 64
+    x, wt = (a.to(torch.float16).to(torch.bfloat16) for a in _head(n, v, w))  # (values that every type holds)
+    y, (t, ids) = _labels(n, v), _teacher(n, v, 5)
+    xo, wo = x.to(dtype).requires_grad_(True), wt.to(dtype).requires_grad_(True)
+    xb, wb = x.requires_grad_(True), wt.requires_grad_(True)
+    a, b = ops.linear_cross_entropy(xo, wo, y.to(torch.int32)), ops.linear_cross_entropy(xb, wb, y)
+    assert torch.equal(a, b)
+    for p, r in zip(torch.autograd.grad(a, (xo, wo)), torch.autograd.grad(b, (xb, wb))):
+        # (rounded to bf16 here, h; to the finer type there, 2^-11, 2^-25 where fp16 is subnormal)
+        assert p.dtype == dtype and bool(((p.double() - r.double()).abs() <= 1.2 * H * r.double().abs() + 2.0 ** -24).all())
+    z = torch.randn(n, v, generator=_gen(9), device="cuda").to(torch.float16).to(dtype).requires_grad_(True)
+    zf = z.detach().float().requires_grad_(True)
+    a, b = ops.distillation_loss(z, t.to(dtype), ids.to(torch.int32), 2.0), ops.distillation_loss(zf, t.to(dtype).float(), ids, 2.0)
+    assert torch.equal(a, b)
+    (p,), (r,) = torch.autograd.grad(a, z), torch.autograd.grad(b, zf)
+    assert p.dtype == dtype and torch.equal(p, r.to(dtype))
+
+
+def test_some_gradients_no_rows_and_views(ops):
+    n, v, w = 130, 1000, 64
+    x, wt = _head(n, v, w)
+    y, (t, ids) = _labels(n, v), _teacher(n, v, 5)
+    x.requires_grad_(True), wt.requires_grad_(True)
+    for f in (lambda a, b: ops.linear_cross_entropy(a, b, y), lambda a, b: ops.linear_distillation_loss(a, b, t, ids, 2.0)):
+        both = torch.autograd.grad(f(x, wt), (x, wt))
+        assert torch.equal(torch.autograd.grad(f(x, wt.detach()), x)[0], both[0])
+        assert torch.equal(torch.autograd.grad(f(x.detach(), wt), wt)[0], both[1])
+        with torch.no_grad():
+            assert torch.equal(f(x, wt), f(x.t().contiguous().t(), wt.t().contiguous().t()))
+    for loss in (ops.linear_cross_entropy(x[:0], wt, y[:0]), ops.linear_distillation_loss(x[:0], wt, t[:0], ids[:0])):
+        dx, dw = torch.autograd.grad(loss, (x, wt))
+        assert float(loss) == 0 and dx.abs().max() == 0 and dw.abs().max() == 0
+    # logits as a view with gaps, as one row for all, and in three axes with an odd width
+    z = torch.randn(6, 7, 331, generator=_gen(4), device="cuda")
+    t3, i3 = t[:42].reshape(6, 7, 5), ids[:42].reshape(6, 7, 5) % 101
+    view = z[:, :, 230:331].requires_grad_(True)
+    copy = view.detach().clone().requires_grad_(True)
+    a, b = ops.distillation_loss(view, t3, i3), ops.distillation_loss(copy, t3, i3)
+    assert torch.equal(a, b) and torch.equal(torch.autograd.grad(a, view)[0], torch.autograd.grad(b, copy)[0])
+    row = z[0, :1, :101]
+    a, b = ops.distillation_loss(row.expand(42, 101), t[:42], i3.reshape(42, 5)), ops.distillation_loss(row.repeat(42, 1), t[:42], i3.reshape(42, 5))
+    assert torch.equal(a, b)
+
+
+def test_two_streams_at_once(ops):
+    sets = [(_head(1500, 5003, 128, s), _labels(1500, 5003, s), _teacher(1500, 5003, 16, s)) for s in (0, 1)]
+    for (x, wt), _, _ in sets:
+        x.requires_grad_(True), wt.requires_grad_(True)
+
+    def run(s):
+        (x, wt), y, teacher = s
+        a, b = ops.linear_cross_entropy(x, wt, y), ops.linear_distillation_loss(x, wt, *teacher, 2.0)
+        return (a.detach(), *torch.autograd.grad(a, (x, wt)), b.detach(), *torch.autograd.grad(b, (x, wt)))
+
+    want = [run(s) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    got = [[], []]
+    for _ in range(3):
+        for i, s in enumerate(streams):
+            with torch.cuda.stream(s):
+                got[i].append(run(sets[i]))
+    torch.cuda.synchronize()
+    for a, g in zip(want, got):
+        for each in g:
+            assert all(torch.equal(p, r) for p, r in zip(a, each))
+
+
+def test_too_many_rows_are_refused(ops):
+    n = 1 << 22
+    ids = torch.zeros(n, 1, dtype=torch.int32, device="cuda")
+    with pytest.raises(ValueError, match="rows at a time"):
+        ops.distillation_loss(torch.zeros(n, 1, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, 1, device="cuda"), ids)
+    with pytest.raises(ValueError, match="rows at a time"):
+        ops.linear_cross_entropy(torch.zeros(1, 64, dtype=torch.bfloat16, device="cuda").expand(n, 64), torch.zeros(5, 64, dtype=torch.bfloat16, device="cuda"), ids[:, 0])

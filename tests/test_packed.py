@@ -124,3 +124,37 @@ def test_gpt2_on_packed_documents():
         model(idx[:10], pack=pack)
     with pytest.raises(ValueError, match="not both"):
         model(idx, tgt, pack=pack, teacher=(t, ids))
+
+
+def test_lists_of_floats_are_refused_and_offsets_of_arrays_taken():
+    import numpy as np
+
+    for bad in ([0.0, 4.5], [], [[0, 4]]):
+        with pytest.raises(ValueError, match="offsets"):
+            ops.pack_sequences(bad, 8)
+    assert torch.equal(ops.pack_sequences(np.array([0, 3, 8]), 8).spans, _pack([0, 3, 8], 8).spans)
+
+
+def test_joint_projection_of_other_strides_and_of_no_rows():
+    pack = _pack([0, 4, 6], 6)
+    a = torch.randn(6, 32, dtype=torch.float64)
+    b = torch.randn(32, 6, dtype=torch.float64).t().copy_(a)
+    assert torch.equal(ops.attention_packed_qkv(a, pack, 2, 1), ops.attention_packed_qkv(b, pack, 2, 1))
+    assert ops.attention_packed_qkv(a[:0], _pack([0], 0), 2, 1).shape == (0, 16)
+
+
+def test_sizes_and_factors_out_of_range():
+    q, k, v = _qkv(6, 4, 2, 8)
+    pack = _pack([0, 6], 6)
+    with pytest.raises(ValueError, match="expected"):
+        ops.attention_packed(q[..., :0], k[..., :0], v[..., :0], pack)
+    for scale in (1e-31, 1e39):
+        with pytest.raises(ValueError, match="scale"):
+            ops.attention_packed(q, k, v, pack, scale=scale)
+    ids, table = torch.zeros(6, dtype=torch.int64), torch.zeros(10, 8)
+    with pytest.raises(TypeError, match="SequencePack"):
+        ops.token_position_embedding(ids, table, table, torch.tensor([0, 6]))
+    with pytest.raises(TypeError, match="int64"):
+        ops.token_position_embedding(ids.float(), table, table, pack)
+    with pytest.raises(ValueError, match="tables on"):
+        ops.token_position_embedding(ids, table.to("meta"), table, pack)

@@ -98,3 +98,20 @@ def test_refusals():
         ops.distillation_loss(x, t.requires_grad_(True), ids)
     with pytest.raises(TypeError, match="int64"):
         ops.distillation_loss(x, t.detach(), ids.float())
+
+
+def test_temperatures_out_of_range():
+    x, t, ids = torch.zeros(3, 8), torch.zeros(3, 2), torch.zeros(3, 2, dtype=torch.int64)
+    for bad in (1e-7, 1e7):
+        with pytest.raises(ValueError, match="temperature"):
+            ops.distillation_loss(x, t, ids, bad)
+
+
+def test_head_distillation_is_the_loss_on_the_projection_in_mixed_types_and_without_rows():
+    x, w = _r(4, 6).to(torch.bfloat16), _r(9, 6, seed=1).float().requires_grad_(True)
+    t, ids = _r(4, 3, seed=2), torch.tensor([[0, 8, 3]] * 4)
+    a = ops.linear_distillation_loss(x, w, t, ids, 2.0)
+    assert abs(float(a) - float(ops.distillation_loss(x.double() @ w.double().t(), t, ids, 2.0))) < 1e-5
+    none = ops.linear_distillation_loss(x[:0], w, t[:0], ids[:0])
+    none.backward()
+    assert float(none) == 0 and w.grad.abs().max() == 0
