@@ -2,7 +2,7 @@
 //
 //   q   : [T, H, D]   bf16   T rows: the tokens of all sequences, one sequence behind the other
 //   k, v: [T, Hk, D]  bf16   query head h reads key / value head h / (H / Hk)
-//   out : [T, H, D]   bf16   lse, delta: [H, T] fp32 (log2 units / minus rowsum(dO * O))   rest: [T, H, D] 8 bits, out's rounding
+//   out : [T, H, D]   bf16   lse, delta: [H, T] fp32, minus log-sum-exp in units of q.k / minus rowsum(dO * O)   rest: [T, H, D] 8 bits, out's rounding
 //   spans: [T] {first, end}: the sequence a row belongs to; {0, 0} for a row outside every sequence (its results are 0)
 //
 //   o_i = sum_j p_ij v_j,  p_ij = exp(scale q_i.k_j - lse_i),  j in [first, i] (causal) or [first, end)
@@ -25,16 +25,17 @@ struct PackedArgs {
     const bf16 *q, *k, *v, *o, *dout;
     bf16 *out, *dq, *dk, *dv;
     uint8_t* rest;        // [T, H, D] e5m2, see rest_place: what rounding took from out, for the backward pass (or nullptr)
-    float* lse;
+    float* lse;           // (both negated: they are what the products' accumulators start from)
     float* delta;
     float* part;          // split dK / dV: [splits][2][T][Hk][D] fp32 partial sums, or nullptr
     const int2* spans;
-    const int* order;     // [nblk]: blocks of 128 rows, the ones with the most tiles first
+    const int4* order;    // [nblk] {block of 128 rows, first and end of the rows it streams}, the ones with the most tiles first
     long long q_row, k_row, v_row, o_row, dq_row, dk_row, dv_row;   // elements between rows ...
     long long q_head, k_head, v_head, dq_head, dk_head, dv_head;    // ... and between heads (o, dout, out: o_row, D)
     int T, H, Hk, group;
     int causal, nblk, splits;
     float scale_log2, scale;
+    float unscale;        // 1 / scale_log2
 };
 
 #define AP_INF __builtin_inff()
@@ -71,11 +72,11 @@ struct Bounds {
     int lo, hi;          // union
     int max_lo, min_hi;  // beyond these an element-wise mask is not needed
 };
-__device__ __forceinline__ Bounds wave_bounds(int2 s) {
+__device__ __forceinline__ Bounds wave_bounds(int2 s, int from, int to) {  // [from, to): the block's, known to hold them where offsets do not fall
     const uint32_t some = static_cast<uint32_t>(__ballot(s.y > s.x));
     if (some == 0) return {INT32_MAX, 0, 0, INT32_MAX};
     const int first = __builtin_ctz(some), last = 31 - __builtin_clz(some);
-    return {__builtin_amdgcn_readlane(s.x, first), __builtin_amdgcn_readlane(s.y, last), __builtin_amdgcn_readlane(s.x, last),
+    return {max(__builtin_amdgcn_readlane(s.x, first), from), min(__builtin_amdgcn_readlane(s.y, last), to), __builtin_amdgcn_readlane(s.x, last),
             __builtin_amdgcn_readlane(s.y, first)};
 }
 
@@ -190,7 +191,7 @@ __device__ __forceinline__ void row_forward(const PackedArgs& p, int h, int row,
         if (p.rest != nullptr)
             p.rest[row * p.o_row + h * (64 * NP) + rest_place<NP>(lane + 64 * e)] = static_cast<uint8_t>(rest_pack(rest_of(x), 0.f, 0.f, 0.f));
     }
-    if (lane == 0) p.lse[static_cast<size_t>(h) * p.T + row] = log2f(l) + m;
+    if (lane == 0) p.lse[static_cast<size_t>(h) * p.T + row] = (log2f(l) + m) * -p.unscale;
 }
 
 template <int NP>
@@ -219,7 +220,7 @@ __device__ __forceinline__ void row_dq(const PackedArgs& p, int h, int row, int 
         }
         a = wave_sum(a);
         b = wave_sum(b);
-        const float ds = fast_exp2(a * p.scale_log2 - lse) * (b - dl);
+        const float ds = fast_exp2((a + lse) * p.scale_log2) * (b - dl);
 #pragma unroll
         for (int e = 0; e < NP; ++e) dq[e] += ds * kv[e];
     }
@@ -250,7 +251,7 @@ __device__ __forceinline__ void row_dkv(const PackedArgs& p, int hk, int h0, int
             }
             a = wave_sum(a);
             b = wave_sum(b);
-            const float pr = fast_exp2(a * p.scale_log2 - p.lse[static_cast<size_t>(h) * p.T + i]);
+            const float pr = fast_exp2((a + p.lse[static_cast<size_t>(h) * p.T + i]) * p.scale_log2);
             const float ds = pr * (b + p.delta[static_cast<size_t>(h) * p.T + i]);
 #pragma unroll
             for (int e = 0; e < NP; ++e) acc[e] += IS_V ? pr * dov[e] : ds * qv[e];
@@ -299,10 +300,13 @@ __device__ __forceinline__ uint32_t bad_rows(const f32x16 (&a)[N], bool counts) 
 // heads (one in eight where the heads are a multiple of eight) whose rows its L2 serves, and every XCD gets blocks of all
 // sizes.  The blocks with the most tiles come first (pack_order_kernel): 16384 rows of documents of 1 to 1024 tokens fill
 // the CUs 2.7 times, and in the order of the rows the last round left them a quarter idle.
-__device__ __forceinline__ void ap_unit(const PackedArgs& p, int heads, int& blk, int& h) {
+__device__ __forceinline__ void ap_unit(const PackedArgs& p, int heads, int& blk, int& h, int& from, int& to) {
     const int rank = blockIdx.x / heads;
     h = blockIdx.x - rank * heads;
-    blk = p.order[rank];
+    const int4 e = p.order[rank];
+    blk = e.x;
+    from = e.y;
+    to = e.z;
 }
 
 template <int NP>
@@ -311,11 +315,10 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
     extern __shared__ __attribute__((aligned(1024))) bf16 ap_smem[];
     bf16* sK = ap_smem;                    // [RING][TILE]
     bf16* sV = ap_smem + RING * TILE;   // [RING][TILE]
-    __shared__ int sB[8];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hi = lane >> 5, lq = lane & 31;
-    int blk, h;
-    ap_unit(p, p.H, blk, h);
+    int blk, h, k_lo, k_hi;
+    ap_unit(p, p.H, blk, h, k_lo, k_hi);
     const int hk = h / p.group;
     const int qw0 = blk * AT_BR + 32 * wave, qrow = qw0 + lq;
     bf16x8 qf[4 * NP];  // B operand of S^T
@@ -325,15 +328,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
         for (int ks = 0; ks < 4 * NP; ++ks) qf[ks] = *reinterpret_cast<const bf16x8*>(qp + 16 * ks);
     }
     const int2 span = ap_keys_of(p, qrow);
-    const Bounds wb = wave_bounds(span);
-    if (lane == 0) {
-        sB[wave] = wb.lo;
-        sB[4 + wave] = wb.hi;
-    }
-    __syncthreads();
-    const int k_lo = min(min(sB[0], sB[1]), min(sB[2], sB[3])), k_hi = max(max(sB[4], sB[5]), max(sB[6], sB[7]));
-    const int nt = k_hi > k_lo ? (k_hi - k_lo + AT_T - 1) / AT_T : 0;
-    const int t_lo = wb.hi > wb.lo ? (wb.lo - k_lo) / AT_T : nt, t_hi = wb.hi > wb.lo ? (wb.hi - k_lo + AT_T - 1) / AT_T : nt;
+    const int nt = (k_hi - k_lo + AT_T - 1) / AT_T;
     const bf16* kbase = p.k + hk * p.k_head;
     const bf16* vbase = p.v + hk * p.v_head;
     const TileDma dma = tile_dma_setup(wave, lane);
@@ -343,9 +338,12 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
         ap_tile_issue<NP>(dma, kbase, p.k_row, k_lo + t * AT_T, k_hi - 1, sK + slot * TILE, wave);
         ap_tile_issue<NP>(dma, vbase, p.v_row, k_lo + t * AT_T, k_hi - 1, sV + slot * TILE, wave);
     };
+    asm volatile("" ::: "memory");  // (the rows' own loads first: the counter of loads under way is in order)
 #pragma unroll
     for (int t = 0; t < RING - 1; ++t)
         if (t < nt) issue(t, t);
+    const Bounds wb = wave_bounds(span, k_lo, k_hi);
+    const int t_lo = wb.hi > wb.lo ? (wb.lo - k_lo) / AT_T : nt, t_hi = wb.hi > wb.lo ? (wb.hi - k_lo + AT_T - 1) / AT_T : nt;
 
     f32x16 o[2 * NP];
 #pragma unroll
@@ -491,7 +489,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
 #pragma unroll
             for (int e = 0; e < 16; ++e) o[d][e] = 0.f;
     }
-    if (hi == 0 && qrow < p.T) p.lse[static_cast<size_t>(h) * p.T + qrow] = some ? log2f(lt) + ref : 0.f;
+    if (hi == 0 && qrow < p.T) p.lse[static_cast<size_t>(h) * p.T + qrow] = some ? (log2f(lt) + ref) * -p.unscale : 0.f;
     const int el = ap_late(lane);
     bf16* orow0 = p.out + qw0 * p.o_row + h * (64 * NP);
     bf16* so = sK + wave * (32 * AT_D);
@@ -537,23 +535,14 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
     extern __shared__ __attribute__((aligned(1024))) bf16 ap_smem[];
     bf16* sK = ap_smem;
     bf16* sV = ap_smem + RING * TILE;
-    __shared__ int sB[8];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hi = lane >> 5, lq = lane & 31;
-    int blk, h;
-    ap_unit(p, p.H, blk, h);
+    int blk, h, k_lo, k_hi;
+    ap_unit(p, p.H, blk, h, k_lo, k_hi);
     const int hk = h / p.group;
     const int qw0 = blk * AT_BR + 32 * wave, qrow = qw0 + lq;
     const int2 span = ap_keys_of(p, qrow);
-    const Bounds wb = wave_bounds(span);
-    if (lane == 0) {
-        sB[wave] = wb.lo;
-        sB[4 + wave] = wb.hi;
-    }
-    __syncthreads();
-    const int k_lo = min(min(sB[0], sB[1]), min(sB[2], sB[3])), k_hi = max(max(sB[4], sB[5]), max(sB[6], sB[7]));
-    const int nt = k_hi > k_lo ? (k_hi - k_lo + AT_T - 1) / AT_T : 0;
-    const int t_lo = wb.hi > wb.lo ? (wb.lo - k_lo) / AT_T : nt, t_hi = wb.hi > wb.lo ? (wb.hi - k_lo + AT_T - 1) / AT_T : nt;
+    const int nt = (k_hi - k_lo + AT_T - 1) / AT_T;
     const bf16* kbase = p.k + hk * p.k_head;
     const bf16* vbase = p.v + hk * p.v_head;
     const TileDma dma = tile_dma_setup(wave, lane);
@@ -562,9 +551,12 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
         ap_tile_issue<NP>(dma, kbase, p.k_row, k_lo + t * AT_T, k_hi - 1, sK + slot * TILE, wave);
         ap_tile_issue<NP>(dma, vbase, p.v_row, k_lo + t * AT_T, k_hi - 1, sV + slot * TILE, wave);
     };
+    asm volatile("" ::: "memory");  // (the rows' own loads first: the counter of loads under way is in order)
 #pragma unroll
     for (int t = 0; t < RING - 1; ++t)
         if (t < nt) issue(t, t);
+    const Bounds wb = wave_bounds(span, k_lo, k_hi);
+    const int t_lo = wb.hi > wb.lo ? (wb.lo - k_lo) / AT_T : nt, t_hi = wb.hi > wb.lo ? (wb.hi - k_lo + AT_T - 1) / AT_T : nt;
     bf16x8 qf[4 * NP], dof[4 * NP];
     float nl = 0.f, ndl = 0.f;  // minus log-sum-exp (log2 units), minus delta
     {
@@ -597,7 +589,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
         ndl = -other_half_sum(dl);
         const size_t off = static_cast<size_t>(h) * p.T + qc;
         if (hi == 0 && qrow < p.T) p.delta[off] = ndl;
-        nl = -p.lse[off];
+        nl = p.lse[off] * p.scale_log2;
     }
     f32x16 dq[2 * NP];
 #pragma unroll
@@ -732,34 +724,23 @@ __device__ __forceinline__ void dkv_store(const PackedArgs& p, f32x16 (&acc)[2 *
     }
 }
 
-__global__ __launch_bounds__(256, 2) void packed_dkv64_kernel(const PackedArgs p) {
+__global__ __launch_bounds__(256, 3) void packed_dkv64_kernel(const PackedArgs p) {
     constexpr int NP = 1;
     constexpr int TILE = NP * AT_TILE;
     extern __shared__ __attribute__((aligned(1024))) bf16 ap_smem[];
     bf16* sQ = ap_smem;
     bf16* sDO = ap_smem + AT_RING * TILE;
-    __shared__ __attribute__((aligned(1024))) float sRow[AT_RING][4][AT_T];  // per tile: lse, -delta, two unused rows (waves 2, 3)
-    __shared__ int sB[8];
+    __shared__ __attribute__((aligned(1024))) float sRow[AT_RING][4][AT_T];  // per tile: lse, delta, two unused rows (waves 2, 3)
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hi = lane >> 5, lq = lane & 31;
-    int blk, u;
-    ap_unit(p, p.Hk * p.splits, blk, u);
+    int blk, u, q_lo, q_hi;
+    ap_unit(p, p.Hk * p.splits, blk, u, q_lo, q_hi);
     const int hk = u / p.splits, split = u - hk * p.splits;
     const int h0 = hk * p.group + split * p.group / p.splits, h1 = hk * p.group + (split + 1) * p.group / p.splits;
     const int kw0 = blk * AT_BR + 32 * wave, key = kw0 + lq;
     const int2 span = ap_queries_of(p, key);
-    const Bounds wb = wave_bounds(span);
-    if (lane == 0) {
-        sB[wave] = wb.lo;
-        sB[4 + wave] = wb.hi;
-    }
-    __syncthreads();
-    const int q_lo = min(min(sB[0], sB[1]), min(sB[2], sB[3])), q_hi = max(max(sB[4], sB[5]), max(sB[6], sB[7]));
-    const int nt1 = q_hi > q_lo ? (q_hi - q_lo + AT_T - 1) / AT_T : 0;  // tiles of one head; the heads follow each other
+    const int nt1 = (q_hi - q_lo + AT_T - 1) / AT_T;  // tiles of one head; the heads follow each other
     const int nt = nt1 * (h1 - h0);
-    const int t_lo = wb.hi > wb.lo ? (wb.lo - q_lo) / AT_T : nt1, t_hi = wb.hi > wb.lo ? (wb.hi - q_lo + AT_T - 1) / AT_T : nt1;
-    const TileDma dma = tile_dma_setup(wave, lane);
-    const FragAddr fa = frag_addr_setup(lane);
     bf16x8 kf[4 * NP], vf[4 * NP];
     {
         const int kc = min(key, p.T - 1);
@@ -774,6 +755,7 @@ __global__ __launch_bounds__(256, 2) void packed_dkv64_kernel(const PackedArgs p
     int is_h = h0, is_t = 0;  // the loader's head and tile
     auto issue = [&](int slot) {
         const int r0 = q_lo + is_t * AT_T;
+        const TileDma dma = tile_dma_setup(wave, ap_late(lane));  // (worked out anew: registers are what bounds this kernel's waves)
         ap_tile_issue<NP>(dma, p.q + is_h * p.q_head, p.q_row, r0, q_hi - 1, sQ + slot * TILE, wave);
         ap_tile_issue<NP>(dma, p.dout + is_h * (64 * NP), p.o_row, r0, q_hi - 1, sDO + slot * TILE, wave);
         const float* rows = (wave & 1 ? p.delta : p.lse) + static_cast<size_t>(is_h) * p.T;
@@ -783,9 +765,12 @@ __global__ __launch_bounds__(256, 2) void packed_dkv64_kernel(const PackedArgs p
             ++is_h;
         }
     };
+    asm volatile("" ::: "memory");  // (the rows' own loads first: the counter of loads under way is in order)
 #pragma unroll
     for (int i = 0; i < 2; ++i)
         if (i < nt) issue(i);
+    const Bounds wb = wave_bounds(span, q_lo, q_hi);
+    const int t_lo = wb.hi > wb.lo ? (wb.lo - q_lo) / AT_T : nt1, t_hi = wb.hi > wb.lo ? (wb.hi - q_lo + AT_T - 1) / AT_T : nt1;
     f32x16 dk[2 * NP], dv[2 * NP];
 #pragma unroll
     for (int d = 0; d < 2 * NP; ++d)
@@ -809,45 +794,47 @@ __global__ __launch_bounds__(256, 2) void packed_dkv64_kernel(const PackedArgs p
             const int cur = next_tile();
             if (t < t_lo || t >= t_hi) continue;
             const int q0 = q_lo + t * AT_T;
-            const TileAt at = tile_at(fa, sq_lds + static_cast<uint32_t>(cur) * (TILE * 2));
+            const TileAt at = tile_at(frag_addr_setup(ap_late(lane)), sq_lds + static_cast<uint32_t>(cur) * (TILE * 2));
             const uint32_t row_tile = srow_lds + static_cast<uint32_t>(cur) * (4 * AT_T * 4) + 16 * hi;
             const bool masked = q0 < wb.max_lo || q0 + AT_T > wb.min_hi;
             auto half = [&](auto qt) {
                 if (q0 + 32 * qt >= wb.hi || q0 + 32 * qt + 32 <= wb.lo) return;  // no key of the wave meets it
+                // (registers: three waves per SIMD have 168 each, 96 of them hold the sums and the keys' own rows; so the row
+                // terms start the products' accumulators, and operands are fetched one after the other)
                 f32x16 s, dp;
-                f32x4 nd[4], l2[4];
-                RowFrags qf, dof;
+                f32x4 l2[4], nd[4];
+                RowFrags f;
+#pragma unroll
+                for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(l2[r4], row_tile + (32 * qt + 8 * r4) * 4);
+                read_rows<qt * 4096>(f, at.row);
+                lds_wait<0>();
+                taken(l2);
+                taken(f);
+#pragma unroll
+                for (int e = 0; e < 16; ++e) s[e] = l2[e >> 2][e & 3];
+#pragma unroll
+                for (int ks = 0; ks < 4; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f, ks), kf[ks], s, 0, 0, 0);
+                asm volatile("" : "+v"(s));  // (the products are issued before the next operand takes their registers)
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(nd[r4], row_tile + AT_T * 4 + (32 * qt + 8 * r4) * 4);
-                read_rows<qt * 4096>(qf, at.row);
-                read_rows<DO_AT + qt * 4096>(dof, at.row);
-                lds_wait<4>();
+                read_rows<DO_AT + qt * 4096>(f, at.row);
+                lds_wait<0>();
                 taken(nd);
-                taken(qf);
+                taken(f);
 #pragma unroll
                 for (int e = 0; e < 16; ++e) dp[e] = nd[e >> 2][e & 3];
 #pragma unroll
-                for (int ks = 0; ks < 4; ++ks) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(qf, ks), kf[ks], ks == 0 ? f32x16{} : s, 0, 0, 0);
-                lds_wait<0>();
-                taken(dof);
-#pragma unroll
-                for (int ks = 0; ks < 4; ++ks) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(dof, ks), vf[ks], dp, 0, 0, 0);
-#pragma unroll
-                for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(l2[r4], row_tile + (32 * qt + 8 * r4) * 4);
-                TrFrags dot[2], qtf[2];  // dO^T and Q^T, on their way during the vector work
-                ap_for<2>([&](auto d) {
-                    read_tr<DO_AT + qt * 4096>(dot[d], at.tr[d]);
-                    read_tr<qt * 4096>(qtf[d], at.tr[d]);
-                });
+                for (int ks = 0; ks < 4; ++ks) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f, ks), vf[ks], dp, 0, 0, 0);
+                asm volatile("" : "+v"(dp));
+                TrFrags t2[2];  // dO^T, on its way during the vector work
+                ap_for<2>([&](auto d) { read_tr<DO_AT + qt * 4096>(t2[d], at.tr[d]); });
                 if (masked) {
                     const int first = q0 + 32 * qt + 4 * hi;
                     mask_outside(s, span.x - first, span.y - first);
                 }
-                lds_wait<15>();  // (the row terms are the oldest four of twenty reads; the counter ends at 15)
-                taken(l2);
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    s[r] = fast_exp2(fmaf(s[r], p.scale_log2, -l2[r >> 2][r & 3]));
+                    s[r] = fast_exp2(s[r] * p.scale_log2);
                     dp[r] *= s[r];
                 }
                 bf16x8 pb[2], dsb[2];
@@ -858,17 +845,20 @@ __global__ __launch_bounds__(256, 2) void packed_dkv64_kernel(const PackedArgs p
                 }
                 lds_wait<0>();
 #pragma unroll
-                for (int d = 0; d < 2; ++d) {
-                    taken(dot[d]);
-                    taken(qtf[d]);
-                }
+                for (int d = 0; d < 2; ++d) taken(t2[d]);
 #pragma unroll
                 for (int j = 0; j < 2; ++j)
 #pragma unroll
-                    for (int d = 0; d < 2; ++d) {
-                        dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(dot[d], j), pb[j], dv[d], 0, 0, 0);
-                        dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(qtf[d], j), dsb[j], dk[d], 0, 0, 0);
-                    }
+                    for (int d = 0; d < 2; ++d) dv[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(t2[d], j), pb[j], dv[d], 0, 0, 0);
+                __builtin_amdgcn_sched_barrier(0);
+                ap_for<2>([&](auto d) { read_tr<qt * 4096>(t2[d], at.tr[d]); });
+                lds_wait<0>();
+#pragma unroll
+                for (int d = 0; d < 2; ++d) taken(t2[d]);
+#pragma unroll
+                for (int j = 0; j < 2; ++j)
+#pragma unroll
+                    for (int d = 0; d < 2; ++d) dk[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(t2[d], j), dsb[j], dk[d], 0, 0, 0);
                 __builtin_amdgcn_sched_barrier(0);
             };
             half(C0{});
@@ -892,25 +882,17 @@ __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs 
     bf16* sQ = ap_smem;                    // [AT_RING][TILE]
     bf16* sDO = ap_smem + AT_RING * TILE;  // [AT_RING][TILE]
     float* sP = reinterpret_cast<float*>(ap_smem + 2 * AT_RING * TILE);  // [2][4 pairs][16 registers / 4][64 lanes][4]
-    __shared__ __attribute__((aligned(1024))) float sRow[AT_RING][8][AT_T];  // a wave's own row terms: lse (P waves) or -delta
-    __shared__ int sB[8];
+    __shared__ __attribute__((aligned(1024))) float sRow[AT_RING][8][AT_T];  // a wave's own row terms: lse (P waves) or delta
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hi = lane >> 5, lq = lane & 31, pair = wave & 3;
     const bool is_p = wave < 4;
-    int blk, u;
-    ap_unit(p, p.Hk * p.splits, blk, u);
+    int blk, u, q_lo, q_hi;
+    ap_unit(p, p.Hk * p.splits, blk, u, q_lo, q_hi);
     const int hk = u / p.splits, split = u - hk * p.splits;
     const int h0 = hk * p.group + split * p.group / p.splits, h1 = hk * p.group + (split + 1) * p.group / p.splits;
     const int kw0 = blk * AT_BR + 32 * pair, key = kw0 + lq;
     const int2 span = ap_queries_of(p, key);
-    const Bounds wb = wave_bounds(span);
-    if (lane == 0 && is_p) {
-        sB[wave] = wb.lo;
-        sB[4 + wave] = wb.hi;
-    }
-    __syncthreads();
-    const int q_lo = min(min(sB[0], sB[1]), min(sB[2], sB[3])), q_hi = max(max(sB[4], sB[5]), max(sB[6], sB[7]));
-    const int nt1 = q_hi > q_lo ? (q_hi - q_lo + AT_T - 1) / AT_T : 0;  // tiles of one head; the heads follow each other
+    const int nt1 = (q_hi - q_lo + AT_T - 1) / AT_T;  // tiles of one head; the heads follow each other
     const int nt = nt1 * (h1 - h0);
     const FragAddr fa = frag_addr_setup(lane);
     // DMA pieces of eight rows: wave w fetches rows 8w .. 8w + 7 of each of the tile's four panels
@@ -943,8 +925,10 @@ __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs 
             ++is_h;
         }
     };
+    asm volatile("" ::: "memory");  // (the rows' own loads first: the counter of loads under way is in order)
     if (nt > 0) issue(0);
     if (nt > 1) issue(1);
+    const Bounds wb = wave_bounds(span, q_lo, q_hi);
     const uint32_t sq_lds = lds_addr(sQ), srow_lds = lds_addr(&sRow[0][wave][0]) + 16 * hi;
     const uint32_t sp_lds = lds_addr(sP) + pair * 4096 + lane * 16;
 
@@ -961,7 +945,11 @@ __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs 
 #pragma unroll
             for (int e = 0; e < 16; ++e) acc[d][e] = 0.f;
         RowFrags f[2];
+        f32x4 rt[4];  // row terms
         auto fetch = [&](int slot, auto half) {
+            const uint32_t row_at = srow_lds + static_cast<uint32_t>(slot) * (8 * AT_T * 4);
+#pragma unroll
+            for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(rt[r4], row_at + (32 * half + 8 * r4) * 4);
             const uint32_t base = sq_lds + static_cast<uint32_t>(slot) * (TILE * 2);
             uint32_t at[4];
 #pragma unroll
@@ -973,15 +961,14 @@ __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs 
             lds_wait<0>();
             taken(f[0]);
             taken(f[1]);
+            taken(rt);
         };
         // queries [q_lo + 64 t + 32 half, + 32) of the current head, tile in ring slot `slot`; then the rows of half2 in slot2
         auto phase = [&](int t, int slot, auto half, int slot2, auto half2) {
-            const uint32_t base = sq_lds + static_cast<uint32_t>(slot) * (TILE * 2), row_at = srow_lds + static_cast<uint32_t>(slot) * (8 * AT_T * 4);
+            const uint32_t base = sq_lds + static_cast<uint32_t>(slot) * (TILE * 2);
             f32x16 c;
-            f32x4 rt[4], pr[4];  // row terms; P of the other wave
+            f32x4 pr[4];  // P of the other wave
             TrFrags ft[4];
-#pragma unroll
-            for (int r4 = 0; r4 < 4; ++r4) lds_read_f32x4(rt[r4], row_at + (32 * half + 8 * r4) * 4);
             if constexpr (!IS_P) {
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) asm volatile("ds_read_b128 %0, %1 offset:%2" : "=v"(pr[r4]) : "v"(sp_lds), "n"(half * 16384 + r4 * 1024) : "memory");
@@ -993,14 +980,14 @@ __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs 
                 ap_for<4>([&](auto d) { read_tr<T_AT + (d >> 1) * PANEL + half * 4096>(ft[d], at[d & 1]); });
             }
 #pragma unroll
-            for (int ks = 0; ks < 8; ++ks) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), own[ks], ks == 0 ? f32x16{} : c, 0, 0, 0);
+            for (int e = 0; e < 16; ++e) c[e] = rt[e >> 2][e & 3];  // (the row term starts the sum)
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), own[ks], c, 0, 0, 0);
             if constexpr (IS_P) {
-                lds_wait<15>();  // (the row terms are the oldest four of twenty reads; the counter ends at 15)
-                taken(rt);
                 const int q0 = q_lo + t * AT_T + 32 * half;
                 if (q0 < wb.max_lo || q0 + 32 > wb.min_hi) mask_outside(c, span.x - q0 - 4 * hi, span.y - q0 - 4 * hi);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) c[r] = fast_exp2(fmaf(c[r], p.scale_log2, -rt[r >> 2][r & 3]));
+                for (int r = 0; r < 16; ++r) c[r] = fast_exp2(c[r] * p.scale_log2);
 #pragma unroll
                 for (int r4 = 0; r4 < 4; ++r4) {
                     const f32x4 v = {c[4 * r4], c[4 * r4 + 1], c[4 * r4 + 2], c[4 * r4 + 3]};
@@ -1011,10 +998,9 @@ __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs 
 #pragma unroll
             for (int d = 0; d < 4; ++d) taken(ft[d]);
             if constexpr (!IS_P) {
-                taken(rt);
                 taken(pr);
 #pragma unroll
-                for (int r = 0; r < 16; ++r) c[r] = (c[r] + rt[r >> 2][r & 3]) * pr[r >> 2][r & 3];
+                for (int r = 0; r < 16; ++r) c[r] *= pr[r >> 2][r & 3];
             }
             const bf16x8 b0 = pack_half(c, 0), b1 = pack_half(c, 1);
             __builtin_amdgcn_sched_barrier(0);
@@ -1103,10 +1089,10 @@ __device__ __forceinline__ int2 pack_span_of(const int* offsets, int n, int rows
     return {0, 0};
 }
 
-// work: [3][blocks], rows that a block of 128 streams: causal query side, causal key side, not causal.  order (if given): the
-// rows' own order of the blocks instead.
+// entries: [3][blocks] {block of 128 rows, first and end of the rows it streams, their number}: causal query side, causal key
+// side, not causal; in the order the kernels take them, or by block for pack_order_kernel.
 __global__ __launch_bounds__(256) void pack_spans_kernel(const int* __restrict__ offsets, int n, int rows, int2* __restrict__ spans,
-                                                        long long* __restrict__ positions, int* __restrict__ work, int* __restrict__ order) {
+                                                        long long* __restrict__ positions, int4* __restrict__ entries, bool sorted) {
     const int row = blockIdx.x * 256 + threadIdx.x;
     if (row >= rows) return;
     const int2 s = pack_span_of(offsets, n, rows, row);
@@ -1116,27 +1102,24 @@ __global__ __launch_bounds__(256) void pack_spans_kernel(const int* __restrict__
         const int last = min(row + AT_BR, rows) - 1, blocks = (rows + AT_BR - 1) / AT_BR, b = row / AT_BR;
         const int2 e = pack_span_of(offsets, n, rows, last);
         const int first = s.y > 0 ? s.x : row, end = e.y > 0 ? e.y : last + 1;  // (a block's edge may lie outside every sequence)
-        if (order != nullptr) {
-            order[b] = blocks - 1 - b;  // causal, query side: the last blocks of a long sequence have the most keys
-            order[blocks + b] = b;
-            order[2 * static_cast<size_t>(blocks) + b] = b;
-        } else {
-            work[b] = last + 1 - first;
-            work[blocks + b] = end - row;
-            work[2 * static_cast<size_t>(blocks) + b] = end - first;
-        }
+        // (in the rows' own order the last blocks come first on the query side: of a long sequence they have the most keys)
+        entries[sorted ? b : blocks - 1 - b] = {b, first, last + 1, last + 1 - first};
+        entries[blocks + b] = {b, row, end, end - row};
+        entries[2 * static_cast<size_t>(blocks) + b] = {b, first, end, end - first};
     }
 }
 
-// order[k][rank] = block, by falling work (equal ones as the rows go).  Counted, not sorted: a few thousand blocks at most.
-__global__ __launch_bounds__(256) void pack_order_kernel(const int* __restrict__ work, int blocks, int* __restrict__ order) {
+// The entries by falling work (equal ones as the rows go).  Counted, not sorted: a few thousand blocks at most.
+__global__ __launch_bounds__(256) void pack_order_kernel(const int4* __restrict__ entries, int blocks, int4* __restrict__ order) {
     __shared__ __attribute__((aligned(16))) int w[256];
-    const int* src = work + static_cast<size_t>(blockIdx.y) * blocks;
-    const int b = blockIdx.x * 256 + threadIdx.x, mine = b < blocks ? src[b] : 0;
+    const int4* src = entries + static_cast<size_t>(blockIdx.y) * blocks;
+    const int b = blockIdx.x * 256 + threadIdx.x;
+    const int4 e = b < blocks ? src[b] : int4{0, 0, 0, 0};
+    const int mine = e.w;
     int rank = 0;
     for (int j0 = 0; j0 < blocks; j0 += 256) {
         __syncthreads();
-        w[threadIdx.x] = j0 + static_cast<int>(threadIdx.x) < blocks ? src[j0 + threadIdx.x] : -1;
+        w[threadIdx.x] = j0 + static_cast<int>(threadIdx.x) < blocks ? src[j0 + threadIdx.x].w : -1;
         __syncthreads();
         const int before = b - j0;  // equal work counts from the blocks in front of this one
 #pragma unroll 16
@@ -1145,22 +1128,23 @@ __global__ __launch_bounds__(256) void pack_order_kernel(const int* __restrict__
             rank += (x.x >= mine + (j >= before)) + (x.y >= mine + (j + 1 >= before)) + (x.z >= mine + (j + 2 >= before)) + (x.w >= mine + (j + 3 >= before));
         }
     }
-    if (b < blocks) order[static_cast<size_t>(blockIdx.y) * blocks + rank] = b;
+    if (b < blocks) order[static_cast<size_t>(blockIdx.y) * blocks + rank] = e;
 }
 
 // Packs of few blocks (one round of workgroups) and of very many (the last round does not matter) keep the rows' own order.
 #define AP_ORDER_FROM 16
 #define AP_ORDER_TO 8192
 
-// offsets: [sequences + 1] int32, not falling.  order: [3][ceil(rows / 128)]; work: scratch of the same size.
-PDT_API int pdt_pack_spans(const int* offsets, int sequences, int rows, void* spans, long long* positions, int* order, int* work, void* stream) {
+// offsets: [sequences + 1] int32, not falling.  order: [3][ceil(rows / 128)] entries of 16 bytes; work: scratch of the same size.
+PDT_API int pdt_pack_spans(const int* offsets, int sequences, int rows, void* spans, long long* positions, void* order, void* work, void* stream) {
     if (sequences < 0 || rows <= 0 || rows >= (1 << 30)) return -1;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int blocks = pdt_cdiv(rows, AT_BR);
     const bool sorted = blocks > AP_ORDER_FROM && blocks <= AP_ORDER_TO;
-    hipLaunchKernelGGL(pack_spans_kernel, dim3(pdt_cdiv(rows, 256)), dim3(256), 0, s, offsets, sequences, rows, static_cast<int2*>(spans), positions, work,
-                       sorted ? nullptr : order);
-    if (sorted) hipLaunchKernelGGL(pack_order_kernel, dim3(pdt_cdiv(blocks, 256), 3), dim3(256), 0, s, work, blocks, order);
+    hipLaunchKernelGGL(pack_spans_kernel, dim3(pdt_cdiv(rows, 256)), dim3(256), 0, s, offsets, sequences, rows, static_cast<int2*>(spans), positions,
+                       static_cast<int4*>(sorted ? work : order), sorted);
+    if (sorted)
+        hipLaunchKernelGGL(pack_order_kernel, dim3(pdt_cdiv(blocks, 256), 3), dim3(256), 0, s, static_cast<const int4*>(work), blocks, static_cast<int4*>(order));
     return pdt_launch_status();
 }
 
@@ -1170,7 +1154,7 @@ static bool ap_stride_ok(const long long* st, int n) {
     return true;
 }
 
-static int ap_args(PackedArgs& a, const void* spans, const int* order, int T, int H, int Hk, int D, float scale, int causal) {
+static int ap_args(PackedArgs& a, const void* spans, const void* order, int T, int H, int Hk, int D, float scale, int causal) {
     if (T <= 0 || H <= 0 || Hk <= 0 || H % Hk != 0 || (D != 64 && D != 128) || !(scale > 0.f) || !(scale < 3.0e38f)) return -1;
     a.spans = static_cast<const int2*>(spans);
     a.T = T; a.H = H; a.Hk = Hk;
@@ -1178,9 +1162,10 @@ static int ap_args(PackedArgs& a, const void* spans, const int* order, int T, in
     a.nblk = pdt_cdiv(T, AT_BR);
     a.causal = causal != 0;
     a.splits = 1;
-    a.order = order + (causal != 0 ? 0 : 2 * static_cast<size_t>(a.nblk));
+    a.order = static_cast<const int4*>(order) + (causal != 0 ? 0 : 2 * static_cast<size_t>(a.nblk));
     a.scale = scale;
     a.scale_log2 = scale * 1.4426950408889634f;
+    a.unscale = 1.f / a.scale_log2;
     if (static_cast<long long>(a.nblk) * H >= (1ll << 31) || T >= (1 << 30)) return -1;
     return 0;
 }
@@ -1206,7 +1191,7 @@ static int ap_launch(K kernel, unsigned long long& granted, unsigned grid, size_
 
 // spans, order: pdt_pack_spans.  st: row and head strides of q, k, v in elements (multiples of 8; 16-byte aligned pointers); out is [T, H, D] without gaps,
 // rest (nullptr without a backward pass) has one byte for each of its elements.
-PDT_API int pdt_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, void* rest, float* lse, const void* spans, const int* order, const long long* st,
+PDT_API int pdt_packed_attention_fwd(const void* q, const void* k, const void* v, void* out, void* rest, float* lse, const void* spans, const void* order, const long long* st,
                                      int T, int H, int Hk, int D, float scale, int causal, void* stream) {
     PackedArgs a = {};
     if (ap_args(a, spans, order, T, H, Hk, D, scale, causal) != 0 || !ap_stride_ok(st, 6)) return -1;
@@ -1239,7 +1224,7 @@ PDT_API int pdt_packed_attention_splits(int T, int H, int Hk) {
 // st: row and head strides of q, k, v, dq, dk, dv; o and dout are [T, H, D] without gaps.  delta: scratch, H * T floats.
 // part: scratch, splits * 2 * T * Hk * D floats, unused (may be nullptr) where splits is 1.
 PDT_API int pdt_packed_attention_bwd(const void* q, const void* k, const void* v, const void* o, const void* rest, const void* dout, const float* lse, float* delta,
-                                     void* dq, void* dk, void* dv, float* part, int splits, const void* spans, const int* order, const long long* st, int T, int H,
+                                     void* dq, void* dk, void* dv, float* part, int splits, const void* spans, const void* order, const long long* st, int T, int H,
                                      int Hk, int D, float scale, int causal, void* stream) {
     PackedArgs a = {};
     if (ap_args(a, spans, order, T, H, Hk, D, scale, causal) != 0 || !ap_stride_ok(st, 12)) return -1;

@@ -22,17 +22,17 @@ BLOCK_ROWS = 128  # rows of a workgroup
 
 
 def pack_plan(offsets, rows: int):
-    """One int64 buffer: ``rows`` positions, ``rows`` spans (two int32), three orders of the blocks and as much scratch."""
+    """One int64 buffer: ``rows`` positions, ``rows`` spans (two int32), three orders of the blocks (four int32 each) and as much scratch."""
     with _on(offsets.device):
         if offsets.dtype == torch.int64:
             offsets = offsets.clamp(-1, rows)  # (what lies beyond is cut off, and must not wrap around in 32 bits)
         offsets = offsets.to(torch.int32).contiguous()
         blocks = -(-rows // BLOCK_ROWS)
-        plan = torch.empty(2 * rows + 3 * blocks, dtype=torch.int64, device=offsets.device)
+        plan = torch.empty(2 * rows + 12 * blocks, dtype=torch.int64, device=offsets.device)
         if rows:
             at = plan.data_ptr()
             order = at + 16 * rows
-            _check(_pack_spans(offsets.data_ptr(), offsets.numel() - 1, rows, at + 8 * rows, at, order, order + 12 * blocks, _stream()), "pack_spans")
+            _check(_pack_spans(offsets.data_ptr(), offsets.numel() - 1, rows, at + 8 * rows, at, order, order + 48 * blocks, _stream()), "pack_spans")
     return plan
 
 
