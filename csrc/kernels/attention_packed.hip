@@ -144,7 +144,7 @@ template <int NP>
 __device__ __forceinline__ int rest_place(int d) { return ((d >> 3) & 1) * (32 * NP) + ((d >> 4) << 3) + (d & 7); }
 __device__ __forceinline__ float rest_of(float x) {
     const float r = (x - bf16_to_f32(f32_to_bf16(x))) * 256.f;
-    return fminf(fmaxf(r, -57344.f), 57344.f);
+    return __builtin_amdgcn_fmed3f(r, -57344.f, 57344.f);  // (NaN comes out as a number: its row is computed again)
 }
 __device__ __forceinline__ uint32_t rest_pack(float a, float b, float c, float d) {
     const int lo = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false);
@@ -310,8 +310,8 @@ __device__ __forceinline__ void ap_unit(const PackedArgs& p, int heads, int& blk
 }
 
 template <int NP>
-__global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const PackedArgs p) {
-    constexpr int TILE = NP * AT_TILE, RING = ap_ring<NP>;
+__global__ __launch_bounds__(256, NP == 1 ? 4 : 2) void packed_fwd_kernel(const PackedArgs p) {
+    constexpr int TILE = NP * AT_TILE, RING = 2;
     extern __shared__ __attribute__((aligned(1024))) bf16 ap_smem[];
     bf16* sK = ap_smem;                    // [RING][TILE]
     bf16* sV = ap_smem + RING * TILE;   // [RING][TILE]
@@ -331,9 +331,9 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
     const int nt = (k_hi - k_lo + AT_T - 1) / AT_T;
     const bf16* kbase = p.k + hk * p.k_head;
     const bf16* vbase = p.v + hk * p.v_head;
+
     const TileDma dma = tile_dma_setup(wave, lane);
     const FragAddr fa = frag_addr_setup(lane);
-
     auto issue = [&](int t, int slot) {
         ap_tile_issue<NP>(dma, kbase, p.k_row, k_lo + t * AT_T, k_hi - 1, sK + slot * TILE, wave);
         ap_tile_issue<NP>(dma, vbase, p.v_row, k_lo + t * AT_T, k_hi - 1, sV + slot * TILE, wave);
@@ -450,6 +450,28 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
             //   S(0) S(1) | softmax(0) | PV(0) | softmax(1) | PV(1)
             const int k0 = k_lo + t * AT_T;
             enter_tile(t);
+            if constexpr (NP == 1) {
+                bool out = false;
+                ap_for<2>([&](auto kt) {
+                    if (out) return;
+                    f32x16 acc;
+                    scores(acc, kt);
+                    read_v(kt);
+                    mask(acc, k0, kt);
+                    const float l = probs(acc);
+                    kt0 = kt;
+                    if (__builtin_expect(__any(!(l <= 1073741824.f)), 0)) {
+                        lds_wait<0>();
+                        out = true;
+                        return;
+                    }
+                    lsum += l;
+                    values(acc);
+                    __builtin_amdgcn_sched_barrier(0);
+                });
+                entered = true;
+                if (out) break;
+            } else {
             f32x16 acc0, acc1;
             scores(acc0, C0{});
             scores(acc1, C1{});
@@ -473,6 +495,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
             }
             lsum += l1;
             values(acc1);
+            }
             entered = false;
             kt0 = 0;
             __builtin_amdgcn_sched_barrier(0);
@@ -482,8 +505,13 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
     asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
     const bool some = span.y > span.x;
     const float lt = other_half_sum(lsum);
-    const float inv = some ? 1.f / lt : 0.f;
-    if (!some) {
+    const float inv = 1.f / lt;
+    if (some) {
+#pragma unroll
+        for (int d = 0; d < 2 * NP; ++d)
+#pragma unroll
+            for (int e = 0; e < 16; ++e) o[d][e] *= inv;
+    } else {
 #pragma unroll
         for (int d = 0; d < 2 * NP; ++d)
 #pragma unroll
@@ -495,7 +523,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
     bf16* so = sK + wave * (32 * AT_D);
 #pragma unroll
     for (int pn = 0; pn < NP; ++pn)
-        store_rows32(so, o + 2 * pn, inv, el, p.T - qw0, [&](int row) { return orow0 + row * p.o_row + 64 * pn; });
+        store_rows32(so, o + 2 * pn, 1.f, el, p.T - qw0, [&](int row) { return orow0 + row * p.o_row + 64 * pn; });
     uint32_t bad = bad_rows(o, some);
     if (p.rest != nullptr) {
         // The backward pass takes dout . out as the row term of dS = P (dP - term).  Where few keys share a row P (dP - term) is
@@ -511,7 +539,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_fwd_kernel(const 
             for (int r2 = 0; r2 < 2; ++r2) {
                 float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) x[e] = rest_of(o[d][8 * r2 + e] * inv);
+                for (int e = 0; e < 8; ++e) x[e] = rest_of(o[d][8 * r2 + e]);
                 float even = __builtin_bit_cast(float, rest_pack(x[0], x[1], x[2], x[3])), odd = __builtin_bit_cast(float, rest_pack(x[4], x[5], x[6], x[7]));
                 swap_rows32(even, odd);
                 w[2 * r2] = __builtin_bit_cast(uint32_t, even);
@@ -1205,7 +1233,7 @@ PDT_API int pdt_packed_attention_fwd(const void* q, const void* k, const void* v
     a.k_row = st[2]; a.k_head = st[3];
     a.v_row = st[4]; a.v_head = st[5];
     a.o_row = static_cast<long long>(H) * D;
-    const size_t lds = static_cast<size_t>(2 * (D == 64 ? ap_ring<1> : ap_ring<2>)) * AT_T * D * sizeof(bf16);
+    const size_t lds = static_cast<size_t>(2 * 2) * AT_T * D * sizeof(bf16);
     const unsigned grid = static_cast<unsigned>(a.nblk) * H;
     static unsigned long long granted[2];
     return D == 64 ? ap_launch(packed_fwd_kernel<1>, granted[0], grid, lds, static_cast<hipStream_t>(stream), a)
