@@ -642,6 +642,8 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
         const int cur = next_tile(t);
         const TileAt at = tile_at(fa, sk_lds + static_cast<uint32_t>(cur) * (TILE * 2));
         const bool masked = k0 < wb.max_lo || k0 + AT_T > wb.min_hi;
+        // (a wave's products go in front of the other waves' vector work, s_setprio: 16384 rows of one document, 1527 -> 1475 us;
+        // the forward and the dK / dV kernels lose 4 to 8 % by it)
         auto half = [&](auto kt) {
             if (k0 + 32 * kt >= wb.hi || k0 + 32 * kt + 32 <= wb.lo) return;  // no row of the wave reaches it
             f32x16 s, dp;
@@ -654,17 +656,21 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
                 lds_wait<0>();
 #pragma unroll
                 for (int pn = 0; pn < NP; ++pn) taken(f[pn]);
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int ks = 0; ks < 4 * NP; ++ks)
                     s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), qf[ks], ks == 0 ? f32x16{} : s, 0, 0, 0);
+                __builtin_amdgcn_s_setprio(0);
                 __builtin_amdgcn_sched_barrier(0);
                 ap_for<NP>([&](auto pn) { read_rows<V_AT + pn * PANEL + kt * 4096>(f[pn], at.row); });  // (under the products just issued)
                 lds_wait<0>();
 #pragma unroll
                 for (int pn = 0; pn < NP; ++pn) taken(f[pn]);
+                __builtin_amdgcn_s_setprio(1);
 #pragma unroll
                 for (int ks = 0; ks < 4 * NP; ++ks)
                     dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), dof[ks], dp, 0, 0, 0);
+                __builtin_amdgcn_s_setprio(0);
             }
             __builtin_amdgcn_sched_barrier(0);
             TrFrags kf[2 * NP];  // on their way during the vector work
@@ -679,10 +685,12 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
             lds_wait<0>();
 #pragma unroll
             for (int d = 0; d < 2 * NP; ++d) taken(kf[d]);
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int d = 0; d < 2 * NP; ++d) dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(kf[d], 0), ds0, dq[d], 0, 0, 0);
 #pragma unroll
             for (int d = 0; d < 2 * NP; ++d) dq[d] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_tr_get(kf[d], 1), ds1, dq[d], 0, 0, 0);
+            __builtin_amdgcn_s_setprio(0);
             __builtin_amdgcn_sched_barrier(0);
         };
         half(C0{});
