@@ -566,7 +566,7 @@ __global__ __launch_bounds__(512) void vocab_join_kernel(const VocabGemm p) {
 struct Targets {
     const long long* ids;    // [rows][top]
     const float* teacher;    // [rows][top], or nullptr: one target of weight 1 (labels)
-    float* p;                // [rows][top], unused for labels
+    float* p;                // [rows][top] weights, of repeated ids at their first entry; unused for labels
     float* base;             // [rows]
     int* valid;              // [rows]
     const bf16 *x, *w;       // behind a projection: [rows][width], [vocab][width]; else nullptr
@@ -577,83 +577,123 @@ struct Targets {
     float inv_tau;
 };
 
-// one wave per row
-__global__ __launch_bounds__(256) void vocab_targets_kernel(const Targets t) {
+// p . (x . W[id]) / tau of a row's targets, eight at a time (their rows of W are on their way together): this wave's share,
+// targets first, first + 8, ... of every `step`; lane's part of the sum.
+template <typename P, typename I>
+__device__ __forceinline__ float vl_target_scores(const Targets& t, int row, int first, int step, int lane, P p_of, I id_of) {
+    const bf16* x = t.x + static_cast<size_t>(row) * t.width;
+    float base = 0.f;
+    for (int k0 = first; k0 < t.top; k0 += step) {
+        const bf16* w[8];
+        float pk[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            pk[i] = k0 + i < t.top ? p_of(k0 + i) : 0.f;
+            w[i] = t.w + (pk[i] != 0.f ? id_of(k0 + i) : 0ll) * t.width;
+        }
+        for (int c = lane * 8; c < t.width; c += 512) {
+            const bf16x8 xv = *reinterpret_cast<const bf16x8*>(x + c);
+            bf16x8 wv[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i)
+                if (pk[i] != 0.f) wv[i] = *reinterpret_cast<const bf16x8*>(w[i] + c);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if (pk[i] == 0.f) continue;  // (not multiplied by 0: what an absent target's row holds does not count)
+                float s = 0.f;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) s = fmaf(bf16_to_f32(xv[e]), bf16_to_f32(wv[i][e]), s);
+                base -= pk[i] * s * t.inv_tau;
+            }
+        }
+    }
+    return base;
+}
+__device__ __forceinline__ void vl_copy_used(const Targets& t, int row, int at, int threads, bool some) {
+    if (t.x_used == nullptr) return;
+    for (int c = at * 8; c < t.width; c += threads * 8) {
+        const size_t o = static_cast<size_t>(row) * t.width + c;
+        *reinterpret_cast<bf16x8*>(t.x_used + o) = some ? *reinterpret_cast<const bf16x8*>(t.x + o) : bf16x8{};
+    }
+}
+
+// labels: one wave per row
+__global__ __launch_bounds__(256) void vocab_labels_kernel(const Targets t) {
     const int lane = threadIdx.x & 63, row = blockIdx.x * 4 + (threadIdx.x >> 6);
     if (row >= t.rows) {
-        if (t.x_used != nullptr)
-            for (int c = lane * 8; c < t.width; c += 512) *reinterpret_cast<bf16x8*>(t.x_used + static_cast<size_t>(row) * t.width + c) = bf16x8{};
+        vl_copy_used(t, row, lane, 64, false);
+        return;
+    }
+    const long long id = t.ids[row];
+    const bool some = id >= 0 && id < t.vocab;
+    const float base = wave_sum(some ? vl_target_scores(t, row, 0, 8, lane, [](int) { return 1.f; }, [&](int) { return id; }) : 0.f);
+    vl_copy_used(t, row, lane, 64, some);
+    if (lane == 0) {
+        t.base[row] = base;
+        t.valid[row] = some ? 1 : 0;
+    }
+}
+
+// a teacher: one workgroup per row, of four waves where there are rows of W to fetch (512 rows of 32 targets, width 768: 12 us,
+// with one wave 21; 8192 rows of 64 targets, width 1024: 153, 174) or targets by the hundred, else of one (8192 rows of 64
+// targets on given logits: 17 us, with four 46).  What is left of an id that repeats is its first entry, with all their weight.
+template <int THREADS>
+__global__ __launch_bounds__(THREADS) void vocab_teacher_kernel(const Targets t) {
+    extern __shared__ __attribute__((aligned(16))) int vl_targets_lds[];
+    __shared__ float red[16];
+    const int tid = threadIdx.x, row = blockIdx.x, padded = (t.top + 3) & ~3;
+    int* id = vl_targets_lds;
+    float *p = reinterpret_cast<float*>(id + padded), *merged = p + padded;
+    if (row >= t.rows) {
+        vl_copy_used(t, row, tid, THREADS, false);
         return;
     }
     const long long* ids = t.ids + static_cast<size_t>(row) * t.top;
-    auto present = [&](int k) { return ids[k] >= 0 && ids[k] < t.vocab; };
+    const float* z = t.teacher + static_cast<size_t>(row) * t.top;
+    float mx = -VL_INF;
+    int any = 0;
+    for (int k = tid; k < padded; k += THREADS) {
+        const bool ok = k < t.top && ids[k] >= 0 && ids[k] < t.vocab;
+        const float v = ok ? z[k] : -VL_INF;
+        id[k] = ok ? static_cast<int>(ids[k]) : -1;
+        p[k] = v;
+        any |= ok && !(v == -VL_INF);  // (NaN counts: it is to be seen in the loss)
+        mx = fmaxf(mx, v);
+    }
+    const bool some = __syncthreads_or(any) != 0;
+    mx = block_max(mx, red);
+    if (mx == -VL_INF) mx = 0.f;
+    float sum = 0.f;
+    for (int k = tid; k < t.top; k += THREADS) sum += vl_exp2((p[k] - mx) * t.inv_tau * VL_LOG2E);
+    sum = block_sum(sum, red);
+    const float ls = log2f(sum), inv = some ? 1.f / sum : 0.f;
     float base = 0.f;
-    bool some = false;
-    if (t.teacher == nullptr) {
-        some = present(0);
-    } else {
-        const float* z = t.teacher + static_cast<size_t>(row) * t.top;
-        float* p = t.p + static_cast<size_t>(row) * t.top;
-        float mx = -VL_INF;
-        bool any = false;
-        for (int k = lane; k < t.top; k += 64)
-            if (present(k)) {
-                any |= !(z[k] == -VL_INF);  // (NaN counts: it is to be seen in the loss)
-                mx = fmaxf(mx, z[k]);
-            }
-        mx = wave_max(mx);
-        some = __any(any);
-        if (mx == -VL_INF) mx = 0.f;
-        float sum = 0.f;
-        for (int k = lane; k < t.top; k += 64)
-            if (present(k)) sum += vl_exp2((z[k] - mx) * t.inv_tau * VL_LOG2E);
-        sum = wave_sum(sum);
-        const float ls = log2f(sum), inv = some ? 1.f / sum : 0.f;
-        for (int k = lane; k < t.top; k += 64) {
-            const float l = (z[k] - mx) * t.inv_tau * VL_LOG2E, pk = present(k) && some ? vl_exp2(l) * inv : 0.f;
-            p[k] = pk;
-            if (pk != 0.f) base += pk * (l - ls) * VL_LN2;
-        }
-        __threadfence_block();  // (the weights are read again by all lanes below)
+    for (int k = tid; k < padded; k += THREADS) {
+        const float l = (p[k] - mx) * t.inv_tau * VL_LOG2E, pk = id[k] >= 0 && some ? vl_exp2(l) * inv : 0.f;
+        p[k] = pk;
+        if (pk != 0.f) base += pk * (l - ls) * VL_LN2;
     }
-    if (t.x != nullptr && some) {
-        // sum_k p_k x . W[id_k], eight targets at a time: their rows of W are on their way together
-        const bf16* x = t.x + static_cast<size_t>(row) * t.width;
-        const float* p = t.teacher == nullptr ? nullptr : t.p + static_cast<size_t>(row) * t.top;
-        for (int k0 = 0; k0 < t.top; k0 += 8) {
-            const bf16* w[8];
-            float pk[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int k = min(k0 + i, t.top - 1);
-                const bool ok = k0 + i < t.top && present(k);
-                pk[i] = ok ? (p == nullptr ? 1.f : p[k]) : 0.f;
-                w[i] = t.w + (pk[i] != 0.f ? ids[k] : 0ll) * t.width;
-            }
-            for (int c = lane * 8; c < t.width; c += 512) {
-                const bf16x8 xv = *reinterpret_cast<const bf16x8*>(x + c);
-                bf16x8 wv[8];
-#pragma unroll
-                for (int i = 0; i < 8; ++i)
-                    if (pk[i] != 0.f) wv[i] = *reinterpret_cast<const bf16x8*>(w[i] + c);
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    if (pk[i] == 0.f) continue;  // (not multiplied by 0: what an absent target's row holds does not count)
-                    float s = 0.f;
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) s = fmaf(bf16_to_f32(xv[e]), bf16_to_f32(wv[i][e]), s);
-                    base -= pk[i] * s * t.inv_tau;
-                }
-            }
+    __syncthreads();
+    for (int k = tid; k < t.top; k += THREADS) {
+        const int mine = id[k];
+        float m = 0.f;
+        bool first = mine >= 0;
+        for (int j = 0; j < padded; j += 4) {
+            const int4 i4 = *reinterpret_cast<const int4*>(id + j);
+            const float4 p4 = *reinterpret_cast<const float4*>(p + j);
+            m += (i4.x == mine ? p4.x : 0.f) + (i4.y == mine ? p4.y : 0.f) + (i4.z == mine ? p4.z : 0.f) + (i4.w == mine ? p4.w : 0.f);
+            first &= !((i4.x == mine && j < k) || (i4.y == mine && j + 1 < k) || (i4.z == mine && j + 2 < k) || (i4.w == mine && j + 3 < k));
         }
+        m = first ? m : 0.f;
+        merged[k] = m;
+        t.p[static_cast<size_t>(row) * t.top + k] = m;
     }
-    if (t.x_used != nullptr)
-        for (int c = lane * 8; c < t.width; c += 512) {
-            const size_t at = static_cast<size_t>(row) * t.width + c;
-            *reinterpret_cast<bf16x8*>(t.x_used + at) = some ? *reinterpret_cast<const bf16x8*>(t.x + at) : bf16x8{};
-        }
-    base = wave_sum(base);
-    if (lane == 0) {
+    __syncthreads();
+    if (t.x != nullptr && some)
+        base += vl_target_scores(t, row, 8 * (tid >> 6), THREADS / 8, tid & 63, [&](int k) { return merged[k]; }, [&](int k) { return static_cast<long long>(id[k]); });
+    vl_copy_used(t, row, tid, THREADS, some);
+    base = block_sum(base, red);
+    if (tid == 0) {
         t.base[row] = base;
         t.valid[row] = some ? 1 : 0;
     }
@@ -685,32 +725,6 @@ __global__ __launch_bounds__(1024) void vocab_mean_kernel(const float* __restric
     if (threadIdx.x == 0) loss[0] = s * scal[1];
 }
 
-// Targets of a row into LDS: id, and the weight of the id (entries that repeat an id add to its first place; others 0).
-// Returns through `own` whether this thread's entry k is the one that writes the id.
-struct TargetLds {
-    int id[VL_MAX_TOP];
-    float p[VL_MAX_TOP];
-};
-__device__ __forceinline__ void vl_load_targets(TargetLds& s, const long long* ids, const float* p, int top, long long vocab) {
-    for (int k = threadIdx.x; k < top; k += blockDim.x) {
-        const bool ok = ids[k] >= 0 && ids[k] < vocab;
-        s.id[k] = ok ? static_cast<int>(ids[k]) : -1;
-        s.p[k] = p != nullptr ? p[k] : 1.f;
-    }
-    __syncthreads();
-}
-__device__ __forceinline__ bool vl_merged(const TargetLds& s, int k, int top, float& p) {
-    const int id = s.id[k];
-    if (id < 0) return false;
-    p = 0.f;
-    for (int j = 0; j < top; ++j)
-        if (s.id[j] == id) {
-            if (j < k) return false;
-            p += s.p[j];
-        }
-    return true;
-}
-
 // ---- behind a projection: one workgroup per row joins the groups; training: exponentials -> q - p in place (e holds rows
 // rounded up to 64)
 struct Rows {
@@ -727,21 +741,24 @@ struct Rows {
     bool stream;
 };
 
-__global__ __launch_bounds__(256) void vocab_rows_kernel(const Rows a) {
+static_assert(VL_MAX_TOP <= 1024, "a thread per target");
+// (of 1024 threads: 8192 rows of 50257 entries 279 us for labels, 298 for 64 targets; with 512 threads 296 and 306, with 256
+// 312 and 328.  At 4.4 to 5.9 TB/s it is bound by memory.)
+__global__ __launch_bounds__(1024) void vocab_rows_kernel(const Rows a) {
+    constexpr int THREADS = 1024;
     __shared__ float red[16];
-    __shared__ TargetLds tg;
     const int row = blockIdx.x, tid = threadIdx.x;
     if (row >= a.rows) {  // rows up to a multiple of 64: zeros for the product over the rows
-        for (long long c = tid * 8; c < a.lde; c += 2048) *reinterpret_cast<bf16x8*>(a.e + row * a.lde + c) = bf16x8{};
+        for (long long c = tid * 8; c < a.lde; c += THREADS * 8) *reinterpret_cast<bf16x8*>(a.e + row * a.lde + c) = bf16x8{};
         return;
     }
     const float2* st = a.stats + static_cast<size_t>(row) * a.groups;
     float m = -VL_INF;
-    for (int g = tid; g < a.groups; g += 256) m = fmaxf(m, st[g].x);
+    for (int g = tid; g < a.groups; g += THREADS) m = fmaxf(m, st[g].x);
     m = block_max(m, red);
     const float ref = m == -VL_INF ? 0.f : m;
     float s = 0.f;
-    for (int g = tid; g < a.groups; g += 256) s += st[g].y * vl_exp2(st[g].x - ref);
+    for (int g = tid; g < a.groups; g += THREADS) s += st[g].y * vl_exp2(st[g].x - ref);
     s = block_sum(s, red);
     const float lse = ref + log2f(s);
     const bool valid = a.valid[row] != 0;
@@ -749,24 +766,15 @@ __global__ __launch_bounds__(256) void vocab_rows_kernel(const Rows a) {
     if (a.e == nullptr) return;
     bf16* e = a.e + row * a.lde;
     if (!valid) {
-        for (long long c = tid * 8; c < a.lde; c += 2048) *reinterpret_cast<bf16x8*>(e + c) = bf16x8{};
+        for (long long c = tid * 8; c < a.lde; c += THREADS * 8) *reinterpret_cast<bf16x8*>(e + c) = bf16x8{};
         return;
     }
-    vl_load_targets(tg, a.ids + static_cast<size_t>(row) * a.top, a.p == nullptr ? nullptr : a.p + static_cast<size_t>(row) * a.top, a.top, a.vocab);
-    float val[VL_MAX_TOP / 256];
-    uint32_t mine = 0;
-#pragma unroll
-    for (int i = 0; i < VL_MAX_TOP / 256; ++i) {
-        const int k = tid + i * 256;
-        float p;
-        if (k < a.top && vl_merged(tg, k, a.top, p)) {
-            const int id = tg.id[k];
-            val[i] = bf16_to_f32(e[id]) * vl_exp2(st[id >> 6].x - lse) - p;
-            mine |= 1u << i;
-        }
-    }
+    const long long* ids = a.ids + static_cast<size_t>(row) * a.top;
+    const float p = tid < a.top ? (a.p == nullptr ? 1.f : a.p[static_cast<size_t>(row) * a.top + tid]) : 0.f;
+    const int at = p != 0.f ? static_cast<int>(ids[tid]) : 0;
+    const float val = p != 0.f ? bf16_to_f32(e[at]) * vl_exp2(st[at >> 6].x - lse) - p : 0.f;
     __syncthreads();  // the targets' exponentials are read
-    for (long long c = tid * 8; c < a.lde; c += 2048) {
+    for (long long c = tid * 8; c < a.lde; c += THREADS * 8) {
         const float f = vl_exp2(st[c >> 6].x - lse);
         bf16x8 v = __builtin_nontemporal_load(reinterpret_cast<const bf16x8*>(e + c));
 #pragma unroll
@@ -774,9 +782,7 @@ __global__ __launch_bounds__(256) void vocab_rows_kernel(const Rows a) {
         vl_store(reinterpret_cast<bf16x8*>(e + c), v, a.stream);
     }
     __syncthreads();  // ... and every one is rewritten
-#pragma unroll
-    for (int i = 0; i < VL_MAX_TOP / 256; ++i)
-        if ((mine >> i) & 1) e[tg.id[tid + i * 256]] = f32_to_bf16(val[i]);
+    if (p != 0.f) e[at] = f32_to_bf16(val);
 }
 
 // ---- on given logits: one workgroup per row
@@ -810,7 +816,6 @@ template <typename T, int THREADS, int NV>
 __global__ __launch_bounds__(THREADS) void logits_distill_kernel(const Logits<T> a) {
     constexpr int W = 16 / sizeof(T);
     __shared__ float red[16];
-    __shared__ TargetLds tg;
     const int row = blockIdx.x, tid = threadIdx.x;
     const T* z = a.z + row * a.ldz;
     const bool valid = a.valid[row] != 0;
@@ -849,7 +854,8 @@ __global__ __launch_bounds__(THREADS) void logits_distill_kernel(const Logits<T>
             for (int c = tid; c < chunks; c += THREADS) f(c, load(c));
         }
     };
-    vl_load_targets(tg, a.ids + static_cast<size_t>(row) * a.top, a.p + static_cast<size_t>(row) * a.top, a.top, a.vocab);
+    const long long* ids = a.ids + static_cast<size_t>(row) * a.top;
+    const float* p = a.p + static_cast<size_t>(row) * a.top;
     float m = -VL_INF;
     each([&](int, vec x) {
 #pragma unroll
@@ -863,7 +869,7 @@ __global__ __launch_bounds__(THREADS) void logits_distill_kernel(const Logits<T>
         for (int e = 0; e < W; ++e) s += vl_exp2((static_cast<float>(x[e]) - ref) * a.scale_log2);
     });
     for (int k = tid; k < a.top; k += THREADS)
-        if (tg.id[k] >= 0 && tg.p[k] != 0.f) t += tg.p[k] * (static_cast<float>(z[tg.id[k]]) - ref);
+        if (p[k] != 0.f) t += p[k] * (static_cast<float>(z[ids[k]]) - ref);
     s = block_sum(s, red);
     t = block_sum(t, red);
     const float ls = log2f(s);
@@ -878,10 +884,8 @@ __global__ __launch_bounds__(THREADS) void logits_distill_kernel(const Logits<T>
         vl_store(reinterpret_cast<vec*>(dz + c * W), r, a.stream);
     });
     __syncthreads();
-    for (int k = tid; k < a.top; k += THREADS) {
-        float p;
-        if (vl_merged(tg, k, a.top, p)) dz[tg.id[k]] = static_cast<T>((q_of(static_cast<float>(z[tg.id[k]])) - p) * g);
-    }
+    for (int k = tid; k < a.top; k += THREADS)
+        if (p[k] != 0.f) dz[ids[k]] = static_cast<T>((q_of(static_cast<float>(z[ids[k]])) - p[k]) * g);
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -947,7 +951,11 @@ static bool vl_sizes_ok(int rows, int vocab, int width) {
 static int vl_targets(const long long* ids, const float* teacher, float* p, float* base, int* valid, float* scal, const void* x, const void* w,
                       void* x_used, int rows, int top, int width, int vocab, float tau, hipStream_t s) {
     Targets t = {ids, teacher, p, base, valid, static_cast<const bf16*>(x), static_cast<const bf16*>(w), static_cast<bf16*>(x_used), rows, top, width, vocab, 1.f / tau};
-    hipLaunchKernelGGL(vocab_targets_kernel, dim3(x_used == nullptr ? pdt_cdiv(rows, 4) : pdt_cdiv(rows, 64) * 16), dim3(256), 0, s, t);
+    const int all = x_used == nullptr ? rows : pdt_cdiv(rows, 64) * 64;
+    const int lds = (top + 3) / 4 * 4 * 12;
+    if (teacher != nullptr && (x != nullptr || top > 128)) hipLaunchKernelGGL(vocab_teacher_kernel<256>, dim3(all), dim3(256), lds, s, t);
+    else if (teacher != nullptr) hipLaunchKernelGGL(vocab_teacher_kernel<64>, dim3(all), dim3(64), lds, s, t);
+    else hipLaunchKernelGGL(vocab_labels_kernel, dim3(pdt_cdiv(all, 4)), dim3(256), 0, s, t);
     hipLaunchKernelGGL(vocab_count_kernel, dim3(1), dim3(1024), 0, s, valid, rows, tau, scal);
     return pdt_launch_status();
 }
@@ -1050,7 +1058,7 @@ PDT_API int pdt_head_loss(const void* x, const void* w, const long long* ids, co
         if (int e = vl_launch<0>(g, s)) return e;
         Rows a = {h.stats, h.e, pitch, ids + static_cast<size_t>(r0) * top, h.r.p == nullptr ? nullptr : h.r.p + static_cast<size_t>(r0) * top,
                   h.r.base + r0, h.r.valid + r0, h.r.row_loss + r0, g.groups, top, n, vocab, big};
-        hipLaunchKernelGGL(vocab_rows_kernel, dim3(train ? pdt_cdiv(n, 64) * 64 : n), dim3(256), 0, s, a);
+        hipLaunchKernelGGL(vocab_rows_kernel, dim3(train ? pdt_cdiv(n, 64) * 64 : n), dim3(1024), 0, s, a);
         g = {};
         g.lda = pitch; g.ldb = width;
         g.N = width;
