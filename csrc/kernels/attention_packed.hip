@@ -40,8 +40,9 @@ struct PackedArgs {
 
 #define AP_INF __builtin_inff()
 
-// Tiles in LDS per streamed operand of the query-side kernels: three (two on their way while one is read) for heads of 64;
-// two for heads of 128, so that two workgroups fit a CU - with three, one wave per SIMD has nothing to cover its softmax.
+// Tiles in LDS per streamed operand of the dQ kernel: three (two on their way while one is read) for heads of 64; two for heads
+// of 128, so that two workgroups fit a CU - with three, one wave per SIMD has nothing to cover its softmax.  The forward kernel
+// has two of either: four workgroups of 64-wide heads fit a CU.
 template <int NP>
 constexpr int ap_ring = NP == 1 ? AT_RING : 2;
 
@@ -309,12 +310,16 @@ __device__ __forceinline__ void ap_unit(const PackedArgs& p, int heads, int& blk
     to = e.z;
 }
 
+// Measured: D = 64, 16381 rows of documents of up to 1024, 16 heads, causal: 47 us - 150 MB of q, k, v, out and rest would take
+// 30 at the rate of a large copy; vector work (exponentials, the ends of short rows) and the waits of workgroups that live for
+// five tiles make up the rest.  D = 128, one document of 16384 rows, 16 heads on 4, causal: 1.08 ms, 1.02 PFLOP/s; matrix pipe and
+// vector ALU are busy 52 % and 45 % of the time, at 1.9 GHz.
 template <int NP>
 __global__ __launch_bounds__(256, NP == 1 ? 4 : 2) void packed_fwd_kernel(const PackedArgs p) {
     constexpr int TILE = NP * AT_TILE, RING = 2;
     extern __shared__ __attribute__((aligned(1024))) bf16 ap_smem[];
-    bf16* sK = ap_smem;                    // [RING][TILE]
-    bf16* sV = ap_smem + RING * TILE;   // [RING][TILE]
+    bf16* sK = ap_smem;                // [RING][TILE]
+    bf16* sV = ap_smem + RING * TILE;  // [RING][TILE]
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int hi = lane >> 5, lq = lane & 31;
     int blk, h, k_lo, k_hi;
@@ -339,9 +344,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 4 : 2) void packed_fwd_kernel(const 
         ap_tile_issue<NP>(dma, vbase, p.v_row, k_lo + t * AT_T, k_hi - 1, sV + slot * TILE, wave);
     };
     asm volatile("" ::: "memory");  // (the rows' own loads first: the counter of loads under way is in order)
-#pragma unroll
-    for (int t = 0; t < RING - 1; ++t)
-        if (t < nt) issue(t, t);
+    if (nt > 0) issue(0, 0);
     const Bounds wb = wave_bounds(span, k_lo, k_hi);
     const int t_lo = wb.hi > wb.lo ? (wb.lo - k_lo) / AT_T : nt, t_hi = wb.hi > wb.lo ? (wb.hi - k_lo + AT_T - 1) / AT_T : nt;
 
@@ -356,12 +359,11 @@ __global__ __launch_bounds__(256, NP == 1 ? 4 : 2) void packed_fwd_kernel(const 
     const uint32_t sk_lds = lds_addr(sK);
 
     int buf = 0;
-    auto next_tile = [&](int t) {  // (the protocol of the fixed-length kernels)
-        if (RING > 2 && t + 1 < nt) asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"n"(4 * NP) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-        if (t + RING - 1 < nt) issue(t + RING - 1, buf == 0 ? RING - 1 : buf - 1);
+    auto next_tile = [&](int t) {
+        asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
         const int cur = buf;
-        buf = buf == RING - 1 ? 0 : buf + 1;
+        buf ^= 1;
+        if (t + 1 < nt) issue(t + 1, buf);
         return cur;
     };
     constexpr int PANEL = AT_TILE * 2, V_AT = RING * TILE * 2;  // bytes
@@ -446,56 +448,34 @@ __global__ __launch_bounds__(256, NP == 1 ? 4 : 2) void packed_fwd_kernel(const 
             ++t;
         } while (t < t_hi && k_lo + t * AT_T <= wb.max_lo);
         for (; t < t_hi; ++t) {
-            // two halves of 32 keys, so that the matrix pipe has work while the vector ALU turns scores into probabilities:
-            //   S(0) S(1) | softmax(0) | PV(0) | softmax(1) | PV(1)
+            // Two halves of 32 keys.  Heads of 128: S(0) S(1) | softmax(0) | PV(0) | softmax(1) | PV(1), so that the matrix pipe has
+            // work while the vector ALU turns scores into probabilities; heads of 64 one after the other, which takes registers
+            // for four waves per SIMD instead of three (16381 rows of documents, 16 heads: 47 us instead of 52).
             const int k0 = k_lo + t * AT_T;
             enter_tile(t);
-            if constexpr (NP == 1) {
-                bool out = false;
-                ap_for<2>([&](auto kt) {
-                    if (out) return;
-                    f32x16 acc;
-                    scores(acc, kt);
-                    read_v(kt);
-                    mask(acc, k0, kt);
-                    const float l = probs(acc);
-                    kt0 = kt;
-                    if (__builtin_expect(__any(!(l <= 1073741824.f)), 0)) {
-                        lds_wait<0>();
-                        out = true;
-                        return;
-                    }
-                    lsum += l;
-                    values(acc);
-                    __builtin_amdgcn_sched_barrier(0);
-                });
-                entered = true;
-                if (out) break;
-            } else {
-            f32x16 acc0, acc1;
-            scores(acc0, C0{});
-            scores(acc1, C1{});
-            read_v(C0{});
-            mask(acc0, k0, 0);
-            const float l0 = probs(acc0);
             entered = true;
-            if (__builtin_expect(__any(!(l0 <= 1073741824.f)), 0)) {
-                lds_wait<0>();  // (the value fragments are read again)
-                break;
+            auto finish = [&](f32x16& acc, auto kt) {  // false: the maximum rose
+                read_v(kt);
+                mask(acc, k0, kt);
+                const float l = probs(acc);
+                kt0 = kt;
+                if (__builtin_expect(__any(!(l <= 1073741824.f)), 0)) {
+                    lds_wait<0>();  // (the value fragments are read again)
+                    return false;
+                }
+                lsum += l;
+                values(acc);
+                return true;
+            };
+            f32x16 acc[NP];
+            scores(acc[0], C0{});
+            if constexpr (NP == 2) scores(acc[1], C1{});
+            if (!finish(acc[0], C0{})) break;
+            if constexpr (NP == 1) {
+                __builtin_amdgcn_sched_barrier(0);
+                scores(acc[0], C1{});
             }
-            lsum += l0;
-            values(acc0);
-            read_v(C1{});
-            mask(acc1, k0, 1);
-            const float l1 = probs(acc1);
-            kt0 = 1;
-            if (__builtin_expect(__any(!(l1 <= 1073741824.f)), 0)) {
-                lds_wait<0>();
-                break;
-            }
-            lsum += l1;
-            values(acc1);
-            }
+            if (!finish(acc[NP - 1], C1{})) break;
             entered = false;
             kt0 = 0;
             __builtin_amdgcn_sched_barrier(0);
@@ -557,6 +537,8 @@ __global__ __launch_bounds__(256, NP == 1 ? 4 : 2) void packed_fwd_kernel(const 
     }
 }
 
+// dQ, and the row terms that dK / dV start from.  Measured as the forward kernel: D = 64 64 us (218 MB, 43 us at a copy's rate);
+// D = 128 1.48 ms, 1.11 PFLOP/s (three products), matrix pipe busy 54 %.
 template <int NP>
 __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const PackedArgs p) {
     constexpr int TILE = NP * AT_TILE, RING = ap_ring<NP>;
@@ -760,6 +742,8 @@ __device__ __forceinline__ void dkv_store(const PackedArgs& p, f32x16 (&acc)[2 *
     }
 }
 
+// dK and dV of 64-wide heads.  Measured as the forward kernel: 72 us (201 MB, 40 us at a copy's rate), 80 with two waves per SIMD,
+// more of each operand on its way and the row terms applied behind the products.
 __global__ __launch_bounds__(256, 3) void packed_dkv64_kernel(const PackedArgs p) {
     constexpr int NP = 1;
     constexpr int TILE = NP * AT_TILE;
@@ -912,6 +896,10 @@ __global__ __launch_bounds__(256, 3) void packed_dkv64_kernel(const PackedArgs p
 // P goes from the one to the other through LDS in fp32, register for register (the two products have the same layout).  The
 // work is a sequence of phases of 32 queries with a barrier each; the dS waves run one phase behind.  Tiles are 64 queries
 // (32 KB with dO) in a ring of three: one arriving, one of the P waves, one that the dS waves may still need.
+// Measured as the forward kernel: 2.3 ms, 0.96 PFLOP/s (four products), matrix pipe busy 43 %: a phase takes 2400 cycles of which
+// the two waves' products are 1024, the rest is each wave's chain from one product over the vector work to the next.  (dS
+// waves half a phase out of step with the P waves, their dK products under the P waves' exponentials: 2.49 ms; products in front of
+// the other waves' vector work by s_setprio: 2.48 ms.)
 __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs p) {
     constexpr int TILE = 2 * AT_TILE, PANEL = AT_TILE * 2, DO_AT = AT_RING * TILE * 2;  // elements; bytes
     extern __shared__ __attribute__((aligned(1024))) bf16 ap_smem[];
@@ -1167,9 +1155,12 @@ __global__ __launch_bounds__(256) void pack_order_kernel(const int4* __restrict_
     if (b < blocks) order[static_cast<size_t>(blockIdx.y) * blocks + rank] = e;
 }
 
-// Packs of few blocks (one round of workgroups) and of very many (the last round does not matter) keep the rows' own order.
-#define AP_ORDER_FROM 16
-#define AP_ORDER_TO 8192
+// Packs of few blocks (one round of workgroups) and of very many (the last round does not matter, the counting does) keep the
+// rows' own order.  Pack, forward and backward in this order and in the rows' own: 18 blocks of one document, 16 heads of 64 131 and
+// 125 us, 32 blocks 233 and 228, 32 blocks with 32 heads of 128 476 and 486, 64 blocks of documents of up to 4096 rows 506 and 530,
+// 4096 blocks, 2 heads of 64 1202 and 1213, 8192 blocks 2690 and 2385.
+#define AP_ORDER_FROM 31
+#define AP_ORDER_TO 4096
 
 // offsets: [sequences + 1] int32, not falling.  order: [3][ceil(rows / 128)] entries of 16 bytes; work: scratch of the same size.
 PDT_API int pdt_pack_spans(const int* offsets, int sequences, int rows, void* spans, long long* positions, void* order, void* work, void* stream) {
@@ -1249,7 +1240,9 @@ PDT_API int pdt_packed_attention_fwd(const void* q, const void* k, const void* v
 }
 
 // How many ways the backward pass splits the query heads of a key head (1: no partial sums).  A key block with all the
-// heads of its group is one workgroup; with few key heads that leaves CUs idle.
+// heads of its group is one workgroup; with few key heads that leaves CUs idle.  Forward and backward with and without: 4096
+// rows, 16 heads of 128 on one key head 333 and 1601 us, 32 on eight 476 and 599 (with up to 1024 workgroups 490); 1024 rows, 16
+// heads of 64 on four 80 and 132.
 PDT_API int pdt_packed_attention_splits(int T, int H, int Hk) {
     const int group = H / Hk, units = pdt_cdiv(T, AT_BR) * Hk;
     int s = 1;

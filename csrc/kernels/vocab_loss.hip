@@ -23,8 +23,9 @@ typedef const __attribute__((address_space(1))) void vl_global_cvoid;
 #define VL_MAX_TOP 1024
 #define VL_MAX_ROWS (1 << 22)  // a workgroup of up to 1024 threads a row, 2^32 threads a launch
 
-// A buffer far larger than the caches is written around them (measured on 8192 x 50257 bf16: the scores kernel 798 -> 757 us,
-// the pass over the rows 365 -> 311 us, distillation on logits 409 -> 379 us); a smaller one is read again from them.
+// A buffer far larger than the caches is written around them: 8192 x 50257 bf16, loss and gradients 2346 -> 2266 us, distillation
+// on logits 393 -> 377 us, 2048 rows 544 -> 537 us.  One that the caches hold is read again from them: 512 rows 188 us, written
+// around them 191; 64 rows 103 and 105.
 #define VL_STREAM_BYTES (64ll << 20)
 template <typename V>
 __device__ __forceinline__ void vl_store(V* at, V v, bool stream) {
@@ -63,6 +64,11 @@ __device__ __forceinline__ float vl_exp2(float x) { return __builtin_amdgcn_exp2
 //
 // Work: whole tiles first, a multiple of the workgroups; the tiles left over (all, where the tiles are few) are cut along k
 // into parts that fill the last round, summed in order by vocab_join_kernel.
+//
+// Measured (a library product of 8192^3 in bf16 runs at 1.5 PFLOP/s): 8192 rows, 50257 entries, width 1024: scores 757 to 800 us
+// (1.05 to 1.1 PFLOP/s: 16 K-steps, then exponentials, maxima and 128 KB of results per tile), dx and dW 635 to 660 us (1.3);
+// 130001 entries, width 2048: 3.5, 3.1 and 3.2 ms (1.25, 1.4, 1.36).  Bound by the matrix pipe between the tiles' ends.  512 rows,
+// width 768: 54, 43 and 51 us; 64 rows, scores alone: 22 us, W read at 3.5 TB/s.
 // ------------------------------------------------------------------------------------------------
 struct VocabGemm {
     const bf16 *a, *b;
@@ -811,7 +817,9 @@ struct ChunkOf {
 };
 
 // The row stays in registers (NV chunks of 16 bytes per thread) between its maximum, its sum and the gradient: one read and
-// one write of the logits.  NV = 0: rows too long for that are read again from the caches.
+// one write of the logits, 4.5 TB/s on 8192 rows of 50257 in bf16 (364 us).  NV = 0: rows too long for that are read again from
+// the caches; rows of all lengths done so: 8192 x 8000 119 us instead of 71, 8192 x 50257 561 instead of 377, 2048 x 131000 319
+// instead of 253 (2048 x 140000, too long: 340).
 template <typename T, int THREADS, int NV>
 __global__ __launch_bounds__(THREADS) void logits_distill_kernel(const Logits<T> a) {
     constexpr int W = 16 / sizeof(T);
@@ -888,6 +896,18 @@ __global__ __launch_bounds__(THREADS) void logits_distill_kernel(const Logits<T>
         if (p[k] != 0.f) dz[ids[k]] = static_cast<T>((q_of(static_cast<float>(z[ids[k]])) - p[k]) * g);
 }
 
+// x *= g[0] unless g[0] == 1 (the gradient of a loss that is the root of the graph): a pass over an fp32 gradient saved
+__global__ __launch_bounds__(256) void vocab_scale_kernel(f32x4* __restrict__ x, const float* __restrict__ g, long long n) {
+    const float gv = g[0];
+    if (gv == 1.f) return;
+    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
+        f32x4 v = x[i];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] *= gv;
+        x[i] = v;
+    }
+}
+
 // ------------------------------------------------------------------------------------------------
 // entry points
 // ------------------------------------------------------------------------------------------------
@@ -911,7 +931,8 @@ static int vl_cus() {
 }
 
 // Tiles in whole rounds of the CUs first; the rest in parts of at least eight K-steps that fill the last round, if it would
-// be less than 3/4 full.
+// be less than 3/4 full.  Loss and gradients with and without: 64 rows of 50257 entries of width 768 103 and 921 us, 512 rows
+// 188 and 987, 2048 rows 537 and 1251, 8192 rows of width 1024 2266 and 2602.
 static void vl_plan(VocabGemm& g, bool split) {
     g.tiles_m = pdt_cdiv(g.M, 256);
     g.tiles_n = pdt_cdiv(g.N, 256);
@@ -1127,4 +1148,13 @@ PDT_API int pdt_distill(const void* z, void* dz, const long long* ids, const flo
     const int e = dtype == 1 ? distill_launch(Logits<bf16>{static_cast<const bf16*>(z), static_cast<bf16*>(dz), ldz, ldd, ids, r.p, r.base, r.valid, r.scal, r.row_loss, top, vocab, c, it, big}, rows, s)
                              : distill_launch(Logits<float>{static_cast<const float*>(z), static_cast<float*>(dz), ldz, ldd, ids, r.p, r.base, r.valid, r.scal, r.row_loss, top, vocab, c, it, big}, rows, s);
     return e != 0 ? e : vl_mean(r.row_loss, r.scal, loss, rows, s);
+}
+
+// fp32 x (16-byte aligned, a multiple of four elements) times a device scalar, in place; nothing is touched where it is 1.
+PDT_API int pdt_scale_by_scalar_f32(float* x, const float* g, long long numel, void* stream) {
+    if (numel <= 0 || (numel % 4) != 0) return -1;
+    const long long blocks = (numel / 4 + 255) / 256;
+    hipLaunchKernelGGL(vocab_scale_kernel, dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(256), 0, static_cast<hipStream_t>(stream),
+                       reinterpret_cast<f32x4*>(x), g, numel / 4);
+    return pdt_launch_status();
 }
