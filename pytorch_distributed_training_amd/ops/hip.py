@@ -108,6 +108,17 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+def _once_differentiable(backward):
+    """``torch.autograd.function.once_differentiable``, whose context costs 4 us of host time: entered only where a graph of the
+    backward pass is recorded (elsewhere gradients are off already)."""
+    guarded = torch.autograd.function.once_differentiable(backward)
+
+    def run(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return run
+
+
 def _on(device: torch.device):
     """The device a kernel is launched on, made current where it is not."""
     return _contextlib.nullcontext() if device.index == torch.cuda.current_device() else torch.cuda.device(device)

@@ -9,7 +9,7 @@ import ctypes
 
 import torch
 
-from .hip import _check, _on, _ptr, _stream
+from .hip import _check, _on, _once_differentiable, _ptr, _stream
 from .hip_transformer import _f, _i, _sig, _vp
 
 _pack_spans = _sig("pdt_pack_spans", [_vp, _i, _i] + [_vp] * 5)
@@ -52,17 +52,20 @@ def _strides(*xs):
 
 
 def _forward(q, k, v, plan, causal: bool, scale: float, train: bool):
+    """(out, what the backward pass needs beside it: a byte per element of out, what its rounding took, then the fp32 row
+    terms ``[h, t]``; without a backward pass the row terms alone)."""
     t, h, d = q.shape
     out = torch.empty((t, h, d), dtype=torch.bfloat16, device=q.device)
-    rest = torch.empty((t, h, d), dtype=torch.uint8, device=q.device) if train else None  # what rounding took from out: the backward pass's row terms need it
-    lse = torch.empty((h, t), dtype=torch.float32, device=q.device)
+    aside = torch.empty(t * h * (1 + d // 4 if train else 1), dtype=torch.float32, device=q.device)
     if out.numel():
-        _check(_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), _ptr(rest), lse.data_ptr(), plan.data_ptr() + 8 * t, plan.data_ptr() + 16 * t, _strides(q, k, v),
-                    t, h, k.shape[1], d, scale, int(causal), _stream()), "packed_attention_fwd")
-    return out, rest, lse
+        rest = aside.data_ptr() if train else None
+        lse = aside.data_ptr() + (t * h * d if train else 0)
+        _check(_fwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest, lse, plan.data_ptr() + 8 * t,
+                    plan.data_ptr() + 16 * t, _strides(q, k, v), t, h, k.shape[1], d, scale, int(causal), _stream()), "packed_attention_fwd")
+    return out, aside
 
 
-def _backward(q, k, v, out, rest, lse, g, plan, causal: bool, scale: float, dq, dk, dv) -> None:
+def _backward(q, k, v, out, aside, g, plan, causal: bool, scale: float, dq, dk, dv) -> None:
     t, h, d = q.shape
     hk = k.shape[1]
     if not q.numel():
@@ -74,7 +77,7 @@ def _backward(q, k, v, out, rest, lse, g, plan, causal: bool, scale: float, dq, 
     delta = torch.empty((h, t), dtype=torch.float32, device=q.device)
     splits = _splits(t, h, hk)
     part = torch.empty((splits, 2, t, hk, d), dtype=torch.float32, device=q.device) if splits > 1 else None
-    _check(_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), rest.data_ptr(), g.data_ptr(), lse.data_ptr(), delta.data_ptr(),
+    _check(_bwd(q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), aside.data_ptr(), g.data_ptr(), aside.data_ptr() + t * h * d, delta.data_ptr(),
                 dq.data_ptr(), dk.data_ptr(), dv.data_ptr(), _ptr(part), splits, plan.data_ptr() + 8 * t, plan.data_ptr() + 16 * t, _strides(q, k, v, dq, dk, dv), t, h, hk, d, scale,
                 int(causal), _stream()), "packed_attention_bwd")
 
@@ -84,18 +87,18 @@ class _AttentionPacked(torch.autograd.Function):
     def forward(ctx, q, k, v, plan, causal: bool, scale: float):
         with _on(q.device):
             q, k, v = _heads(q), _heads(k), _heads(v)
-            out, rest, lse = _forward(q, k, v, plan, causal, scale, any(ctx.needs_input_grad[:3]))
-        ctx.save_for_backward(q, k, v, out, rest, lse, plan)
+            out, aside = _forward(q, k, v, plan, causal, scale, any(ctx.needs_input_grad[:3]))
+        ctx.save_for_backward(q, k, v, out, aside, plan)
         ctx.meta = (causal, scale)
         return out
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, g):
-        q, k, v, out, rest, lse, plan = ctx.saved_tensors
+        q, k, v, out, aside, plan = ctx.saved_tensors
         with _on(q.device):
             dq, dk, dv = (torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) for x in (q, k, v))
-            _backward(q, k, v, out, rest, lse, g, plan, *ctx.meta, dq, dk, dv)
+            _backward(q, k, v, out, aside, g, plan, *ctx.meta, dq, dk, dv)
         return dq, dk, dv, None, None, None
 
 
@@ -116,19 +119,19 @@ class _AttentionPackedQKV(torch.autograd.Function):
                 qkv = qkv.to(torch.bfloat16)
             if not qkv.is_contiguous() or qkv.data_ptr() % 16:
                 qkv = qkv.clone(memory_format=torch.contiguous_format)
-            out, rest, lse = _forward(*_split_qkv(qkv, heads, kv_heads), plan, causal, scale, ctx.needs_input_grad[0])
-        ctx.save_for_backward(qkv, out, rest, lse, plan)
+            out, aside = _forward(*_split_qkv(qkv, heads, kv_heads), plan, causal, scale, ctx.needs_input_grad[0])
+        ctx.save_for_backward(qkv, out, aside, plan)
         ctx.meta = (heads, kv_heads, causal, scale)
         return out.flatten(1)
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, g):
-        qkv, out, rest, lse, plan = ctx.saved_tensors
+        qkv, out, aside, plan = ctx.saved_tensors
         heads, kv_heads, causal, scale = ctx.meta
         with _on(qkv.device):
             dqkv = torch.empty_like(qkv)
-            _backward(*_split_qkv(qkv, heads, kv_heads), out, rest, lse, g.reshape(out.shape), plan, causal, scale,
+            _backward(*_split_qkv(qkv, heads, kv_heads), out, aside, g.reshape(out.shape), plan, causal, scale,
                       *_split_qkv(dqkv, heads, kv_heads))
         return dqkv, None, None, None, None, None
 

@@ -10,7 +10,7 @@ import os
 
 import torch
 
-from .hip import SHADOWS, _axpy_dev, _check, _grad_sink, _on, _ptr, _round_up, _scale_by_scalar, _stream
+from .hip import SHADOWS, _axpy_dev, _check, _grad_sink, _on, _once_differentiable, _ptr, _round_up, _scale_by_scalar, _stream
 from .hip_transformer import _f, _i, _ll, _sig, _vp
 
 _head_scratch = _sig("pdt_head_loss_scratch", [_i] * 8)
@@ -84,7 +84,7 @@ class _HeadLoss(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, g):
         dx, dw = ctx.grads
         ctx.grads = [None, None]
@@ -92,7 +92,7 @@ class _HeadLoss(torch.autograd.Function):
             raise RuntimeError("the loss behind a projection handed its gradients out already (backward ran twice)")
         weight = ctx.weight
         with _on(g.device):
-            g1 = g.reshape(1).to(torch.float32).contiguous()
+            g1 = g if g.dtype == torch.float32 else g.to(torch.float32)
             for d in (dx, dw):
                 if d is not None and d.dtype == torch.bfloat16:
                     _check(_scale_by_scalar(d.data_ptr(), g1.data_ptr(), d.numel(), _stream()), "scale_by_scalar")
@@ -144,18 +144,20 @@ class _LogitsDistill(torch.autograd.Function):
         return loss
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
+    @_once_differentiable
     def backward(ctx, g):
         dz, ctx.dz = ctx.dz, None
         if dz is None:
             raise RuntimeError("the distillation loss handed its gradient out already (backward ran twice)")
         with _on(g.device):
-            g1 = g.reshape(1).to(torch.float32).contiguous()
+            g1 = g if g.dtype == torch.float32 else g.to(torch.float32)
             if dz.dtype == torch.bfloat16:
                 _check(_scale_by_scalar(dz.data_ptr(), g1.data_ptr(), dz.numel(), _stream()), "scale_by_scalar")
             else:
                 _check(_scale_f32(dz.data_ptr(), g1.data_ptr(), dz.numel(), _stream()), "scale_by_scalar_f32")
-        return dz[:, :ctx.shape[-1]].reshape(ctx.shape), None, None, None
+        if dz.shape[1] != ctx.shape[-1]:
+            dz = dz[:, :ctx.shape[-1]]
+        return dz.reshape(ctx.shape), None, None, None
 
 
 def logits_distill(logits, ids, teacher, tau: float):
