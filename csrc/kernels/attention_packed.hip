@@ -538,7 +538,7 @@ __global__ __launch_bounds__(256, NP == 1 ? 4 : 2) void packed_fwd_kernel(const 
 }
 
 // dQ, and the row terms that dK / dV start from.  Measured as the forward kernel: D = 64 64 us (218 MB, 43 us at a copy's rate);
-// D = 128 1.48 ms, 1.11 PFLOP/s (three products), matrix pipe busy 54 %.
+// D = 128 1.44 to 1.48 ms, 1.11 to 1.14 PFLOP/s (three products), matrix pipe busy 60 % at 1.85 GHz.
 template <int NP>
 __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const PackedArgs p) {
     constexpr int TILE = NP * AT_TILE, RING = ap_ring<NP>;
@@ -896,7 +896,7 @@ __global__ __launch_bounds__(256, 3) void packed_dkv64_kernel(const PackedArgs p
 // P goes from the one to the other through LDS in fp32, register for register (the two products have the same layout).  The
 // work is a sequence of phases of 32 queries with a barrier each; the dS waves run one phase behind.  Tiles are 64 queries
 // (32 KB with dO) in a ring of three: one arriving, one of the P waves, one that the dS waves may still need.
-// Measured as the forward kernel: 2.3 ms, 0.96 PFLOP/s (four products), matrix pipe busy 43 %: a phase takes 2400 cycles of which
+// Measured as the forward kernel: 2.3 ms, 0.96 PFLOP/s (four products), matrix pipe busy 46 %: a phase takes 2400 cycles of which
 // the two waves' products are 1024, the rest is each wave's chain from one product over the vector work to the next.  (dS
 // waves half a phase out of step with the P waves, their dK products under the P waves' exponentials: 2.49 ms; products in front of
 // the other waves' vector work by s_setprio: 2.48 ms.)
