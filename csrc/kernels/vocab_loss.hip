@@ -130,6 +130,31 @@ __device__ __forceinline__ void vl_wait_lds() {
     __builtin_amdgcn_sched_barrier(0);
 }
 
+// v of this lane and of lane ^ 16 (or ^ 32), in either order, on the vector ALU
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+template <int LANES>
+__device__ __forceinline__ void vl_both(float v, float& a, float& b) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, v);
+    u32x2 r;
+    if constexpr (LANES == 16) r = __builtin_amdgcn_permlane16_swap(x, x, false, false);
+    else r = __builtin_amdgcn_permlane32_swap(x, x, false, false);
+    const uint32_t lo = r[0], hi = r[1];  // (a bit cast of a vector's element itself reads element 0)
+    a = __builtin_bit_cast(float, lo);
+    b = __builtin_bit_cast(float, hi);
+}
+__device__ __forceinline__ float vl_max4(float v) {  // over lanes l, l ^ 16, l ^ 32, l ^ 48
+    float a, b;
+    vl_both<16>(v, a, b);
+    vl_both<32>(fmaxf(a, b), a, b);
+    return fmaxf(a, b);
+}
+__device__ __forceinline__ float vl_sum4(float v) {
+    float a, b;
+    vl_both<16>(v, a, b);
+    vl_both<32>(a + b, a, b);
+    return a + b;
+}
+
 template <bool KMAJOR>
 __device__ __forceinline__ int vl_swz(int row) { return KMAJOR ? (row & 3) | ((row >> 1) & 4) : row & 7; }
 
@@ -477,8 +502,7 @@ __global__ __launch_bounds__(512) void vocab_gemm_kernel(const VocabGemm p) {
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e) mx = fmaxf(mx, acc[i][j][e]);
-                    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-                    mx = fmaxf(mx, __shfl_xor(mx, 32, 64)) * p.scale_log2;
+                    mx = vl_max4(mx) * p.scale_log2;
                     const float ref = mx == -VL_INF ? 0.f : mx;  // (a group beyond the vocabulary, or one that is masked out)
                     float sum = 0.f;
 #pragma unroll
@@ -488,8 +512,7 @@ __global__ __launch_bounds__(512) void vocab_gemm_kernel(const VocabGemm p) {
                             acc[i][j][e] = vl_exp2(fmaf(acc[i][j][e], p.scale_log2, -ref));
                             sum += acc[i][j][e];
                         }
-                    sum += __shfl_xor(sum, 16, 64);
-                    sum += __shfl_xor(sum, 32, 64);
+                    sum = vl_sum4(sum);
                     if (g4 == 0 && m < p.M && nw < p.N) p.stats[static_cast<size_t>(m) * p.groups + (nw >> 6)] = float2{mx, sum};
                     if (p.e == nullptr) continue;
                 }
