@@ -896,8 +896,9 @@ __global__ __launch_bounds__(256, 3) void packed_dkv64_kernel(const PackedArgs p
 // P goes from the one to the other through LDS in fp32, register for register (the two products have the same layout).  The
 // work is a sequence of phases of 32 queries with a barrier each; the dS waves run one phase behind.  Tiles are 64 queries
 // (32 KB with dO) in a ring of three: one arriving, one of the P waves, one that the dS waves may still need.
-// Measured as the forward kernel: 2.3 ms, 0.96 PFLOP/s (four products), matrix pipe busy 46 %: a phase takes 2400 cycles of which
-// the two waves' products are 1024, the rest is each wave's chain from one product over the vector work to the next.  (dS
+// Measured as the forward kernel: 2.25 to 2.33 ms, 0.94 to 0.98 PFLOP/s (four products), matrix pipe busy 46 %: a phase takes 2400 cycles of which
+// the two waves' products are 1024, the rest is each wave's chain from one product over the vector work to the next.  (Products issued behind the wait for
+// the other operands instead of between their reads: 3 % slower; all reads issued first: the same; dS
 // waves half a phase out of step with the P waves, their dK products under the P waves' exponentials: 2.49 ms; products in front of
 // the other waves' vector work by s_setprio: 2.48 ms.)
 __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs p) {
@@ -1007,6 +1008,7 @@ __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs 
             for (int e = 0; e < 16; ++e) c[e] = rt[e >> 2][e & 3];  // (the row term starts the sum)
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks) c = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), own[ks], c, 0, 0, 0);
+            asm volatile("" : "+v"(c));  // (issued before any wait below)
             if constexpr (IS_P) {
                 const int q0 = q_lo + t * AT_T + 32 * half;
                 if (q0 < wb.max_lo || q0 + 32 > wb.min_hi) mask_outside(c, span.x - q0 - 4 * hi, span.y - q0 - 4 * hi);
@@ -1018,7 +1020,7 @@ __global__ __launch_bounds__(512, 2) void packed_dkv128_kernel(const PackedArgs 
                     asm volatile("ds_write_b128 %0, %1 offset:%2" ::"v"(sp_lds), "v"(v), "n"(half * 16384 + r4 * 1024) : "memory");
                 }
             }
-            lds_wait<0>();
+            lds_wait<IS_P ? 4 : 0>();  // (the four writes of P may be under way until the phase ends)
 #pragma unroll
             for (int d = 0; d < 4; ++d) taken(ft[d]);
             if constexpr (!IS_P) {
