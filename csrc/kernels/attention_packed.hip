@@ -642,6 +642,9 @@ __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const P
 #pragma unroll
                 for (int ks = 0; ks < 4 * NP; ++ks)
                     s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_rows_get(f[ks >> 2], ks & 3), qf[ks], ks == 0 ? f32x16{} : s, 0, 0, 0);
+                // 64-wide heads: issued before the wait below; 128-wide ones as one run of sixteen behind it (long document: 1462 us,
+                // 1505 the other way), in front of which the other wave of the SIMD does its vector work
+                if constexpr (NP == 1) asm volatile("" : "+v"(s));
                 __builtin_amdgcn_s_setprio(0);
                 __builtin_amdgcn_sched_barrier(0);
                 ap_for<NP>([&](auto pn) { read_rows<V_AT + pn * PANEL + kt * 4096>(f[pn], at.row); });  // (under the products just issued)
