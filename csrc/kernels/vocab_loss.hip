@@ -65,8 +65,8 @@ __device__ __forceinline__ float vl_exp2(float x) { return __builtin_amdgcn_exp2
 // Work: whole tiles first, a multiple of the workgroups; the tiles left over (all, where the tiles are few) are cut along k
 // into parts that fill the last round, summed in order by vocab_join_kernel.
 //
-// Measured (a library product of 8192^3 in bf16 runs at 1.5 PFLOP/s): 8192 rows, 50257 entries, width 1024: scores 757 to 800 us
-// (1.05 to 1.1 PFLOP/s: 16 K-steps, then exponentials, maxima and 128 KB of results per tile), dx and dW 635 to 660 us (1.3);
+// Measured (a library product of 8192^3 in bf16 runs at 1.5 PFLOP/s): 8192 rows, 50257 entries, width 1024: scores 768 us
+// (1.1 PFLOP/s: 16 K-steps, then exponentials, maxima and 128 KB of results per tile), dx and dW 635 to 660 us (1.3);
 // 130001 entries, width 2048: 3.5, 3.1 and 3.2 ms (1.25, 1.4, 1.36).  Bound by the matrix pipe between the tiles' ends.  512 rows,
 // width 768: 54, 43 and 51 us; 64 rows, scores alone: 22 us, W read at 3.5 TB/s.
 // ------------------------------------------------------------------------------------------------

@@ -68,7 +68,7 @@ def _forward(q, k, v, plan, causal: bool, scale: float, train: bool):
 def _backward(q, k, v, out, aside, g, plan, causal: bool, scale: float, dq, dk, dv) -> None:
     t, h, d = q.shape
     hk = k.shape[1]
-    if not q.numel():
+    if t == 0:
         return
     if g.dtype != torch.bfloat16:
         g = g.to(torch.bfloat16)
@@ -97,7 +97,7 @@ class _AttentionPacked(torch.autograd.Function):
     def backward(ctx, g):
         q, k, v, out, aside, plan = ctx.saved_tensors
         with _on(q.device):
-            dq, dk, dv = (torch.empty(x.shape, dtype=torch.bfloat16, device=x.device) for x in (q, k, v))
+            dq, dk, dv = torch.empty_like(q), torch.empty_like(k), torch.empty_like(v)
             _backward(q, k, v, out, aside, g, plan, *ctx.meta, dq, dk, dv)
         return dq, dk, dv, None, None, None
 

@@ -417,3 +417,27 @@ def test_pack_devices_and_embedding_refusals(ops):
     wpe = torch.arange(10.0, device="cuda")[:, None].repeat(1, 64)
     got = ops.token_position_embedding(torch.zeros(12, dtype=torch.int64, device="cuda"), table, wpe, long)
     assert got[:, 0].tolist() == [0, 1, 2, 3, 4, 5, 6, 7, 8, 9, 9, 9]
+
+
+def test_gradients_of_views_that_are_not_dense(ops):
+    """Keys and values as slices of wider tensors, one head of several, one row of several: gradients of any layout."""
+    t, d = 140, 64
+    q, k, v, do = _inputs(t, 4, 2, d, seed=21)
+    pack = ops.pack_sequences([0, 75, t], t, device="cuda")
+    want = [x.detach().requires_grad_(True) for x in (q, k, v)]
+    a = torch.autograd.grad(ops.attention_packed(*want, pack), want, do)
+    wide = torch.zeros(2, t, 5, 3 * d, dtype=torch.bfloat16, device="cuda")
+    views = [wide[0, :, :4, :d], wide[0, :, 1:3, d:2 * d], wide[1].transpose(0, 1)[3:5, :, 2 * d:].transpose(0, 1)]
+    views = [x.copy_(y).detach().requires_grad_(True) for x, y in zip(views, (q, k, v))]
+    b = torch.autograd.grad(ops.attention_packed(views[0], views[1], views[2], pack), views, do)
+    # (the first two views overlap in nothing but their memory's rows; every gradient is its own tensor)
+    assert all(torch.equal(x, y) for x, y in zip(a, b))
+    one = ops.pack_sequences([0, 1], 1, device="cuda")
+    row = [x[5:6].detach().requires_grad_(True) for x in (q, k, v)]
+    col = [x.transpose(0, 1).contiguous().transpose(0, 1)[5:6].detach().requires_grad_(True) for x in (q, k, v)]
+    for x, y in zip(*(torch.autograd.grad(ops.attention_packed(*r, one), r, do[5:6]) for r in (row, col))):
+        assert torch.equal(x, y)
+    single = [x[:, 1:2].detach().requires_grad_(True) for x in (q, k, v)]
+    dense = [x.detach().contiguous().requires_grad_(True) for x in single]
+    for x, y in zip(*(torch.autograd.grad(ops.attention_packed(*r, pack), r, do[:, 1:2]) for r in (single, dense))):
+        assert torch.equal(x, y)
