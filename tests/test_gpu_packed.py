@@ -441,3 +441,59 @@ def test_gradients_of_views_that_are_not_dense(ops):
     dense = [x.detach().contiguous().requires_grad_(True) for x in single]
     for x, y in zip(*(torch.autograd.grad(ops.attention_packed(*r, pack), r, do[:, 1:2]) for r in (single, dense))):
         assert torch.equal(x, y)
+
+
+def test_captured_training_step_of_packed_gpt2(ops):
+    """Forward and backward of the packed model, its pack included, replayed over other documents; gradients land in .grad."""
+    from pytorch_distributed_training_amd.models.gpt2 import gpt2_tiny
+
+    torch.manual_seed(0)
+    model = ops.prepare_module(gpt2_tiny(vocab_size=2000, n_ctx=64).cuda())
+    params = list(model.parameters())
+    for p in params:
+        p.grad = torch.zeros_like(p)
+    rows = 165
+    offsets = torch.tensor([0, 60, 124, 160], dtype=torch.int32, device="cuda")
+    idx, targets = (torch.randint(0, 2000, (rows,), device="cuda") for _ in range(2))
+
+    def step():
+        for p in params:
+            p.grad.zero_()
+        loss = model(idx, targets, pack=ops.pack_sequences(offsets, rows))
+        loss.backward()
+        return loss.detach()
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        got = step()
+    for new in ([0, 1, 2, 66], [0, 64, 64, 128], [5, 50, 110, 165]):
+        offsets.copy_(torch.tensor(new, dtype=torch.int32))
+        idx.random_(0, 2000)
+        targets.random_(0, 2000)
+        targets[new[-1]:] = -100
+        graph.replay()
+        torch.cuda.synchronize()
+        loss, grads = float(got), [p.grad.clone() for p in params]
+        assert float(step()) == loss
+        for g, p in zip(grads, params):
+            # sums of up to 165 fp32 terms in another order: 165 x 2^-24 of their absolute sum, ten times the result's size at most
+            assert float((g - p.grad).norm()) <= 10 * 165 * 2.0 ** -24 * float(p.grad.norm()) + 1e-12
+
+
+def test_second_derivatives_are_refused(ops):
+    q, k, v, do = _inputs(20, 2, 2, 64)
+    pack = ops.pack_sequences([0, 20], 20, device="cuda")
+    q.requires_grad_(True)
+    do.requires_grad_(True)
+    (dq,) = torch.autograd.grad(ops.attention_packed(q, k, v, pack), q, do, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dq.float().sum().backward()
+    x, w = torch.randn(4, 64, device="cuda", requires_grad=True), torch.randn(10, 64, device="cuda")
+    (dx,) = torch.autograd.grad(ops.linear_cross_entropy(x, w, torch.zeros(4, dtype=torch.int64, device="cuda")) ** 2, x, create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        dx.float().sum().backward()
