@@ -299,7 +299,7 @@ __device__ __forceinline__ uint32_t bad_rows(const f32x16 (&a)[N], bool counts) 
 
 // (block, head) of a workgroup, heads fastest: consecutive workgroups go to the eight XCDs in turn, so an XCD keeps to a few
 // heads (one in eight where the heads are a multiple of eight) whose rows its L2 serves, and every XCD gets blocks of all
-// sizes.  The blocks with the most tiles come first (pack_order_kernel): 16384 rows of documents of 1 to 1024 tokens fill
+// sizes.  The blocks with the most tiles come first (pack_spans_kernel): 16384 rows of documents of 1 to 1024 tokens fill
 // the CUs 2.7 times, and in the order of the rows the last round left them a quarter idle.
 __device__ __forceinline__ void ap_unit(const PackedArgs& p, int heads, int& blk, int& h, int& from, int& to) {
     const int rank = blockIdx.x / heads;
@@ -1102,39 +1102,94 @@ __global__ __launch_bounds__(256) void packed_join_kernel(const PackedArgs p, in
     }
 }
 
-// Sequence of every row: offsets[s] <= row < offsets[s + 1], cut to the rows there are.  The last sequence that starts at or
+// Sequence of a row: offsets[s] <= row < offsets[s + 1], cut to the rows there are.  The last sequence that starts at or
 // before the row is the only one that can hold it (empty sequences share their start with the one behind them).
-__device__ __forceinline__ int2 pack_span_of(const int* offsets, int n, int rows, int row) {
-    int lo = 0, hi = n;  // offsets[0 .. lo) start at or before the row
+template <typename At>
+__device__ __forceinline__ int2 pack_span_of(At offset, int n, int rows, int row) {
+    int lo = 0, hi = n;  // offsets 0 .. lo - 1 start at or before the row
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
-        if (offsets[mid] <= row) lo = mid + 1;
+        if (offset(mid) <= row) lo = mid + 1;
         else hi = mid;
     }
     if (lo > 0) {
-        const int first = max(offsets[lo - 1], 0), end = min(offsets[lo], rows);
+        const int first = max(offset(lo - 1), 0), end = min(offset(lo), rows);
         if (row < end) return {first, end};
     }
     return {0, 0};
 }
 
-// entries: [3][blocks] {block of 128 rows, first and end of the rows it streams, their number}: causal query side, causal key
-// side, not causal; in the order the kernels take them, or by block for pack_order_kernel.
+// {block of 128 rows, first and end of the rows it streams, their number}: causal query side, causal key side, not causal
+template <typename At>
+__device__ __forceinline__ int4 pack_entry(At offset, int n, int rows, int b, int kind) {
+    const int row = b * AT_BR, last = min(row + AT_BR, rows) - 1;
+    const int2 s = pack_span_of(offset, n, rows, row), e = pack_span_of(offset, n, rows, last);
+    const int from = kind == 1 || s.y == 0 ? row : s.x, to = kind == 0 || e.y == 0 ? last + 1 : e.y;  // (a block's edge may lie outside every sequence)
+    return {b, from, to, to - from};
+}
+
+// blocks whose work comes before that of block b: more of it, or as much and in front (w[j]: work of block j0 + j, -1 behind the last)
+__device__ __forceinline__ int pack_rank(const int* w, int count, int mine, int before) {
+    int rank = 0;
+#pragma unroll 16
+    for (int j = 0; j < count; j += 4) {
+        const int4 x = *reinterpret_cast<const int4*>(w + j);
+        rank += (x.x >= mine + (j >= before)) + (x.y >= mine + (j + 1 >= before)) + (x.z >= mine + (j + 2 >= before)) + (x.w >= mine + (j + 3 >= before));
+    }
+    return rank;
+}
+
+// Packs of few blocks (one round of workgroups) and of very many (the last round does not matter, the counting does) keep the
+// rows' own order.  Pack, forward and backward in this order and in the rows' own: 18 blocks of one document, 16 heads of 64 131 and
+// 125 us, 32 blocks 233 and 228, 32 blocks with 32 heads of 128 476 and 486, 64 blocks of documents of up to 4096 rows 506 and 530,
+// 4096 blocks, 2 heads of 64 1202 and 1213, 8192 blocks 2690 and 2385.
+#define AP_ORDER_FROM 31
+#define AP_ORDER_TO 4096
+#define AP_ORDER_ONCE 512    // blocks that one workgroup puts in order, in the launch that makes the spans
+#define AP_OFFSETS_LDS 2048  // offsets that are searched in LDS
+enum { AP_OWN_ORDER, AP_ORDERED, AP_TO_BE_ORDERED };
+
+// Spans and positions of the rows, a row per thread, and the blocks' entries: in the rows' own order (on the causal query side the
+// last blocks first: of a long sequence they have the most keys); by three workgroups in front of the others in the order of
+// falling work; or by block, for pack_order_kernel.
 __global__ __launch_bounds__(256) void pack_spans_kernel(const int* __restrict__ offsets, int n, int rows, int2* __restrict__ spans,
-                                                        long long* __restrict__ positions, int4* __restrict__ entries, bool sorted) {
-    const int row = blockIdx.x * 256 + threadIdx.x;
+                                                        long long* __restrict__ positions, int4* __restrict__ entries, int mode) {
+    __shared__ int off[AP_OFFSETS_LDS];
+    __shared__ __attribute__((aligned(16))) int w[AP_ORDER_ONCE];
+    const bool near = n < AP_OFFSETS_LDS;
+    if (near) {
+        for (int i = threadIdx.x; i <= n; i += 256) off[i] = offsets[i];
+        __syncthreads();
+    }
+    auto offset = [&](int i) { return near ? off[i] : offsets[i]; };
+    const int blocks = (rows + AT_BR - 1) / AT_BR, front = mode == AP_ORDERED ? 3 : 0;
+    if (static_cast<int>(blockIdx.x) < front) {
+        const int kind = blockIdx.x;
+        int4 e[AP_ORDER_ONCE / 256];
+#pragma unroll
+        for (int i = 0; i < AP_ORDER_ONCE / 256; ++i) {
+            const int b = threadIdx.x + 256 * i;
+            e[i] = b < blocks ? pack_entry(offset, n, rows, b, kind) : int4{0, 0, 0, -1};
+            w[b] = e[i].w;
+        }
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < AP_ORDER_ONCE / 256; ++i) {
+            const int b = threadIdx.x + 256 * i;
+            if (b < blocks) entries[static_cast<size_t>(kind) * blocks + pack_rank(w, (blocks + 3) & ~3, e[i].w, b)] = e[i];
+        }
+        return;
+    }
+    const int row = (blockIdx.x - front) * 256 + threadIdx.x;
     if (row >= rows) return;
-    const int2 s = pack_span_of(offsets, n, rows, row);
+    const int2 s = pack_span_of(offset, n, rows, row);
     spans[row] = s;
     positions[row] = s.y > 0 ? row - s.x : 0;
-    if (row % AT_BR == 0) {
-        const int last = min(row + AT_BR, rows) - 1, blocks = (rows + AT_BR - 1) / AT_BR, b = row / AT_BR;
-        const int2 e = pack_span_of(offsets, n, rows, last);
-        const int first = s.y > 0 ? s.x : row, end = e.y > 0 ? e.y : last + 1;  // (a block's edge may lie outside every sequence)
-        // (in the rows' own order the last blocks come first on the query side: of a long sequence they have the most keys)
-        entries[sorted ? b : blocks - 1 - b] = {b, first, last + 1, last + 1 - first};
-        entries[blocks + b] = {b, row, end, end - row};
-        entries[2 * static_cast<size_t>(blocks) + b] = {b, first, end, end - first};
+    if (mode != AP_ORDERED && row % AT_BR == 0) {
+        const int b = row / AT_BR;
+        entries[mode == AP_OWN_ORDER ? blocks - 1 - b : b] = pack_entry(offset, n, rows, b, 0);
+        entries[blocks + b] = pack_entry(offset, n, rows, b, 1);
+        entries[2 * static_cast<size_t>(blocks) + b] = pack_entry(offset, n, rows, b, 2);
     }
 }
 
@@ -1144,38 +1199,25 @@ __global__ __launch_bounds__(256) void pack_order_kernel(const int4* __restrict_
     const int4* src = entries + static_cast<size_t>(blockIdx.y) * blocks;
     const int b = blockIdx.x * 256 + threadIdx.x;
     const int4 e = b < blocks ? src[b] : int4{0, 0, 0, 0};
-    const int mine = e.w;
     int rank = 0;
     for (int j0 = 0; j0 < blocks; j0 += 256) {
         __syncthreads();
         w[threadIdx.x] = j0 + static_cast<int>(threadIdx.x) < blocks ? src[j0 + threadIdx.x].w : -1;
         __syncthreads();
-        const int before = b - j0;  // equal work counts from the blocks in front of this one
-#pragma unroll 16
-        for (int j = 0; j < 256; j += 4) {
-            const int4 x = *reinterpret_cast<const int4*>(w + j);
-            rank += (x.x >= mine + (j >= before)) + (x.y >= mine + (j + 1 >= before)) + (x.z >= mine + (j + 2 >= before)) + (x.w >= mine + (j + 3 >= before));
-        }
+        rank += pack_rank(w, 256, e.w, b - j0);
     }
     if (b < blocks) order[static_cast<size_t>(blockIdx.y) * blocks + rank] = e;
 }
-
-// Packs of few blocks (one round of workgroups) and of very many (the last round does not matter, the counting does) keep the
-// rows' own order.  Pack, forward and backward in this order and in the rows' own: 18 blocks of one document, 16 heads of 64 131 and
-// 125 us, 32 blocks 233 and 228, 32 blocks with 32 heads of 128 476 and 486, 64 blocks of documents of up to 4096 rows 506 and 530,
-// 4096 blocks, 2 heads of 64 1202 and 1213, 8192 blocks 2690 and 2385.
-#define AP_ORDER_FROM 31
-#define AP_ORDER_TO 4096
 
 // offsets: [sequences + 1] int32, not falling.  order: [3][ceil(rows / 128)] entries of 16 bytes; work: scratch of the same size.
 PDT_API int pdt_pack_spans(const int* offsets, int sequences, int rows, void* spans, long long* positions, void* order, void* work, void* stream) {
     if (sequences < 0 || rows <= 0 || rows >= (1 << 30)) return -1;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const int blocks = pdt_cdiv(rows, AT_BR);
-    const bool sorted = blocks > AP_ORDER_FROM && blocks <= AP_ORDER_TO;
-    hipLaunchKernelGGL(pack_spans_kernel, dim3(pdt_cdiv(rows, 256)), dim3(256), 0, s, offsets, sequences, rows, static_cast<int2*>(spans), positions,
-                       static_cast<int4*>(sorted ? work : order), sorted);
-    if (sorted)
+    const int mode = blocks <= AP_ORDER_FROM || blocks > AP_ORDER_TO ? AP_OWN_ORDER : blocks <= AP_ORDER_ONCE ? AP_ORDERED : AP_TO_BE_ORDERED;
+    hipLaunchKernelGGL(pack_spans_kernel, dim3(pdt_cdiv(rows, 256) + (mode == AP_ORDERED ? 3 : 0)), dim3(256), 0, s, offsets, sequences, rows,
+                       static_cast<int2*>(spans), positions, static_cast<int4*>(mode == AP_TO_BE_ORDERED ? work : order), mode);
+    if (mode == AP_TO_BE_ORDERED)
         hipLaunchKernelGGL(pack_order_kernel, dim3(pdt_cdiv(blocks, 256), 3), dim3(256), 0, s, static_cast<const int4*>(work), blocks, static_cast<int4*>(order));
     return pdt_launch_status();
 }

@@ -497,3 +497,46 @@ def test_second_derivatives_are_refused(ops):
     (dx,) = torch.autograd.grad(ops.linear_cross_entropy(x, w, torch.zeros(4, dtype=torch.int64, device="cuda")) ** 2, x, create_graph=True)
     with pytest.raises(RuntimeError, match="once_differentiable"):
         dx.float().sum().backward()
+
+
+def _random_lengths(rows, longest, seed):
+    g = torch.Generator().manual_seed(seed)
+    lengths = []
+    while sum(lengths) < rows:
+        lengths.append(min(int(torch.randint(0, longest + 1, (1,), generator=g)), rows - sum(lengths)))
+    return lengths
+
+
+@pytest.mark.parametrize("rows,longest", [(3968, 400), (3969, 400), (5000, 300), (65536, 5000), (66000, 60)])
+def test_order_of_the_blocks(ops, rows, longest):
+    """In the rows' own order, put in order within the launch and by a second one, offsets searched in LDS and in memory."""
+    offsets = _offsets(_random_lengths(rows - 212, longest, rows), 5)
+    pack = ops.pack_sequences(torch.tensor(offsets, dtype=torch.int32, device="cuda"), rows)
+    spans = ops.pack_sequences(offsets, rows).spans
+    assert torch.equal(pack.spans.cpu(), spans)
+    blocks = -(-rows // 128)
+    order = pack.plan[2 * rows:2 * rows + 6 * blocks].cpu().view(torch.int32).view(3, blocks, 4)
+    row = torch.arange(0, rows, 128)
+    last = (row + 127).clamp(max=rows - 1)
+    first = torch.where(spans[row, 1] > 0, spans[row, 0], row)
+    end = torch.where(spans[last, 1] > 0, spans[last, 1], last + 1)
+    for got, a, b, reverse in zip(order, (first, row, first), (last + 1, end, end), (True, False, False)):
+        work = b - a
+        if blocks <= 31:
+            want = torch.arange(blocks).flip(0) if reverse else torch.arange(blocks)
+        else:
+            want = torch.sort(-work, stable=True).indices
+        assert torch.equal(got.long(), torch.stack([want, a[want], b[want], work[want]], 1))
+
+
+@pytest.mark.parametrize("h,hk,d", [(2, 1, 64), (2, 2, 128)])
+def test_many_blocks(ops, h, hk, d):
+    rows = 5000
+    offsets = _offsets(_random_lengths(rows - 100, 500, 3), 40)
+    q, k, v, do = _inputs(rows, h, hk, d, seed=3)
+    leaves = [x.requires_grad_(True) for x in (q, k, v)]
+    pack = ops.pack_sequences(torch.tensor(offsets, device="cuda"), rows)
+    for causal in (True, False):
+        out = ops.attention_packed(*leaves, pack, causal=causal)
+        got = (out.detach(), *torch.autograd.grad(out, leaves, do))
+        _check(got, *_expected(q.detach(), k.detach(), v.detach(), do, offsets, causal, d ** -0.5))
