@@ -728,7 +728,7 @@ __global__ __launch_bounds__(THREADS) void vocab_teacher_kernel(const Targets t)
     }
 }
 
-// scal[0] = tau / rows with a target (0 without any), scal[1] = tau^2 / rows with a target
+// scal[0] = tau / rows with a target (0 without any)
 __global__ __launch_bounds__(1024) void vocab_count_kernel(const int* __restrict__ valid, int rows, float tau, float* __restrict__ scal) {
     __shared__ int red[16];
     int c = 0;
@@ -741,17 +741,20 @@ __global__ __launch_bounds__(1024) void vocab_count_kernel(const int* __restrict
         int n = 0;
         for (int i = 0; i < 16; ++i) n += red[i];
         scal[0] = n > 0 ? tau / n : 0.f;
-        scal[1] = n > 0 ? tau * tau / n : 0.f;
     }
 }
 
-__global__ __launch_bounds__(1024) void vocab_mean_kernel(const float* __restrict__ row_loss, int rows, const float* __restrict__ scal,
+__global__ __launch_bounds__(1024) void vocab_mean_kernel(const float* __restrict__ row_loss, const int* __restrict__ valid, int rows, float tau,
                                                          float* __restrict__ loss) {
     __shared__ float red[16];
-    float s = 0.f;
-    for (int i = threadIdx.x; i < rows; i += 1024) s += row_loss[i];
+    float s = 0.f, n = 0.f;  // (fewer than 2^22 rows: counted exactly)
+    for (int i = threadIdx.x; i < rows; i += 1024) {
+        s += row_loss[i];
+        n += valid[i];
+    }
     s = block_sum(s, red);
-    if (threadIdx.x == 0) loss[0] = s * scal[1];
+    n = block_sum(n, red);
+    if (threadIdx.x == 0) loss[0] = n > 0.f ? s * (tau * tau / n) : 0.f;
 }
 
 // ---- behind a projection: one workgroup per row joins the groups; training: exponentials -> q - p in place (e holds rows
@@ -824,9 +827,11 @@ struct Logits {
     const float* p;
     const float* base;
     const int* valid;
-    const float* scal;
+    const float* scal;       // nullptr: every workgroup counts the rows with a target itself
+    const int* every;        // valid of all rows
     float* row_loss;
-    int top, vocab;
+    int top, vocab, rows;
+    float tau;
     float scale_log2, inv_tau;
     bool stream;
 };
@@ -906,7 +911,14 @@ __global__ __launch_bounds__(THREADS) void logits_distill_kernel(const Logits<T>
     const float ls = log2f(s);
     if (tid == 0) a.row_loss[row] = a.base[row] - t * a.inv_tau + ls * VL_LN2;
     if (dz == nullptr) return;
-    const float g = a.scal[0];
+    float g;
+    if (a.scal != nullptr) {
+        g = a.scal[0];
+    } else {
+        float n = 0.f;
+        for (int i = tid; i < a.rows; i += THREADS) n += a.every[i];
+        g = a.tau / block_sum(n, red);
+    }
     auto q_of = [&](float x) { return vl_exp2((x - ref) * a.scale_log2 - ls); };
     each([&](int c, vec x) {  // (rows of dz are padded to whole chunks, on 16-byte boundaries)
         vec r;
@@ -1000,12 +1012,12 @@ static int vl_targets(const long long* ids, const float* teacher, float* p, floa
     if (teacher != nullptr && (x != nullptr || top > 128)) hipLaunchKernelGGL(vocab_teacher_kernel<256>, dim3(all), dim3(256), lds, s, t);
     else if (teacher != nullptr) hipLaunchKernelGGL(vocab_teacher_kernel<64>, dim3(all), dim3(64), lds, s, t);
     else hipLaunchKernelGGL(vocab_labels_kernel, dim3(pdt_cdiv(all, 4)), dim3(256), 0, s, t);
-    hipLaunchKernelGGL(vocab_count_kernel, dim3(1), dim3(1024), 0, s, valid, rows, tau, scal);
+    if (scal != nullptr) hipLaunchKernelGGL(vocab_count_kernel, dim3(1), dim3(1024), 0, s, valid, rows, tau, scal);
     return pdt_launch_status();
 }
 
-static int vl_mean(const float* row_loss, const float* scal, float* loss, int rows, hipStream_t s) {
-    hipLaunchKernelGGL(vocab_mean_kernel, dim3(1), dim3(1024), 0, s, row_loss, rows, scal, loss);
+static int vl_mean(const float* row_loss, const int* valid, float* loss, int rows, float tau, hipStream_t s) {
+    hipLaunchKernelGGL(vocab_mean_kernel, dim3(1), dim3(1024), 0, s, row_loss, valid, rows, tau, loss);
     return pdt_launch_status();
 }
 
@@ -1028,7 +1040,7 @@ struct RowScratch {
         base = m.take<float>(rows);
         row_loss = m.take<float>(rows);
         valid = m.take<int>(rows);
-        scal = m.take<float>(2);
+        scal = m.take<float>(1);
     }
 };
 struct HeadScratch {
@@ -1084,7 +1096,7 @@ PDT_API int pdt_head_loss(const void* x, const void* w, const long long* ids, co
     hipStream_t s = static_cast<hipStream_t>(stream);
     const long long pitch = (vocab + 63ll) / 64 * 64;
     const bool big = 2 * pitch * chunk >= VL_STREAM_BYTES;
-    if (int e = vl_targets(ids, teacher, h.r.p, h.r.base, h.r.valid, h.r.scal, x, w, h.x_used, rows, top, width, vocab, tau, s)) return e;
+    if (int e = vl_targets(ids, teacher, h.r.p, h.r.base, h.r.valid, train ? h.r.scal : nullptr, x, w, h.x_used, rows, top, width, vocab, tau, s)) return e;
     for (int r0 = 0; r0 < rows; r0 += chunk) {
         const int n = rows - r0 < chunk ? rows - r0 : chunk;
         VocabGemm g = {};
@@ -1127,7 +1139,7 @@ PDT_API int pdt_head_loss(const void* x, const void* w, const long long* ids, co
             if (int e = vl_launch<2>(g, s)) return e;
         }
     }
-    return vl_mean(h.r.row_loss, h.r.scal, loss, rows, s);
+    return vl_mean(h.r.row_loss, h.r.valid, loss, rows, tau, s);
 }
 
 template <typename T>
@@ -1166,11 +1178,13 @@ PDT_API int pdt_distill(const void* z, void* dz, const long long* ids, const flo
     if (scratch == nullptr || static_cast<long long>(m.used) > scratch_bytes) return -1;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const float it = 1.f / tau, c = VL_LOG2E * it;
-    if (int e = vl_targets(ids, teacher, r.p, r.base, r.valid, r.scal, nullptr, nullptr, nullptr, rows, top, 0, vocab, tau, s)) return e;
+    // up to 1024 rows every workgroup counts the ones with a target itself: a launch less
+    float* scal = rows > 1024 && dz != nullptr ? r.scal : nullptr;
+    if (int e = vl_targets(ids, teacher, r.p, r.base, r.valid, scal, nullptr, nullptr, nullptr, rows, top, 0, vocab, tau, s)) return e;
     const bool big = ldd * rows * (dtype == 1 ? 2 : 4) >= VL_STREAM_BYTES;
-    const int e = dtype == 1 ? distill_launch(Logits<bf16>{static_cast<const bf16*>(z), static_cast<bf16*>(dz), ldz, ldd, ids, r.p, r.base, r.valid, r.scal, r.row_loss, top, vocab, c, it, big}, rows, s)
-                             : distill_launch(Logits<float>{static_cast<const float*>(z), static_cast<float*>(dz), ldz, ldd, ids, r.p, r.base, r.valid, r.scal, r.row_loss, top, vocab, c, it, big}, rows, s);
-    return e != 0 ? e : vl_mean(r.row_loss, r.scal, loss, rows, s);
+    const int e = dtype == 1 ? distill_launch(Logits<bf16>{static_cast<const bf16*>(z), static_cast<bf16*>(dz), ldz, ldd, ids, r.p, r.base, r.valid, scal, r.valid, r.row_loss, top, vocab, rows, tau, c, it, big}, rows, s)
+                             : distill_launch(Logits<float>{static_cast<const float*>(z), static_cast<float*>(dz), ldz, ldd, ids, r.p, r.base, r.valid, scal, r.valid, r.row_loss, top, vocab, rows, tau, c, it, big}, rows, s);
+    return e != 0 ? e : vl_mean(r.row_loss, r.valid, loss, rows, tau, s);
 }
 
 // fp32 x (16-byte aligned, a multiple of four elements) times a device scalar, in place; nothing is touched where it is 1.

@@ -179,7 +179,7 @@ def linear_cross_entropy(x, weight, labels):
     if x.is_cuda and labels.numel():
         from . import hip_vocab
 
-        return hip_vocab.head_loss(x, weight, labels.reshape(-1, 1).to(torch.int64).contiguous(), None, 1.0)
+        return hip_vocab.head_loss(x, weight, _rows(labels, 1, torch.int64), None, 1.0)
     return _ref.linear_cross_entropy(x, weight, labels)
 
 
@@ -210,10 +210,18 @@ def linear_distillation_loss(x, weight, teacher_logits, teacher_ids, temperature
     return _ref.distillation_loss(_ref.linear(x.to(up), weight.to(up)), teacher_logits, teacher_ids, tau)
 
 
+def _rows(x, width: int, dtype):
+    """[rows, width] in ``dtype`` without gaps; the tensor itself where it is that (host time counts in small calls)."""
+    if x.dim() != 2 or x.shape[1] != width:
+        x = x.reshape(-1, width)
+    if x.dtype != dtype:
+        x = x.to(dtype)
+    return x if x.is_contiguous() else x.contiguous()
+
+
 def _teacher_rows(teacher_logits, teacher_ids):
     top = teacher_ids.shape[-1]
-    return (teacher_ids.reshape(-1, top).to(torch.int64).contiguous(),
-            teacher_logits.detach().reshape(-1, top).to(torch.float32).contiguous())
+    return _rows(teacher_ids, top, torch.int64), _rows(teacher_logits, top, torch.float32)
 
 
 def layer_norm(x, weight, bias, eps: float = 1e-5, link=None):

@@ -451,3 +451,9 @@ def test_too_many_rows_are_refused(ops):
         ops.distillation_loss(torch.zeros(n, 1, dtype=torch.bfloat16, device="cuda"), torch.zeros(n, 1, device="cuda"), ids)
     with pytest.raises(ValueError, match="rows at a time"):
         ops.linear_cross_entropy(torch.zeros(1, 64, dtype=torch.bfloat16, device="cuda").expand(n, 64), torch.zeros(5, 64, dtype=torch.bfloat16, device="cuda"), ids[:, 0])
+
+
+@pytest.mark.parametrize("n", [1023, 1024, 1025, 3000])
+def test_distillation_on_many_rows(ops, n):
+    """Rows with a target counted by every workgroup, and by a launch of its own."""
+    test_distillation_on_logits(ops, torch.bfloat16, n, 130, 5, 2.0)
