@@ -931,16 +931,32 @@ __global__ __launch_bounds__(THREADS) void logits_distill_kernel(const Logits<T>
         if (p[k] != 0.f) dz[ids[k]] = static_cast<T>((q_of(static_cast<float>(z[ids[k]])) - p[k]) * g);
 }
 
-// x *= g[0] unless g[0] == 1 (the gradient of a loss that is the root of the graph): a pass over an fp32 gradient saved
-__global__ __launch_bounds__(256) void vocab_scale_kernel(f32x4* __restrict__ x, const float* __restrict__ g, long long n) {
+// Up to two gradients times g[0], in place, unless it is 1 (a loss that is the root of its graph): nothing is touched then, and
+// the grid is one round of workgroups so that finding out is short.
+struct Gradients {
+    void* at[2];
+    long long n[2];  // 16-byte vectors
+    bool f32[2];
+};
+__global__ __launch_bounds__(256) void vocab_scale_kernel(const Gradients a, const float* __restrict__ g) {
     const float gv = g[0];
     if (gv == 1.f) return;
-    for (long long i = blockIdx.x * 256ll + threadIdx.x; i < n; i += gridDim.x * 256ll) {
-        f32x4 v = x[i];
+    for (int k = 0; k < 2; ++k)
+        for (long long i = blockIdx.x * 256ll + threadIdx.x; i < a.n[k]; i += gridDim.x * 256ll) {
+            if (a.f32[k]) {
+                f32x4* x = static_cast<f32x4*>(a.at[k]) + i;
+                f32x4 v = *x;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) v[e] *= gv;
-        x[i] = v;
-    }
+                for (int e = 0; e < 4; ++e) v[e] *= gv;
+                *x = v;
+            } else {
+                bf16x8* x = static_cast<bf16x8*>(a.at[k]) + i;
+                bf16x8 v = *x;
+#pragma unroll
+                for (int e = 0; e < 8; ++e) v[e] = f32_to_bf16(bf16_to_f32(v[e]) * gv);
+                *x = v;
+            }
+        }
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -1187,11 +1203,13 @@ PDT_API int pdt_distill(const void* z, void* dz, const long long* ids, const flo
     return e != 0 ? e : vl_mean(r.row_loss, r.valid, loss, rows, tau, s);
 }
 
-// fp32 x (16-byte aligned, a multiple of four elements) times a device scalar, in place; nothing is touched where it is 1.
-PDT_API int pdt_scale_by_scalar_f32(float* x, const float* g, long long numel, void* stream) {
-    if (numel <= 0 || (numel % 4) != 0) return -1;
-    const long long blocks = (numel / 4 + 255) / 256;
-    hipLaunchKernelGGL(vocab_scale_kernel, dim3(static_cast<unsigned>(blocks < 8192 ? blocks : 8192)), dim3(256), 0, static_cast<hipStream_t>(stream),
-                       reinterpret_cast<f32x4*>(x), g, numel / 4);
+// x and y (nullptr: none; bf16, or fp32 where the flag says so; 16-byte aligned, whole 16-byte vectors) times a device scalar, in
+// place; nothing is touched where it is 1.
+PDT_API int pdt_scale_gradients(void* x, long long nx, int x_f32, void* y, long long ny, int y_f32, const float* g, void* stream) {
+    if (nx < 0 || ny < 0 || (nx % (x_f32 != 0 ? 4 : 8)) != 0 || (ny % (y_f32 != 0 ? 4 : 8)) != 0) return -1;
+    const Gradients a = {{x, y}, {x == nullptr ? 0 : nx / (x_f32 != 0 ? 4 : 8), y == nullptr ? 0 : ny / (y_f32 != 0 ? 4 : 8)}, {x_f32 != 0, y_f32 != 0}};
+    const long long most = a.n[0] > a.n[1] ? a.n[0] : a.n[1], blocks = (most + 255) / 256;
+    if (most == 0) return 0;
+    hipLaunchKernelGGL(vocab_scale_kernel, dim3(static_cast<unsigned>(blocks < 2048 ? blocks : 2048)), dim3(256), 0, static_cast<hipStream_t>(stream), a, g);
     return pdt_launch_status();
 }

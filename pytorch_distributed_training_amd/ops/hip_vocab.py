@@ -10,13 +10,13 @@ import os
 
 import torch
 
-from .hip import SHADOWS, _axpy_dev, _check, _grad_sink, _on, _once_differentiable, _ptr, _round_up, _scale_by_scalar, _stream
+from .hip import SHADOWS, _axpy_dev, _check, _grad_sink, _on, _once_differentiable, _ptr, _round_up, _stream
 from .hip_transformer import _f, _i, _ll, _sig, _vp
 
 _head_scratch = _sig("pdt_head_loss_scratch", [_i] * 8)
 _head_scratch.restype = _ll
 _head = _sig("pdt_head_loss", [_vp] * 9 + [_ll] + [_i] * 5 + [_f, _vp])
-_scale_f32 = _sig("pdt_scale_by_scalar_f32", [_vp, _vp, _ll, _vp])
+_scale_gradients = _sig("pdt_scale_gradients", [_vp, _ll, _i, _vp, _ll, _i, _vp, _vp])
 _distill_scratch = _sig("pdt_distill_scratch", [_i] * 2)
 _distill_scratch.restype = _ll
 _distill = _sig("pdt_distill", [_vp] * 6 + [_ll] + [_i] * 3 + [_ll, _ll, _f, _i, _vp])
@@ -73,6 +73,14 @@ def _head_forward(x, weight, ids, teacher, tau: float, want_dx: bool, want_dw: b
     return loss, dx, dw
 
 
+def _scale(g, *grads) -> None:
+    """Gradients (bf16 or fp32, up to two) times a device scalar, in place."""
+    args = []
+    for d in (*grads, None)[:2]:
+        args += (None, 0, 0) if d is None else (d.data_ptr(), d.numel(), int(d.dtype == torch.float32))
+    _check(_scale_gradients(*args, g.data_ptr(), _stream()), "scale_gradients")
+
+
 class _HeadLoss(torch.autograd.Function):
     """Loss of ``x W^T`` against a few targets per row.  The rows are worked off in chunks; the forward pass leaves ``dx``
     and ``dW`` for an incoming gradient of 1, the backward pass multiplies them by the incoming one (a device scalar)."""
@@ -93,17 +101,13 @@ class _HeadLoss(torch.autograd.Function):
         weight = ctx.weight
         with _on(g.device):
             g1 = g if g.dtype == torch.float32 else g.to(torch.float32)
-            for d in (dx, dw):
-                if d is not None and d.dtype == torch.bfloat16:
-                    _check(_scale_by_scalar(d.data_ptr(), g1.data_ptr(), d.numel(), _stream()), "scale_by_scalar")
-            if dw is not None and dw.dtype == torch.float32:
-                sink = _grad_sink(weight, tuple(weight.shape))
-                if sink is not None:
-                    _check(_axpy_dev(sink.data_ptr(), dw.data_ptr(), g1.data_ptr(), dw.numel(), _stream()), "axpy")
-                    dw = None
-                else:
-                    _check(_scale_f32(dw.data_ptr(), g1.data_ptr(), dw.numel(), _stream()), "scale_by_scalar_f32")
-                    dw = dw.to(weight.dtype)
+            sink = _grad_sink(weight, tuple(weight.shape)) if dw is not None and dw.dtype == torch.float32 else None
+            if sink is not None:
+                _check(_axpy_dev(sink.data_ptr(), dw.data_ptr(), g1.data_ptr(), dw.numel(), _stream()), "axpy")
+                dw = None
+            _scale(g1, dx, dw)
+            if dw is not None:
+                dw = dw.to(weight.dtype)
         return None if dx is None else dx.view(ctx.shape), dw, None, None, None
 
 
@@ -151,10 +155,7 @@ class _LogitsDistill(torch.autograd.Function):
             raise RuntimeError("the distillation loss handed its gradient out already (backward ran twice)")
         with _on(g.device):
             g1 = g if g.dtype == torch.float32 else g.to(torch.float32)
-            if dz.dtype == torch.bfloat16:
-                _check(_scale_by_scalar(dz.data_ptr(), g1.data_ptr(), dz.numel(), _stream()), "scale_by_scalar")
-            else:
-                _check(_scale_f32(dz.data_ptr(), g1.data_ptr(), dz.numel(), _stream()), "scale_by_scalar_f32")
+            _scale(g1, dz)
         if dz.shape[1] != ctx.shape[-1]:
             dz = dz[:, :ctx.shape[-1]]
         return dz.reshape(ctx.shape), None, None, None
