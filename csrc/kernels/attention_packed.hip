@@ -160,28 +160,67 @@ __device__ __forceinline__ float rest_dot(uint32_t rest, const bf16* g, const bf
     return s;
 }
 
-// ---- one row by a whole wave (lane = element lane, lane + 64), over its own interval only
+// ---- one row by a whole wave, over its own interval only.  64 rows of the other side at a time: a lane forms the products with
+// one of them, then the lanes take elements lane, lane + 64 of the sums.  (One document of 16384 rows, 16 heads of 128 on 4,
+// the first value NaN and with it every row: 77 ms forward, 7 ms backward, which ends a row whose elements are all NaN.)
+template <int NP>
+__device__ __forceinline__ float row_dot(const bf16* a, const bf16* b) {
+    float s = 0.f;
+#pragma unroll 2
+    for (int c = 0; c < 64 * NP; c += 8) {
+        const bf16x8 x = *reinterpret_cast<const bf16x8*>(a + c), y = *reinterpret_cast<const bf16x8*>(b + c);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) s = fmaf(bf16_to_f32(x[e]), bf16_to_f32(y[e]), s);
+    }
+    return s;
+}
+// acc[e] += sum over the `count` lanes from 0 of w times element lane + 64 e of row (first + lane's number)
+template <int NP>
+__device__ __forceinline__ void row_add(float (&acc)[NP], float w, int count, const bf16* first, long long pitch, int lane) {
+    auto some = [&](int t0, auto n) {
+        bf16 x[n][NP];
+#pragma unroll
+        for (int t = 0; t < n; ++t)
+#pragma unroll
+            for (int e = 0; e < NP; ++e) x[t][e] = first[(t0 + t) * pitch + lane + 64 * e];
+#pragma unroll
+        for (int t = 0; t < n; ++t) {
+            const float wt = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, w), t0 + t));
+#pragma unroll
+            for (int e = 0; e < NP; ++e) acc[e] = fmaf(wt, bf16_to_f32(x[t][e]), acc[e]);
+        }
+    };
+    int t = 0;
+    for (; t + 8 <= count; t += 8) some(t, std::integral_constant<int, 8>{});
+    for (; t < count; ++t) some(t, std::integral_constant<int, 1>{});
+}
+template <int NP>
+__device__ __forceinline__ bool row_is_nan(const float (&acc)[NP]) {  // every element is, and stays so whatever is added
+    bool nan = true;
+#pragma unroll
+    for (int e = 0; e < NP; ++e) nan &= acc[e] != acc[e];
+    return __all(nan);
+}
+
 template <int NP>
 __device__ __forceinline__ void row_forward(const PackedArgs& p, int h, int row, int lane) {
     const int hk = h / p.group;
     const int2 s = ap_keys_of(p, row);
-    float qv[NP], o[NP], m = -AP_INF, l = 0.f;
+    const bf16 *q = p.q + row * p.q_row + h * p.q_head, *k = p.k + hk * p.k_head, *v = p.v + hk * p.v_head;
+    float o[NP], m = -AP_INF, l = 0.f;
 #pragma unroll
-    for (int e = 0; e < NP; ++e) {
-        qv[e] = bf16_to_f32(p.q[row * p.q_row + h * p.q_head + lane + 64 * e]);
-        o[e] = 0.f;
-    }
-    for (int j = s.x; j < s.y; ++j) {
-        float a = 0.f;
-#pragma unroll
-        for (int e = 0; e < NP; ++e) a += qv[e] * bf16_to_f32(p.k[j * p.k_row + hk * p.k_head + lane + 64 * e]);
-        a = wave_sum(a) * p.scale_log2;
-        const float mn = fmaxf(m, a), ref = mn == -AP_INF ? 0.f : mn;
-        const float alpha = fast_exp2(m - ref), w = fast_exp2(a - ref);
-        l = l * alpha + w;
-#pragma unroll
-        for (int e = 0; e < NP; ++e) o[e] = o[e] * alpha + w * bf16_to_f32(p.v[j * p.v_row + hk * p.v_head + lane + 64 * e]);
+    for (int e = 0; e < NP; ++e) o[e] = 0.f;
+    for (int j0 = s.x; j0 < s.y; j0 += 64) {
+        const int count = min(64, s.y - j0);
+        const float a = row_dot<NP>(q, k + (j0 + min(lane, count - 1)) * p.k_row) * p.scale_log2;
+        const float mn = fmaxf(m, wave_max(lane < count ? a : -AP_INF)), ref = mn == -AP_INF ? 0.f : mn;
+        const float alpha = fast_exp2(m - ref), w = lane < count ? fast_exp2(a - ref) : 0.f;
+        l = l * alpha + wave_sum(w);
         m = mn;
+        if (l != l) break;  // a score is NaN: so is the row
+#pragma unroll
+        for (int e = 0; e < NP; ++e) o[e] *= alpha;
+        if (!row_is_nan<NP>(o)) row_add<NP>(o, w, count, v + j0 * p.v_row, p.v_row, lane);
     }
 #pragma unroll
     for (int e = 0; e < NP; ++e) {
@@ -199,31 +238,24 @@ template <int NP>
 __device__ __forceinline__ void row_dq(const PackedArgs& p, int h, int row, int lane) {
     const int hk = h / p.group;
     const int2 s = ap_keys_of(p, row);
+    const bf16 *q = p.q + row * p.q_row + h * p.q_head, *k = p.k + hk * p.k_head, *v = p.v + hk * p.v_head;
+    const bf16* g = p.dout + row * p.o_row + h * (64 * NP);
     const float lse = p.lse[static_cast<size_t>(h) * p.T + row];
-    float qv[NP], dov[NP], dq[NP], dl = 0.f;
+    float dq[NP], dl = 0.f;
 #pragma unroll
     for (int e = 0; e < NP; ++e) {
         const long long at = row * p.o_row + h * (64 * NP) + lane + 64 * e;
-        qv[e] = bf16_to_f32(p.q[row * p.q_row + h * p.q_head + lane + 64 * e]);
-        dov[e] = bf16_to_f32(p.dout[at]);
         const int rest = p.rest[row * p.o_row + h * (64 * NP) + rest_place<NP>(lane + 64 * e)];
-        dl += dov[e] * (bf16_to_f32(p.o[at]) + __builtin_amdgcn_cvt_f32_bf8(rest, 0) * (1.f / 256.f));
+        dl += bf16_to_f32(g[lane + 64 * e]) * (bf16_to_f32(p.o[at]) + __builtin_amdgcn_cvt_f32_bf8(rest, 0) * (1.f / 256.f));
         dq[e] = 0.f;
     }
     dl = wave_sum(dl);
-    for (int j = s.x; j < s.y; ++j) {
-        float a = 0.f, b = 0.f, kv[NP];
-#pragma unroll
-        for (int e = 0; e < NP; ++e) {
-            kv[e] = bf16_to_f32(p.k[j * p.k_row + hk * p.k_head + lane + 64 * e]);
-            a += qv[e] * kv[e];
-            b += dov[e] * bf16_to_f32(p.v[j * p.v_row + hk * p.v_head + lane + 64 * e]);
-        }
-        a = wave_sum(a);
-        b = wave_sum(b);
-        const float ds = fast_exp2((a + lse) * p.scale_log2) * (b - dl);
-#pragma unroll
-        for (int e = 0; e < NP; ++e) dq[e] += ds * kv[e];
+    for (int j0 = s.x; j0 < s.y; j0 += 64) {
+        const int count = min(64, s.y - j0);
+        const long long j = j0 + min(lane, count - 1);
+        const float ds = fast_exp2((row_dot<NP>(q, k + j * p.k_row) + lse) * p.scale_log2) * (row_dot<NP>(g, v + j * p.v_row) - dl);
+        row_add<NP>(dq, ds, count, k + j0 * p.k_row, p.k_row, lane);
+        if (row_is_nan<NP>(dq)) break;
     }
 #pragma unroll
     for (int e = 0; e < NP; ++e) p.dq[row * p.dq_row + h * p.dq_head + lane + 64 * e] = f32_to_bf16(dq[e] * p.scale);
@@ -233,30 +265,26 @@ __device__ __forceinline__ void row_dq(const PackedArgs& p, int h, int row, int 
 template <int NP, bool IS_V>
 __device__ __forceinline__ void row_dkv(const PackedArgs& p, int hk, int h0, int h1, int split, int row, int lane) {
     const int2 s = ap_queries_of(p, row);
-    float kv[NP], vv[NP], acc[NP];
+    const bf16 *k = p.k + row * p.k_row + hk * p.k_head, *v = p.v + row * p.v_row + hk * p.v_head;
+    float acc[NP];
 #pragma unroll
-    for (int e = 0; e < NP; ++e) {
-        kv[e] = bf16_to_f32(p.k[row * p.k_row + hk * p.k_head + lane + 64 * e]);
-        vv[e] = bf16_to_f32(p.v[row * p.v_row + hk * p.v_head + lane + 64 * e]);
-        acc[e] = 0.f;
-    }
-    for (int h = h0; h < h1; ++h)
-        for (int i = s.x; i < s.y; ++i) {
-            float a = 0.f, b = 0.f, qv[NP], dov[NP];
-#pragma unroll
-            for (int e = 0; e < NP; ++e) {
-                qv[e] = bf16_to_f32(p.q[i * p.q_row + h * p.q_head + lane + 64 * e]);
-                dov[e] = bf16_to_f32(p.dout[i * p.o_row + h * (64 * NP) + lane + 64 * e]);
-                a += qv[e] * kv[e];
-                b += dov[e] * vv[e];
+    for (int e = 0; e < NP; ++e) acc[e] = 0.f;
+    for (int h = h0; h < h1; ++h) {
+        const bf16 *q = p.q + h * p.q_head, *g = p.dout + h * (64 * NP);
+        for (int i0 = s.x; i0 < s.y; i0 += 64) {
+            const int count = min(64, s.y - i0);
+            const long long i = i0 + min(lane, count - 1);
+            const size_t term = static_cast<size_t>(h) * p.T + i;
+            float w = fast_exp2((row_dot<NP>(k, q + i * p.q_row) + p.lse[term]) * p.scale_log2);
+            if constexpr (!IS_V) w *= row_dot<NP>(v, g + i * p.o_row) + p.delta[term];
+            if constexpr (IS_V) row_add<NP>(acc, w, count, g + i0 * p.o_row, p.o_row, lane);
+            else row_add<NP>(acc, w, count, q + i0 * p.q_row, p.q_row, lane);
+            if (row_is_nan<NP>(acc)) {
+                h = h1;
+                break;
             }
-            a = wave_sum(a);
-            b = wave_sum(b);
-            const float pr = fast_exp2((a + p.lse[static_cast<size_t>(h) * p.T + i]) * p.scale_log2);
-            const float ds = pr * (b + p.delta[static_cast<size_t>(h) * p.T + i]);
-#pragma unroll
-            for (int e = 0; e < NP; ++e) acc[e] += IS_V ? pr * dov[e] : ds * qv[e];
         }
+    }
 #pragma unroll
     for (int e = 0; e < NP; ++e) {
         const float x = IS_V ? acc[e] : acc[e] * p.scale;
@@ -899,7 +927,7 @@ __global__ __launch_bounds__(256, 3) void packed_dkv64_kernel(const PackedArgs p
 // P goes from the one to the other through LDS in fp32, register for register (the two products have the same layout).  The
 // work is a sequence of phases of 32 queries with a barrier each; the dS waves run one phase behind.  Tiles are 64 queries
 // (32 KB with dO) in a ring of three: one arriving, one of the P waves, one that the dS waves may still need.
-// Measured as the forward kernel: 2.25 to 2.33 ms, 0.94 to 0.98 PFLOP/s (four products), matrix pipe busy 46 %: a phase takes 2400 cycles of which
+// Measured as the forward kernel: 2.25 to 2.33 ms, 0.94 to 0.98 PFLOP/s (four products), matrix pipe busy 46 to 49 %: a phase takes 2400 cycles of which
 // the two waves' products are 1024, the rest is each wave's chain from one product over the vector work to the next.  (Products issued behind the wait for
 // the other operands instead of between their reads: 3 % slower; all reads issued first: the same; dS
 // waves half a phase out of step with the P waves, their dK products under the P waves' exponentials: 2.49 ms; products in front of

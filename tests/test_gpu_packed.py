@@ -540,3 +540,27 @@ def test_many_blocks(ops, h, hk, d):
         out = ops.attention_packed(*leaves, pack, causal=causal)
         got = (out.detach(), *torch.autograd.grad(out, leaves, do))
         _check(got, *_expected(q.detach(), k.detach(), v.detach(), do, offsets, causal, d ** -0.5))
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("causal", [True, False])
+def test_rows_done_one_by_one_are_right(ops, d, causal):
+    """One element of one value is NaN: its column of the output is, every other number of the document is as it was (all of
+    its rows take the slow path), and its neighbours do not notice."""
+    offsets, h, hk = [0, 70, 410, 433], 4, 2
+    t = offsets[-1]
+    q, k, v, do = _inputs(t, h, hk, d, seed=d)
+    val, err = _expected(q, k, v, do, offsets, causal, d ** -0.5)
+    bad = v.clone()
+    bad[75, 1, 7] = math.nan
+    leaves = [x.requires_grad_(True) for x in (q, k, bad)]
+    pack = ops.pack_sequences(offsets, t, device="cuda")
+    out = ops.attention_packed(*leaves, pack, causal=causal)
+    got = [out.detach(), *torch.autograd.grad(out, leaves, do)]
+    seen = slice(75, 410) if causal else slice(70, 410)  # rows that attend to it, through the second key head: heads 2 and 3
+    assert bool(torch.isnan(got[0][seen, 2:, 7]).all()) and bool(torch.isnan(got[1][seen, 2:]).all())
+    # every key that one of those rows attends to gets a NaN, and nothing of dv, which does not depend on v
+    assert bool(torch.isnan(got[2][70:410, 1]).all())
+    for x, y in ((got[0][seen, 2:, 7], val[0][seen, 2:, 7]), (got[1][seen, 2:], val[1][seen, 2:]), (got[2][70:410, 1], val[2][70:410, 1])):
+        x.copy_(y)
+    _check([x.double() for x in got], val, [e + H * y.abs() for y, e in zip(val, err)])  # (the copies are rounded to bf16)
