@@ -24,28 +24,28 @@ BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
 def listed():
     return [
         # a handful of short prompts to score: the latency of one call
-        attention("attention: few short documents", 200, 96, 16, 16, 64, causal=True, train=False),
+        attention("attention, few short documents", 200, 96, 16, 16, 64, causal=True, train=False),
         # one training batch of documents cut at the 1024-token context, 16 heads
-        attention("attention: documents", 16381, 1024, 16, 16, 64, causal=True, train=True),
+        attention("attention, documents", 16381, 1024, 16, 16, 64, causal=True, train=True),
         # grouped heads, documents of very different lengths
-        attention("attention: grouped heads", 8192, 4096, 32, 8, 128, causal=True, train=True),
+        attention("attention, grouped heads", 8192, 4096, 32, 8, 128, causal=True, train=True),
         # one long document, grouped heads
-        attention("attention: long document", 16384, 16384, 16, 4, 128, causal=True, train=True, lengths=0),
+        attention("attention, long document", 16384, 16384, 16, 4, 128, causal=True, train=True, lengths=0),
         # images of different sizes as token sequences, every token sees its whole image
-        attention("attention: images", 12601, 197, 12, 12, 64, causal=False, train=True),
+        attention("attention, images", 12601, 197, 12, 12, 64, causal=False, train=True),
         # the loss of a few sequences' last tokens: bound by reading the vocabulary's weights
-        head_loss("loss: few rows", 64, 50257, 768, train=False),
+        head_loss("loss, few rows", 64, 50257, 768, train=False),
         # one step of a medium language model
-        head_loss("loss: 50k vocabulary", 8192, 50257, 1024, train=True),
+        head_loss("loss, 50k vocabulary", 8192, 50257, 1024, train=True),
         # a large multilingual vocabulary
-        head_loss("loss: 130k vocabulary", 8192, 130001, 2048, train=True),
+        head_loss("loss, 130k vocabulary", 8192, 130001, 2048, train=True),
         # an image classifier that learns from a larger one's best five classes
-        distill("distillation: 1000 classes", 256, 1000, 5, "bf16"),
+        distill("distillation, 1000 classes", 256, 1000, 5, "bf16"),
         # logits of a language model against stored top-64 logits
-        distill("distillation: 50k vocabulary", 8192, 50257, 64, "bf16"),
+        distill("distillation, 50k vocabulary", 8192, 50257, 64, "bf16"),
         # the same from the hidden states, a small and a usual step
-        head_distill("head distillation: few rows", 512, 50257, 768, 32),
-        head_distill("head distillation: 50k vocabulary", 8192, 50257, 1024, 64),
+        head_distill("head distillation, few rows", 512, 50257, 768, 32),
+        head_distill("head distillation, 50k vocabulary", 8192, 50257, 1024, 64),
     ]
 
 
