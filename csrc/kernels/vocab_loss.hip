@@ -821,7 +821,7 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(const Rows a) {
 template <typename T>
 struct Logits {
     const T* z;
-    T* dz;                   // [rows][ldd], or nullptr
+    T* dz;                   // [rows][ldd], or nullptr; entries behind the vocabulary become zeros
     long long ldz, ldd;
     const long long* ids;
     const float* p;
@@ -860,7 +860,7 @@ __global__ __launch_bounds__(THREADS) void logits_distill_kernel(const Logits<T>
     if (!valid) {
         if (tid == 0) a.row_loss[row] = 0.f;
         if (dz != nullptr)
-            for (int c = tid; c < a.vocab; c += THREADS) dz[c] = static_cast<T>(0.f);
+            for (int c = tid; c < a.ldd; c += THREADS) dz[c] = static_cast<T>(0.f);
         return;
     }
     typedef typename ChunkOf<T>::vec vec;
@@ -924,8 +924,13 @@ __global__ __launch_bounds__(THREADS) void logits_distill_kernel(const Logits<T>
         vec r;
 #pragma unroll
         for (int e = 0; e < W; ++e) r[e] = static_cast<T>(q_of(static_cast<float>(x[e])) * g);
+        if ((c + 1) * W > a.vocab) {
+#pragma unroll
+            for (int e = 0; e < W; ++e) r[e] = c * W + e < a.vocab ? r[e] : static_cast<T>(0.f);
+        }
         vl_store(reinterpret_cast<vec*>(dz + c * W), r, a.stream);
     });
+    for (int c = chunks * W + tid; c < a.ldd; c += THREADS) dz[c] = static_cast<T>(0.f);
     __syncthreads();
     for (int k = tid; k < a.top; k += THREADS)
         if (p[k] != 0.f) dz[ids[k]] = static_cast<T>((q_of(static_cast<float>(z[ids[k]])) - p[k]) * g);
@@ -1182,8 +1187,8 @@ PDT_API long long pdt_distill_scratch(int rows, int top) {
     return static_cast<long long>(m.used);
 }
 
-// dtype: 0 fp32, 1 bf16 logits.  dz (may be nullptr) has the logits' type, 16-byte aligned rows of pitch ldd and room for
-// whole 16-byte chunks.
+// dtype: 0 fp32, 1 bf16 logits.  dz (may be nullptr) has the logits' type and 16-byte aligned rows of pitch ldd that hold whole
+// 16-byte chunks; it is written up to the pitch, zeros behind the vocabulary.
 PDT_API int pdt_distill(const void* z, void* dz, const long long* ids, const float* teacher, float* loss, void* scratch, long long scratch_bytes, int rows,
                         int vocab, int top, long long ldz, long long ldd, float tau, int dtype, void* stream) {
     if (rows <= 0 || rows >= VL_MAX_ROWS || vocab <= 0 || vocab >= (1 << 24) || top <= 0 || top > VL_MAX_TOP || ldz < 0 || !(tau > 0.f) ||

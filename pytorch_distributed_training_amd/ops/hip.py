@@ -198,7 +198,7 @@ class ZeroArena:
         self._threads: set = set()
 
     def _check_thread(self) -> None:
-        """The arena (like the shadow-weight cache and the padded-gradient cache of this module) is process-wide state
+        """The arena (like the shadow-weight cache of this module) is process-wide state
         that assumes ONE training loop: regions are handed out by the thread that runs forward and by autograd's
         device thread that runs backward, strictly one after the other.  A third thread means two loops share the
         process (two models trained concurrently): their steps would clear each other's accumulators."""
@@ -1361,7 +1361,19 @@ def global_avgpool(a):
 # ------------------------------------------------------------------------------------------------
 # Linear
 # ------------------------------------------------------------------------------------------------
-_PADDED_GRADS: Dict[int, int] = {}  # data_ptr of a zero-padded gradient buffer -> its row stride
+def zero_padded(buf: torch.Tensor) -> torch.Tensor:
+    """Notes of a ``[rows, pitch]`` buffer that a loss hands out cut to its first columns that the others hold zeros.  The note is
+    the memory's own: it ends with it, so another buffer at the same address (a sum of two gradients frees the one, a later
+    step gets its place) is never taken for it."""
+    buf.untyped_storage()._pdt_zero_padded = buf.shape[1]
+    return buf
+
+
+def padded_form(g: torch.Tensor, pitch: int) -> Optional[torch.Tensor]:
+    """The ``[rows, pitch]`` buffer that ``g`` is cut from, where its other columns are known to hold zeros."""
+    if g.stride() != (pitch, 1) or g.storage_offset() != 0 or getattr(g.untyped_storage(), "_pdt_zero_padded", 0) != pitch:
+        return None
+    return torch.as_strided(g, (g.shape[0], pitch), (pitch, 1))
 
 
 class _Linear(torch.autograd.Function):
@@ -1416,11 +1428,11 @@ class _Linear(torch.autograd.Function):
             g2 = g2.to(torch.bfloat16)
         if npad == n:
             gp = g2 if g2.is_contiguous() else g2.contiguous()
-        elif _PADDED_GRADS.pop(g2.data_ptr(), None) == npad and g2.stride() == (npad, 1):
-            gp = torch.as_strided(g2, (M, npad), (npad, 1))  # produced zero-padded by the loss kernel
         else:
-            gp = torch.zeros((M, npad), dtype=torch.bfloat16, device=g.device)
-            gp[:, :n].copy_(g2)
+            gp = padded_form(g2, npad)  # produced zero-padded by the loss kernel
+            if gp is None:
+                gp = torch.zeros((M, npad), dtype=torch.bfloat16, device=g.device)
+                gp[:, :n].copy_(g2)
         dx = dw = db = None
         if ctx.needs_input_grad[0]:
             wt, npad_w = SHADOWS.dgrad(weight, 1)  # [k][npad]
@@ -1619,10 +1631,7 @@ class _SoftmaxCE(torch.autograd.Function):
             ctx.fused[0] = None
             g1 = g.reshape(1).to(torch.float32).contiguous()
             _check(_scale_by_scalar(dbuf.data_ptr(), g1.data_ptr(), dbuf.numel(), _stream()), "scale_by_scalar")
-            if pad_to != classes:
-                _PADDED_GRADS[dbuf.data_ptr()] = pad_to
-                return dbuf[:, :classes], None
-            return dbuf, None
+            return (zero_padded(dbuf)[:, :classes] if pad_to != classes else dbuf), None
         logits, labels, lse = ctx.saved_tensors
         rows, classes = logits.shape
         ld = logits.stride(0)
@@ -1632,10 +1641,7 @@ class _SoftmaxCE(torch.autograd.Function):
         dt = 1 if logits.dtype == torch.bfloat16 else 0
         _check(_ce_bwd(logits.data_ptr(), labels.data_ptr(), lse.data_ptr(), g1.data_ptr(), dbuf.data_ptr(), rows, classes,
                        ld, pad_to, pad_to, dt, _stream()), "softmax_ce_bwd")
-        if pad_to != classes:
-            _PADDED_GRADS[dbuf.data_ptr()] = pad_to
-            return dbuf[:, :classes], None
-        return dbuf, None
+        return (zero_padded(dbuf)[:, :classes] if pad_to != classes else dbuf), None
 
 
 def softmax_cross_entropy(logits, labels):

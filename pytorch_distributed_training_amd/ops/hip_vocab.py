@@ -10,7 +10,7 @@ import os
 
 import torch
 
-from .hip import SHADOWS, _axpy_dev, _check, _grad_sink, _on, _once_differentiable, _ptr, _round_up, _stream
+from .hip import SHADOWS, _axpy_dev, _check, _grad_sink, _on, _once_differentiable, _ptr, _round_up, _stream, zero_padded
 from .hip_transformer import _f, _i, _ll, _sig, _vp
 
 _head_scratch = _sig("pdt_head_loss_scratch", [_i] * 8)
@@ -118,7 +118,7 @@ def head_loss(x, weight, ids, teacher, tau: float):
 
 
 def _distill_forward(logits, ids, teacher, tau: float, want: bool):
-    """(loss, gradient of the logits for an incoming one of 1, rows padded to whole 128 bytes)."""
+    """(loss, gradient of the logits for an incoming one of 1, rows padded with zeros to 64 entries as ``ops.linear`` takes them)."""
     vocab = logits.shape[-1]
     dev = logits.device
     with _on(dev):
@@ -157,7 +157,7 @@ class _LogitsDistill(torch.autograd.Function):
             g1 = g if g.dtype == torch.float32 else g.to(torch.float32)
             _scale(g1, dz)
         if dz.shape[1] != ctx.shape[-1]:
-            dz = dz[:, :ctx.shape[-1]]
+            dz = zero_padded(dz)[:, :ctx.shape[-1]]
         return dz.reshape(ctx.shape), None, None, None
 
 

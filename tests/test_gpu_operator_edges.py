@@ -1,0 +1,93 @@
+"""Packed attention, vocabulary losses and the losses beside them on the GPU, where they meet other parts: the linear layer's
+padded gradients, over-long documents, forward-mode derivatives, rows without a label, students close to their teacher,
+results far from 1 (needs an MI355X).
+
+h = 2^-8 is half a step of bf16 relative to the value; sums of n products in 32 bits are off by n 2^-24 of their absolute sum.
+"""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+H = 2.0 ** -8
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ops():
+    from pytorch_distributed_training_amd import ops as m
+
+    return m
+
+
+def _gen(seed):
+    return torch.Generator("cuda").manual_seed(seed)
+
+
+def _bf16(*shape, seed=0, std=1.0):
+    return (torch.randn(*shape, generator=_gen(seed), device="cuda") * std).to(torch.bfloat16)
+
+
+def _distill_64(z, teacher, ids, tau):
+    """Gradient of the logits in 64 bits (every row has a target, no id twice in a row)."""
+    p = torch.softmax(teacher.double() / tau, 1)
+    dz = torch.softmax(z.double() / tau, 1).scatter_add(1, ids, -p)
+    return dz * (tau / len(z))
+
+
+@pytest.mark.parametrize("vocab", [1000, 2010, 1020])
+@pytest.mark.parametrize("left_out", [False, True])
+def test_distillation_behind_a_linear_layer(ops, vocab, left_out):
+    """Distillation alone behind a projection whose rows are padded, in memory that held NaN, after a step that added
+    cross-entropy and distillation on the same logits: the gradient of x against the formula's."""
+    n, width, top, tau = 64, 128, 5, 2.0
+    weight = torch.nn.Parameter(_bf16(vocab, width, seed=1, std=2.0 / math.sqrt(width)).float())
+    x = _bf16(n, width, seed=2)
+    ids = (torch.arange(n, device="cuda")[:, None] * 13 + torch.arange(top, device="cuda") * 7) % vocab
+    teacher = torch.randn(n, top, generator=_gen(3), device="cuda")
+    labels = ids[:, 0].contiguous()
+    if left_out:
+        ids = ids.clone()
+        ids[5] = -1
+    pitch = (vocab + 63) // 64 * 64
+    for _ in range(3):
+        a = x.clone().requires_grad_(True)
+        z = ops.linear(a, weight)
+        (ops.softmax_cross_entropy(z, labels) + ops.distillation_loss(z, teacher, ids, tau)).backward()
+        del z
+        for fill in [torch.full((n, pitch), math.nan, dtype=torch.bfloat16, device="cuda") for _ in range(8)]:
+            del fill
+        b = x.clone().requires_grad_(True)
+        z = ops.linear(b, weight)
+        ops.distillation_loss(z, teacher, ids, tau).backward()
+        dz = _distill_64(z.detach(), teacher, ids.clamp(min=0), tau)
+        if left_out:
+            dz[5] = 0
+            dz *= n / (n - 1)
+        w = weight.detach().double()
+        want = dz @ w
+        # the gradient of the logits rounded once, the result once; the sums in 32 bits, the probabilities to 2e-5
+        bound = (H + 2e-5 + vocab * U) * (dz.abs() @ w.abs()) + 2e-5 * tau / n * (torch.softmax(z.detach().double() / tau, 1) @ w.abs()) + H * want.abs()
+        assert bool(torch.isfinite(b.grad).all())
+        over = (b.grad.double() - want).abs() - 1.05 * bound
+        assert float(over.max()) <= 0, float(over.max())
+        weight.grad = None
+
+
+def test_distillation_gradient_is_taken_as_it_is(ops):
+    """The rows' padding is written with zeros, left-out rows' too, whatever the memory held."""
+    from pytorch_distributed_training_amd.ops import hip_vocab
+
+    for dtype in (torch.bfloat16, torch.float32):
+        for vocab in (1000, 1001, 63, 1023):
+            n = 7
+            pitch = (vocab + 63) // 64 * 64
+            z = _bf16(n, vocab, seed=vocab).to(dtype)
+            ids = torch.randint(0, vocab, (n, 3), generator=_gen(4), device="cuda")
+            ids[2] = -1
+            full = torch.full((n, pitch), math.nan, dtype=dtype, device="cuda")
+            del full
+            _, dz = hip_vocab._distill_forward(z, ids, torch.zeros(n, 3, device="cuda"), 1.0, True)
+            assert dz.shape[1] == pitch and bool((dz[:, vocab:] == 0).all()) and bool(torch.isfinite(dz).all())

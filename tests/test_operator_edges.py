@@ -1,0 +1,25 @@
+"""Limits and bookkeeping of the packed and vocabulary operators that need no GPU."""
+import pytest
+import torch
+
+
+def test_padding_is_known_of_the_buffer_itself():
+    """What a loss says of its gradient's padding ends with the buffer: another one at the same address says nothing."""
+    from pytorch_distributed_training_amd.ops import hip
+
+    def at(memory):
+        return torch.frombuffer(memory, dtype=torch.bfloat16).view(6, 64)
+
+    memory = bytearray(6 * 64 * 2)
+    buf = hip.zero_padded(at(memory))
+    g = buf[:, :50]
+    assert hip.padded_form(g, 64).shape == (6, 64) and hip.padded_form(g, 64).data_ptr() == buf.data_ptr()
+    assert hip.padded_form(g.reshape(2, 3, 50).reshape(6, 50), 64) is not None  # a view of a view
+    assert hip.padded_form(g, 128) is None and hip.padded_form(g[1:], 64) is None and hip.padded_form(g[:, 1:], 64) is None
+    total = g + g  # a sum with another loss's gradient is dense, and the buffer goes unused
+    assert hip.padded_form(total, 64) is None
+    address = buf.data_ptr()
+    del buf, g
+    later = at(memory)[:, :50]
+    assert later.data_ptr() == address and later.stride() == (64, 1)
+    assert hip.padded_form(later, 64) is None
