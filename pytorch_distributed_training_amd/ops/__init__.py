@@ -315,7 +315,7 @@ def token_position_embedding(ids, wte, wpe, pack: Optional[SequencePack] = None)
     """Input embedding of a language model: ``wte[ids] + wpe[position]`` for ``ids`` of shape ``[B, S]``, or of shape
     ``[rows]`` with ``pack``, where positions count from the start of each sequence (and are 0 outside).  A sequence longer
     than the table is refused where the pack knows its lengths; of one made from offsets on the GPU the tokens behind the
-    table's end take its last row."""
+    table's end take its last row, and their gradients go to it."""
     if pack is not None:
         if not isinstance(pack, SequencePack):
             raise TypeError("pack: a SequencePack, made by ops.pack_sequences")
@@ -331,7 +331,7 @@ def token_position_embedding(ids, wte, wpe, pack: Optional[SequencePack] = None)
         from . import hip_transformer as ht
 
         if pack is not None:
-            return ht.packed_embedding(ids, pack.positions, wte, wpe)
+            return ht.packed_embedding(ids, pack, wte, wpe)
         return ht.token_position_embedding(ids, wte, wpe)
     if pack is not None:
         return _ref.packed_embedding(ids, pack.positions, wte, wpe)

@@ -278,10 +278,11 @@ def token_position_embedding(ids, wte, wpe):
 
 class _PackedEmbedding(torch.autograd.Function):
     """``wte[ids] + wpe[positions]`` -> bf16 ``[rows, D]`` for packed sequences: rows of equal position lie anywhere, so the
-    position table's gradient is a scatter-add like the token table's."""
+    position table's gradient is a scatter-add like the token table's.  Positions behind the table's end (``inside``: there
+    are none) read its last row, and their gradients go there."""
 
     @staticmethod
-    def forward(ctx, ids, positions, wte, wpe):
+    def forward(ctx, ids, positions, wte, wpe, inside: bool):
         ids_c = ids.to(torch.int64).contiguous()
         vocab, d = wte.shape
         if wpe.shape[1] != d or not wte.is_contiguous() or not wpe.is_contiguous():
@@ -294,27 +295,29 @@ class _PackedEmbedding(torch.autograd.Function):
                 _check(_emb_pos_fwd(ids_c.data_ptr(), wte.data_ptr(), wpe.data_ptr(), positions.data_ptr(), out.data_ptr(), ids_c.numel(), d,
                                     vocab, wpe.shape[0], _stream()), "embedding_pos_fwd")
         ctx.save_for_backward(ids_c, positions)
-        ctx.tables = (wte, wpe)
+        ctx.tables, ctx.inside = (wte, wpe), inside
         return out
 
     @staticmethod
     def backward(ctx, g):
         grads = []
         g2 = _bf16c(g)
-        for need, table, ids in zip(ctx.needs_input_grad[2:], ctx.tables, ctx.saved_tensors):
+        for need, table, at, bounded in zip(ctx.needs_input_grad[2:], ctx.tables, ctx.saved_tensors, (True, ctx.inside)):
             if not need:
                 grads.append(None)
                 continue
             buf, own = _param_grad_target(table, tuple(table.shape), g.device)
-            if ids.numel():
+            if at.numel():
                 with _on(g.device):
-                    _embedding_grad(ids, g2, buf, table.shape[1], table.shape[0])
+                    if not bounded:
+                        at = at.clamp(max=table.shape[0] - 1)
+                    _embedding_grad(at, g2, buf, table.shape[1], table.shape[0])
             grads.append(None if own else buf)
-        return None, None, *grads
+        return None, None, *grads, None
 
 
-def packed_embedding(ids, positions, wte, wpe):
-    return _PackedEmbedding.apply(ids, positions, wte, wpe)
+def packed_embedding(ids, pack, wte, wpe):
+    return _PackedEmbedding.apply(ids, pack.positions, wte, wpe, pack.longest is not None and pack.longest <= wpe.shape[0])
 
 
 class _VitAssemble(torch.autograd.Function):

@@ -91,3 +91,27 @@ def test_distillation_gradient_is_taken_as_it_is(ops):
             del full
             _, dz = hip_vocab._distill_forward(z, ids, torch.zeros(n, 3, device="cuda"), 1.0, True)
             assert dz.shape[1] == pitch and bool((dz[:, vocab:] == 0).all()) and bool(torch.isfinite(dz).all())
+
+
+@pytest.mark.parametrize("deterministic", [False, True])
+def test_gradient_of_positions_behind_the_tables_end(ops, deterministic):
+    """Tokens behind the position table's end read its last row, so their gradients are its."""
+    offsets = torch.tensor([0, 40, 47, 52], device="cuda")
+    rows, d = 53, 64
+    wte, wpe = torch.randn(30, d, generator=_gen(0), device="cuda"), torch.randn(16, d, generator=_gen(1), device="cuda")
+    wte.requires_grad_(True), wpe.requires_grad_(True)
+    ids = torch.randint(0, 30, (rows,), generator=_gen(2), device="cuda")
+    g = _bf16(rows, d, seed=3)
+    pack = ops.pack_sequences(offsets, rows)
+    at = pack.positions.clamp(max=15)
+    ops.set_deterministic(deterministic)
+    try:
+        out = ops.token_position_embedding(ids, wte, wpe, pack)
+        a, b = torch.autograd.grad(out, (wte, wpe), g)
+    finally:
+        ops.set_deterministic(False)
+    assert torch.equal(out.detach(), (wte[ids] + wpe[at]).to(torch.bfloat16))
+    for got, index in ((a, ids), (b, at)):
+        want = torch.zeros(got.shape, dtype=torch.float64, device="cuda").index_add_(0, index, g.double())
+        terms = torch.zeros(got.shape, dtype=torch.float64, device="cuda").index_add_(0, index, g.double().abs())
+        assert bool(((got.double() - want).abs() <= rows * U * terms).all())
