@@ -26,6 +26,7 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad as _forward_ad
 
 from .. import native
 
@@ -117,6 +118,14 @@ def _once_differentiable(backward):
         return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
     return run
+
+
+def _derivative_wanted(*inputs: torch.Tensor) -> bool:
+    """Whether a call on these has to go through its autograd function: one of them requires a gradient, or carries a tangent
+    (forward mode knows neither ``requires_grad`` nor ``no_grad``; the function refuses it instead of dropping it)."""
+    if torch.is_grad_enabled() and any(x.requires_grad for x in inputs):
+        return True
+    return any(_forward_ad.unpack_dual(x).tangent is not None for x in inputs)
 
 
 def _on(device: torch.device):

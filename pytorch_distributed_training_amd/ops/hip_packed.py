@@ -9,7 +9,7 @@ import ctypes
 
 import torch
 
-from .hip import _check, _on, _once_differentiable, _ptr, _stream
+from .hip import _check, _derivative_wanted, _on, _once_differentiable, _ptr, _stream
 from .hip_transformer import _f, _i, _sig, _vp
 
 _pack_spans = _sig("pdt_pack_spans", [_vp, _i, _i] + [_vp] * 5)
@@ -143,7 +143,7 @@ def _check_head_dim(d: int) -> None:
 
 def attention_packed(q, k, v, pack, causal: bool, scale: float):
     _check_head_dim(q.shape[2])
-    if not (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad)):
+    if not _derivative_wanted(q, k, v):
         with _on(q.device):
             return _forward(_heads(q), _heads(k), _heads(v), pack.plan, causal, scale, False)[0]
     return _AttentionPacked.apply(q, k, v, pack.plan, bool(causal), scale)

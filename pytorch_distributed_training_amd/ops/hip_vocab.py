@@ -10,7 +10,7 @@ import os
 
 import torch
 
-from .hip import SHADOWS, _axpy_dev, _check, _grad_sink, _on, _once_differentiable, _ptr, _round_up, _stream, zero_padded
+from .hip import SHADOWS, _axpy_dev, _check, _derivative_wanted, _grad_sink, _on, _once_differentiable, _ptr, _round_up, _stream, zero_padded
 from .hip_transformer import _f, _i, _ll, _sig, _vp
 
 _head_scratch = _sig("pdt_head_loss_scratch", [_i] * 8)
@@ -112,7 +112,7 @@ class _HeadLoss(torch.autograd.Function):
 
 
 def head_loss(x, weight, ids, teacher, tau: float):
-    if not (torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad)):
+    if not _derivative_wanted(x, weight):
         return _head_forward(x, weight, ids, teacher, tau, False, False)[0]
     return _HeadLoss.apply(x, weight, ids, teacher, tau)
 
@@ -162,6 +162,6 @@ class _LogitsDistill(torch.autograd.Function):
 
 
 def logits_distill(logits, ids, teacher, tau: float):
-    if not (torch.is_grad_enabled() and logits.requires_grad):
+    if not _derivative_wanted(logits):
         return _distill_forward(logits, ids, teacher, tau, False)[0]
     return _LogitsDistill.apply(logits, ids, teacher, tau)

@@ -115,3 +115,29 @@ def test_gradient_of_positions_behind_the_tables_end(ops, deterministic):
         want = torch.zeros(got.shape, dtype=torch.float64, device="cuda").index_add_(0, index, g.double())
         terms = torch.zeros(got.shape, dtype=torch.float64, device="cuda").index_add_(0, index, g.double().abs())
         assert bool(((got.double() - want).abs() <= rows * U * terms).all())
+
+
+def test_forward_mode_derivatives_are_refused(ops):
+    """Not dropped: a dual tensor goes the way of a tensor that requires a gradient, and is refused there."""
+    from torch.autograd import forward_ad
+
+    q, k, v = _bf16(6, 2, 64), _bf16(6, 2, 64, seed=1), _bf16(6, 2, 64, seed=2)
+    pack = ops.pack_sequences([0, 6], 6, device="cuda")
+    x, w, z = _bf16(6, 64), _bf16(70, 64, seed=3), _bf16(6, 70, seed=4)
+    labels, teacher = torch.arange(6, device="cuda"), torch.randn(6, 2, generator=_gen(5), device="cuda")
+    ids = torch.arange(12, device="cuda").view(6, 2)
+    calls = {
+        "attention": (lambda a, b, c: ops.attention_packed(a, b, c, pack), [q, k, v]),
+        "joint": (lambda a: ops.attention_packed_qkv(a, pack, 2), [torch.cat([q, k, v], 1).flatten(1)]),
+        "loss": (lambda a, b: ops.linear_cross_entropy(a, b, labels), [x, w]),
+        "head distillation": (lambda a, b, t: ops.linear_distillation_loss(a, b, t, ids), [x, w, teacher]),
+        "distillation": (lambda a, t: ops.distillation_loss(a, t, ids), [z, teacher]),
+    }
+    for name, (call, inputs) in calls.items():
+        plain = call(*inputs)
+        for i in range(len(inputs)):
+            for grad in (True, False):
+                with forward_ad.dual_level(), torch.set_grad_enabled(grad):
+                    with pytest.raises((NotImplementedError, ValueError)):
+                        call(*(forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(inputs)))
+                    assert torch.equal(call(*inputs), plain), name

@@ -23,3 +23,20 @@ def test_padding_is_known_of_the_buffer_itself():
     later = at(memory)[:, :50]
     assert later.data_ptr() == address and later.stride() == (64, 1)
     assert hip.padded_form(later, 64) is None
+
+
+def test_no_tangent_of_the_teacher():
+    from torch.autograd import forward_ad
+
+    from pytorch_distributed_training_amd import ops
+
+    z, t, ids = torch.randn(3, 5), torch.randn(3, 2), torch.tensor([[0, 1], [2, 3], [4, 0]])
+    x, w = torch.randn(3, 8), torch.randn(5, 8)
+    with forward_ad.dual_level():
+        dual = forward_ad.make_dual(t, torch.ones_like(t))
+        with pytest.raises(ValueError, match="teacher"):
+            ops.distillation_loss(z, dual, ids)
+        with pytest.raises(ValueError, match="teacher"):
+            ops.linear_distillation_loss(x, w, dual, ids)
+        tangent = forward_ad.unpack_dual(ops.distillation_loss(forward_ad.make_dual(z, torch.ones_like(z)), t, ids)).tangent
+        assert abs(float(tangent)) < 1e-6  # (a shift of all logits changes nothing)
