@@ -1,9 +1,10 @@
-// Fused softmax cross-entropy (mean over rows) for bf16 or fp32 logits.
+// Fused softmax cross-entropy for bf16 or fp32 logits, mean over the rows whose label is one of the classes: a label outside
+// (-100, say) leaves its row out, without gradient and not counted; 0 where no row has one.
 //
 // Forward: one pass per row computes max, log-sum-exp and the row loss (online softmax, so the
 //          row is read once even when it does not fit in registers); the row's lse is kept.
-// Backward: dlogits = (exp(x - lse) - onehot) * (g / rows), written in the logits' dtype in one
-//          pass; probabilities are never materialised.
+// Backward: dlogits = (exp(x - lse) - onehot) * (g / rows with a label), written in the logits' dtype in
+//          one pass; probabilities are never materialised.
 // Rows of up to 1024 classes are handled by one wave each (4 rows per workgroup); longer rows
 // (language-model vocabularies) by one 256-thread workgroup each.
 //
@@ -33,6 +34,18 @@ __device__ __forceinline__ void online_merge(float& m, float& s, float m2, float
     const float mn = fmaxf(m, m2);
     s = s * __expf(m - mn) + s2 * __expf(m2 - mn);
     m = mn;
+}
+
+// rows with a label, 1 where there are none (the sums they divide are 0 then)
+__device__ __forceinline__ float label_count(const long long* __restrict__ labels, long long rows, int classes, float* red) {
+    float c = 0.f;
+    for (long long i = threadIdx.x; i < rows; i += blockDim.x) c += labels[i] >= 0 && labels[i] < classes ? 1.f : 0.f;
+    return fmaxf(block_sum(c, red), 1.f);  // (whole numbers: exact up to 2^24 rows, and every thread's share far below)
+}
+__global__ __launch_bounds__(1024) void label_count_kernel(const long long* __restrict__ labels, long long rows, int classes, float* __restrict__ count) {
+    __shared__ float red[16];
+    const float c = label_count(labels, rows, classes, red);
+    if (threadIdx.x == 0) count[0] = c;
 }
 
 // ---- wave-per-row forward
@@ -104,9 +117,9 @@ __global__ __launch_bounds__(256) void ce_fwd_block_kernel(const T* __restrict__
 template <typename T>
 __global__ __launch_bounds__(256) void ce_bwd_kernel(const T* __restrict__ logits, const long long* __restrict__ labels,
                                                     const float* __restrict__ lse, const float* __restrict__ gout,
-                                                    T* __restrict__ dlogits, int rows, int classes, long long ld_row,
-                                                    long long ld_drow, int pad_to) {
-    const float g = gout[0] / rows;
+                                                    const float* __restrict__ count, T* __restrict__ dlogits, int rows,
+                                                    int classes, long long ld_row, long long ld_drow, int pad_to) {
+    const float g = gout[0] / count[0];
     // one workgroup walks whole rows so lse/label are loaded once per row
     for (int row = blockIdx.x; row < rows; row += gridDim.x) {
         const float l = lse[row];
@@ -124,13 +137,13 @@ __global__ __launch_bounds__(256) void ce_bwd_kernel(const T* __restrict__ logit
 
 // ---- long bf16 rows, forward and gradient in one pass: a 512-thread workgroup holds its row in registers
 // (NV 16-byte vectors per thread), so the logits are read from memory once and the gradient
-// (softmax - onehot) / rows is written straight away; the backward pass only has to scale it by the
+// (softmax - onehot) / (rows with a label) is written straight away; the backward pass only has to scale it by the
 // incoming gradient, which for a loss that is the root of the graph is 1.
 template <int NV>
 __global__ __launch_bounds__(512) void ce_fused_row_kernel(const bf16* __restrict__ logits, const long long* __restrict__ labels,
                                                           float* __restrict__ row_loss, bf16* __restrict__ dlogits,
                                                           int rows, int classes, long long ld_row, long long ld_drow,
-                                                          int pad_to, float inv_rows) {
+                                                          int pad_to, const float* __restrict__ count) {
     __shared__ float red[16];
     const int row = blockIdx.x;
     const bf16* x = logits + row * ld_row;
@@ -176,7 +189,7 @@ __global__ __launch_bounds__(512) void ce_fused_row_kernel(const bf16* __restric
     if (dlogits == nullptr) return;
     // (dlogits may be the logits buffer itself: every thread has its part of the row in registers by now, and the
     // block reductions above are barriers between the last load and the first store)
-    const float g = valid ? inv_rows : 0.f;
+    const float g = valid ? 1.f / count[0] : 0.f;
     const float ll2 = l * 1.4426950408889634f;
     bf16* d = dlogits + row * ld_drow;
     const int pvec = pad_to >> 3;
@@ -189,7 +202,7 @@ __global__ __launch_bounds__(512) void ce_fused_row_kernel(const bf16* __restric
             for (int e = 0; e < 8; ++e) {
                 const int c = vi * 8 + e;
                 float r = 0.f;
-                if (vi < nvec && c < classes)
+                if (vi < nvec && c < classes && valid)
                     r = (__builtin_amdgcn_exp2f(bf16_to_f32(v[i][e]) * 1.4426950408889634f - ll2) - (c == y ? 1.f : 0.f)) * g;
                 o[e] = f32_to_bf16(r);
             }
@@ -210,18 +223,24 @@ __global__ __launch_bounds__(256) void scale_by_scalar_kernel(bf16* __restrict__
     }
 }
 
-// deterministic mean of a float vector -> out[0]  (single workgroup)
-__global__ __launch_bounds__(1024) void mean_kernel(const float* __restrict__ x, float* __restrict__ out, long long n,
-                                                   float scale) {
+// Sum of the row losses over the rows with a label (single workgroup, fixed order): counted from the labels and left in
+// count, or - where labels is nullptr - as count says.
+__global__ __launch_bounds__(1024) void ce_mean_kernel(const float* __restrict__ row_loss, const long long* __restrict__ labels, long long rows,
+                                                      int classes, float* __restrict__ count, float* __restrict__ loss) {
     __shared__ float red[16];
     float s = 0.f;
-    for (long long i = threadIdx.x; i < n; i += 1024) s += x[i];
+    for (long long i = threadIdx.x; i < rows; i += 1024) s += row_loss[i];
     const float t = block_sum(s, red);
-    if (threadIdx.x == 0) out[0] = t * scale;
+    const float c = labels != nullptr ? label_count(labels, rows, classes, red) : count[0];
+    if (threadIdx.x == 0) {
+        loss[0] = t * (1.f / c);
+        if (labels != nullptr) count[0] = c;
+    }
 }
 
-// dtype: 0 = fp32 logits, 1 = bf16 logits.  row_loss/lse: [rows] fp32.  loss: [1] fp32.
-PDT_API int pdt_softmax_ce_fwd(const void* logits, const long long* labels, float* row_loss, float* lse, float* loss,
+// dtype: 0 = fp32 logits, 1 = bf16 logits.  row_loss/lse: [rows] fp32.  loss: [1] fp32.  count: [1] fp32,
+// the rows with a label (at least 1), for the backward pass.
+PDT_API int pdt_softmax_ce_fwd(const void* logits, const long long* labels, float* row_loss, float* lse, float* loss, float* count,
                                int rows, int classes, long long ld_row, int dtype, void* stream) {
     if (rows <= 0 || classes <= 0 || ld_row < classes) return -1;
     hipStream_t s = static_cast<hipStream_t>(stream);
@@ -234,28 +253,30 @@ PDT_API int pdt_softmax_ce_fwd(const void* logits, const long long* labels, floa
         if (dtype == 1) hipLaunchKernelGGL(ce_fwd_block_kernel<bf16>, g, b, 0, s, static_cast<const bf16*>(logits), labels, row_loss, lse, classes, ld_row);
         else hipLaunchKernelGGL(ce_fwd_block_kernel<float>, g, b, 0, s, static_cast<const float*>(logits), labels, row_loss, lse, classes, ld_row);
     }
-    hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(1024), 0, s, row_loss, loss, static_cast<long long>(rows), 1.f / rows);
+    hipLaunchKernelGGL(ce_mean_kernel, dim3(1), dim3(1024), 0, s, row_loss, labels, static_cast<long long>(rows), classes, count, loss);
     return pdt_launch_status();
 }
 
 // dlogits has row stride ld_drow; columns [classes, pad_to) are written as zeros (pad_to <= ld_drow).
-PDT_API int pdt_softmax_ce_bwd(const void* logits, const long long* labels, const float* lse, const float* gout,
+PDT_API int pdt_softmax_ce_bwd(const void* logits, const long long* labels, const float* lse, const float* gout, const float* count,
                                void* dlogits, int rows, int classes, long long ld_row, long long ld_drow, int pad_to,
                                int dtype, void* stream) {
     if (rows <= 0 || classes <= 0 || ld_row < classes || pad_to < classes || ld_drow < pad_to) return -1;
     hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 g(rows < 8192 ? rows : 8192), b(256);
-    if (dtype == 1) hipLaunchKernelGGL(ce_bwd_kernel<bf16>, g, b, 0, s, static_cast<const bf16*>(logits), labels, lse, gout, static_cast<bf16*>(dlogits), rows, classes, ld_row, ld_drow, pad_to);
-    else hipLaunchKernelGGL(ce_bwd_kernel<float>, g, b, 0, s, static_cast<const float*>(logits), labels, lse, gout, static_cast<float*>(dlogits), rows, classes, ld_row, ld_drow, pad_to);
+    if (dtype == 1) hipLaunchKernelGGL(ce_bwd_kernel<bf16>, g, b, 0, s, static_cast<const bf16*>(logits), labels, lse, gout, count, static_cast<bf16*>(dlogits), rows, classes, ld_row, ld_drow, pad_to);
+    else hipLaunchKernelGGL(ce_bwd_kernel<float>, g, b, 0, s, static_cast<const float*>(logits), labels, lse, gout, count, static_cast<float*>(dlogits), rows, classes, ld_row, ld_drow, pad_to);
     return pdt_launch_status();
 }
 
-// Forward and gradient in one pass for bf16 logits with long rows (see ce_fused_row_kernel).  dlogits may be
-// nullptr (no gradient wanted); it has row stride ld_drow and columns [classes, pad_to) are written as zeros.
-// Needs classes > 1024, ld_row, ld_drow and pad_to multiples of 8, ld_row >= classes rounded up to 8, and at
-// most 65536 classes.  The gradient is for an incoming gradient of 1: scale with pdt_scale_by_scalar.
-PDT_API int pdt_softmax_ce_fused(const void* logits, const long long* labels, float* row_loss, float* loss, void* dlogits,
-                                 int rows, int classes, long long ld_row, long long ld_drow, int pad_to, void* stream) {
+// Forward and gradient in one pass for bf16 logits with long rows (see ce_fused_row_kernel): row losses and the logits'
+// gradient for an incoming one of 1 (scale with pdt_scale_by_scalar), of a batch of which count[0] rows have a label
+// (pdt_label_count); pdt_label_mean takes the mean.  A batch may come in chunks of rows.  dlogits may be nullptr (no gradient
+// wanted) or the logits buffer itself: a language-model head then needs no second [rows, vocabulary] buffer; it has row stride
+// ld_drow and columns [classes, pad_to) are written as zeros.  Needs classes > 1024, ld_row, ld_drow and pad_to multiples of
+// 8, ld_row >= classes rounded up to 8, and at most 65536 classes.
+PDT_API int pdt_softmax_ce_fused(const void* logits, const long long* labels, float* row_loss, void* dlogits, int rows, int classes,
+                                 long long ld_row, long long ld_drow, int pad_to, const float* count, void* stream) {
     const int c8 = (classes + 7) / 8 * 8;
     if (rows <= 0 || classes <= 1024 || classes > 65536 || (ld_row % 8) != 0 || ld_row < c8) return -1;
     if (dlogits != nullptr && ((ld_drow % 8) != 0 || (pad_to % 8) != 0 || pad_to < c8 || ld_drow < pad_to || pad_to > 65536)) return -1;
@@ -263,31 +284,7 @@ PDT_API int pdt_softmax_ce_fused(const void* logits, const long long* labels, fl
     const int need = (((dlogits != nullptr ? pad_to : c8) >> 3) + 511) / 512;
     const bf16* x = static_cast<const bf16*>(logits);
     bf16* d = static_cast<bf16*>(dlogits);
-#define PDT_CE(NV) hipLaunchKernelGGL(ce_fused_row_kernel<NV>, dim3(rows), dim3(512), 0, s, x, labels, row_loss, d, rows, classes, ld_row, ld_drow, pad_to, 1.f / rows)
-    if (need <= 4) PDT_CE(4);
-    else if (need <= 8) PDT_CE(8);
-    else if (need <= 13) PDT_CE(13);
-    else PDT_CE(16);
-#undef PDT_CE
-    hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(1024), 0, s, row_loss, loss, static_cast<long long>(rows), 1.f / rows);
-    return pdt_launch_status();
-}
-
-// The same pass over one chunk of `rows` rows of a batch of `total_rows` rows: the gradient is scaled by
-// 1 / total_rows and no mean is taken (pdt_mean_f32 over the row losses of all chunks does that).  `dlogits` may be
-// the logits buffer itself (in-place): a language-model head then needs no second [rows, vocabulary] buffer.
-PDT_API int pdt_softmax_ce_fused_chunk(const void* logits, const long long* labels, float* row_loss, void* dlogits,
-                                       int rows, int classes, long long ld_row, long long ld_drow, int pad_to,
-                                       long long total_rows, void* stream) {
-    const int c8 = (classes + 7) / 8 * 8;
-    if (rows <= 0 || total_rows < rows || classes <= 1024 || classes > 65536 || (ld_row % 8) != 0 || ld_row < c8) return -1;
-    if (dlogits != nullptr && ((ld_drow % 8) != 0 || (pad_to % 8) != 0 || pad_to < c8 || ld_drow < pad_to || pad_to > 65536)) return -1;
-    hipStream_t s = static_cast<hipStream_t>(stream);
-    const int need = (((dlogits != nullptr ? pad_to : c8) >> 3) + 511) / 512;
-    const bf16* x = static_cast<const bf16*>(logits);
-    bf16* d = static_cast<bf16*>(dlogits);
-    const float inv = 1.f / static_cast<float>(total_rows);
-#define PDT_CE(NV) hipLaunchKernelGGL(ce_fused_row_kernel<NV>, dim3(rows), dim3(512), 0, s, x, labels, row_loss, d, rows, classes, ld_row, ld_drow, pad_to, inv)
+#define PDT_CE(NV) hipLaunchKernelGGL(ce_fused_row_kernel<NV>, dim3(rows), dim3(512), 0, s, x, labels, row_loss, d, rows, classes, ld_row, ld_drow, pad_to, count)
     if (need <= 4) PDT_CE(4);
     else if (need <= 8) PDT_CE(8);
     else if (need <= 13) PDT_CE(13);
@@ -296,10 +293,17 @@ PDT_API int pdt_softmax_ce_fused_chunk(const void* logits, const long long* labe
     return pdt_launch_status();
 }
 
-// out[0] = scale * sum(x[0..n)) (deterministic, one workgroup)
-PDT_API int pdt_mean_f32(const float* x, float* out, long long n, float scale, void* stream) {
-    if (n <= 0) return -1;
-    hipLaunchKernelGGL(mean_kernel, dim3(1), dim3(1024), 0, static_cast<hipStream_t>(stream), x, out, n, scale);
+// count[0] = rows with a label, at least 1
+PDT_API int pdt_label_count(const long long* labels, long long rows, int classes, float* count, void* stream) {
+    if (rows <= 0 || classes <= 0) return -1;
+    hipLaunchKernelGGL(label_count_kernel, dim3(1), dim3(1024), 0, static_cast<hipStream_t>(stream), labels, rows, classes, count);
+    return pdt_launch_status();
+}
+
+// loss[0] = sum(row_loss) / count[0] (one workgroup, fixed order)
+PDT_API int pdt_label_mean(const float* row_loss, long long rows, const float* count, float* loss, void* stream) {
+    if (rows <= 0) return -1;
+    hipLaunchKernelGGL(ce_mean_kernel, dim3(1), dim3(1024), 0, static_cast<hipStream_t>(stream), row_loss, nullptr, rows, 0, const_cast<float*>(count), loss);
     return pdt_launch_status();
 }
 

@@ -49,8 +49,8 @@ class GPT2(nn.Module):
     def forward(self, idx: torch.Tensor, targets: Optional[torch.Tensor] = None, pack: Optional[ops.SequencePack] = None,
                 teacher: Optional[tuple] = None, temperature: float = 1.0) -> torch.Tensor:
         """``idx`` ``[B, S]``, or ``[rows]`` with ``pack`` (:func:`ops.pack_sequences`): documents one behind the other,
-        each with positions of its own from 0 and attending to itself alone.  ``targets`` of the shape of ``idx`` (packed:
-        tokens whose target lies outside the vocabulary, -100 at a document's end say, do not count), or ``teacher``:
+        each with positions of its own from 0 and attending to itself alone.  ``targets`` of the shape of ``idx`` (tokens
+        whose target lies outside the vocabulary, -100 at a document's end say, do not count), or ``teacher``:
         (logits, ids) of the shape of ``idx`` plus ``K``, see :func:`ops.distillation_loss`."""
         if targets is not None and teacher is not None:
             raise ValueError("targets or a teacher, not both")

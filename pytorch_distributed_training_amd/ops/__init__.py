@@ -113,6 +113,8 @@ def gelu_mlp(x, w1, b1, w2, b2, residual=None, link=None):
 
 
 def softmax_cross_entropy(logits, labels):
+    """Mean cross-entropy over the rows that have a label: -100 leaves its row out, without gradient and not counted (on GPU
+    every label that is none of the classes does; on CPU the others are an error).  0 where no row has one."""
     if logits.is_cuda:
         return _hip().softmax_cross_entropy(logits, labels)
     return _ref.softmax_cross_entropy(logits, labels)
@@ -120,11 +122,13 @@ def softmax_cross_entropy(logits, labels):
 
 def lm_head_loss(x, weight, labels):
     """Mean cross-entropy of the logits ``x W^T`` (no bias) against ``labels``: a language model's tied output
-    projection and loss.  On GPU the rows are processed in chunks through one scratch buffer, so the
+    projection and loss, over the rows whose label lies in the vocabulary (0 without any).  On GPU the rows are processed in chunks through one scratch buffer, so the
     ``[rows, vocabulary]`` logits of the whole batch never exist (see ``ops.hip._LMHeadLoss``)."""
     if x.is_cuda and 1024 < weight.shape[0] <= 65536 and _LM_HEAD_FUSED:
         return _hip().lm_head_loss(x, weight, labels)
     logits = linear(x, weight, None)
+    if not x.is_cuda:
+        labels = _ref.without_others(labels, weight.shape[0])
     return softmax_cross_entropy(logits.reshape(-1, logits.shape[-1]), labels.reshape(-1))
 
 

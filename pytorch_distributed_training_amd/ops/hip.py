@@ -62,11 +62,11 @@ _bn_relu_maxpool_fwd = _sig("pdt_bn_relu_maxpool_fwd", [_vp, _vp, _vp, _vp, _vp,
 _maxpool_bn_bwd_apply = _sig("pdt_maxpool_bn_bwd_apply", [_vp, _vp, _vp, _vp, _vp, _vp, _i, _i, _i, _i, _vp])
 _avgpool_fwd = _sig("pdt_avgpool_fwd", [_vp, _vp, _i, _i, _i, _vp])
 _avgpool_bwd = _sig("pdt_avgpool_bwd", [_vp, _vp, _i, _i, _i, _vp])
-_ce_fwd = _sig("pdt_softmax_ce_fwd", [_vp, _vp, _vp, _vp, _vp, _i, _i, _ll, _i, _vp])
-_ce_bwd = _sig("pdt_softmax_ce_bwd", [_vp, _vp, _vp, _vp, _vp, _i, _i, _ll, _ll, _i, _i, _vp])
-_ce_fused = _sig("pdt_softmax_ce_fused", [_vp, _vp, _vp, _vp, _vp, _i, _i, _ll, _ll, _i, _vp])
-_ce_fused_chunk = _sig("pdt_softmax_ce_fused_chunk", [_vp, _vp, _vp, _vp, _i, _i, _ll, _ll, _i, _ll, _vp])
-_mean_f32 = _sig("pdt_mean_f32", [_vp, _vp, _ll, _f, _vp])
+_ce_fwd = _sig("pdt_softmax_ce_fwd", [_vp] * 6 + [_i, _i, _ll, _i, _vp])
+_ce_bwd = _sig("pdt_softmax_ce_bwd", [_vp] * 6 + [_i, _i, _ll, _ll, _i, _i, _vp])
+_ce_fused = _sig("pdt_softmax_ce_fused", [_vp, _vp, _vp, _vp, _i, _i, _ll, _ll, _i, _vp, _vp])
+_label_count = _sig("pdt_label_count", [_vp, _ll, _i, _vp, _vp])
+_label_mean = _sig("pdt_label_mean", [_vp, _ll, _vp, _vp, _vp])
 _axpy_dev = _sig("pdt_axpy_dev_scalar_f32", [_vp, _vp, _vp, _ll, _vp])
 _scale_by_scalar = _sig("pdt_scale_by_scalar", [_vp, _vp, _ll, _vp])
 _nchw_to_nhwc = _sig("pdt_nchw_to_nhwc_bf16", [_vp, _vp, _i, _i, _i, _i, _i, _vp])
@@ -1610,6 +1610,7 @@ class _SoftmaxCE(torch.autograd.Function):
         dev = logits.device
         row_loss = torch.empty(rows, dtype=torch.float32, device=dev)
         loss = torch.empty(1, dtype=torch.float32, device=dev)
+        count = torch.empty(1, dtype=torch.float32, device=dev)  # rows whose label is one of the classes, at least 1
         ld = logits.stride(0)
         ctx.fused = None
         if logits.dtype == torch.bfloat16 and 1024 < classes <= 65536 and ld % 8 == 0 and ld >= _round_up(classes, 8):
@@ -1620,15 +1621,17 @@ class _SoftmaxCE(torch.autograd.Function):
             dbuf = None
             if ctx.needs_input_grad[0]:
                 dbuf = torch.empty((rows, pad_to), dtype=torch.bfloat16, device=dev)
-            _check(_ce_fused(logits.data_ptr(), labels.data_ptr(), row_loss.data_ptr(), loss.data_ptr(), _ptr(dbuf), rows,
-                             classes, ld, pad_to, pad_to, _stream()), "softmax_ce_fused")
+            _check(_label_count(labels.data_ptr(), rows, classes, count.data_ptr(), _stream()), "label_count")
+            _check(_ce_fused(logits.data_ptr(), labels.data_ptr(), row_loss.data_ptr(), _ptr(dbuf), rows, classes, ld, pad_to,
+                             pad_to, count.data_ptr(), _stream()), "softmax_ce_fused")
+            _check(_label_mean(row_loss.data_ptr(), rows, count.data_ptr(), loss.data_ptr(), _stream()), "label_mean")
             ctx.fused = [dbuf, classes, pad_to]
             return loss.reshape(())
         lse = torch.empty(rows, dtype=torch.float32, device=dev)
         dt = 1 if logits.dtype == torch.bfloat16 else 0
-        _check(_ce_fwd(logits.data_ptr(), labels.data_ptr(), row_loss.data_ptr(), lse.data_ptr(), loss.data_ptr(), rows,
-                       classes, logits.stride(0), dt, _stream()), "softmax_ce_fwd")
-        ctx.save_for_backward(logits, labels, lse)
+        _check(_ce_fwd(logits.data_ptr(), labels.data_ptr(), row_loss.data_ptr(), lse.data_ptr(), loss.data_ptr(), count.data_ptr(),
+                       rows, classes, logits.stride(0), dt, _stream()), "softmax_ce_fwd")
+        ctx.save_for_backward(logits, labels, lse, count)
         return loss.reshape(())
 
     @staticmethod
@@ -1641,14 +1644,14 @@ class _SoftmaxCE(torch.autograd.Function):
             g1 = g.reshape(1).to(torch.float32).contiguous()
             _check(_scale_by_scalar(dbuf.data_ptr(), g1.data_ptr(), dbuf.numel(), _stream()), "scale_by_scalar")
             return (zero_padded(dbuf)[:, :classes] if pad_to != classes else dbuf), None
-        logits, labels, lse = ctx.saved_tensors
+        logits, labels, lse, count = ctx.saved_tensors
         rows, classes = logits.shape
         ld = logits.stride(0)
         pad_to = ld if ld >= classes and ld - classes < 64 else classes
         dbuf = torch.empty((rows, pad_to), dtype=logits.dtype, device=logits.device)
         g1 = g.reshape(1).to(torch.float32).contiguous()
         dt = 1 if logits.dtype == torch.bfloat16 else 0
-        _check(_ce_bwd(logits.data_ptr(), labels.data_ptr(), lse.data_ptr(), g1.data_ptr(), dbuf.data_ptr(), rows, classes,
+        _check(_ce_bwd(logits.data_ptr(), labels.data_ptr(), lse.data_ptr(), g1.data_ptr(), count.data_ptr(), dbuf.data_ptr(), rows, classes,
                        ld, pad_to, pad_to, dt, _stream()), "softmax_ce_bwd")
         return (zero_padded(dbuf)[:, :classes] if pad_to != classes else dbuf), None
 
@@ -1662,7 +1665,8 @@ LM_HEAD_CHUNK_ROWS = int(_os.environ.get("PDT_LM_HEAD_CHUNK_ROWS", "32768"))
 
 class _LMHeadLoss(torch.autograd.Function):
     """mean cross-entropy of ``x W^T`` against ``labels`` - a language model's output projection and loss - without
-    ever holding the ``[rows, vocabulary]`` logits (or their gradient) of the whole batch.
+    ever holding the ``[rows, vocabulary]`` logits (or their gradient) of the whole batch; over the rows whose label lies
+    in the vocabulary.
 
     Rows are processed in chunks.  Per chunk: logits GEMM into a scratch buffer -> softmax-cross-entropy kernel that
     turns the buffer into the logits' gradient in place (each row sits in the registers of one workgroup) -> the
@@ -1702,20 +1706,22 @@ class _LMHeadLoss(torch.autograd.Function):
         dx = torch.empty((M, k), dtype=torch.bfloat16, device=dev) if want_dx else None
         dw = torch.zeros((n, k), dtype=torch.float32, device=dev) if want_dw else None
         wt = SHADOWS.dgrad(weight, 1)[0] if want_dx else None  # [k][npad]
+        count = torch.empty(1, dtype=torch.float32, device=dev)
+        _check(_label_count(labels.data_ptr(), M, n, count.data_ptr(), _stream()), "label_count")
         one = [(0, 0, 0)]
         for r0 in range(0, M, rows_c):
             rows = min(rows_c, M - r0)
             xc = x2[r0:r0 + rows]
             _launch_gather_gemm(xc, wb, scratch, None, None, rows, n, k, npad, k, one, 1, 1, 1, 1, 1, 1, 1, 1, 0, 0)
             grad_buf = scratch if (want_dx or want_dw) else None
-            _check(_ce_fused_chunk(scratch.data_ptr(), labels[r0:r0 + rows].data_ptr(), row_loss[r0:r0 + rows].data_ptr(),
-                                   _ptr(grad_buf), rows, n, npad, npad, npad, M, _stream()), "softmax_ce_fused_chunk")
+            _check(_ce_fused(scratch.data_ptr(), labels[r0:r0 + rows].data_ptr(), row_loss[r0:r0 + rows].data_ptr(), _ptr(grad_buf),
+                             rows, n, npad, npad, npad, count.data_ptr(), _stream()), "softmax_ce_fused")
             if want_dx:
                 _launch_gather_gemm(scratch, wt, dx[r0:r0 + rows], None, None, rows, k, npad, k, npad, one, 1, 1, 1, 1, 1, 1, 1, 1,
                                     0, 0)
             if want_dw:
                 _launch_wgrad(scratch, xc, dw, rows, n, npad, k, one, k, 1, 1, 1, 1, 1)
-        _check(_mean_f32(row_loss.data_ptr(), loss.data_ptr(), M, 1.0 / M, _stream()), "mean")
+        _check(_label_mean(row_loss.data_ptr(), M, count.data_ptr(), loss.data_ptr(), _stream()), "label_mean")
         ctx.grads = [dx, dw]
         ctx.weight = weight
         ctx.lead, ctx.k = lead, k

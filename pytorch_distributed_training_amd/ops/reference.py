@@ -72,17 +72,23 @@ def linear(x, weight, bias=None, activation: Optional[str] = None, residual=None
 
 
 def softmax_cross_entropy(logits: torch.Tensor, labels: torch.Tensor) -> torch.Tensor:
-    """Mean softmax cross-entropy over all rows (role of ``nn.CrossEntropyLoss()`` at
+    """Mean softmax cross-entropy over the rows with a label (not -100), 0 without any (role of ``nn.CrossEntropyLoss()`` at
     /root/reference/src/main.py:62,76)."""
-    return F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), labels.reshape(-1))
+    y = labels.reshape(-1)
+    return F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), y, reduction="mean" if bool((y != -100).any()) else "sum")
+
+
+def without_others(labels, vocab: int):
+    """Labels outside the vocabulary as -100."""
+    y = labels.reshape(-1).to(torch.int64)
+    return torch.where((y >= 0) & (y < vocab), y, torch.full_like(y, -100))
 
 
 def linear_cross_entropy(x, weight, labels):
     """Mean cross-entropy of ``x W^T`` over the rows whose label lies in the vocabulary; 0 without any."""
     up = torch.promote_types(x.dtype, torch.float32)
     z = F.linear(x.reshape(-1, x.shape[-1]).to(up), weight.to(up))
-    y = labels.reshape(-1).to(torch.int64)
-    y = torch.where((y >= 0) & (y < weight.shape[0]), y, torch.full_like(y, -100))
+    y = without_others(labels, weight.shape[0])
     return F.cross_entropy(z, y, ignore_index=-100, reduction="sum") / (y >= 0).sum().clamp(min=1)
 
 

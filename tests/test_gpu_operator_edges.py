@@ -141,3 +141,70 @@ def test_forward_mode_derivatives_are_refused(ops):
                     with pytest.raises((NotImplementedError, ValueError)):
                         call(*(forward_ad.make_dual(t, torch.ones_like(t)) if i == j else t for j, t in enumerate(inputs)))
                     assert torch.equal(call(*inputs), plain), name
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("classes", [10, 1000, 1032, 5003, 66000])
+@pytest.mark.parametrize("labelled", ["all", "some", "none"])
+def test_cross_entropy_over_the_rows_with_a_label(ops, dtype, classes, labelled):
+    n = 37
+    z = _bf16(n, classes, seed=classes, std=2.0).to(dtype).requires_grad_(True)
+    y = torch.randint(0, classes, (n,), generator=_gen(6), device="cuda")
+    if labelled != "all":
+        y[::3] = -100
+        y[1], y[2] = classes, -1
+    if labelled == "none":
+        y[:] = -100
+    loss = ops.softmax_cross_entropy(z, y)
+    (g,) = torch.autograd.grad(loss * 2, z)
+    has = (y >= 0) & (y < classes)
+    count = has.sum().clamp(min=1)
+    z64 = z.detach().double()
+    logp = torch.log_softmax(z64, 1)
+    each = -logp.gather(1, y.clamp(0, classes - 1)[:, None])[:, 0] * has
+    dz = logp.exp()
+    dz[torch.arange(n, device="cuda"), y.clamp(0, classes - 1)] -= 1.0
+    dz *= (2.0 * has / count)[:, None]
+    # exponentials and sums in 32 bits: 2e-5 of the loss's terms and of the probabilities (their exponents are below 2^6)
+    assert abs(float(loss) - float(each.sum() / count)) <= 2e-5 * (1 + float(each.sum() / count))
+    # four factors and differences in 32 bits; bf16: rounded once (the longer rows' gradient in the forward pass: doubling it is exact)
+    rounding = 4 * U + (H if dtype == torch.bfloat16 else 0)
+    assert bool(((g.double() - dz).abs() <= rounding * dz.abs() + 2e-5 * 2.0 * (logp.exp() / count) * has[:, None] + 1e-38).all())
+    assert bool((g[~has] == 0).all())
+
+
+@pytest.mark.parametrize("vocab", [1000, 1100, 66000])
+@pytest.mark.parametrize("packed", [False, True])
+def test_gpt2_targets_mean_the_same_at_every_vocabulary(ops, vocab, packed):
+    """Targets outside the vocabulary do not count, in a batch or packed, on either side of what the fused head takes; the
+    gradients agree with the fp32 model on the CPU in direction and size."""
+    import copy
+
+    from pytorch_distributed_training_amd.models.gpt2 import gpt2_tiny
+
+    torch.manual_seed(0)
+    ref = gpt2_tiny(vocab_size=vocab, n_ctx=32)
+    gpu = ops.prepare_module(copy.deepcopy(ref).cuda())
+    idx = torch.randint(0, vocab, (2, 32))
+    targets = torch.randint(0, vocab, (2, 32))
+    targets[0, 5:] = -100
+    targets[1, ::2] = -100
+    if packed:
+        idx, targets = idx.flatten(), targets.flatten()
+        a = ref(idx, targets, pack=ops.pack_sequences([0, 32, 64], 64))
+        b = gpu(idx.cuda(), targets.cuda(), pack=ops.pack_sequences([0, 32, 64], 64, device="cuda"))
+    else:
+        a, b = ref(idx, targets), gpu(idx.cuda(), targets.cuda())
+    a.backward(), b.backward()
+    # bf16 activations through two blocks: each rounds at 2^-8 of the value a dozen times, at random
+    assert abs(float(a) - float(b)) < 12 * H
+    for (name, p), r in zip(ref.named_parameters(), gpu.parameters()):
+        g, w = r.grad.cpu().double().flatten(), p.grad.double().flatten()
+        assert float((g - w).norm()) <= 12 * H * float(w.norm()) + 1e-9, (name, float((g - w).norm() / w.norm()))
+
+
+def test_fused_head_without_any_label(ops):
+    x, w = _bf16(8, 64).requires_grad_(True), torch.nn.Parameter(_bf16(2000, 64, seed=1).float())
+    loss = ops.lm_head_loss(x, w, torch.full((8,), -100, device="cuda"))
+    loss.backward()
+    assert float(loss) == 0.0 and bool((x.grad == 0).all()) and bool((w.grad == 0).all())
