@@ -10,7 +10,8 @@
 // holds a 256 x 256 tile of z in fp32 registers and leaves, per row and group of 64 vocabulary entries, the maximum and
 // the sum of 2^(z - maximum) in fp32 and (training) the exponentials themselves in bf16 - relative to their group's
 // maximum, so the rounding (2^-8 at most) is relative to the value however small the probability.  Once a row's groups
-// are joined, one pass turns the exponentials into q - p in place, and two more products give dx = (q - p) W and
+// are joined, one pass turns the exponentials into q - p in place (at the targets from their scores in fp32, see
+// vl_target_scores), and two more products give dx = (q - p) W and
 // dW = (q - p)^T x; the factor tau / rows is applied to their fp32 sums.
 #include "common.h"
 #include <type_traits>
@@ -596,6 +597,7 @@ struct Targets {
     const long long* ids;    // [rows][top]
     const float* teacher;    // [rows][top], or nullptr: one target of weight 1 (labels)
     float* p;                // [rows][top] weights, of repeated ids at their first entry; unused for labels
+    float* z;                // [rows][top] scores of the targets in units of log2, or nullptr (no gradient, or given logits)
     float* base;             // [rows]
     int* valid;              // [rows]
     const bf16 *x, *w;       // behind a projection: [rows][width], [vocab][width]; else nullptr
@@ -603,20 +605,41 @@ struct Targets {
                              // must not meet its zero gradient in the product that gives dW; rows rounded up to 64, zeros behind the last
     int rows, top, width;
     long long vocab;
-    float inv_tau;
+    float inv_tau, scale_log2;
 };
 
-// p . (x . W[id]) / tau of a row's targets, eight at a time (their rows of W are on their way together): this wave's share,
-// targets first, first + 8, ... of every `step`; lane's part of the sum.
+// sum of s[lane / 8] over the wave: every exchange halves the values a lane still has to do with
+__device__ __forceinline__ float vl_sums8(const float (&s)[8], int lane) {
+    float v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = s[i];
+#pragma unroll
+    for (int n = 4, bit = 32; n > 0; n >>= 1, bit >>= 1)
+#pragma unroll
+        for (int i = 0; i < n; ++i) {
+            const float keep = lane & bit ? v[i + n] : v[i], give = lane & bit ? v[i] : v[i + n];
+            v[i] = keep + __shfl_xor(give, bit, 64);
+        }
+    float r = v[0];
+#pragma unroll
+    for (int o = 4; o > 0; o >>= 1) r += __shfl_xor(r, o, 64);
+    return r;
+}
+
+// - p . (x . W[id]) / tau of a row's targets, eight at a time (their rows of W are on their way together): this wave's share,
+// targets first, first + 8, ... of every `step`; lane's part of the sum.  The scores themselves are kept for q - p at the
+// targets: a student close to its teacher leaves little of that difference, and q from a rounded exponential would be most of
+// its error (70 rows of 64 targets, teacher within 0.003 of the student: dx off by 17 % of it, from these scores by 0.24 %).
 template <typename P, typename I>
 __device__ __forceinline__ float vl_target_scores(const Targets& t, int row, int first, int step, int lane, P p_of, I id_of) {
     const bf16* x = t.x + static_cast<size_t>(row) * t.width;
     float base = 0.f;
     for (int k0 = first; k0 < t.top; k0 += step) {
         const bf16* w[8];
-        float pk[8];
+        float pk[8], s[8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
+            s[i] = 0.f;
             pk[i] = k0 + i < t.top ? p_of(k0 + i) : 0.f;
             w[i] = t.w + (pk[i] != 0.f ? id_of(k0 + i) : 0ll) * t.width;
         }
@@ -629,10 +652,17 @@ __device__ __forceinline__ float vl_target_scores(const Targets& t, int row, int
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if (pk[i] == 0.f) continue;  // (not multiplied by 0: what an absent target's row holds does not count)
-                float s = 0.f;
 #pragma unroll
-                for (int e = 0; e < 8; ++e) s = fmaf(bf16_to_f32(xv[e]), bf16_to_f32(wv[i][e]), s);
-                base -= pk[i] * s * t.inv_tau;
+                for (int e = 0; e < 8; ++e) s[i] = fmaf(bf16_to_f32(xv[e]), bf16_to_f32(wv[i][e]), s[i]);
+            }
+        }
+        const float sum = vl_sums8(s, lane);
+        if ((lane & 7) == 0) {
+            const int k = k0 + (lane >> 3);
+            const float p = k < t.top ? p_of(k) : 0.f;
+            if (p != 0.f) {
+                base -= p * sum * t.inv_tau;
+                if (t.z != nullptr) t.z[static_cast<size_t>(row) * t.top + k] = sum * t.scale_log2;
             }
         }
     }
@@ -765,6 +795,7 @@ struct Rows {
     long long lde;
     const long long* ids;
     const float* p;          // nullptr: labels
+    const float* z;          // scores of the targets
     const float* base;
     const int* valid;
     float* row_loss;
@@ -804,8 +835,7 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(const Rows a) {
     const long long* ids = a.ids + static_cast<size_t>(row) * a.top;
     const float p = tid < a.top ? (a.p == nullptr ? 1.f : a.p[static_cast<size_t>(row) * a.top + tid]) : 0.f;
     const int at = p != 0.f ? static_cast<int>(ids[tid]) : 0;
-    const float val = p != 0.f ? bf16_to_f32(e[at]) * vl_exp2(st[at >> 6].x - lse) - p : 0.f;
-    __syncthreads();  // the targets' exponentials are read
+    const float val = p != 0.f ? vl_exp2(a.z[static_cast<size_t>(row) * a.top + tid] - lse) - p : 0.f;
     for (long long c = tid * 8; c < a.lde; c += THREADS * 8) {
         const float f = vl_exp2(st[c >> 6].x - lse);
         bf16x8 v = __builtin_nontemporal_load(reinterpret_cast<const bf16x8*>(e + c));
@@ -813,7 +843,7 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(const Rows a) {
         for (int k = 0; k < 8; ++k) v[k] = f32_to_bf16(bf16_to_f32(v[k]) * f);
         vl_store(reinterpret_cast<bf16x8*>(e + c), v, a.stream);
     }
-    __syncthreads();  // ... and every one is rewritten
+    __syncthreads();  // every entry is rewritten
     if (p != 0.f) e[at] = f32_to_bf16(val);
 }
 
@@ -1025,9 +1055,9 @@ static bool vl_sizes_ok(int rows, int vocab, int width) {
            static_cast<long long>(pdt_cdiv(rows, 256)) * pdt_cdiv(width, 256) < (1ll << 30);
 }
 
-static int vl_targets(const long long* ids, const float* teacher, float* p, float* base, int* valid, float* scal, const void* x, const void* w,
+static int vl_targets(const long long* ids, const float* teacher, float* p, float* z, float* base, int* valid, float* scal, const void* x, const void* w,
                       void* x_used, int rows, int top, int width, int vocab, float tau, hipStream_t s) {
-    Targets t = {ids, teacher, p, base, valid, static_cast<const bf16*>(x), static_cast<const bf16*>(w), static_cast<bf16*>(x_used), rows, top, width, vocab, 1.f / tau};
+    Targets t = {ids, teacher, p, z, base, valid, static_cast<const bf16*>(x), static_cast<const bf16*>(w), static_cast<bf16*>(x_used), rows, top, width, vocab, 1.f / tau, VL_LOG2E / tau};
     const int all = x_used == nullptr ? rows : pdt_cdiv(rows, 64) * 64;
     const int lds = (top + 3) / 4 * 4 * 12;
     if (teacher != nullptr && (x != nullptr || top > 128)) hipLaunchKernelGGL(vocab_teacher_kernel<256>, dim3(all), dim3(256), lds, s, t);
@@ -1068,11 +1098,12 @@ struct HeadScratch {
     RowScratch r;
     float2* stats;
     bf16 *e, *x_used;
-    float* part;
+    float *z, *part;
     HeadScratch(Scratch& m, int rows, int top, int vocab, int width, int chunk, bool teacher, bool dx, bool dw) : r(m, rows, top, teacher) {
         const size_t groups = pdt_cdiv(vocab, 64);
         stats = m.take<float2>(chunk * groups);
         e = dx || dw ? m.take<bf16>(static_cast<size_t>(pdt_cdiv(chunk, 64)) * 64 * groups * 64) : nullptr;
+        z = dx || dw ? m.take<float>(static_cast<size_t>(rows) * top) : nullptr;
         x_used = dw ? m.take<bf16>(static_cast<size_t>(pdt_cdiv(rows, 64)) * 64 * width) : nullptr;
         size_t need = 0;
         for (int k = 0; k < 2; ++k) {  // a whole chunk, and the last one
@@ -1117,7 +1148,7 @@ PDT_API int pdt_head_loss(const void* x, const void* w, const long long* ids, co
     hipStream_t s = static_cast<hipStream_t>(stream);
     const long long pitch = (vocab + 63ll) / 64 * 64;
     const bool big = 2 * pitch * chunk >= VL_STREAM_BYTES;
-    if (int e = vl_targets(ids, teacher, h.r.p, h.r.base, h.r.valid, train ? h.r.scal : nullptr, x, w, h.x_used, rows, top, width, vocab, tau, s)) return e;
+    if (int e = vl_targets(ids, teacher, h.r.p, h.z, h.r.base, h.r.valid, train ? h.r.scal : nullptr, x, w, h.x_used, rows, top, width, vocab, tau, s)) return e;
     for (int r0 = 0; r0 < rows; r0 += chunk) {
         const int n = rows - r0 < chunk ? rows - r0 : chunk;
         VocabGemm g = {};
@@ -1134,7 +1165,7 @@ PDT_API int pdt_head_loss(const void* x, const void* w, const long long* ids, co
         vl_plan(g, false);
         if (int e = vl_launch<0>(g, s)) return e;
         Rows a = {h.stats, h.e, pitch, ids + static_cast<size_t>(r0) * top, h.r.p == nullptr ? nullptr : h.r.p + static_cast<size_t>(r0) * top,
-                  h.r.base + r0, h.r.valid + r0, h.r.row_loss + r0, g.groups, top, n, vocab, big};
+                  h.z == nullptr ? nullptr : h.z + static_cast<size_t>(r0) * top, h.r.base + r0, h.r.valid + r0, h.r.row_loss + r0, g.groups, top, n, vocab, big};
         hipLaunchKernelGGL(vocab_rows_kernel, dim3(train ? pdt_cdiv(n, 64) * 64 : n), dim3(1024), 0, s, a);
         g = {};
         g.lda = pitch; g.ldb = width;
@@ -1201,7 +1232,7 @@ PDT_API int pdt_distill(const void* z, void* dz, const long long* ids, const flo
     const float it = 1.f / tau, c = VL_LOG2E * it;
     // up to 1024 rows every workgroup counts the ones with a target itself: a launch less
     float* scal = rows > 1024 && dz != nullptr ? r.scal : nullptr;
-    if (int e = vl_targets(ids, teacher, r.p, r.base, r.valid, scal, nullptr, nullptr, nullptr, rows, top, 0, vocab, tau, s)) return e;
+    if (int e = vl_targets(ids, teacher, r.p, nullptr, r.base, r.valid, scal, nullptr, nullptr, nullptr, rows, top, 0, vocab, tau, s)) return e;
     const bool big = ldd * rows * (dtype == 1 ? 2 : 4) >= VL_STREAM_BYTES;
     const int e = dtype == 1 ? distill_launch(Logits<bf16>{static_cast<const bf16*>(z), static_cast<bf16*>(dz), ldz, ldd, ids, r.p, r.base, r.valid, scal, r.valid, r.row_loss, top, vocab, rows, tau, c, it, big}, rows, s)
                              : distill_launch(Logits<float>{static_cast<const float*>(z), static_cast<float*>(dz), ldz, ldd, ids, r.p, r.base, r.valid, scal, r.valid, r.row_loss, top, vocab, rows, tau, c, it, big}, rows, s);

@@ -208,3 +208,31 @@ def test_fused_head_without_any_label(ops):
     loss = ops.lm_head_loss(x, w, torch.full((8,), -100, device="cuda"))
     loss.backward()
     assert float(loss) == 0.0 and bool((x.grad == 0).all()) and bool((w.grad == 0).all())
+
+
+@pytest.mark.parametrize("near", [0.0, 0.003, 0.03])
+def test_students_close_to_their_teacher(ops, near):
+    """q - p at the targets is a small difference there: both are formed in 32 bits, and only the difference is rounded."""
+    n, vocab, width, top, tau = 70, 4000, 256, 64, 1.0
+    # small whole numbers and eighths: every score is exact in 32 bits; the highest share two groups of 64 entries, so that
+    # most of them are not the largest of their group
+    x = torch.randint(-3, 4, (n, width), generator=_gen(1), device="cuda").to(torch.bfloat16).requires_grad_(True)
+    w = torch.randint(-3, 4, (vocab, width), generator=_gen(2), device="cuda").to(torch.bfloat16) / 8
+    w[128:] /= 4
+    w.requires_grad_(True)
+    x64, w64 = x.detach().double(), w.detach().double()
+    z = x64 @ w64.t()
+    ids = z.topk(top, 1).indices
+    teacher = (z.gather(1, ids) + near * torch.randn(n, top, generator=_gen(3), device="cuda")).float()
+    loss = ops.linear_distillation_loss(x, w, teacher, ids, tau)
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    q, p = torch.softmax(z, 1), torch.softmax(teacher.double(), 1)
+    dz = q.scatter_add(1, ids, -p) / n
+    # q of entries that are no targets: an exponential and its multiple, each rounded; q - p at the targets: rounded once;
+    # exponents below 2^6 and sums in 32 bits: 2e-5 of q and p
+    others = q.scatter(1, ids, 0.0) / n
+    f = 2.01 * H * others + H * (dz - others).abs() + 2e-5 * (q / n).scatter_add(1, ids, p / n)
+    for got, want, bound in ((dx, dz @ w64, f @ w64.abs()), (dw, dz.t() @ x64, f.t() @ x64.abs())):
+        terms = dz.abs() @ w64.abs() if got is dx else dz.abs().t() @ x64.abs()
+        over = (got.double() - want).abs() - 1.05 * (bound + H * want.abs() + vocab * U * terms)
+        assert float(over.max()) <= 0, float(over.max())
