@@ -139,14 +139,18 @@ __device__ __forceinline__ void taken(RowFrags& f) { asm volatile("" : "+v"(f.v[
 __device__ __forceinline__ void taken(TrFrags& f) { asm volatile("" : "+v"(f.lo[0]), "+v"(f.lo[1]), "+v"(f.hi[0]), "+v"(f.hi[1])); }
 __device__ __forceinline__ void taken(f32x4 (&f)[4]) { asm volatile("" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3])); }
 
-// What rounding to bf16 took from an output, 2^-9 of it at most, in 8 bits (e5m2, times 256, saturating): an eighth of it is
-// all that is lost.  The bytes of a row lie as the dQ kernel's lanes read them: element d at half d / 8 % 2, 8 (d / 16) + d % 8.
+// What rounding to bf16 took from an output, half a step of it (2^-8 of the value) at most, in 8 bits (e5m2) relative to the output's own
+// exponent: with out = m 2^e, 0.5 <= |m| < 1, the rest is 2^(e - 9) at most, and times 2^(24 - e) that is 2^15, 29 octaves above
+// e5m2's smallest normal number.  So an eighth of the rest is all that is lost, whatever the size of the values.  The bytes of a row
+// lie as the dQ kernel's lanes read them: element d at half d / 8 % 2, 8 (d / 16) + d % 8.
 template <int NP>
 __device__ __forceinline__ int rest_place(int d) { return ((d >> 3) & 1) * (32 * NP) + ((d >> 4) << 3) + (d & 7); }
 __device__ __forceinline__ float rest_of(float x) {
-    const float r = (x - bf16_to_f32(f32_to_bf16(x))) * 256.f;
+    const float out = bf16_to_f32(f32_to_bf16(x));
+    const float r = __builtin_amdgcn_ldexpf(x - out, 24 - __builtin_amdgcn_frexp_expf(out));
     return __builtin_amdgcn_fmed3f(r, -57344.f, 57344.f);  // (NaN comes out as a number: its row is computed again)
 }
+__device__ __forceinline__ float rest_add(float out, float r) { return out + __builtin_amdgcn_ldexpf(r, __builtin_amdgcn_frexp_expf(out) - 24); }
 __device__ __forceinline__ uint32_t rest_pack(float a, float b, float c, float d) {
     const int lo = __builtin_amdgcn_cvt_pk_bf8_f32(a, b, 0, false);
     return static_cast<uint32_t>(__builtin_amdgcn_cvt_pk_bf8_f32(c, d, lo, true));
@@ -156,7 +160,7 @@ __device__ __forceinline__ float rest_dot(uint32_t rest, const bf16* g, const bf
     const f32x2 a = __builtin_amdgcn_cvt_pk_f32_bf8(static_cast<int>(rest), false), b = __builtin_amdgcn_cvt_pk_f32_bf8(static_cast<int>(rest), true);
     const float r[4] = {a[0], a[1], b[0], b[1]};
 #pragma unroll
-    for (int e = 0; e < 4; ++e) s = fmaf(bf16_to_f32(g[e]), fmaf(r[e], 1.f / 256.f, bf16_to_f32(o[e])), s);
+    for (int e = 0; e < 4; ++e) s = fmaf(bf16_to_f32(g[e]), rest_add(bf16_to_f32(o[e]), r[e]), s);
     return s;
 }
 
@@ -246,7 +250,7 @@ __device__ __forceinline__ void row_dq(const PackedArgs& p, int h, int row, int 
     for (int e = 0; e < NP; ++e) {
         const long long at = row * p.o_row + h * (64 * NP) + lane + 64 * e;
         const int rest = p.rest[row * p.o_row + h * (64 * NP) + rest_place<NP>(lane + 64 * e)];
-        dl += bf16_to_f32(g[lane + 64 * e]) * (bf16_to_f32(p.o[at]) + __builtin_amdgcn_cvt_f32_bf8(rest, 0) * (1.f / 256.f));
+        dl += bf16_to_f32(g[lane + 64 * e]) * rest_add(bf16_to_f32(p.o[at]), __builtin_amdgcn_cvt_f32_bf8(rest, 0));
         dq[e] = 0.f;
     }
     dl = wave_sum(dl);

@@ -236,3 +236,53 @@ def test_students_close_to_their_teacher(ops, near):
         terms = dz.abs() @ w64.abs() if got is dx else dz.abs().t() @ x64.abs()
         over = (got.double() - want).abs() - 1.05 * (bound + H * want.abs() + vocab * U * terms)
         assert float(over.max()) <= 0, float(over.max())
+
+
+def _uniform(n_rows, keys, hk, d, seed, value_scale):
+    """Documents of `keys` rows (a power of two) whose keys all get the same weight, exactly; their values share a large part,
+    so that dS = P (dout.v - dout.out) is a small difference; dout has the sign of what rounding takes from out."""
+    base = torch.rand(n_rows // keys, 1, hk, d, generator=_gen(seed), device="cuda") + 1.5
+    near = torch.randn(n_rows // keys, keys, hk, d, generator=_gen(seed + 1), device="cuda") * 0.02
+    v = ((base + near) * value_scale).to(torch.bfloat16).reshape(n_rows, hk, d)
+    out = v.double().reshape(-1, keys, hk, d).mean(1, keepdim=True).expand(-1, keys, hk, d).reshape(n_rows, hk, d)
+    taken = out - out.to(torch.bfloat16).double()
+    return v, out, taken, torch.where(taken >= 0, 1.0, -1.0).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("keys", [2, 8, 32])
+@pytest.mark.parametrize("value_scale", [2.0 ** -30, 2.0 ** -14, 1.0, 2.0 ** 20])
+@pytest.mark.parametrize("beside_nan", [False, True])
+def test_row_terms_from_unrounded_outputs(ops, d, keys, value_scale, beside_nan):
+    """The backward pass knows out to an eighth of what its rounding took, whatever the size of the values; rows that share
+    tiles with NaN (done one by one) know it too."""
+    rows, heads = 256, 2
+    v, out, taken, dout = _uniform(rows, keys, heads, d, keys, value_scale)
+    other = _bf16(rows, heads, d, seed=9)
+    zero = torch.zeros_like(other)
+    clean = torch.ones(rows, dtype=torch.bool, device="cuda")
+    if beside_nan:
+        v = v.clone()
+        for first in range(0, rows, 64):
+            v[first:first + keys] = math.nan
+            clean[first:first + keys] = False
+    pack = ops.pack_sequences(list(range(0, rows + 1, keys)), rows, device="cuda")
+    scale = d ** -0.5
+    v64, g64, o64 = torch.nan_to_num(v.double()), dout.double(), other.double()
+    by = lambda x: x.reshape(rows // keys, keys, heads, d).transpose(1, 2)  # [documents, heads, keys, d]
+    back = lambda x: x.transpose(1, 2).reshape(rows, heads, d)
+    p = 1.0 / keys
+    dp = by(g64) @ by(v64).transpose(2, 3)
+    ds = p * (dp - (by(g64) * by(out)).sum(-1, keepdim=True))
+    # dS rounded once; the row term off by an eighth of what rounding took; sums of d products in 32 bits
+    term = (by(g64).abs() * by(taken).abs()).sum(-1, keepdim=True) / 8 + (d + 16) * U * (by(g64).abs() * by(out).abs()).sum(-1, keepdim=True)
+    f = H * ds.abs() + p * (term + (d + 16) * U * (by(g64).abs() @ by(v64).abs().transpose(2, 3)))
+    for q, k, index in ((zero, other, 0), (other, zero, 1)):  # scores of 0 either way: weights of 1 / keys
+        q, k = q.clone().requires_grad_(True), k.clone().requires_grad_(True)
+        res = ops.attention_packed(q, k, v, pack, causal=False)
+        assert torch.equal(res.detach()[clean], out[clean].to(torch.bfloat16))
+        got = torch.autograd.grad(res, (q, k), dout)[index]
+        side, ff = (ds, f) if index == 0 else (ds.transpose(2, 3), f.transpose(2, 3))
+        want, bound = back(scale * side @ by(o64)), back(scale * ff @ by(o64).abs())
+        over = ((got.double() - want).abs() - 1.05 * (bound + H * want.abs() + 1e-37))[clean]
+        assert float(over.max()) <= 0, float((over / bound[clean]).max())
