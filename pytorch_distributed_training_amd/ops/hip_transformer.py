@@ -13,7 +13,7 @@ from typing import Optional
 
 import torch
 
-from .hip import _check, _colsum, _grad_sink, _lib, _on, _ptr, _stream
+from .hip import _check, _colsum, _grad_sink, _lib, _on, _once_differentiable, _ptr, _stream
 
 _vp, _i, _f, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
 
@@ -299,6 +299,7 @@ class _PackedEmbedding(torch.autograd.Function):
         return out
 
     @staticmethod
+    @_once_differentiable
     def backward(ctx, g):
         grads = []
         g2 = _bf16c(g)

@@ -286,3 +286,14 @@ def test_row_terms_from_unrounded_outputs(ops, d, keys, value_scale, beside_nan)
         want, bound = back(scale * side @ by(o64)), back(scale * ff @ by(o64).abs())
         over = ((got.double() - want).abs() - 1.05 * (bound + H * want.abs() + 1e-37))[clean]
         assert float(over.max()) <= 0, float((over / bound[clean]).max())
+
+
+def test_second_derivative_of_the_packed_embedding_is_refused(ops):
+    wte, wpe = (torch.randn(10, 64, device="cuda", requires_grad=True) for _ in range(2))
+    g = torch.ones(6, 64, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    pack = ops.pack_sequences([0, 6], 6, device="cuda")
+    out = ops.token_position_embedding(torch.arange(6, device="cuda"), wte, wpe, pack)
+    for table in (wte, wpe):
+        (d,) = torch.autograd.grad(out, table, g, create_graph=True, retain_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            (d * d).sum().backward()
