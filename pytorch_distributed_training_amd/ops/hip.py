@@ -109,13 +109,23 @@ def _stream() -> int:
     return torch.cuda.current_stream().cuda_stream
 
 
+_with_graph = _threading.local()  # .on: this thread is in a backward pass whose own graph is recorded
+
+
 def _once_differentiable(backward):
     """``torch.autograd.function.once_differentiable``, whose context costs 4 us of host time: entered only where a graph of the
-    backward pass is recorded (elsewhere gradients are off already)."""
+    backward pass is recorded (elsewhere gradients are off already).  There every gradient goes back to autograd (see
+    :func:`_grad_sink`) and refuses its derivative, also where the incoming gradient is a constant: by the inputs it has one."""
     guarded = torch.autograd.function.once_differentiable(backward)
 
     def run(ctx, *grads):
-        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+        if not torch.is_grad_enabled():
+            return backward(ctx, *grads)
+        _with_graph.on = True
+        try:
+            return guarded(ctx, *(g if g.requires_grad else g.detach().requires_grad_() for g in grads))
+        finally:
+            _with_graph.on = False
 
     return run
 
@@ -254,7 +264,9 @@ def _grad_sink(param: torch.Tensor, phys_shape) -> Optional[torch.Tensor]:
     gradient reducers are notified exactly as for ordinary gradients.
     """
     g = param.grad
-    if g is None or g.dtype != torch.float32 or not getattr(param, "_pdt_sink_ok", False) or torch.is_grad_enabled():
+    if g is None or g.dtype != torch.float32 or not getattr(param, "_pdt_sink_ok", False):
+        return None
+    if torch.is_grad_enabled() or getattr(_with_graph, "on", False):
         return None
     if g.shape != param.shape or g.stride() != param.stride():
         return None

@@ -297,3 +297,31 @@ def test_second_derivative_of_the_packed_embedding_is_refused(ops):
         (d,) = torch.autograd.grad(out, table, g, create_graph=True, retain_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             (d * d).sum().backward()
+
+
+def test_gradients_with_a_graph_are_not_added_on_the_quiet(ops):
+    """Under create_graph a parameter whose .grad the kernels may add into gets a gradient that refuses its own derivative."""
+    x, ids = _bf16(6, 64).requires_grad_(True), torch.arange(6, device="cuda")
+    pack = ops.pack_sequences([0, 6], 6, device="cuda")
+    for call in (lambda w: ops.linear_cross_entropy(x, w, ids), lambda w: ops.token_position_embedding(ids, w, w, pack).float().pow(2).sum()):
+        plain = torch.nn.Parameter(_bf16(70, 64, seed=1).float())
+        call(plain).backward()
+        w = torch.nn.Parameter(plain.detach().clone())
+        w.grad, w._pdt_sink_ok = torch.zeros_like(w), True
+        call(w).backward(create_graph=True)
+        assert torch.equal(w.grad.detach(), plain.grad)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            w.grad.pow(2).sum().backward()
+
+
+def test_derivatives_of_gradients_by_the_inputs_are_refused(ops):
+    """Also where the incoming gradient is a constant (a gradient penalty on a loss)."""
+    ids, pack = torch.arange(12, device="cuda").view(6, 2), ops.pack_sequences([0, 6], 6, device="cuda")
+    x, z, q = (_bf16(*s, seed=i).requires_grad_(True) for i, s in enumerate([(6, 64), (6, 70), (6, 1, 64)]))
+    w, do = _bf16(70, 64, seed=4), _bf16(6, 1, 64, seed=5)
+    calls = [(x, ops.linear_cross_entropy(x, w, ids[:, 0]), None), (z, ops.distillation_loss(z, torch.zeros(6, 2, device="cuda"), ids), None),
+             (q, ops.attention_packed(q, do, do, pack), do), (q, ops.attention_packed_qkv(torch.cat([q, do, do], 1).flatten(1), pack, 1), do.flatten(1))]
+    for leaf, out, g in calls:
+        (d,) = torch.autograd.grad(out, leaf, g, create_graph=True)
+        with pytest.raises(RuntimeError, match="once_differentiable"):
+            (leaf.float().sum() + d.float().pow(2).sum()).backward()
