@@ -22,7 +22,7 @@ typedef const __attribute__((address_space(1))) void vl_global_cvoid;
 #define VL_INF __builtin_inff()
 #define VL_GROUP 64   // vocabulary entries that share a maximum
 #define VL_MAX_TOP 1024
-#define VL_MAX_ROWS (1 << 22)  // a workgroup of up to 1024 threads a row, 2^32 threads a launch
+#define VL_MAX_ROWS ((1 << 22) - 63)  // rows stay below: rounded up to 64, with up to 1024 threads each, a launch has fewer than 2^32
 
 // A buffer far larger than the caches is written around them: 8192 x 50257 bf16, loss and gradients 2346 -> 2266 us, distillation
 // on logits 393 -> 377 us, 2048 rows 544 -> 537 us.  One that the caches hold is read again from them: 512 rows 188 us, written

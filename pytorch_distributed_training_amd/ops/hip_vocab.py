@@ -24,7 +24,7 @@ _distill = _sig("pdt_distill", [_vp] * 6 + [_ll] + [_i] * 3 + [_ll, _ll, _f, _i,
 # Rows worked off at a time: their exponentials (2 bytes per row and vocabulary entry) are the one large buffer.  8192 rows
 # of 130 001 entries, width 2048: 10.6 ms in one piece (2.1 GB), 11.6 in pieces of 1 GB, 14.1 in pieces of 256 MB.
 CHUNK_BYTES = int(os.environ.get("PDT_VOCAB_CHUNK_MB", "8192")) << 20
-MAX_ROWS = 1 << 22  # rows of a call stay below (a workgroup of up to 1024 threads each, 2^32 threads in a launch)
+MAX_ROWS = (1 << 22) - 63  # rows of a call stay below (rounded up to 64, with up to 1024 threads each: fewer than 2^32 in a launch)
 
 
 def _check_rows(n: int) -> None:

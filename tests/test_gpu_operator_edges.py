@@ -325,3 +325,25 @@ def test_derivatives_of_gradients_by_the_inputs_are_refused(ops):
         (d,) = torch.autograd.grad(out, leaf, g, create_graph=True)
         with pytest.raises(RuntimeError, match="once_differentiable"):
             (leaf.float().sum() + d.float().pow(2).sum()).backward()
+
+
+def test_as_many_rows_as_there_may_be(ops):
+    """2^22 - 64 equal rows: the loss is a row's, the gradients are the row's share of them."""
+    n, vocab = (1 << 22) - 64, 50
+    row, w = _bf16(1, 64), (_bf16(vocab, 64, seed=1) / 8).requires_grad_(True)
+    x = row.repeat(n, 1).requires_grad_(True)
+    loss = ops.linear_cross_entropy(x, w, torch.full((n,), 7, device="cuda", dtype=torch.int32))
+    dx, dw = torch.autograd.grad(loss, (x, w))
+    r, w64 = row.double(), w.detach().double()
+    q = torch.softmax(r @ w64.t(), 1)
+    want = -torch.log(q[0, 7])
+    d = q.clone()
+    d[0, 7] -= 1
+    # sums over the rows: a term is off by n 2^-24 of the sum at most where it is added one by one; 256 workgroups and 16 terms
+    # a product and more share them: 1024 + 256
+    sums = (n / 256 / 16 + 256) * U
+    assert abs(float(loss) - float(want)) <= (1e-5 + 4096 * U) * float(want)  # (a thread adds 4096 row losses)
+    f = 2 * H * q + H * d.abs() + 2e-5 * q
+    assert torch.equal(dx[0], dx[-1]) and torch.equal(dx[0], dx[n // 2 + 1])
+    assert bool(((dx[:1].double() * n - d @ w64).abs() <= 1.05 * (f @ w64.abs() + H * (d @ w64).abs())).all())
+    assert bool(((dw.double() - d.t() @ r).abs() <= 1.05 * (f.t() @ r.abs() + (H + sums) * (d.t() @ r).abs())).all())

@@ -59,3 +59,15 @@ def test_cross_entropy_over_the_rows_with_a_label(labels):
     else:
         with pytest.raises(IndexError):
             ops.softmax_cross_entropy(z, y)
+
+
+def test_rows_of_a_launch():
+    """Rows are rounded up to 64 in the passes over them, with 1024 threads each: 2^22 - 64 rows are the last that stay below 2^32 threads."""
+    from pytorch_distributed_training_amd.ops import hip_vocab
+
+    assert hip_vocab.MAX_ROWS == (1 << 22) - 63  # the first that is refused
+    for rows, taken in (((1 << 22) - 64, True), ((1 << 22) - 63, False), ((1 << 22) - 1, False), (1 << 22, False)):
+        assert (hip_vocab._head_scratch(rows, 1, 50, 64, rows, 0, 1, 1) > 0) == taken
+        assert (hip_vocab._distill_scratch(rows, 1) > 0) == taken
+    with pytest.raises(ValueError, match="rows at a time"):
+        hip_vocab._check_rows((1 << 22) - 63)
