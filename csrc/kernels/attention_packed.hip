@@ -1273,6 +1273,8 @@ static int ap_args(PackedArgs& a, const void* spans, const void* order, int T, i
     a.scale_log2 = scale * 1.4426950408889634f;
     a.unscale = 1.f / a.scale_log2;
     if (static_cast<long long>(a.nblk) * H >= (1ll << 31) || T >= (1 << 30)) return -1;
+    // (out's rows, [H, D] without gaps: as the other strides, see ap_stride_ok.  Inputs whose rows overlap may have shorter ones.)
+    if (static_cast<long long>(H) * D >= (1 << 24)) return -1;
     return 0;
 }
 

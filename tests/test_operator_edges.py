@@ -71,3 +71,17 @@ def test_rows_of_a_launch():
         assert (hip_vocab._distill_scratch(rows, 1) > 0) == taken
     with pytest.raises(ValueError, match="rows at a time"):
         hip_vocab._check_rows((1 << 22) - 63)
+
+
+def test_rows_of_all_heads_fit_the_tiles_offsets():
+    """Inputs whose rows overlap can have more heads than a row's stride: out and its gradient are [T, H, D] without gaps, and the
+    offsets of 64 of their rows are 32 bits."""
+    import ctypes
+
+    from pytorch_distributed_training_amd.ops import hip_packed
+
+    strides = (ctypes.c_longlong * 12)(*([8] * 12))
+    heads = (1 << 24) // 64
+    one = 1 << 20  # (an address that is never read: the call is refused)
+    assert hip_packed._fwd(one, one, one, one, one, one, one, one, strides, 2, heads, 1, 64, 0.1, 1, None) == -1
+    assert hip_packed._bwd(*[one] * 12, 1, one, one, strides, 2, heads, 1, 64, 0.1, 1, None) == -1
