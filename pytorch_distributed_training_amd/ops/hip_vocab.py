@@ -81,23 +81,31 @@ def _scale(g, *grads) -> None:
     _check(_scale_gradients(*args, g.data_ptr(), _stream()), "scale_gradients")
 
 
+def _check_capture(ctx) -> None:
+    """A graph of the backward pass alone would scale the forward pass's buffers again at every replay."""
+    if not ctx.captured and torch.cuda.is_current_stream_capturing():
+        raise RuntimeError("the backward pass of a vocabulary loss is captured without its forward pass; capture both, in one graph or one each")
+
+
 class _HeadLoss(torch.autograd.Function):
     """Loss of ``x W^T`` against a few targets per row.  The rows are worked off in chunks; the forward pass leaves ``dx``
-    and ``dW`` for an incoming gradient of 1, the backward pass multiplies them by the incoming one (a device scalar)."""
+    and ``dW`` for an incoming gradient of 1, the backward pass multiplies them by the incoming one (a device scalar; where it
+    is neither 1 nor another power of two, gradients in bf16 are rounded a second time)."""
 
     @staticmethod
     def forward(ctx, x, weight, ids, teacher, tau: float):
         loss, *ctx.grads = _head_forward(x, weight, ids, teacher, tau, *ctx.needs_input_grad[:2])
-        ctx.weight, ctx.shape = weight, x.shape
+        ctx.weight, ctx.shape, ctx.captured = weight, x.shape, torch.cuda.is_current_stream_capturing()
         return loss
 
     @staticmethod
     @_once_differentiable
     def backward(ctx, g):
         dx, dw = ctx.grads
-        ctx.grads = [None, None]
         if dx is None and dw is None:
             raise RuntimeError("the loss behind a projection handed its gradients out already (backward ran twice)")
+        _check_capture(ctx)
+        ctx.grads = [None, None]
         weight = ctx.weight
         with _on(g.device):
             g1 = g if g.dtype == torch.float32 else g.to(torch.float32)
@@ -144,15 +152,17 @@ class _LogitsDistill(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, ids, teacher, tau: float):
         loss, ctx.dz = _distill_forward(logits, ids, teacher, tau, True)
-        ctx.shape = logits.shape
+        ctx.shape, ctx.captured = logits.shape, torch.cuda.is_current_stream_capturing()
         return loss
 
     @staticmethod
     @_once_differentiable
     def backward(ctx, g):
-        dz, ctx.dz = ctx.dz, None
+        dz = ctx.dz
         if dz is None:
             raise RuntimeError("the distillation loss handed its gradient out already (backward ran twice)")
+        _check_capture(ctx)
+        ctx.dz = None
         with _on(g.device):
             g1 = g if g.dtype == torch.float32 else g.to(torch.float32)
             _scale(g1, dz)

@@ -347,3 +347,50 @@ def test_as_many_rows_as_there_may_be(ops):
     assert torch.equal(dx[0], dx[-1]) and torch.equal(dx[0], dx[n // 2 + 1])
     assert bool(((dx[:1].double() * n - d @ w64).abs() <= 1.05 * (f @ w64.abs() + H * (d @ w64).abs())).all())
     assert bool(((dw.double() - d.t() @ r).abs() <= 1.05 * (f.t() @ r.abs() + (H + sums) * (d.t() @ r).abs())).all())
+
+
+def test_backward_pass_alone_is_not_captured(ops, monkeypatch):
+    """The losses' gradients lie in the forward pass's buffers and are scaled in place: a graph that holds the backward pass without
+    the forward pass would scale them again at every replay, so it is refused (the stream is only said to be captured here)."""
+    x, w, z = _bf16(6, 64).requires_grad_(True), _bf16(70, 64, seed=1), _bf16(6, 70, seed=2).requires_grad_(True)
+    ids, teacher = torch.arange(12, device="cuda").view(6, 2), torch.zeros(6, 2, device="cuda")
+    for leaf, loss in ((x, ops.linear_cross_entropy(x, w, ids[:, 0])), (z, ops.distillation_loss(z, teacher, ids))):
+        with monkeypatch.context() as m:
+            m.setattr(torch.cuda, "is_current_stream_capturing", lambda: True)
+            with pytest.raises(RuntimeError, match="captured"):
+                torch.autograd.grad(loss, leaf, retain_graph=True)
+        (g,) = torch.autograd.grad(loss, leaf)  # nothing was taken
+        assert bool(torch.isfinite(g).all())
+
+
+def test_forward_and_backward_in_a_graph_each(ops):
+    """As torch's own graphed callables record them: the forward pass's graph, then the backward pass's, replayed in turn with eager work
+    between; every round's gradients are those of its inputs and its factor."""
+    x, w = _bf16(40, 64).requires_grad_(True), _bf16(70, 64, seed=1).requires_grad_(True)
+    z, t = _bf16(40, 70, seed=2).requires_grad_(True), torch.randn(40, 2, generator=_gen(3), device="cuda")
+    ids = torch.randint(0, 70, (40, 2), generator=_gen(4), device="cuda")
+    factor = torch.tensor(3.0, device="cuda")
+    for call, leaves in ((lambda: ops.linear_cross_entropy(x, w, ids[:, 0]), (x, w)), (lambda: ops.distillation_loss(z, t, ids), (z,))):
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            torch.autograd.grad(call(), leaves, factor)
+        torch.cuda.current_stream().wait_stream(side)
+        first, second = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+        with torch.cuda.graph(first):
+            loss = call()
+        with torch.cuda.graph(second, pool=first.pool()):
+            got = torch.autograd.grad(loss, leaves, factor)
+        for n in range(3):
+            with torch.no_grad():
+                for leaf in leaves:
+                    leaf.normal_(generator=_gen(10 + n))
+                factor.fill_(2.0 + n)
+            first.replay()
+            second.replay()
+            torch.cuda.synchronize()
+            kept = [loss.detach().clone()] + [g.clone() for g in got]
+            again = call()
+            want = [again.detach(), *torch.autograd.grad(again, leaves, factor)]
+            assert all(torch.equal(a, b) for a, b in zip(kept, want))
+            del again
