@@ -21,7 +21,8 @@ _distill_scratch = _sig("pdt_distill_scratch", [_i] * 2)
 _distill_scratch.restype = _ll
 _distill = _sig("pdt_distill", [_vp] * 6 + [_ll] + [_i] * 3 + [_ll, _ll, _f, _i, _vp])
 
-# Rows worked off at a time: their exponentials (2 bytes per row and vocabulary entry) are the one large buffer.  8192 rows
+# Rows worked off at a time: their exponentials (2 bytes per row and vocabulary entry; the size of the logits in bf16) are the one
+# large buffer, without a gradient the groups' statistics (8 bytes per row and 64 entries).  8192 rows
 # of 130 001 entries, width 2048: 10.6 ms in one piece (2.1 GB), 11.6 in pieces of 1 GB, 14.1 in pieces of 256 MB.
 CHUNK_BYTES = int(os.environ.get("PDT_VOCAB_CHUNK_MB", "8192")) << 20
 MAX_ROWS = (1 << 22) - 63  # rows of a call stay below (rounded up to 64, with up to 1024 threads each: fewer than 2^32 in a launch)
@@ -56,7 +57,8 @@ def _head_forward(x, weight, ids, teacher, tau: float, want_dx: bool, want_dw: b
         x2, w = _matrix(x, width), _weight(weight)
         n, top = ids.shape
         _check_rows(n)
-        chunk = n if not (want_dx or want_dw) else min(n, CHUNK_BYTES // (2 * _round_up(vocab, 64)))
+        groups = -(-vocab // 64)
+        chunk = min(n, CHUNK_BYTES // (groups * (128 if want_dx or want_dw else 8)))
         if chunk < n:
             chunk = min(n, max(256, chunk - chunk % 256))
         # one chunk and a bf16 weight: the gradient is rounded once, in the product's epilogue; else it is summed in fp32

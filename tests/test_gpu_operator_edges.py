@@ -394,3 +394,28 @@ def test_forward_and_backward_in_a_graph_each(ops):
             want = [again.detach(), *torch.autograd.grad(again, leaves, factor)]
             assert all(torch.equal(a, b) for a, b in zip(kept, want))
             del again
+
+
+def test_losses_without_a_gradient_in_pieces(ops, monkeypatch):
+    """Rows are worked off in pieces without a gradient too: the row statistics (8 bytes per 64 entries) of one piece at a time."""
+    from pytorch_distributed_training_amd.ops import hip_vocab
+
+    n, vocab, width = 2000, 50257, 64
+    x, w = _bf16(n, width), _bf16(vocab, width, seed=1)
+    y = torch.randint(0, vocab, (n,), generator=_gen(2), device="cuda")
+    teacher, ids = torch.randn(n, 3, generator=_gen(3), device="cuda"), torch.randint(0, vocab, (n, 3), generator=_gen(4), device="cuda")
+    groups = (vocab + 63) // 64
+
+    def peak(call):
+        torch.cuda.synchronize()
+        torch.cuda.reset_peak_memory_stats()
+        before = torch.cuda.memory_allocated()
+        return call(), torch.cuda.max_memory_allocated() - before
+
+    for call in (lambda: ops.linear_cross_entropy(x, w, y), lambda: ops.linear_distillation_loss(x, w, teacher, ids, 2.0)):
+        whole, much = peak(call)
+        with monkeypatch.context() as m:
+            m.setattr(hip_vocab, "CHUNK_BYTES", 300 * 8 * groups)
+            pieces, little = peak(call)
+        assert torch.equal(whole, pieces)
+        assert much >= n * 8 * groups and little < 256 * 8 * groups + (1 << 20)
