@@ -597,7 +597,7 @@ struct Targets {
     const long long* ids;    // [rows][top]
     const float* teacher;    // [rows][top], or nullptr: one target of weight 1 (labels)
     float* p;                // [rows][top] weights, of repeated ids at their first entry; unused for labels
-    float* z;                // [rows][top] scores of the targets in units of log2, or nullptr (no gradient, or given logits)
+    float* z;                // [rows][top] scores of the targets, or nullptr (no gradient, or given logits)
     float* base;             // [rows]
     int* valid;              // [rows]
     const bf16 *x, *w;       // behind a projection: [rows][width], [vocab][width]; else nullptr
@@ -605,7 +605,7 @@ struct Targets {
                              // must not meet its zero gradient in the product that gives dW; rows rounded up to 64, zeros behind the last
     int rows, top, width;
     long long vocab;
-    float inv_tau, scale_log2;
+    float inv_tau;
 };
 
 // sum of s[lane / 8] over the wave: every exchange halves the values a lane still has to do with
@@ -662,7 +662,7 @@ __device__ __forceinline__ float vl_target_scores(const Targets& t, int row, int
             const float p = k < t.top ? p_of(k) : 0.f;
             if (p != 0.f) {
                 base -= p * sum * t.inv_tau;
-                if (t.z != nullptr) t.z[static_cast<size_t>(row) * t.top + k] = sum * t.scale_log2;
+                if (t.z != nullptr) t.z[static_cast<size_t>(row) * t.top + k] = sum;
             }
         }
     }
@@ -802,6 +802,7 @@ struct Rows {
     int groups, top, rows;
     long long vocab;
     bool stream;
+    float scale_log2;
 };
 
 static_assert(VL_MAX_TOP <= 1024, "a thread per target");
@@ -823,9 +824,10 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(const Rows a) {
     float s = 0.f;
     for (int g = tid; g < a.groups; g += THREADS) s += st[g].y * vl_exp2(st[g].x - ref);
     s = block_sum(s, red);
-    const float lse = ref + log2f(s);
+    // (probabilities from differences to the maximum: rounding ref + ls would show in them where exponents are large, at low temperatures)
+    const float ls = log2f(s);
     const bool valid = a.valid[row] != 0;
-    if (tid == 0) a.row_loss[row] = valid ? a.base[row] + lse * VL_LN2 : 0.f;
+    if (tid == 0) a.row_loss[row] = valid ? a.base[row] + (ref + ls) * VL_LN2 : 0.f;
     if (a.e == nullptr) return;
     bf16* e = a.e + row * a.lde;
     if (!valid) {
@@ -835,9 +837,9 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(const Rows a) {
     const long long* ids = a.ids + static_cast<size_t>(row) * a.top;
     const float p = tid < a.top ? (a.p == nullptr ? 1.f : a.p[static_cast<size_t>(row) * a.top + tid]) : 0.f;
     const int at = p != 0.f ? static_cast<int>(ids[tid]) : 0;
-    const float val = p != 0.f ? vl_exp2(a.z[static_cast<size_t>(row) * a.top + tid] - lse) - p : 0.f;
+    const float val = p != 0.f ? vl_exp2(fmaf(a.z[static_cast<size_t>(row) * a.top + tid], a.scale_log2, -ref) - ls) - p : 0.f;
     for (long long c = tid * 8; c < a.lde; c += THREADS * 8) {
-        const float f = vl_exp2(st[c >> 6].x - lse);
+        const float f = vl_exp2(st[c >> 6].x - ref - ls);
         bf16x8 v = __builtin_nontemporal_load(reinterpret_cast<const bf16x8*>(e + c));
 #pragma unroll
         for (int k = 0; k < 8; ++k) v[k] = f32_to_bf16(bf16_to_f32(v[k]) * f);
@@ -1057,7 +1059,7 @@ static bool vl_sizes_ok(int rows, int vocab, int width) {
 
 static int vl_targets(const long long* ids, const float* teacher, float* p, float* z, float* base, int* valid, float* scal, const void* x, const void* w,
                       void* x_used, int rows, int top, int width, int vocab, float tau, hipStream_t s) {
-    Targets t = {ids, teacher, p, z, base, valid, static_cast<const bf16*>(x), static_cast<const bf16*>(w), static_cast<bf16*>(x_used), rows, top, width, vocab, 1.f / tau, VL_LOG2E / tau};
+    Targets t = {ids, teacher, p, z, base, valid, static_cast<const bf16*>(x), static_cast<const bf16*>(w), static_cast<bf16*>(x_used), rows, top, width, vocab, 1.f / tau};
     const int all = x_used == nullptr ? rows : pdt_cdiv(rows, 64) * 64;
     const int lds = (top + 3) / 4 * 4 * 12;
     if (teacher != nullptr && (x != nullptr || top > 128)) hipLaunchKernelGGL(vocab_teacher_kernel<256>, dim3(all), dim3(256), lds, s, t);
@@ -1165,7 +1167,7 @@ PDT_API int pdt_head_loss(const void* x, const void* w, const long long* ids, co
         vl_plan(g, false);
         if (int e = vl_launch<0>(g, s)) return e;
         Rows a = {h.stats, h.e, pitch, ids + static_cast<size_t>(r0) * top, h.r.p == nullptr ? nullptr : h.r.p + static_cast<size_t>(r0) * top,
-                  h.z == nullptr ? nullptr : h.z + static_cast<size_t>(r0) * top, h.r.base + r0, h.r.valid + r0, h.r.row_loss + r0, g.groups, top, n, vocab, big};
+                  h.z == nullptr ? nullptr : h.z + static_cast<size_t>(r0) * top, h.r.base + r0, h.r.valid + r0, h.r.row_loss + r0, g.groups, top, n, vocab, big, g.scale_log2};
         hipLaunchKernelGGL(vocab_rows_kernel, dim3(train ? pdt_cdiv(n, 64) * 64 : n), dim3(1024), 0, s, a);
         g = {};
         g.lda = pitch; g.ldb = width;

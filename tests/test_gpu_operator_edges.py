@@ -419,3 +419,28 @@ def test_losses_without_a_gradient_in_pieces(ops, monkeypatch):
             pieces, little = peak(call)
         assert torch.equal(whole, pieces)
         assert much >= n * 8 * groups and little < 256 * 8 * groups + (1 << 20)
+
+
+@pytest.mark.parametrize("tau", [1e-3, 0.05])
+def test_students_equal_to_their_teacher_at_low_temperatures(ops, tau):
+    """Exponents of 10^4 and more: q is formed from differences to the row's maximum, so that it agrees with p to 32 bits."""
+    n, vocab, width, top = 40, 700, 128, 8
+    x = torch.randint(-3, 4, (n, width), generator=_gen(1), device="cuda").to(torch.bfloat16).requires_grad_(True)
+    w = (torch.randint(-3, 4, (vocab, width), generator=_gen(2), device="cuda").to(torch.bfloat16) / 8).requires_grad_(True)
+    x64, w64 = x.detach().double(), w.detach().double()
+    with torch.no_grad():
+        w[1], w[2] = w[0], w[0]  # a few entries that share the maximum
+        x.abs_()
+        w[:3] = w[:3].abs() + 0.125
+    x64, w64 = x.detach().double(), w.detach().double()
+    z = x64 @ w64.t()
+    ids = z.topk(top, 1).indices
+    teacher = z.gather(1, ids).float()
+    dx, dw = torch.autograd.grad(ops.linear_distillation_loss(x, w, teacher, ids, tau), (x, w))
+    q, p = torch.softmax(z / tau, 1), torch.softmax(teacher.double() / tau, 1)
+    dz = q.scatter_add(1, ids, -p) * (tau / n)
+    others = q.scatter(1, ids, 0.0) * (tau / n)
+    f = 2.01 * H * others + H * (dz - others).abs() + 2e-5 * (tau / n) * q.scatter_add(1, ids, p)
+    for got, want, bound in ((dx, dz @ w64, f @ w64.abs()), (dw, dz.t() @ x64, f.t() @ x64.abs())):
+        over = (got.double() - want).abs() - 1.05 * (bound + H * want.abs())
+        assert float(over.max()) <= 0, float(over.max())
