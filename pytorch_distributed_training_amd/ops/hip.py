@@ -133,9 +133,12 @@ def _once_differentiable(backward):
 def _derivative_wanted(*inputs: torch.Tensor) -> bool:
     """Whether a call on these has to go through its autograd function: one of them requires a gradient, or carries a tangent
     (forward mode knows neither ``requires_grad`` nor ``no_grad``; the function refuses it instead of dropping it)."""
-    if torch.is_grad_enabled() and any(x.requires_grad for x in inputs):
-        return True
-    return any(_forward_ad.unpack_dual(x).tangent is not None for x in inputs)
+    if torch.is_grad_enabled():
+        for x in inputs:
+            if x.requires_grad:
+                return True
+    # (outside every dual level, nearly always, no tensor is looked at: half a microsecond each)
+    return getattr(_forward_ad, "_current_level", 0) >= 0 and any(_forward_ad.unpack_dual(x).tangent is not None for x in inputs)
 
 
 def _on(device: torch.device):
