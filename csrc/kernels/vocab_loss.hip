@@ -66,8 +66,8 @@ __device__ __forceinline__ float vl_exp2(float x) { return __builtin_amdgcn_exp2
 // Work: whole tiles first, a multiple of the workgroups; the tiles left over (all, where the tiles are few) are cut along k
 // into parts that fill the last round, summed in order by vocab_join_kernel.
 //
-// Measured (a library product of 8192^3 in bf16 runs at 1.5 PFLOP/s): 8192 rows, 50257 entries, width 1024: scores 768 us
-// (1.1 PFLOP/s: 16 K-steps, then exponentials, maxima and 128 KB of results per tile), dx and dW 635 to 660 us (1.3);
+// Measured (a library product of 8192^3 in bf16 runs at 1.5 PFLOP/s): 8192 rows, 50257 entries, width 1024: scores 750 to 800 us by
+// the card (1.1 PFLOP/s: 16 K-steps, then exponentials, maxima and 128 KB of results per tile), dx and dW 635 to 680 us (1.3);
 // 130001 entries, width 2048: 3.5, 3.1 and 3.2 ms (1.25, 1.4, 1.36).  Bound by the matrix pipe between the tiles' ends.  512 rows,
 // width 768: 54, 43 and 51 us; 64 rows, scores alone: 22 us, W read at 3.5 TB/s.
 // ------------------------------------------------------------------------------------------------
@@ -608,19 +608,23 @@ struct Targets {
     float inv_tau;
 };
 
-// sum of s[lane / 8] over the wave: every exchange halves the values a lane still has to do with
+// a + (a of lane ^ LANES) in the lanes whose bit LANES is clear, the same of b in the others
+template <int LANES>
+__device__ __forceinline__ float vl_halves(float a, float b) {
+    const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+    u32x2 r;
+    if constexpr (LANES == 16) r = __builtin_amdgcn_permlane16_swap(x, y, false, false);
+    else r = __builtin_amdgcn_permlane32_swap(x, y, false, false);
+    const uint32_t lo = r[0], hi = r[1];
+    return __builtin_bit_cast(float, lo) + __builtin_bit_cast(float, hi);
+}
+// sum of s[lane / 8] over the wave: the first three exchanges each halve the values a lane still has to do with
 __device__ __forceinline__ float vl_sums8(const float (&s)[8], int lane) {
-    float v[8];
+    float v[4];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) v[i] = s[i];
-#pragma unroll
-    for (int n = 4, bit = 32; n > 0; n >>= 1, bit >>= 1)
-#pragma unroll
-        for (int i = 0; i < n; ++i) {
-            const float keep = lane & bit ? v[i + n] : v[i], give = lane & bit ? v[i] : v[i + n];
-            v[i] = keep + __shfl_xor(give, bit, 64);
-        }
-    float r = v[0];
+    for (int i = 0; i < 4; ++i) v[i] = vl_halves<32>(s[i], s[i + 4]);
+    const float a = vl_halves<16>(v[0], v[2]), b = vl_halves<16>(v[1], v[3]);
+    float r = (lane & 8 ? b : a) + __shfl_xor(lane & 8 ? a : b, 8, 64);
 #pragma unroll
     for (int o = 4; o > 0; o >>= 1) r += __shfl_xor(r, o, 64);
     return r;
@@ -694,7 +698,7 @@ __global__ __launch_bounds__(256) void vocab_labels_kernel(const Targets t) {
 }
 
 // a teacher: one workgroup per row, of four waves where there are rows of W to fetch (512 rows of 32 targets, width 768: 12 us,
-// with one wave 21; 8192 rows of 64 targets, width 1024: 153, 174) or targets by the hundred, else of one (8192 rows of 64
+// with one wave 17; 8192 rows of 64 targets, width 1024: 157, 172) or targets by the hundred, else of one (8192 rows of 64
 // targets on given logits: 17 us, with four 46).  What is left of an id that repeats is its first entry, with all their weight.
 template <int THREADS>
 __global__ __launch_bounds__(THREADS) void vocab_teacher_kernel(const Targets t) {
@@ -806,8 +810,8 @@ struct Rows {
 };
 
 static_assert(VL_MAX_TOP <= 1024, "a thread per target");
-// (of 1024 threads: 8192 rows of 50257 entries 279 us for labels, 298 for 64 targets; with 512 threads 296 and 306, with 256
-// 312 and 328.  At 4.4 to 5.9 TB/s it is bound by memory.)
+// (of 1024 threads: 8192 rows of 50257 entries 290 us for labels, 314 for 64 targets; with 512 threads 297 and 321, with 256
+// 312 and 337.  At 5.2 to 5.7 TB/s it is bound by memory.)
 __global__ __launch_bounds__(1024) void vocab_rows_kernel(const Rows a) {
     constexpr int THREADS = 1024;
     __shared__ float red[16];
@@ -816,6 +820,11 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(const Rows a) {
         for (long long c = tid * 8; c < a.lde; c += THREADS * 8) *reinterpret_cast<bf16x8*>(a.e + row * a.lde + c) = bf16x8{};
         return;
     }
+    // this thread's target, on its way under the sums (what it holds counts where p is not 0)
+    const size_t target = static_cast<size_t>(row) * a.top + tid;
+    const bool one = a.e != nullptr && tid < a.top;
+    const float p = one ? (a.p == nullptr ? 1.f : a.p[target]) : 0.f, z = one ? a.z[target] : 0.f;
+    const int at = one ? static_cast<int>(a.ids[target]) : 0;
     const float2* st = a.stats + static_cast<size_t>(row) * a.groups;
     float m = -VL_INF;
     for (int g = tid; g < a.groups; g += THREADS) m = fmaxf(m, st[g].x);
@@ -834,10 +843,6 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(const Rows a) {
         for (long long c = tid * 8; c < a.lde; c += THREADS * 8) *reinterpret_cast<bf16x8*>(e + c) = bf16x8{};
         return;
     }
-    const long long* ids = a.ids + static_cast<size_t>(row) * a.top;
-    const float p = tid < a.top ? (a.p == nullptr ? 1.f : a.p[static_cast<size_t>(row) * a.top + tid]) : 0.f;
-    const int at = p != 0.f ? static_cast<int>(ids[tid]) : 0;
-    const float val = p != 0.f ? vl_exp2(fmaf(a.z[static_cast<size_t>(row) * a.top + tid], a.scale_log2, -ref) - ls) - p : 0.f;
     for (long long c = tid * 8; c < a.lde; c += THREADS * 8) {
         const float f = vl_exp2(st[c >> 6].x - ref - ls);
         bf16x8 v = __builtin_nontemporal_load(reinterpret_cast<const bf16x8*>(e + c));
@@ -846,7 +851,7 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(const Rows a) {
         vl_store(reinterpret_cast<bf16x8*>(e + c), v, a.stream);
     }
     __syncthreads();  // every entry is rewritten
-    if (p != 0.f) e[at] = f32_to_bf16(val);
+    if (p != 0.f) e[at] = f32_to_bf16(vl_exp2(fmaf(z, a.scale_log2, -ref) - ls) - p);
 }
 
 // ---- on given logits: one workgroup per row
