@@ -884,7 +884,9 @@ struct ChunkOf {
 // The row stays in registers (NV chunks of 16 bytes per thread) between its maximum, its sum and the gradient: one read and
 // one write of the logits, 4.5 TB/s on 8192 rows of 50257 in bf16 (364 us).  NV = 0: rows too long for that are read again from
 // the caches; rows of all lengths done so: 8192 x 8000 119 us instead of 71, 8192 x 50257 561 instead of 377, 2048 x 131000 319
-// instead of 253 (2048 x 140000, too long: 340).
+// instead of 253 (2048 x 140000, too long: 340).  Chunks that a thread holds but the row does not fill cost occupancy: with 13 instead
+// of 16 of 512 threads bf16 rows of 33000 entries take 251 us instead of 271, of 50257 394 instead of 414, of 53000 the same 371
+// (loss and gradient, 8192 rows); with 1024 threads, fp32 or bf16, there is no difference, so they have 16 alone.
 template <typename T, int THREADS, int NV>
 __global__ __launch_bounds__(THREADS) void logits_distill_kernel(const Logits<T> a) {
     constexpr int W = 16 / sizeof(T);
@@ -1211,7 +1213,6 @@ static int distill_launch(const Logits<T>& a, int rows, hipStream_t s) {
     else if (chunks <= 8 * 512) PDT_LD(512, 8);
     else if (chunks <= 13 * 512) PDT_LD(512, 13);
     else if (chunks <= 16 * 512) PDT_LD(512, 16);
-    else if (chunks <= 13 * 1024) PDT_LD(1024, 13);
     else if (chunks <= 16 * 1024) PDT_LD(1024, 16);
     else PDT_LD(1024, 0);
 #undef PDT_LD
