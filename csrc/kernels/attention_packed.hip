@@ -342,7 +342,7 @@ __device__ __forceinline__ void ap_unit(const PackedArgs& p, int heads, int& blk
     to = e.z;
 }
 
-// Measured: D = 64, 16381 rows of documents of up to 1024, 16 heads, causal: 47 us - 150 MB of q, k, v, out and rest would take
+// Measured: D = 64, 16381 rows of documents of up to 1024, 16 heads, causal: 49 us - 150 MB of q, k, v, out and rest would take
 // 30 at the rate of a large copy; vector work (exponentials, the ends of short rows) and the waits of workgroups that live for
 // five tiles make up the rest.  D = 128, one document of 16384 rows, 16 heads on 4, causal: 1.08 ms, 1.02 PFLOP/s; matrix pipe and
 // vector ALU are busy 52 % and 45 % of the time, at 1.9 GHz.
@@ -569,8 +569,8 @@ __global__ __launch_bounds__(256, NP == 1 ? 4 : 2) void packed_fwd_kernel(const 
     }
 }
 
-// dQ, and the row terms that dK / dV start from.  Measured as the forward kernel: D = 64 64 us (218 MB, 43 us at a copy's rate);
-// D = 128 1.44 to 1.48 ms, 1.11 to 1.14 PFLOP/s (three products), matrix pipe busy 60 % at 1.85 GHz.
+// dQ, and the row terms that dK / dV start from.  Measured as the forward kernel: D = 64 65 us (218 MB, 43 us at a copy's rate);
+// D = 128 1.42 to 1.48 ms, 1.11 to 1.14 PFLOP/s (three products), matrix pipe busy 60 % at 1.85 GHz.
 template <int NP>
 __global__ __launch_bounds__(256, NP == 1 ? 3 : 2) void packed_dq_kernel(const PackedArgs p) {
     constexpr int TILE = NP * AT_TILE, RING = ap_ring<NP>;
@@ -777,7 +777,7 @@ __device__ __forceinline__ void dkv_store(const PackedArgs& p, f32x16 (&acc)[2 *
     }
 }
 
-// dK and dV of 64-wide heads.  Measured as the forward kernel: 72 us (201 MB, 40 us at a copy's rate), 80 with two waves per SIMD,
+// dK and dV of 64-wide heads.  Measured as the forward kernel: 74 us (201 MB, 40 us at a copy's rate), 80 with two waves per SIMD,
 // more of each operand on its way and the row terms applied behind the products.
 __global__ __launch_bounds__(256, 3) void packed_dkv64_kernel(const PackedArgs p) {
     constexpr int NP = 1;
@@ -931,7 +931,7 @@ __global__ __launch_bounds__(256, 3) void packed_dkv64_kernel(const PackedArgs p
 // P goes from the one to the other through LDS in fp32, register for register (the two products have the same layout).  The
 // work is a sequence of phases of 32 queries with a barrier each; the dS waves run one phase behind.  Tiles are 64 queries
 // (32 KB with dO) in a ring of three: one arriving, one of the P waves, one that the dS waves may still need.
-// Measured as the forward kernel: 2.25 to 2.33 ms, 0.94 to 0.98 PFLOP/s (four products), matrix pipe busy 46 to 49 %: a phase takes 2400 cycles of which
+// Measured as the forward kernel: 2.20 to 2.33 ms, 0.94 to 1.0 PFLOP/s (four products), matrix pipe busy 46 to 49 %: a phase takes 2400 cycles of which
 // the two waves' products are 1024, the rest is each wave's chain from one product over the vector work to the next.  (Products issued behind the wait for
 // the other operands instead of between their reads: 3 % slower; all reads issued first: the same; dS
 // waves half a phase out of step with the P waves, their dK products under the P waves' exponentials: 2.49 ms; products in front of
@@ -1171,10 +1171,11 @@ __device__ __forceinline__ int pack_rank(const int* w, int count, int mine, int 
     return rank;
 }
 
-// Packs of few blocks (one round of workgroups) and of very many (the last round does not matter, the counting does) keep the
-// rows' own order.  Pack, forward and backward in this order and in the rows' own: 18 blocks of one document, 16 heads of 64 131 and
-// 125 us, 32 blocks 233 and 228, 32 blocks with 32 heads of 128 476 and 486, 64 blocks of documents of up to 4096 rows 506 and 530,
-// 4096 blocks, 2 heads of 64 1202 and 1213, 8192 blocks 2690 and 2385.
+// Packs of few blocks and of very many (the last round does not matter, the counting does) keep the rows' own order.  Pack, forward
+// and backward in order of falling work and in the rows' own, from a graph: documents of 1 to 4096 rows, 16 heads of 64, 24 blocks
+// 123 and 123 us, 32 blocks 148 and 151, 48 210 and 229, 64 300 and 312, 128 304 and 358, 256 790 and 836; 32 heads of 128 on eight,
+// 24 blocks 243 and 242, 32 blocks 282 and 302, 64 867 and 864; 4 heads of 64, 32 blocks 138 and 138, 128 182 and 189.  One document
+// (ordered either way): within 1 %.  4096 blocks, 2 heads of 64 1202 and 1213, 8192 blocks 2690 and 2385.
 #define AP_ORDER_FROM 31
 #define AP_ORDER_TO 4096
 #define AP_ORDER_ONCE 512    // blocks that one workgroup puts in order, in the launch that makes the spans
