@@ -633,7 +633,7 @@ __device__ __forceinline__ float vl_sums8(const float (&s)[8], int lane) {
 // - p . (x . W[id]) / tau of a row's targets, eight at a time (their rows of W are on their way together): this wave's share,
 // targets first, first + 8, ... of every `step`; lane's part of the sum.  The scores themselves are kept for q - p at the
 // targets: a student close to its teacher leaves little of that difference, and q from a rounded exponential would be most of
-// its error (70 rows of 64 targets, teacher within 0.003 of the student: dx off by 17 % of it, from these scores by 0.24 %).
+// its error (70 rows of 64 targets, teacher within 0.003 of the student: dx off by 17 % of it, from these scores by 0.2 %).
 template <typename P, typename I>
 __device__ __forceinline__ float vl_target_scores(const Targets& t, int row, int first, int step, int lane, P p_of, I id_of) {
     const bf16* x = t.x + static_cast<size_t>(row) * t.width;
@@ -810,8 +810,8 @@ struct Rows {
 };
 
 static_assert(VL_MAX_TOP <= 1024, "a thread per target");
-// (of 1024 threads: 8192 rows of 50257 entries 290 us for labels, 314 for 64 targets; with 512 threads 297 and 321, with 256
-// 312 and 337.  At 5.2 to 5.7 TB/s it is bound by memory.)
+// (of 1024 threads: 8192 rows of 50257 entries 285 us for labels, 297 for 64 targets; before the targets' lines were read first 290
+// and 314, with 512 threads 297 and 321, with 256 312 and 337.  At 5.5 to 5.8 TB/s it is bound by memory.)
 __global__ __launch_bounds__(1024) void vocab_rows_kernel(const Rows a) {
     constexpr int THREADS = 1024;
     __shared__ float red[16];
@@ -843,6 +843,11 @@ __global__ __launch_bounds__(1024) void vocab_rows_kernel(const Rows a) {
         for (long long c = tid * 8; c < a.lde; c += THREADS * 8) *reinterpret_cast<bf16x8*>(e + c) = bf16x8{};
         return;
     }
+    // The loop goes around the caches, and a store of two bytes behind it would fetch its line again: the targets' lines are read into
+    // them before any thread gets there (the value is of no use; 64 targets a row: 315 -> 297 us, labels 290 -> 285).
+    float line = p != 0.f ? bf16_to_f32(e[at]) : 0.f;
+    asm volatile("" : "+v"(line));
+    __syncthreads();
     for (long long c = tid * 8; c < a.lde; c += THREADS * 8) {
         const float f = vl_exp2(st[c >> 6].x - ref - ls);
         bf16x8 v = __builtin_nontemporal_load(reinterpret_cast<const bf16x8*>(e + c));
