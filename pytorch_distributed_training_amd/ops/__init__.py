@@ -13,7 +13,6 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd import forward_ad
 
 from . import reference as _ref
 from .packing import SequencePack, pack_sequences  # noqa: F401
@@ -166,7 +165,7 @@ def _check_teacher(lead, teacher_logits, teacher_ids, temperature: float, device
     _check_targets(tuple(lead) + (top,), teacher_ids, device, what, "teacher ids")
     if teacher_logits.shape != teacher_ids.shape or teacher_logits.device != device or not teacher_logits.is_floating_point():
         raise ValueError(f"{what}: teacher logits must be floating-point, of the ids' shape and device")
-    if teacher_logits.requires_grad or forward_ad.unpack_dual(teacher_logits).tangent is not None:
+    if teacher_logits.requires_grad or _ref.any_tangent(teacher_logits):
         raise ValueError(f"{what}: no gradient flows to the teacher; pass its logits detached")
     temperature = float(temperature)
     if not 1e-6 <= temperature <= 1e6:  # (its square and its inverse are fp32 factors)

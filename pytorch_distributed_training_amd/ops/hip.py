@@ -26,9 +26,9 @@ from typing import Dict, List, Optional, Sequence, Tuple
 
 import torch
 import torch.nn as nn
-from torch.autograd import forward_ad as _forward_ad
 
 from .. import native
+from .reference import any_tangent
 
 _lib = native.kernels()
 _vp, _i, _f, _ll = ctypes.c_void_p, ctypes.c_int, ctypes.c_float, ctypes.c_longlong
@@ -137,8 +137,7 @@ def _derivative_wanted(*inputs: torch.Tensor) -> bool:
         for x in inputs:
             if x.requires_grad:
                 return True
-    # (outside every dual level, nearly always, no tensor is looked at: half a microsecond each)
-    return getattr(_forward_ad, "_current_level", 0) >= 0 and any(_forward_ad.unpack_dual(x).tangent is not None for x in inputs)
+    return any_tangent(*inputs)
 
 
 def _on(device: torch.device):
