@@ -6,8 +6,10 @@ embeddings) that stresses the bucket reducer and the fused AdamW step.
 The forward pass returns logits; with ``targets`` it returns the mean next-token
 cross-entropy from the fused output-projection + loss operator, which works through the rows
 in chunks and never materialises logits or probabilities for the whole batch; with ``teacher``
-the divergence from a teacher's top logits, in the same way.  Documents of different lengths
-train without padding, packed one behind the other along one axis (``pack``).
+the divergence from a teacher's top logits.  Documents of different lengths train without
+padding, packed one behind the other along one axis (``pack``).  These two, and vocabularies
+beyond 65 536 entries, hold a bf16 buffer of rows x vocabulary, of 8 GiB at most, while they
+train (:func:`ops.linear_cross_entropy`).
 """
 
 from __future__ import annotations

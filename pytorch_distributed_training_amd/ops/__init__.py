@@ -176,8 +176,10 @@ def _check_teacher(lead, teacher_logits, teacher_ids, temperature: float, device
 def linear_cross_entropy(x, weight, labels):
     """Mean cross-entropy of the logits ``x W^T`` (``x`` ``[..., width]``, ``weight`` ``[vocabulary, width]``, no bias)
     against ``labels`` ``[...]``, over the rows that have a label: a label outside ``[0, vocabulary)`` (-100, say) leaves
-    its row out, without gradient and not counted.  0 where no row has one.  On GPU the vocabulary, of any size, is worked
-    off in tiles and the logits are never stored; matrix products take bf16, loss and sums are fp32."""
+    its row out, without gradient and not counted.  0 where no row has one.  On GPU the vocabulary (below 2^22 entries) is
+    worked off in tiles; matrix products take bf16, loss and sums are fp32.  With a gradient one buffer of rows x vocabulary in
+    bf16 is held, of ``PDT_VOCAB_CHUNK_MB`` (8192) MB at most: beyond, rows are worked off in pieces; without one, an eighth of
+    a byte per entry."""
     _check_head(x, weight, "linear_cross_entropy")
     _check_targets(x.shape[:-1], labels, x.device, "linear_cross_entropy", "labels")
     if x.is_cuda and labels.numel():
@@ -203,7 +205,7 @@ def distillation_loss(logits, teacher_logits, teacher_ids, temperature: float = 
 
 
 def linear_distillation_loss(x, weight, teacher_logits, teacher_ids, temperature: float = 1.0):
-    """:func:`distillation_loss` of the logits ``x W^T``, which on GPU are never stored (see :func:`linear_cross_entropy`)."""
+    """:func:`distillation_loss` of the logits ``x W^T``, on GPU without storing them (see :func:`linear_cross_entropy`)."""
     _check_head(x, weight, "linear_distillation_loss")
     tau = _check_teacher(x.shape[:-1], teacher_logits, teacher_ids, temperature, x.device, "linear_distillation_loss")
     if x.is_cuda and teacher_ids.numel():
