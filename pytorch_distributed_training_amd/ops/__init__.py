@@ -121,8 +121,9 @@ def softmax_cross_entropy(logits, labels):
 
 def lm_head_loss(x, weight, labels):
     """Mean cross-entropy of the logits ``x W^T`` (no bias) against ``labels``: a language model's tied output
-    projection and loss, over the rows whose label lies in the vocabulary (0 without any).  On GPU the rows are processed in chunks through one scratch buffer, so the
-    ``[rows, vocabulary]`` logits of the whole batch never exist (see ``ops.hip._LMHeadLoss``)."""
+    projection and loss, over the rows whose label lies in the vocabulary (0 without any).  On GPU the rows are processed
+    in chunks through one scratch buffer, so the ``[rows, vocabulary]`` logits of the whole batch never exist (see
+    ``ops.hip._LMHeadLoss``)."""
     if x.is_cuda and 1024 < weight.shape[0] <= 65536 and _LM_HEAD_FUSED:
         return _hip().lm_head_loss(x, weight, labels)
     logits = linear(x, weight, None)

@@ -82,7 +82,8 @@ def softmax_cross_entropy(logits: torch.Tensor, labels: torch.Tensor) -> torch.T
     """Mean softmax cross-entropy over the rows with a label (not -100), 0 without any (role of ``nn.CrossEntropyLoss()`` at
     /root/reference/src/main.py:62,76)."""
     y = labels.reshape(-1)
-    return F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), y, reduction="mean" if bool((y != -100).any()) else "sum")
+    none = not y.is_cuda and not bool((y != -100).any())  # (not asked of the GPU, which would have to be waited for: NaN there)
+    return F.cross_entropy(logits.float().reshape(-1, logits.shape[-1]), y, reduction="sum" if none else "mean")
 
 
 def without_others(labels, vocab: int):
